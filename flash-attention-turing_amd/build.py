@@ -25,7 +25,9 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
-KERNEL_SOURCES = ["fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip"]
+KERNEL_SOURCES = ["fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip", "fa_diff_fwd.hip", "fa_diff_bwd.hip",
+                  "fa_diff_kv.hip", "fa_kvpages.hip"]
+EXTENSION_SOURCES = ["flash_api.cpp", "diff_api.cpp", "kvpages_api.cpp"]
 LIB_NAME = "libfa_mi355x.so"
 
 HIP_FLAGS = [
@@ -76,7 +78,7 @@ def build_library(jobs: int, out_dir: str = HERE, obj_dir: str = None) -> str:
     return lib
 
 
-def build_extension(out_dir: str = HERE) -> str:
+def build_extension(out_dir: str = HERE, obj_dir: str = None) -> str:
     """Link the extension against the libfa_mi355x.so already built in out_dir;
     it finds that library at run time next to itself (rpath $ORIGIN)."""
     import torch
@@ -87,19 +89,31 @@ def build_extension(out_dir: str = HERE) -> str:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     incs = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], f"{ROCM}/include", INCLUDE]
     libdirs = cpp_extension.library_paths()
-    cmd = [
-        "g++",
+    objdir = obj_dir or os.path.join(HERE, "_build")
+    os.makedirs(objdir, exist_ok=True)
+    flags = [
         "-O2",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1",
         "-DTORCH_EXTENSION_NAME=flash_attn_turing",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         *[f"-I{p}" for p in incs],
-        os.path.join(CSRC, "flash_api.cpp"),
+    ]
+
+    def compile_one(src):
+        obj = os.path.join(objdir, os.path.splitext(src)[0] + ".o")
+        _run(["g++", *flags, "-c", os.path.join(CSRC, src), "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(EXTENSION_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, EXTENSION_SOURCES))
+    _run([
+        "g++",
+        "-shared",
+        *objs,
         "-o",
         out + ".tmp",
         *[f"-L{p}" for p in libdirs],
@@ -114,8 +128,7 @@ def build_extension(out_dir: str = HERE) -> str:
         "-lamdhip64",
         "-Wl,-rpath,$ORIGIN",
         *[f"-Wl,-rpath,{p}" for p in libdirs],
-    ]
-    _run(cmd)
+    ])
     os.replace(out + ".tmp", out)
     return out
 

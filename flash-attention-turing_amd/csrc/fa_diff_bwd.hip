@@ -1,0 +1,683 @@
+// Differential attention, backward.
+//
+//   dP = dO v^T (shared by both maps), D_m = rowsum(P_m * dP) = dO . O_m
+//   dS_1 = P_1 (dP - D_1),  dS_2 = -lam P_2 (dP - D_2)
+//   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P_1 - lam P_2)^T dO
+//   dlam = -D_2, summed over the rows and heads that share a lam
+// with P_m = exp(scale S_m - LSE_m), 0 where masked.  o = O_1 - lam O_2 and the
+// forward's O_2 give D_2 = dO . O_2 and D_1 = dO . o + lam D_2.
+//
+// dQ kernel: 4 waves x 32 queries, S^T and dP^T with keys on the MFMA M
+// dimension, so a lane owns one query.  dQ_2's factor -lam belongs to the query
+// and is applied once at the end.  D_m from 16-bit O_m is off by up to half a
+// unit in its last place: enough for dS, where it weighs as the other
+// roundings do, but neither for dlam, which is D_2 itself, nor for rows of a few keys, whose dP -
+// D_m cancels.  So the kernel sums dS_2, which is D_2's error, in fp32
+// (sum_j P_2 (dP - D) = D_2 - D), and rows whose keys lie in the first block
+// take both D_m from that block's own P_m and dP.
+//
+// dK/dV kernel: 4 waves x 32 keys of one KV head, S and dP with queries on M.
+// It loops over the heads of the GQA group and sums them in fp32 registers.
+#include <algorithm>
+#include <type_traits>
+
+#include "fa_diff_common.h"
+
+namespace fa {
+
+constexpr int kDbThreads = 256;
+constexpr int kDbPlanes = 5;  // fp32 planes of the workspace: -D1, -D2, LSE1 * log2(e), LSE2 * log2(e), lam
+
+__host__ __device__ __forceinline__ int64_t diff_plane(const fa_diff_bwd_args &a) {
+    return int64_t(a.batch) * a.nheads * a.lse_seqlen;
+}
+
+template <int HD, bool BF, bool CAUSAL>
+__global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bwd_args a, const int num_m_blocks,
+                                                                const int lg) {
+    constexpr int NT = kDbThreads, BM = 128, BN = 64;
+    constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
+    constexpr int HG = HD / 32;  // MFMA K steps of one map's channels
+    constexpr int PIPE = 3;
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int packs = a.nheads >> lg, P = BM >> lg;
+    int b, h, mb;
+    if (a.work_order && a.cu_seqlens_q) {
+        const int nnb = (a.seqlen_k + 127) / 128;
+        const int it = a.work_order[int64_t(a.batch) * nnb + blockIdx.x / packs];
+        if (it < 0) return;
+        b = __builtin_amdgcn_readfirstlane(it / num_m_blocks);
+        mb = __builtin_amdgcn_readfirstlane(it - b * num_m_blocks);
+        h = (blockIdx.x % packs) << lg;
+    } else {
+        const int bp_count = a.batch * packs, bp = blockIdx.x % bp_count;
+        mb = blockIdx.x / bp_count;
+        if (CAUSAL) mb = num_m_blocks - 1 - mb;
+        b = bp / packs;
+        h = (bp - b * packs) << lg;
+    }
+    const int hk = h / (a.nheads / a.nheads_k);
+    const bool packed_q = a.cu_seqlens_q != nullptr, packed_k = a.cu_seqlens_k != nullptr;
+    const SeqInfo si = seq_info(b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
+    const int sq = si.sq, sk = si.sk, m0 = mb * P;
+    if (m0 >= sq) return;
+    h += wave >> (2 - lg);
+
+    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, si.k_start, hk);
+    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, si.k_start, hk);
+    const int64_t krs = a.k.row_stride, vrs = a.v.row_stride;
+    const int causal_off = sk - sq;
+    int n_end = sk;
+    if (CAUSAL) n_end = max(0, min(sk, m0 + P + causal_off));
+    const int n_blocks = (n_end + BN - 1) / BN;
+    const float cs = a.softmax_scale * kLog2e;
+
+    TileCopier<HD, BN, NT> kcp, vcp;
+    kcp.init(krs, wave, lane);
+    vcp.init(vrs, wave, lane);
+    auto issue = [&](int nb, int st) FA_INLINE {
+        const int n0 = nb * BN;
+        if (n0 + BN <= sk) {
+            kcp.template copy_to<true>(lds_addr(smem) + st * STAGE, kp + int64_t(n0) * krs, krs);
+            vcp.template copy_to<true>(lds_addr(smem) + st * STAGE + TILE, vp + int64_t(n0) * vrs, vrs);
+        } else {
+            dma_tile<HD, BN, NT>(smem + st * STAGE, kp, krs, n0, sk - 1, wave, lane);
+            dma_tile<HD, BN, NT>(smem + st * STAGE + TILE, vp, vrs, n0, sk - 1, wave, lane);
+        }
+    };
+    if (n_blocks > 0) issue(0, 0);
+
+    // Q^T, dO^T as B operands and this lane's half of the row's D.
+    const int q_lo = m0 + 32 * (wave & ((P >> 5) - 1));
+    const int qi = q_lo + (lane & 31);
+    const bool qv = qi < sq;
+    const int qr = qv ? qi : 0;
+    f16x8 qB[HD / 16], doB[HD / 16];
+    float d1 = 0.f, d2 = 0.f;
+    {
+        const f16 *qp = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, h) + qr * a.q.row_stride + 8 * hh;
+        const f16 *dop =
+            (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, si.q_start, h) + qr * a.dout.row_stride + 8 * hh;
+        const f16 *op = (const f16 *)a.o.ptr + base_off(a.o, packed_q, b, si.q_start, h) + qr * a.o.row_stride + 8 * hh;
+        const f16 *o2p =
+            (const f16 *)a.o2.ptr + base_off(a.o2, packed_q, b, si.q_start, h) + qr * a.o2.row_stride + 8 * hh;
+#pragma unroll
+        for (int g = 0; g < HD / 16; ++g) {
+            qB[g] = as_h8(qv ? ldg16(qp + 16 * g) : zero_u4());
+            doB[g] = as_h8(qv ? ldg16(dop + 16 * g) : zero_u4());
+            const f16x8 ov = as_h8(qv ? ldg16(op + 16 * g) : zero_u4());
+            const f16x8 o2v = as_h8(qv ? ldg16(o2p + 16 * g) : zero_u4());
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float x = elem<BF>(doB[g], t);
+                d1 += elem<BF>(ov, t) * x;
+                d2 += elem<BF>(o2v, t) * x;
+            }
+        }
+    }
+    const float lam = qv ? diff_lam(a.lam, b, si.q_start + qi, h) : 0.f;
+    const int64_t lrow = (int64_t(b) * a.nheads + h) * a.lse_seqlen;
+    const int64_t plane = diff_plane(a);
+    const float lse1 = qv ? a.lse[lrow + qi] * kLog2e : 0.f, lse2 = qv ? a.lse[plane + lrow + qi] * kLog2e : 0.f;
+    d2 = sum_xor32(d2);
+    d1 = fmaf(lam, d2, sum_xor32(d1));
+    // All keys of the wave's rows in block 0: D_m from that block.
+    const bool one = (CAUSAL ? min(sk, q_lo + 32 + causal_off) : sk) <= BN;
+    if (one) d1 = d2 = 0.f;
+    float ds2_sum = 0.f;  // this lane half's sum of P_2 (dP - D_2)
+
+    f32x16 dq[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) dq[i] = zero16();
+    TileReader<HD> rd;
+    rd.init(lane);
+
+    auto block = [&](int nb, auto mask_tag) FA_INLINE {
+        constexpr bool MASK = decltype(mask_tag)::value;
+        const int buf = nb & 1, n0 = nb * BN;
+        wait_vmem();
+        __syncthreads();  // block nb is in LDS; every wave is done with stage buf ^ 1
+        if (nb + 1 < n_blocks) issue(nb + 1, buf ^ 1);
+        if (CAUSAL && MASK && n0 > q_lo + 31 + causal_off) return;
+        if (q_lo >= sq) return;
+        const int soff = buf * STAGE;
+        static_assert(STAGE % 512 == 0, "stage offsets must be multiples of 512 bytes");
+        int ab = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff;
+        asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
+        const int lim = (CAUSAL ? min(sk - 1, qi + causal_off) : sk - 1) - n0;
+        f16x8 op[PIPE];
+        f32x16 dp[2];
+        // dP^T from -D_1 on, so that the product comes out as dP - D_1.
+        {
+            float nd = -d1;
+            asm volatile("" : "+v"(nd));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[0][i] = dp[1][i] = nd;
+        }
+        auto rd_dp = [&](int u) FA_INLINE {
+            op[u % PIPE] = rd.a_operand_at(smem + TILE + 32 * (u & 1) * (HD * 2), ab, u >> 1);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < PIPE - 1; ++u) rd_dp(u);
+#pragma unroll
+        for (int u = 0; u < HD / 8; ++u) {
+            if (u + PIPE - 1 < HD / 8) rd_dp(u + PIPE - 1);
+            dp[u & 1] = mfma16<BF>(op[u % PIPE], doB[u >> 1], dp[u & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            f32x16 s[2];
+            auto rd_k = [&](int u) FA_INLINE {
+                op[u % PIPE] = rd.a_operand_at(smem + 32 * (u & 1) * (HD * 2), ab, m * HG + (u >> 1));
+            };
+#pragma unroll
+            for (int u = 0; u < PIPE - 1; ++u) rd_k(u);
+#pragma unroll
+            for (int u = 0; u < 2 * HG; ++u) {
+                if (u + PIPE - 1 < 2 * HG) rd_k(u + PIPE - 1);
+                s[u & 1] = mfma16<BF>(op[u % PIPE], qB[m * HG + (u >> 1)], u < 2 ? zero16() : s[u & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const float lse = m == 0 ? lse1 : lse2;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float x = exp2_fast(fmaf(s[t][r], cs, -lse));
+                    if constexpr (MASK) x = t * 32 + acc_lrow(r, hh) > lim ? 0.f : x;
+                    s[t][r] = x;
+                }
+            float e = m == 0 ? 0.f : d1 - d2;
+            if constexpr (MASK) {
+                if (one) {
+                    float d = 0.f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) d = fmaf(s[t][r], dp[t][r], d);
+                    d = sum_xor32(d);
+                    e = -d;
+                    (m == 0 ? d1 : d2) = d;
+                }
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[t][r] *= dp[t][r] + e;
+                    if (m == 1) sum += s[t][r];
+                }
+            ds2_sum += sum;
+            f16x8 dsB[4];
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg) dsB[gg] = pack16<BF>(s[gg >> 1], 8 * (gg & 1));
+            // dQ_m^T += K_m^T dS_m^T: step u is key step u / HG, channel tile u % (HG / 1) of the map.
+            constexpr int DT = HD / 64;  // 32-channel tiles of a map
+            auto rd_dq = [&](int u) FA_INLINE {
+                op[u % PIPE] = rd.tr_operand_at(smem + 16 * (u / DT) * (HD * 2), tb0, tb1, m * DT + u % DT);
+            };
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < PIPE - 1; ++u) rd_dq(u);
+#pragma unroll
+            for (int u = 0; u < 4 * DT; ++u) {
+                if (u + PIPE - 1 < 4 * DT) rd_dq(u + PIPE - 1);
+                dq[m * DT + u % DT] = mfma16<BF>(op[u % PIPE], dsB[u / DT], dq[m * DT + u % DT]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    // Blocks [0, n_full) are fully visible to every row of the workgroup; where
+    // a wave's rows see block 0 alone, that block is taken as a masked one.
+    int n_full = min(n_blocks, sk / BN);
+    if (CAUSAL) n_full = min(n_full, max(0, (m0 + causal_off + 1) / BN));
+    if (n_full == 1 && (CAUSAL ? min(sk, m0 + 32 + causal_off) : sk) <= BN) n_full = 0;
+    for (int nb = 0; nb < n_full; ++nb) block(nb, std::false_type{});
+    for (int nb = n_full; nb < n_blocks; ++nb) block(nb, std::true_type{});
+
+    ds2_sum = sum_xor32(ds2_sum);
+    if (!qv) return;
+    if (hh == 0) {
+        float *w = a.dsum + lrow + qi;
+        w[0] = -d1;
+        w[plane] = -(d2 + ds2_sum);
+        w[2 * plane] = lse1;
+        w[3 * plane] = lse2;
+        w[4 * plane] = lam;
+    }
+    int qo = qi;
+    asm volatile("" : "+v"(qo));
+    f16 *row = (f16 *)a.dq.ptr + base_off(a.dq, packed_q, b, si.q_start, h) + int64_t(qo) * a.dq.row_stride;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt) {
+        const float f = dt < HD / 64 ? a.softmax_scale : -lam * a.softmax_scale;
+#pragma unroll
+        for (int a4 = 0; a4 < 4; ++a4)
+            *reinterpret_cast<f16x4 *>(row + dt * 32 + 8 * a4 + 4 * hh) =
+                pack4<BF>(dq[dt][4 * a4] * f, dq[dt][4 * a4 + 1] * f, dq[dt][4 * a4 + 2] * f, dq[dt][4 * a4 + 3] * f);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dK/dV: workgroup = 128 keys of one (batch, KV head), wave w keys 32 w .. + 31.
+// K rows live in registers (S's B operands), V rows in LDS (dP's), and every
+// 32-query block of Q, dO and the rows' D, LSE and lam goes HBM -> LDS in two
+// stages.  With lp = lam P_2: P = P_1 - lp feeds dV, dS_1 = P_1 (dP - D_1) and
+// lp (dP - D_2) feed dK; the latter's sign is applied at the end.
+template <int HD, bool BF, bool CAUSAL>
+__global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_bwd_args a, const int nnb) {
+    constexpr int NT = kDbThreads, BN = 128, BM = 32;
+    constexpr int QTILE = BM * HD * 2, STAGE = 2 * QTILE + 1024;  // Q, dO, 3 pairs of row planes
+    constexpr int HG = HD / 32, DT = HD / 64;
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + BN * HD * 2];
+
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int b, hk, nb;
+    if (a.work_order && a.cu_seqlens_k) {
+        const int it = a.work_order[blockIdx.x / a.nheads_k];
+        if (it < 0) return;
+        b = __builtin_amdgcn_readfirstlane(it / nnb);
+        nb = __builtin_amdgcn_readfirstlane(it - b * nnb);
+        hk = blockIdx.x % a.nheads_k;
+    } else {
+        const int bh_count = a.batch * a.nheads_k, bhk = blockIdx.x % bh_count;
+        nb = blockIdx.x / bh_count;  // the key blocks that most queries see first
+        b = bhk / a.nheads_k;
+        hk = bhk - b * a.nheads_k;
+    }
+    const int G = a.nheads / a.nheads_k;
+    const bool packed_q = a.cu_seqlens_q != nullptr, packed_k = a.cu_seqlens_k != nullptr;
+    const SeqInfo si = seq_info(b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
+    const int sq = si.sq, sk = si.sk, k0 = nb * BN;
+    if (k0 >= sk) return;
+
+    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, si.k_start, hk);
+    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, si.k_start, hk);
+    const int causal_off = sk - sq;
+    const float cs = a.softmax_scale * kLog2e;
+    const int64_t qrs = a.q.row_stride, dors = a.dout.row_stride;
+    const int kw0 = k0 + wave * 32, key = kw0 + col;
+    TileReader<HD> rd;
+    rd.init(lane);
+    // V rows: row r of each 32-row group at position sigma(r), so that the B
+    // operand of key col is the conflict-free A-operand pattern.
+    {
+        constexpr int KCH = HD / 8;
+        char *tile = smem + 2 * STAGE;
+#pragma unroll
+        for (int i = 0; i < BN * KCH / NT; ++i) {
+            const int base = (i * (NT / 64) + wave) * 64;
+            const int p = base + lane, pos = p / KCH, c = p % KCH;
+            const int64_t r = min(k0 + ((pos & ~31) | sigma(pos & 31)), sk - 1);
+            g2l16(vp + r * a.v.row_stride + 8 * (c ^ swz<KCH>(pos)), tile + base * 16);
+        }
+    }
+    f16x8 kreg[HD / 16];
+    {
+        const f16 *kr = kp + int64_t(min(key, sk - 1)) * a.k.row_stride + 8 * hh;
+#pragma unroll
+        for (int g = 0; g < HD / 16; ++g) kreg[g] = *reinterpret_cast<const f16x8 *>(kr + 16 * g);
+    }
+    f32x16 dk[HD / 32], dv[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) dk[i] = dv[i] = zero16();
+
+    const int m_first = CAUSAL ? max(0, k0 - causal_off) / BM : 0;
+    const int n_qb = max(0, (sq + BM - 1) / BM - m_first);
+    TileCopier<HD, BM, NT> qcp, ocp;
+    qcp.init(qrs, wave, lane);
+    ocp.init(dors, wave, lane);
+    // Running pointers of the next (head, query block) to copy.
+    const int64_t plane = diff_plane(a);
+    const f16 *nq = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, hk * G);
+    const f16 *ndo = (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, si.q_start, hk * G);
+    const float *nd = a.dsum + (int64_t(b) * a.nheads + hk * G) * a.lse_seqlen;
+    int nh = 0, ni = 0;
+    const uint32_t smem_l = lds_addr(smem);
+    auto issue_next = [&](int st) FA_INLINE {
+        const int q0 = (m_first + ni) * BM;
+        if (q0 + BM <= sq) {
+            qcp.copy_to(smem_l + st * STAGE, nq + int64_t(q0) * qrs, qrs);
+            ocp.copy_to(smem_l + st * STAGE + QTILE, ndo + int64_t(q0) * dors, dors);
+        } else {
+            dma_tile<HD, BM, NT>(smem + st * STAGE, nq, qrs, q0, sq - 1, wave, lane);
+            dma_tile<HD, BM, NT>(smem + st * STAGE + QTILE, ndo, dors, q0, sq - 1, wave, lane);
+        }
+        // Planes 2w and 2w + 1 of the 32 rows by wave w (lanes 0..31 and 32..63).
+        if (wave < 3) {
+            const int64_t pl = min(2 * wave + hh, kDbPlanes - 1);
+            g2l4_to(nd + pl * plane + min(q0 + col, sq - 1), smem_l + st * STAGE + 2 * QTILE + wave * 256);
+        }
+        if (++ni == n_qb) {
+            ni = 0;
+            ++nh;
+            nq += a.q.head_stride;
+            ndo += a.dout.head_stride;
+            nd += a.lse_seqlen;
+        }
+    };
+    const int vb0 = rd.a_base + 2 * STAGE + 32 * wave * (HD * 2);
+    static_assert(STAGE % 512 == 0 && QTILE % 512 == 0, "tile offsets must be multiples of 512 bytes");
+
+    auto block = [&](int j, int qh0, auto mask_tag) FA_INLINE {
+        constexpr bool MASK = decltype(mask_tag)::value;
+        const int soff = (j & 1) * STAGE;
+        const float *lf = reinterpret_cast<const float *>(smem + soff + 2 * QTILE);  // planes of 32 rows
+        int qb = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff, vb = vb0;
+        asm volatile("" : "+v"(qb), "+v"(tb0), "+v"(tb1), "+v"(vb));
+        constexpr int PIPE = 2, NG = HD / 16;
+        f16x8 qa[PIPE], oa[PIPE], va[PIPE];
+        auto ld = [&](int g) FA_INLINE {
+            qa[g % PIPE] = rd.a_operand_at(smem, qb, g);
+            oa[g % PIPE] = rd.a_operand_at(smem + QTILE, qb, g);
+            va[g % PIPE] = rd.a_operand_at(smem, vb, g);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < PIPE - 1; ++g) ld(g);
+        f32x16 s[2], dp;
+#pragma unroll
+        for (int r8 = 0; r8 < 2; ++r8)  // accumulators 8 r8 + u: row 16 r8 + 8 hh + u
+#pragma unroll
+            for (int u = 0; u < 8; u += 4) {
+                const f32x4 d = *reinterpret_cast<const f32x4 *>(lf + 16 * r8 + 8 * hh + u);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) dp[8 * r8 + u + t] = d[t];
+            }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (g + PIPE - 1 < NG) ld(g + PIPE - 1);
+            const int m = g / HG;
+            s[m] = mfma16<BF>(qa[g % PIPE], kreg[g], g % HG == 0 ? zero16() : s[m]);
+            dp = mfma16<BF>(oa[g % PIPE], va[g % PIPE], dp);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // Query row c = 16 r8 + u (from qh0 + 8 hh) is live for m_lo <= c < m_hi.
+        const int mbase = qh0 + 8 * hh;
+        const int m_lo = CAUSAL ? key - causal_off - mbase : -(1 << 30), m_hi = sq - mbase;
+        f16x8 pB[2], d1B[2], d2B[2];
+#pragma unroll
+        for (int r8 = 0; r8 < 2; ++r8) {
+#pragma unroll
+            for (int u4 = 0; u4 < 8; u4 += 4) {
+                const float *row = lf + 16 * r8 + 8 * hh + u4;
+                const f32x4 nd1 = *reinterpret_cast<const f32x4 *>(row), nd2 = *reinterpret_cast<const f32x4 *>(row + 32);
+                const f32x4 l1 = *reinterpret_cast<const f32x4 *>(row + 64), l2 = *reinterpret_cast<const f32x4 *>(row + 96);
+                const f32x4 lam = *reinterpret_cast<const f32x4 *>(row + 128);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int r = 8 * r8 + u4 + t;
+                    float p1 = exp2_fast(fmaf(s[0][r], cs, -l1[t]));
+                    float p2 = exp2_fast(fmaf(s[1][r], cs, -l2[t])) * lam[t];
+                    if constexpr (MASK) {
+                        const int c = 16 * r8 + u4 + t;
+                        const bool off = c < m_lo || c >= m_hi;
+                        p1 = off ? 0.f : p1;
+                        p2 = off ? 0.f : p2;
+                    }
+                    const float x = dp[r];
+                    s[0][r] = p1 - p2;
+                    dp[r] = p1 * x;
+                    s[1][r] = p2 * (x + (nd2[t] - nd1[t]));
+                }
+            }
+            pB[r8] = pack16<BF>(s[0], 8 * r8);
+            d1B[r8] = pack16<BF>(dp, 8 * r8);
+            d2B[r8] = pack16<BF>(s[1], 8 * r8);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int NT2 = 2 * (HD / 32);
+        f16x8 ta[PIPE], tq[PIPE];
+        auto ldt = [&](int t) FA_INLINE {
+            ta[t % PIPE] = rd.tr_operand_at(smem + QTILE + 16 * (t & 1) * (HD * 2), tb0, tb1, t >> 1);
+            tq[t % PIPE] = rd.tr_operand_at(smem + 16 * (t & 1) * (HD * 2), tb0, tb1, t >> 1);
+        };
+#pragma unroll
+        for (int t = 0; t < PIPE - 1; ++t) ldt(t);
+#pragma unroll
+        for (int t = 0; t < NT2; ++t) {
+            if (t + PIPE - 1 < NT2) ldt(t + PIPE - 1);
+            dv[t >> 1] = mfma16<BF>(ta[t % PIPE], pB[t & 1], dv[t >> 1]);
+            dk[t >> 1] = mfma16<BF>(tq[t % PIPE], (t >> 1) < DT ? d1B[t & 1] : d2B[t & 1], dk[t >> 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // Per head four straight loops: blocks that see none of the wave's keys,
+    // diagonal blocks, full blocks, a ragged last block.
+    int j = 0;
+    auto step = [&](int i, auto mask_tag, bool compute) FA_INLINE {
+        wait_vmem();
+        __syncthreads();
+        if (nh < G) issue_next((j & 1) ^ 1);
+        if (compute) block(j, (m_first + i) * BM, mask_tag);
+        ++j;
+    };
+    auto clampi = [](int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); };
+    auto first_at = [&](int x) { return ((x + BM - 1) >> 5) - m_first; };
+    const int i1 = CAUSAL ? clampi(first_at(kw0 - 31 - causal_off), 0, n_qb) : 0;
+    const int i2 = CAUSAL ? clampi(first_at(kw0 + 31 - causal_off), i1, n_qb) : 0;
+    const int i3 = clampi(first_at(sq - 31), i2, n_qb);
+    if (n_qb > 0)
+        issue_next(0);
+    else
+        wait_vmem();
+    for (int hidx = 0; hidx < G && n_qb > 0; ++hidx) {
+        for (int i = 0; i < i1; ++i) step(i, std::true_type{}, false);
+        for (int i = i1; i < i2; ++i) step(i, std::true_type{}, true);
+        for (int i = i2; i < i3; ++i) step(i, std::false_type{}, true);
+        for (int i = i3; i < n_qb; ++i) step(i, std::true_type{}, true);
+    }
+
+    if (key >= sk) return;
+    f16 *dkrow = (f16 *)a.dk.ptr + base_off(a.dk, packed_k, b, si.k_start, hk) + int64_t(key) * a.dk.row_stride;
+    f16 *dvrow = (f16 *)a.dv.ptr + base_off(a.dv, packed_k, b, si.k_start, hk) + int64_t(key) * a.dv.row_stride;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt) {
+        const float f = dt < DT ? a.softmax_scale : -a.softmax_scale;
+#pragma unroll
+        for (int a4 = 0; a4 < 4; ++a4) {
+            const int c = 4 * a4;
+            *reinterpret_cast<f16x4 *>(dkrow + dt * 32 + 8 * a4 + 4 * hh) =
+                pack4<BF>(dk[dt][c] * f, dk[dt][c + 1] * f, dk[dt][c + 2] * f, dk[dt][c + 3] * f);
+            *reinterpret_cast<f16x4 *>(dvrow + dt * 32 + 8 * a4 + 4 * hh) =
+                pack4<BF>(dv[dt][c], dv[dt][c + 1], dv[dt][c + 2], dv[dt][c + 3]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dlam from the rows' -D_2 (plane 1 of the workspace, written by the dQ kernel).
+// A lam for each row: one value each, transposed.  One that rows share: one
+// workgroup per head sums its rows in fp64 in a fixed order, and for a lam of
+// all heads the second launch sums the heads.
+__global__ __launch_bounds__(1024) void diff_dlam_rows_kernel(const fa_diff_bwd_args a) {
+    const int b = blockIdx.y;
+    const int64_t start = a.cu_seqlens_q ? a.cu_seqlens_q[b] : 0;
+    const int sq = a.cu_seqlens_q ? min(a.cu_seqlens_q[b + 1] - int(start), a.lse_seqlen) : a.seqlen_q;
+    const int64_t n = int64_t(sq) * a.nheads;
+    for (int64_t i = int64_t(blockIdx.x) * 1024 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 1024) {
+        const int64_t row = i / a.nheads;
+        const int h = int(i - row * a.nheads);
+        a.dlam.ptr[b * a.dlam.batch_stride + (start + row) * a.dlam.row_stride + h * a.dlam.head_stride] =
+            a.dsum[diff_plane(a) + (int64_t(b) * a.nheads + h) * a.lse_seqlen + row];
+    }
+}
+
+__device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[16];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double s = 0;
+    for (int i = 0; i < int(blockDim.x >> 6); ++i) s += part[i];
+    return s;
+}
+
+// Head blockIdx.x; the sum goes to dlam (a lam for each head) or, for a lam of
+// all heads, to plane 0 of the workspace, which nothing reads any more.
+__global__ __launch_bounds__(1024) void diff_dlam_head_kernel(const fa_diff_bwd_args a, double *const sums) {
+    const int h = blockIdx.x;
+    const float *nd2 = a.dsum + diff_plane(a);
+    double x = 0;
+    for (int b = 0; b < a.batch; ++b) {
+        const int sq =
+            a.cu_seqlens_q ? min(a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b], a.lse_seqlen) : a.seqlen_q;
+        const float *row = nd2 + (int64_t(b) * a.nheads + h) * a.lse_seqlen;
+        for (int i = threadIdx.x; i < sq; i += 1024) x += row[i];
+    }
+    x = block_sum(x);
+    if (threadIdx.x == 0) {
+        if (sums)
+            sums[h] = x;
+        else
+            a.dlam.ptr[h * a.dlam.head_stride] = float(x);
+    }
+}
+
+__global__ __launch_bounds__(64) void diff_dlam_all_kernel(const fa_diff_bwd_args a, const double *const sums) {
+    double x = 0;
+    for (int h = threadIdx.x; h < a.nheads; h += 64) x += sums[h];
+    x = block_sum(x);
+    if (threadIdx.x == 0) a.dlam.ptr[0] = float(x);
+}
+
+// Packed batches: work orders and zeros in the gradients of rows of no sequence.
+__global__ __launch_bounds__(kOrderThreads) void diff_dkdv_order_kernel(const fa_diff_bwd_args a, const int nnb,
+                                                                        const int order_wgs) {
+    if (int(blockIdx.x) >= order_wgs) {
+        for (const fa_tensor *t : {&a.dk, &a.dv})
+            zero_gaps(*t, a.cu_seqlens_k, a.batch, a.seqlen_k, a.dkv_rows, a.nheads_k, a.head_dim,
+                      blockIdx.x - order_wgs, gridDim.x - order_wgs);
+        return;
+    }
+    order_items(a.batch * nnb, [&](int it) {
+        const int b = it / nnb, nb = it - b * nnb;
+        const int sk = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b], sq = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b];
+        const int k0 = nb * 128;
+        if (k0 >= sk) return -1;
+        const int rows = a.causal ? max(0, min(sq, sk - k0)) : max(sq, 0);
+        return min(rows >> 6, kOrderBuckets - 1);
+    }, a.work_order, false);
+}
+
+__global__ __launch_bounds__(kOrderThreads) void diff_dq_order_kernel(const fa_diff_bwd_args a, const int nnb,
+                                                                      const int nmb, const int P, const int order_wgs) {
+    if (int(blockIdx.x) >= order_wgs) {
+        zero_gaps(a.dq, a.cu_seqlens_q, a.batch, a.lse_seqlen, a.dq_rows, a.nheads, a.head_dim, blockIdx.x - order_wgs,
+                  gridDim.x - order_wgs);
+        return;
+    }
+    order_items(a.batch * nmb, [&](int it) {
+        const int b = it / nmb, mb = it - b * nmb;
+        const int sq = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b], sk = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b];
+        const int m0 = mb * P;
+        if (m0 >= sq) return -1;
+        const int keys = a.causal ? max(0, min(sk, m0 + P + sk - sq)) : sk;
+        return min(keys >> 6, kOrderBuckets - 1);
+    }, a.work_order + int64_t(a.batch) * nnb, false);
+}
+
+static int check_diff_bwd(const fa_diff_bwd_args *p) {
+    if (!p) return FA_ERR_INVALID_ARG;
+    const fa_diff_bwd_args &a = *p;
+    if (a.head_dim != 64 && a.head_dim != 128) return FA_ERR_UNSUPPORTED;
+    if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
+    if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_k < 0 || a.nheads <= 0 || a.nheads_k <= 0 ||
+        a.nheads % a.nheads_k != 0 || a.lse_seqlen < a.seqlen_q || (!a.cu_seqlens_q) != (!a.cu_seqlens_k) ||
+        a.batch > 65535)
+        return FA_ERR_INVALID_ARG;
+    if (!a.lse || !a.lam.ptr) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.o, &a.o2, &a.dout, &a.dq, &a.dk, &a.dv})
+        if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
+    if (!a.dsum || (reinterpret_cast<uintptr_t>(a.dsum) & 7u) || a.dsum_bytes < int64_t(fa_diff_bwd_ws_bytes(&a)))
+        return FA_ERR_WORKSPACE;
+    return FA_OK;
+}
+
+// Bytes of the planes, rounded so that the heads' fp64 sums, which follow, are aligned.
+static int64_t plane_bytes(const fa_diff_bwd_args &a) { return (kDbPlanes * diff_plane(a) * 4 + 7) & ~int64_t(7); }
+
+template <int HD, bool BF>
+static int launch_diff_bwd(const fa_diff_bwd_args &a, hipStream_t s) {
+    const int group = a.nheads / a.nheads_k;
+    int lg = 0;  // heads of a GQA group in a dQ workgroup
+    while (lg < 2 && group % (2 << lg) == 0) ++lg;
+    const int P = 128 >> lg, nmb = (a.lse_seqlen + P - 1) / P, nnb = (a.seqlen_k + 127) / 128;
+    const int64_t q_grid = int64_t(nmb) * a.batch * (a.nheads >> lg), k_grid = int64_t(nnb) * a.batch * a.nheads_k;
+    if (q_grid > 0x7fffffff || k_grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    int rc;
+    if (a.cu_seqlens_q && (a.work_order || a.dq_rows > 0)) {
+        const int order_wgs = a.work_order ? 1 : 0;
+        hipLaunchKernelGGL(diff_dq_order_kernel, dim3(order_wgs + (a.dq_rows > 0 ? kZeroBlocks : 0)),
+                           dim3(kOrderThreads), 0, s, a, nnb, nmb, P, order_wgs);
+        if ((rc = int(hipGetLastError()))) return rc;
+    }
+    if (q_grid > 0) {
+        if (a.causal)
+            hipLaunchKernelGGL((diff_dq_kernel<HD, BF, true>), dim3(unsigned(q_grid)), dim3(kDbThreads), 0, s, a, nmb, lg);
+        else
+            hipLaunchKernelGGL((diff_dq_kernel<HD, BF, false>), dim3(unsigned(q_grid)), dim3(kDbThreads), 0, s, a, nmb, lg);
+        if ((rc = int(hipGetLastError()))) return rc;
+    }
+    if (a.cu_seqlens_k && (a.work_order || a.dkv_rows > 0)) {
+        const int order_wgs = a.work_order ? 1 : 0;
+        hipLaunchKernelGGL(diff_dkdv_order_kernel, dim3(order_wgs + (a.dkv_rows > 0 ? kZeroBlocks : 0)),
+                           dim3(kOrderThreads), 0, s, a, nnb, order_wgs);
+        if ((rc = int(hipGetLastError()))) return rc;
+    }
+    if (k_grid > 0) {
+        if (a.causal)
+            hipLaunchKernelGGL((diff_dkdv_kernel<HD, BF, true>), dim3(unsigned(k_grid)), dim3(kDbThreads), 0, s, a, nnb);
+        else
+            hipLaunchKernelGGL((diff_dkdv_kernel<HD, BF, false>), dim3(unsigned(k_grid)), dim3(kDbThreads), 0, s, a, nnb);
+        if ((rc = int(hipGetLastError()))) return rc;
+    }
+    if (!a.dlam.ptr) return FA_OK;
+    if (a.dlam.row_stride != 0) {
+        if (a.batch == 0 || a.lse_seqlen == 0) return FA_OK;
+        const int64_t n = int64_t(a.lse_seqlen) * a.nheads;
+        hipLaunchKernelGGL(diff_dlam_rows_kernel, dim3(unsigned(std::min<int64_t>((n + 1023) / 1024, 1024)), a.batch),
+                           dim3(1024), 0, s, a);
+        return int(hipGetLastError());
+    }
+    double *sums = a.dlam.head_stride != 0
+                       ? nullptr
+                       : reinterpret_cast<double *>(reinterpret_cast<char *>(a.dsum) + plane_bytes(a));
+    hipLaunchKernelGGL(diff_dlam_head_kernel, dim3(a.nheads), dim3(1024), 0, s, a, sums);
+    if ((rc = int(hipGetLastError())) || !sums) return rc;
+    hipLaunchKernelGGL(diff_dlam_all_kernel, dim3(1), dim3(64), 0, s, a, sums);
+    return int(hipGetLastError());
+}
+
+}  // namespace fa
+
+extern "C" size_t fa_diff_bwd_ws_bytes(const fa_diff_bwd_args *a) {
+    if (!a || a->batch < 0 || a->nheads <= 0 || a->lse_seqlen < 0) return 0;
+    return size_t(fa::plane_bytes(*a) + 8 * int64_t(a->nheads));
+}
+
+extern "C" size_t fa_diff_bwd_order_len(const fa_diff_bwd_args *a) {
+    if (!a || a->batch <= 0) return 0;
+    return size_t(a->batch) *
+           (size_t((std::max(a->seqlen_k, 0) + 127) / 128) + size_t((std::max(a->lse_seqlen, 0) + 31) / 32));
+}
+
+extern "C" int fa_diff_bwd(const fa_diff_bwd_args *args, void *stream) {
+    const int rc = fa::check_diff_bwd(args);
+    if (rc) return rc;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const fa_diff_bwd_args &a = *args;
+    if (a.dtype == FA_BF16)
+        return a.head_dim == 128 ? fa::launch_diff_bwd<128, true>(a, s) : fa::launch_diff_bwd<64, true>(a, s);
+    return a.head_dim == 128 ? fa::launch_diff_bwd<128, false>(a, s) : fa::launch_diff_bwd<64, false>(a, s);
+}

@@ -8,6 +8,15 @@ the reference module (flash_attention_interface.py:448-922):
     flash_attn_varlen_func, flash_attn_varlen_qkvpacked_func,
     flash_attn_varlen_kvpacked_func, flash_attn_with_kvcache
 
+Beside them, without a counterpart in the reference: differential attention
+
+    flash_diff_attn_func, flash_diff_attn_varlen_func, flash_diff_attn_with_kvcache
+
+and the pages of a paged cache
+
+    flash_attn_kvcache_alloc, flash_attn_kvcache_copy_pages, flash_attn_kvcache_fork,
+    flash_attn_kvcache_free, flash_attn_kvcache_compact
+
 and the autograd classes FlashAttnFunc, FlashAttnQKVPackedFunc,
 FlashAttnKVPackedFunc, FlashAttnVarlenFunc, FlashAttnVarlenQKVPackedFunc,
 FlashAttnVarlenKVPackedFunc (:172-445).  Every call goes to the native
@@ -366,7 +375,16 @@ _KV_STATUS = {}
 _KV_STATUS_ERRORS = (
     (1, ValueError, "cache capacity is insufficient for the requested append length"),
     (2, RuntimeError, "cache_batch_idx entries must be within cache batch bounds"),
+    (4, RuntimeError, "block_table entries in use must be pages of the cache"),
+    (8, RuntimeError, "the cache has fewer free pages than the call needs"),
+    (16, ValueError, "a list of pages or rows holds one that is out of range, taken or named twice"),
 )
+
+
+def _raise_kv_status(bits: int) -> None:
+    for bit, exc, msg in _KV_STATUS_ERRORS:
+        if bits & bit:
+            raise exc(msg)
 
 
 def _kv_status(device: torch.device) -> torch.Tensor:
@@ -394,7 +412,8 @@ def flash_attn_kvcache_check(device: Optional[Union[torch.device, int]] = None) 
     whose cache_batch_idx is outside the cache, is left unchanged in the cache
     and gets O = 0 (LSE 0); this function then raises the error the default
     (validate=True) call raises at once: ValueError for the capacity,
-    RuntimeError for the cache row.  It reads the device (a synchronisation),
+    RuntimeError for the cache row.  The calls on the pages of a cache and
+    flash_diff_attn_with_kvcache report here as well.  It reads the device (a synchronisation),
     so call it outside captured graphs, for instance after each replay or
     every few steps.  It also allocates the device's status word, which must
     exist before a validate=False call is captured.
@@ -403,9 +422,7 @@ def flash_attn_kvcache_check(device: Optional[Union[torch.device, int]] = None) 
     bits = int(st.item())
     if bits:
         st.zero_()
-        for bit, exc, msg in _KV_STATUS_ERRORS:
-            if bits & bit:
-                raise exc(msg)
+        _raise_kv_status(bits)
 
 
 def flash_attn_with_kvcache(
@@ -530,3 +547,244 @@ def flash_attn_with_kvcache(
         lengths_checked=validate,
     )
     return (out, lse) if return_softmax_lse else out
+
+
+# ---------------------------------------------------------------------------
+# Differential attention (no counterpart in the reference).
+
+
+class FlashDiffAttnFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, softmax_scale, causal, is_grad_enabled):
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        save = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        out, o2, lse = flash_attn_gpu.diff_fwd(q, k, v, lam, softmax_scale, causal, save)
+        if save:
+            ctx.save_for_backward(q, k, v, lam, out, o2, lse)
+            ctx.softmax_scale, ctx.causal = softmax_scale, causal
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, lam, out, o2, lse = ctx.saved_tensors
+        dq, dk, dv, dlam = flash_attn_gpu.diff_bwd(
+            q, k, v, lam, out, o2, lse, maybe_contiguous(dout), ctx.softmax_scale, ctx.causal, ctx.needs_input_grad[3]
+        )
+        return dq, dk, dv, dlam, None, None, None
+
+
+class FlashDiffAttnVarlenFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+                is_grad_enabled):
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        save = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        out, o2, lse = flash_attn_gpu.diff_varlen_fwd(
+            q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal, save
+        )
+        if save:
+            ctx.save_for_backward(q, k, v, lam, out, o2, lse, cu_seqlens_q, cu_seqlens_k)
+            ctx.max_seqlen_q, ctx.max_seqlen_k = max_seqlen_q, max_seqlen_k
+            ctx.softmax_scale, ctx.causal = softmax_scale, causal
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, lam, out, o2, lse, cu_seqlens_q, cu_seqlens_k = ctx.saved_tensors
+        dq, dk, dv, dlam = flash_attn_gpu.diff_varlen_bwd(
+            q, k, v, lam, out, o2, lse, maybe_contiguous(dout), cu_seqlens_q, cu_seqlens_k, ctx.max_seqlen_q,
+            ctx.max_seqlen_k, ctx.softmax_scale, ctx.causal, ctx.needs_input_grad[3],
+        )
+        return dq, dk, dv, dlam, None, None, None, None, None, None, None
+
+
+def _check_diff_args(q, lam, softmax_scale):
+    _validate_supported_head_dim(q.shape[-1])
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("differential attention needs float16 or bfloat16 tensors")
+    if not isinstance(lam, torch.Tensor) or lam.dtype != torch.float32:
+        raise TypeError("lam must be a torch.float32 tensor")
+    # One map's channels are half of the head's.
+    return (q.shape[-1] // 2) ** (-0.5) if softmax_scale is None else softmax_scale
+
+
+def flash_diff_attn_func(q, k, v, lam, softmax_scale: Optional[float] = None, causal: bool = False) -> torch.Tensor:
+    """Differential attention, (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v.
+
+    q (batch, seqlen_q, nheads, headdim); k, v (batch, seqlen_k, nheads_k, headdim), fp16 or bf16.  The first
+    headdim / 2 channels of q and k are the first map's, the others the second's; headdim is 64 or 128 and
+    softmax_scale defaults to (headdim / 2) ** -0.5.  lam is fp32: a scalar tensor, (nheads,), or one value for each
+    query and head, (batch, seqlen_q, nheads).  causal, grouped heads and rows without a visible key are as in
+    flash_attn_func.  Returns out (batch, seqlen_q, nheads, headdim); q, k, v and lam get gradients."""
+    softmax_scale = _check_diff_args(q, lam, softmax_scale)
+    return FlashDiffAttnFunc.apply(q, k, v, lam, softmax_scale, causal, torch.is_grad_enabled())
+
+
+def flash_diff_attn_varlen_func(
+    q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int, max_seqlen_k: int,
+    softmax_scale: Optional[float] = None, causal: bool = False,
+) -> torch.Tensor:
+    """flash_diff_attn_func on packed sequences: q (total_q, nheads, headdim); k, v (total_k, nheads_k, headdim);
+    cu_seqlens_* int32 (batch_size + 1,); lam a scalar, (nheads,) or (total_q, nheads).  Rows that no sequence covers
+    are 0 in out and in the gradients."""
+    softmax_scale = _check_diff_args(q, lam, softmax_scale)
+    return FlashDiffAttnVarlenFunc.apply(
+        q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+        torch.is_grad_enabled(),
+    )
+
+
+def flash_diff_attn_with_kvcache(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    lam: torch.Tensor,
+    k: Optional[torch.Tensor] = None,
+    v: Optional[torch.Tensor] = None,
+    cache_seqlens: Optional[Union[torch.Tensor, int]] = None,
+    cache_batch_idx: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    causal: bool = False,
+    num_splits: int = 0,
+    return_softmax_lse: bool = False,
+    validate: bool = True,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Differential attention with a KV cache, for inference.
+
+    The caches, k, v, cache_seqlens, cache_batch_idx and block_table are those of flash_attn_with_kvcache (fp16 or
+    bf16; both maps' keys are the halves of a key's channels, so the two functions take the same caches; pages are a
+    multiple of 64 tokens here); lam is a scalar, (nheads,) or (batch, seqlen_q, nheads).  num_splits > 0 cuts the
+    cache's capacity into that many pieces.  return_softmax_lse adds the log-sum-exp of both maps, fp32 (2, batch,
+    nheads, seqlen_q).
+
+    validate as there: True checks lengths, rows and pages on the host; False leaves that to the kernels, which
+    record what is wrong for flash_attn_kvcache_check(): a sequence with a bad length or row is neither appended to
+    nor attended over, a page outside the cache is not written and page 0 is read in its place."""
+    softmax_scale = _check_diff_args(q, lam, softmax_scale)
+    if (k is None) != (v is None):
+        raise ValueError("k and v must either both be provided or both be None")
+    batch = q.shape[0]
+    capacity = _cache_capacity(k_cache, block_table)
+    if cache_seqlens is None:
+        if k is not None:
+            raise ValueError("cache_seqlens is required when appending k and v")
+        cache_seqlens = capacity
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((batch,), cache_seqlens, dtype=torch.int32, device=k_cache.device)
+    elif not isinstance(cache_seqlens, torch.Tensor):
+        raise TypeError("cache_seqlens must be an int or a torch.Tensor")
+    for name, t, shape in (("cache_seqlens", cache_seqlens, (batch,)), ("cache_batch_idx", cache_batch_idx, (batch,)),
+                           ("block_table", block_table, (batch, None))):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise TypeError(f"{name} must be a torch.int32 tensor")
+        if t.dim() != len(shape) or t.shape[0] != batch:
+            raise ValueError(f"{name} must have batch_size rows")
+    if block_table is not None and cache_batch_idx is not None:
+        raise NotImplementedError("Paged KV cache does not support cache_batch_idx")
+    if num_splits < 0:
+        raise ValueError("num_splits must be non-negative")
+    if validate and batch > 0:
+        lens = cache_seqlens.cpu()
+        used = lens + (0 if k is None else k.shape[1])
+        if int(lens.min()) < 0 or int(used.max()) > capacity:
+            raise ValueError("cache capacity is insufficient for the requested append length")
+        if cache_batch_idx is not None:
+            rows = cache_batch_idx.cpu()
+            if int(rows.min()) < 0 or int(rows.max()) >= k_cache.shape[0]:
+                raise RuntimeError("cache_batch_idx entries must be within cache batch bounds")
+        if block_table is not None and block_table.shape[1] > 0:
+            pages = block_table.cpu()
+            needed = torch.arange(pages.shape[1]) * k_cache.shape[1] < used[:, None]
+            if bool((needed & ((pages < 0) | (pages >= k_cache.shape[0]))).any()):
+                raise RuntimeError("block_table entries in use must be pages of the cache")
+    status = None if validate or not q.is_cuda else _kv_status(q.device)
+    q, k, v, cache_seqlens, cache_batch_idx, block_table = (
+        maybe_contiguous(t) for t in (q, k, v, cache_seqlens, cache_batch_idx, block_table)
+    )
+    out, lse = flash_attn_gpu.diff_fwd_kvcache(
+        q, k_cache, v_cache, lam, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, causal, num_splits,
+        status,
+    )
+    return (out, lse) if return_softmax_lse else out
+
+
+# ---------------------------------------------------------------------------
+# The pages of a paged KV cache (no counterpart in the reference).
+#
+# The state is four tensors of the caller's: the pools k_cache and v_cache [num_blocks, page_block_size, nheads_k,
+# headdim], block_table int32 [rows, max_num_blocks_per_seq] (-1: no page), cache_seqlens int32 [rows] and page_refs
+# int32 [num_blocks], the number of table entries that name each page (0: free).  A new cache has a table of -1 and
+# zeros elsewhere.  All calls work in place on the device, on the current stream, with no host read when validate is
+# False.  validate=True reads what the kernels found wrong (a synchronisation) and raises it; False leaves it for
+# flash_attn_kvcache_check().  Either way a call that gives out pages changes nothing when something is wrong.
+
+
+def _kv_pages_call(fn, device, validate, *args):
+    status = torch.zeros(1, dtype=torch.int32, device=device) if validate else _kv_status(device)
+    fn(*args, status)
+    if validate:
+        _raise_kv_status(int(status.item()))
+
+
+def _check_pages(block_table=None, cache_seqlens=None, page_refs=None, **lists) -> None:
+    for name, t in (("block_table", block_table), ("cache_seqlens", cache_seqlens), ("page_refs", page_refs),
+                    *lists.items()):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise TypeError(f"{name} must be a torch.int32 tensor")
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor")
+
+
+def flash_attn_kvcache_alloc(block_table, cache_seqlens, page_refs, seqlen_new: Union[int, torch.Tensor],
+                             page_block_size: int, validate: bool = True) -> None:
+    """Give every row the pages that its next seqlen_new tokens (an int, or int32 [rows], 0 for none) need and its
+    table lacks: the lowest free pages first, in the order of the rows."""
+    _check_pages(block_table, cache_seqlens, page_refs)
+    per_row = seqlen_new if isinstance(seqlen_new, torch.Tensor) else None
+    if per_row is not None:
+        _check_pages(seqlen_new=per_row)
+    elif seqlen_new < 0:
+        raise ValueError("seqlen_new must be non-negative")
+    if page_block_size <= 0:
+        raise ValueError("page_block_size must be positive")
+    _kv_pages_call(flash_attn_gpu.kvpages_alloc, block_table.device, validate, block_table, cache_seqlens, page_refs,
+                   0 if per_row is not None else seqlen_new, per_row, page_block_size)
+
+
+def flash_attn_kvcache_copy_pages(k_cache, v_cache, src: torch.Tensor, dst: torch.Tensor, validate: bool = True) -> None:
+    """Copy page src[i] of both pools to page dst[i], all pairs at once.  A page that one pair writes may be in no
+    other pair; such pairs, and those out of range, are not copied and reported."""
+    _check_pages(src=src, dst=dst)
+    _kv_pages_call(flash_attn_gpu.kvpages_copy, src.device, validate, k_cache, v_cache, src, dst)
+
+
+def flash_attn_kvcache_fork(k_cache, v_cache, block_table, cache_seqlens, page_refs, parents: torch.Tensor,
+                            children: torch.Tensor, validate: bool = True) -> None:
+    """Make row children[i] (empty, in the list once, no parent itself) a fork of row parents[i]: it shares the
+    parent's full pages, and where the parent's last page is partly filled it gets a free page (lowest first, in the
+    list's order) with a copy of that page's tokens; the rest of that page is left as it was."""
+    _check_pages(block_table, cache_seqlens, page_refs, parents=parents, children=children)
+    _kv_pages_call(flash_attn_gpu.kvpages_fork, block_table.device, validate, k_cache, v_cache, block_table,
+                   cache_seqlens, page_refs, parents, children)
+
+
+def flash_attn_kvcache_free(block_table, cache_seqlens, page_refs, rows: torch.Tensor, validate: bool = True) -> None:
+    """Empty the rows: each of their pages loses a reference (and is free at 0), their table entries become -1 and
+    their lengths 0.  Empty rows, and a row named twice, are nothing special; a row out of range is reported."""
+    _check_pages(block_table, cache_seqlens, page_refs, rows=rows)
+    _kv_pages_call(flash_attn_gpu.kvpages_free, block_table.device, validate, block_table, cache_seqlens, page_refs,
+                   rows)
+
+
+def flash_attn_kvcache_compact(k_cache, v_cache, block_table, page_refs) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Move the pages in use to the front of the pools: with n of them, the k-th free page below n takes the contents
+    of the k-th used page from n on.  Returns the table and the counts afterwards (new tensors) and n (int32 [1]).
+    The moved pages stay as they were in their old places, so the old table stays right for work that is already
+    queued, until those pages are given out again."""
+    _check_pages(block_table, page_refs=page_refs)
+    return flash_attn_gpu.kvpages_compact(k_cache, v_cache, block_table, page_refs)

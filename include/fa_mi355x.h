@@ -273,6 +273,148 @@ int fa_fwd_kvcache(const fa_kvcache_args *args, void *stream);
 #define FA_NOALLOC_SCRATCH_BYTES (16u << 20)
 int fa_fwd_kvcache_noalloc(const fa_kvcache_args *args, void *stream);
 
+/*
+ * Differential attention.  A head's q and k hold two maps in the two halves of
+ * their head_dim channels (map 1 the first half, map 2 the second), v has
+ * head_dim channels:
+ *   o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v.
+ * All tensors are laid out as those of fa_fwd / fa_bwd; dtype is FA_FP16 or
+ * FA_BF16 for all of them.  No counterpart in the reference.
+ */
+enum { FA_FP16 = 0, FA_BF16 = 1 };
+
+/* lam, fp32: element [batch b][row i][head h] at ptr + b * batch_stride + i *
+ * row_stride + h * head_stride (strides in elements, 0 where it is shared; for
+ * packed tensors the row counts from the first packed row and batch_stride is 0). */
+typedef struct fa_diff_lam {
+    const float *ptr;
+    int64_t batch_stride, row_stride, head_stride;
+} fa_diff_lam;
+
+typedef struct fa_diff_fwd_args {
+    fa_tensor q, k, v, o;
+    fa_tensor o2;                   /* map 2's own output softmax(S2) v, which the backward reads, or ptr NULL */
+    fa_diff_lam lam;
+    float *lse;                     /* fp32 [2][batch][nheads][lse_seqlen], map 1's first */
+    const int32_t *cu_seqlens_q;    /* [batch+1], both or neither                */
+    const int32_t *cu_seqlens_k;
+    int32_t batch, seqlen_q, seqlen_k, nheads, nheads_k, head_dim;
+    int32_t lse_seqlen;             /* seqlen_q, or max_seqlen_q for packed batches */
+    float softmax_scale;
+    int32_t causal;                 /* bottom-right aligned                      */
+    int32_t dtype;
+    int32_t o_rows;                 /* as fa_fwd_args.o_rows                     */
+    int32_t *work_order;            /* fa_diff_fwd_order_len(args) int32s for packed batches, or NULL */
+} fa_diff_fwd_args;
+
+size_t fa_diff_fwd_order_len(const fa_diff_fwd_args *args);
+int fa_diff_fwd(const fa_diff_fwd_args *args, void *stream);
+
+/* dlam as fa_diff_lam, written. */
+typedef struct fa_diff_dlam {
+    float *ptr;
+    int64_t batch_stride, row_stride, head_stride;
+} fa_diff_dlam;
+
+typedef struct fa_diff_bwd_args {
+    fa_tensor q, k, v, o, o2, dout; /* inputs; o and o2 as the forward wrote them */
+    fa_tensor dq, dk, dv;           /* outputs, every row of a sequence written   */
+    fa_diff_lam lam;
+    fa_diff_dlam dlam;              /* gradient of lam, or ptr NULL: row_stride not 0 gives every row
+                                       its own (each row of a sequence written); else the sum over all rows, of each
+                                       head (head_stride not 0) or of all of them (one value) */
+    const float *lse;               /* as the forward wrote it                    */
+    const int32_t *cu_seqlens_q, *cu_seqlens_k;
+    int32_t batch, seqlen_q, seqlen_k, nheads, nheads_k, head_dim, lse_seqlen;
+    float softmax_scale;
+    int32_t causal, dtype;
+    int32_t dq_rows, dkv_rows;      /* as in fa_bwd_args                          */
+    int32_t *work_order;            /* fa_diff_bwd_order_len(args) int32s for packed batches, or NULL */
+    float *dsum;                    /* workspace of dsum_bytes >= fa_diff_bwd_ws_bytes(args), 8-byte aligned */
+    int64_t dsum_bytes;
+} fa_diff_bwd_args;
+
+size_t fa_diff_bwd_ws_bytes(const fa_diff_bwd_args *args);
+size_t fa_diff_bwd_order_len(const fa_diff_bwd_args *args);
+int fa_diff_bwd(const fa_diff_bwd_args *args, void *stream);
+
+/*
+ * Differential attention over a key-value cache, laid out and checked on the
+ * device as in fa_kvcache_args: k_new / v_new are appended at cache_seqlens,
+ * then seqlen_q queries attend over L = cache_seqlens + seqlen_new keys.
+ */
+typedef struct fa_diff_kvcache_args {
+    fa_tensor q, k_cache, v_cache, k_new, v_new, o;
+    fa_diff_lam lam;                /* [batch][seqlen_q][nheads] by its strides   */
+    float *lse;                     /* fp32 [2][batch][nheads][seqlen_q]          */
+    const int32_t *cache_seqlens;   /* [batch] tokens before the append           */
+    const int32_t *cache_batch_idx; /* [batch] or NULL (contiguous caches)        */
+    const int32_t *block_table;     /* [batch][block_table_stride] or NULL        */
+    int64_t block_table_stride;
+    int32_t batch, seqlen_q, nheads, nheads_k, head_dim, seqlen_new;
+    int32_t page_block_size;        /* paged: a multiple of 64                    */
+    int32_t num_pages;              /* paged: pages of the cache; a table entry in use outside them reads page
+                                       0, is not appended to and ORs FA_KV_BAD_PAGE into *status */
+    int32_t num_splits;             /* pieces of cache_capacity, 0: chosen        */
+    float softmax_scale;
+    int32_t causal, dtype;
+    int32_t cache_capacity;         /* tokens one sequence's cache holds          */
+    int32_t cache_batch;            /* rows of a contiguous cache                 */
+    int32_t *status;                /* device word: 1 (capacity) or 2 (cache row) is ORed in, or NULL */
+    void *ws;                       /* fa_diff_kvcache_ws_bytes(args) bytes, 256-byte aligned */
+    int64_t ws_bytes;
+} fa_diff_kvcache_args;
+
+size_t fa_diff_kvcache_ws_bytes(const fa_diff_kvcache_args *args);
+int fa_diff_kvcache(const fa_diff_kvcache_args *args, void *stream);
+
+/*
+ * Pages of a paged key-value cache.  page_refs[p] is the number of block_table
+ * entries that name page p (0: free); a table entry of -1 names none.  All arrays
+ * are on the device, nothing is read on the host, and what is wrong is ORed into
+ * *status (a call that gives out pages then changes nothing).  No counterpart in
+ * the reference.
+ */
+enum {
+    FA_KV_BAD_PAGE = 4,  /* a block_table entry in use names no page of the cache */
+    FA_KV_NO_PAGES = 8,  /* fewer free pages than the call needs                   */
+    FA_KV_BAD_LIST = 16  /* a list's row or page is out of range, taken or named twice */
+};
+
+typedef struct fa_kvpages_args {
+    fa_tensor k_cache, v_cache;     /* [num_pages][page_block_size][nheads_k][head_bytes], strides in BYTES, multiples of 16 */
+    int32_t nheads_k, head_bytes;
+    int32_t page_block_size, num_pages;
+    int32_t *block_table;           /* [rows][max_pages]                          */
+    int64_t block_table_stride;
+    int32_t rows, max_pages;
+    int32_t *cache_seqlens;         /* [rows] tokens in the cache                 */
+    int32_t *page_refs;             /* [num_pages]                                */
+    const int32_t *from, *to;       /* [n]: pages (copy), parents and children (fork), rows (free: from) */
+    int32_t n;
+    int32_t seqlen_new;             /* alloc: tokens that every row makes room for ... */
+    const int32_t *seqlens_new;     /* ... or [rows], or NULL                     */
+    int32_t *out_table;             /* compact: [rows][max_pages], apart from block_table */
+    int64_t out_table_stride;
+    int32_t *out_refs, *out_used;   /* compact: [num_pages], apart from page_refs; [1] pages in use */
+    int32_t *status;                /* device int32 error word, or NULL           */
+    void *ws;                       /* fa_kvpages_ws_bytes(args) bytes (not for copy and free) */
+    int64_t ws_bytes;
+} fa_kvpages_args;
+
+size_t fa_kvpages_ws_bytes(const fa_kvpages_args *args);
+/* Rows get pages for tokens [cache_seqlens, cache_seqlens + new), lowest free pages first, in row order. */
+int fa_kvpages_alloc(const fa_kvpages_args *args, void *stream);
+/* Page to[i] = page from[i], all at once; pairs that touch each other's pages are not copied (FA_KV_BAD_LIST). */
+int fa_kvpages_copy(const fa_kvpages_args *args, void *stream);
+/* Row to[i] (empty) shares the full pages of row from[i] and gets a page with a copy of the tokens of a last, partly
+ * filled one. */
+int fa_kvpages_fork(const fa_kvpages_args *args, void *stream);
+/* Rows from[i] give their pages back and become empty. */
+int fa_kvpages_free(const fa_kvpages_args *args, void *stream);
+/* The used pages move to the front of the pool: out_table and out_refs are the table and the counts afterwards. */
+int fa_kvpages_compact(const fa_kvpages_args *args, void *stream);
+
 /* Human-readable text for a return code (FA_* or hipError_t). */
 const char *fa_error_string(int code);
 

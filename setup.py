@@ -35,8 +35,9 @@ class HipBuild(build_ext):
         out_dir = os.path.dirname(os.path.abspath(self.get_ext_fullpath(ext.name)))
         os.makedirs(out_dir, exist_ok=True)
         jobs = int(os.environ.get("MAX_JOBS", "4"))
-        fa_build.build_library(jobs, out_dir=out_dir, obj_dir=os.path.join(os.path.abspath(self.build_temp), "hip"))
-        fa_build.build_extension(out_dir=out_dir)
+        temp = os.path.abspath(self.build_temp)
+        fa_build.build_library(jobs, out_dir=out_dir, obj_dir=os.path.join(temp, "hip"))
+        fa_build.build_extension(out_dir=out_dir, obj_dir=os.path.join(temp, "ext"))
 
 
 setup(
@@ -49,8 +50,10 @@ setup(
     ext_modules=[
         Extension(
             "flash_attn_turing",
-            sources=[f"{PKG_DIR}/csrc/flash_api.cpp"]
-            + [f"{PKG_DIR}/csrc/{f}" for f in ("fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip")],
+            sources=[f"{PKG_DIR}/csrc/{f}" for f in ("flash_api.cpp", "diff_api.cpp", "kvpages_api.cpp")]
+            + [f"{PKG_DIR}/csrc/{f}" for f in ("fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip",
+                                               "fa_diff_fwd.hip", "fa_diff_bwd.hip", "fa_diff_kv.hip",
+                                               "fa_kvpages.hip")],
         )
     ],
     cmdclass={"build_ext": HipBuild},
