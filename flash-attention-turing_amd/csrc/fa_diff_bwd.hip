@@ -14,7 +14,12 @@
 // roundings do, but neither for dlam, which is D_2 itself, nor for rows of a few keys, whose dP -
 // D_m cancels.  So the kernel sums dS_2, which is D_2's error, in fp32
 // (sum_j P_2 (dP - D) = D_2 - D), and rows whose keys lie in the first block
-// take both D_m from that block's own P_m and dP.
+// take both D_m from that block's own P_m and dP.  The matrix cores' sums lean
+// towards minus infinity by a small part of a unit (here about 3e-8), the same
+// way in every row, and the D_2 of 10^5 rows and more, whose signs vary, sum to
+// so little that this showed in a dlam they share (1.5e-4 of it at 2 x 4096
+// rows, 8 heads).  So every second query computes with -dO: its lane's sums are the
+// negatives, at no cost until the end, and the leanings of neighbours cancel.
 //
 // dK/dV kernel: 4 waves x 32 keys of one KV head, S and dP with queries on M.
 // It loops over the heads of the GQA group and sums them in fp32 registers.
@@ -95,6 +100,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     const int qi = q_lo + (lane & 31);
     const bool qv = qi < sq;
     const int qr = qv ? qi : 0;
+    const float sgn = qi & 1 ? -1.f : 1.f;  // dO, D_m, dS_m and dQ below are sgn times their values
     f16x8 qB[HD / 16], doB[HD / 16];
     float d1 = 0.f, d2 = 0.f;
     {
@@ -107,7 +113,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
 #pragma unroll
         for (int g = 0; g < HD / 16; ++g) {
             qB[g] = as_h8(qv ? ldg16(qp + 16 * g) : zero_u4());
-            doB[g] = as_h8(qv ? ldg16(dop + 16 * g) : zero_u4());
+            const u32x4 dx = qv ? ldg16(dop + 16 * g) : zero_u4();
+            doB[g] = as_h8(qi & 1 ? neg_h8(dx) : dx);
             const f16x8 ov = as_h8(qv ? ldg16(op + 16 * g) : zero_u4());
             const f16x8 o2v = as_h8(qv ? ldg16(o2p + 16 * g) : zero_u4());
 #pragma unroll
@@ -246,8 +253,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     if (!qv) return;
     if (hh == 0) {
         float *w = a.dsum + lrow + qi;
-        w[0] = -d1;
-        w[plane] = -(d2 + ds2_sum);
+        w[0] = -sgn * d1;
+        w[plane] = -sgn * (d2 + ds2_sum);
         w[2 * plane] = lse1;
         w[3 * plane] = lse2;
         w[4 * plane] = lam;
@@ -257,7 +264,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     f16 *row = (f16 *)a.dq.ptr + base_off(a.dq, packed_q, b, si.q_start, h) + int64_t(qo) * a.dq.row_stride;
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt) {
-        const float f = dt < HD / 64 ? a.softmax_scale : -lam * a.softmax_scale;
+        const float f = sgn * (dt < HD / 64 ? a.softmax_scale : -lam * a.softmax_scale);
 #pragma unroll
         for (int a4 = 0; a4 < 4; ++a4)
             *reinterpret_cast<f16x4 *>(row + dt * 32 + 8 * a4 + 4 * hh) =
