@@ -53,22 +53,104 @@ __device__ __forceinline__ float elem(const f16x8 v, int i) {
         return float(v[i]);
 }
 
+// max(a, b, c) in one instruction and without the canonicalisation of each
+// operand that fmaxf adds.  A NaN among them is passed over, as by fmaxf.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max16(const f32x16 &s) {
+    float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]);
+    a = max3(a, s[6], s[7]);
+    b = max3(b, s[8], s[9]);
+    a = max3(a, s[10], s[11]);
+    b = max3(b, s[12], s[13]);
+    return max3(max3(a, s[14], s[15]), b, b);
+}
+// max_xor32 (fa_common.h) without the canonicalisations.
+__device__ __forceinline__ float max2_xor32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+    return max3(a, b, b);
+}
+// A wave-uniform float in a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
 // lam of (batch, row of the tensor, head); strides in elements, 0 where it is shared.
 __device__ __forceinline__ float diff_lam(const fa_diff_lam &l, int b, int64_t row, int h) {
     return l.ptr[int64_t(b) * l.batch_stride + row * l.row_stride + int64_t(h) * l.head_stride];
 }
 
+// A wave-uniform address as scalar registers.  (The builtin returns an int:
+// widened as it is, a low half from 2^31 on would set all of the high half.)
+template <class T>
+__device__ __forceinline__ const T *uniform(const T *p) {
+    const uint64_t u = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(u)), hi = __builtin_amdgcn_readfirstlane(uint32_t(u >> 32));
+    return reinterpret_cast<const T *>(uint64_t(hi) << 32 | lo);
+}
+
 // A wave-uniform int32 of memory that no kernel in flight writes, through the
 // scalar cache: a vector load would wait for the tile copies that are in flight.
 __device__ __forceinline__ int scalar_load(const int32_t *p) {
-    const uint64_t u = reinterpret_cast<uint64_t>(p);
-    // (The builtin returns an int: widened as it is, a low half from 2^31 on would set all of the high half.)
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(u)), hi = __builtin_amdgcn_readfirstlane(uint32_t(u >> 32));
-    const uint64_t s = uint64_t(hi) << 32 | lo;
     int v;
-    asm volatile("s_load_dword %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(s) : "memory");
+    asm volatile("s_load_dword %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(uniform(p)) : "memory");
     return v;
 }
+
+// g2l16 (fa_common.h) with the address as a wave-uniform base and a 32-bit byte
+// offset per lane: no 64-bit address is formed or held per lane and copy.  Same
+// waiting rules.
+__device__ __forceinline__ void g2l16_at(const f16 *base, uint32_t off, uint32_t l) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(off), "s"(base), "s"(l)
+        : "memory");
+}
+// Row strides (elements) with which a tile's lane offsets, below 128 rows, stay
+// under 2^32 bytes.
+constexpr int64_t kDiffMaxRowStride = int64_t(1) << 23;
+
+// Copies of a [ROWS][HD] tile by NT threads into the swizzled layout of
+// TileCopier (fa_common.h), from a wave-uniform first row.  rows: how many there
+// are; the rows past them re-read the last one.
+template <int HD, int ROWS, int NT>
+struct DiffCopier {
+    static constexpr int KCH = HD / 8, CPT = ROWS * KCH / NT, WAVES = NT / 64, RSTEP = NT / KCH;
+    static_assert(RSTEP % 16 == 0, "row step must keep the swizzle");
+    uint32_t rc;  // the lane's row, and 16 times its swizzled chunk in the high half
+    uint32_t lds0;
+    __device__ __forceinline__ void init(int wave, int lane) {
+        const int p = wave * 64 + lane, row = p / KCH;
+        rc = row | ((p % KCH) ^ swz<KCH>(row)) << 20;
+        lds0 = wave * 1024;
+    }
+    __device__ __forceinline__ void copy(uint32_t tile_l, const f16 *row0, int64_t rs, int rows) const {
+        const uint32_t l0 = __builtin_amdgcn_readfirstlane(tile_l + lds0), rsb = uint32_t(rs) * 2;
+        uint32_t x = rc;
+        asm volatile("" : "+v"(x));  // the offsets are formed here, not held between copies
+        row0 = uniform(row0);
+        const uint32_t row = x & 0xffff, c = x >> 16;
+        if (rows >= ROWS) {
+            const uint32_t off = row * rsb + c;
+#pragma unroll
+            for (int i = 0; i < CPT; ++i) g2l16_at(row0 + i * RSTEP * rs, off, l0 + i * WAVES * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CPT; ++i)
+                g2l16_at(row0, min(int(row) + i * RSTEP, rows - 1) * rsb + c, l0 + i * WAVES * 1024);
+        }
+    }
+};
 
 // Page at table entry pg of sequence b, checked: one outside the cache becomes
 // page 0 and is reported, so that no access leaves the cache.

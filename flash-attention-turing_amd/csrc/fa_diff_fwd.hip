@@ -20,7 +20,7 @@
 namespace fa {
 
 constexpr int kDiffBN = 64;       // keys per block
-constexpr int kDiffThreads = 256;  // 4 waves of 32 queries
+constexpr int kDiffRows = 128, kDiffThreads = 256;  // 4 waves of 32 rows
 
 // A call as the kernel takes it: the tensors, and the cache that k and v are
 // (cache_seqlens set).
@@ -32,28 +32,30 @@ struct DiffFwd {
     int32_t *status;
 };
 
-// One map's 64-key block of S^T -> P^T operands: mask (keys past lim, relative
-// to the block), running maximum, rescale of O, exponentials, row sum.  P is
+// One map's 32 keys of S^T -> P^T operands: mask (keys past lim, relative to the
+// first), running maximum, rescale of O, exponentials, row sum.  P is
 // rounded to 16 bits for the product with V, as in ordinary attention; O and
 // the LSE are normalised by the fp32 sum of the unrounded P.
+// The maximum m that P is taken against is raised, and O and the sum rescaled,
+// only when some row of the wave finds a score more than kDiffSlack doublings
+// above it: with scores of unit variance an exact maximum rises in every second
+// block of a row of 4096 keys, and the 128 multiplications were a third of the
+// VALU work that bounds the kernel.  P stays below 2^kDiffSlack; its rounding is
+// relative and as large as elsewhere (only a row's largest P, 1 against an exact
+// maximum, is no longer free of it).
+constexpr float kDiffSlack = 4.f;
+
 template <int HD, bool BF, bool MASK>
-__device__ __forceinline__ void diff_softmax(f32x16 (&s)[2], f16x8 (&pB)[4], f32x16 (&o)[HD / 32], float &m, float &l,
+__device__ __forceinline__ void diff_softmax(f32x16 &s, f16x8 (&pB)[2], f32x16 (&o)[HD / 32], float &m, float &l,
                                              float cscale, int lim, int hh) {
     if constexpr (MASK) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (kt * 32 + acc_lrow(e, hh) > lim) s[kt][e] = -INFINITY;
+        for (int e = 0; e < 16; ++e)
+            if (acc_lrow(e, hh) > lim) s[e] = -INFINITY;
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kt][e]);
-    mx = max_xor32(mx);
+    const float mx = max2_xor32(max16(s));
     const float mx_t = MASK && mx == -INFINITY ? -INFINITY : mx * cscale;
-    if (__builtin_amdgcn_ballot_w64(mx_t > m) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mx_t > m + kDiffSlack) != 0) {
         const float m_new = fmaxf(m, mx_t);
         const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
         l *= alpha;
@@ -66,127 +68,200 @@ __device__ __forceinline__ void diff_softmax(f32x16 (&s)[2], f16x8 (&pB)[4], f32
     const float m_use = m == -INFINITY ? 0.f : m;
     float rs = 0.f;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float x = s[kt][e];
-            float p = exp2_fast(fmaf(x, cscale, -m_use));
-            if constexpr (MASK) p = x == -INFINITY ? 0.f : p;
-            s[kt][e] = p;
-            rs += p;
-        }
+    for (int e = 0; e < 16; ++e) {
+        const float x = s[e];
+        float p = exp2_fast(fmaf(x, cscale, -m_use));
+        if constexpr (MASK) p = x == -INFINITY ? 0.f : p;
+        s[e] = p;
+        rs += p;
+    }
     l += rs;
-#pragma unroll
-    for (int gg = 0; gg < 4; ++gg) pB[gg] = pack16<BF>(s[gg >> 1], 8 * (gg & 1));
+    pB[0] = pack16<BF>(s, 0);
+    pB[1] = pack16<BF>(s, 8);
 }
 
-template <int HD, bool BF, bool CAUSAL, bool CACHE>
-__global__ __launch_bounds__(kDiffThreads, 2) void diff_fwd_kernel(const DiffFwd p, const int num_m_blocks,
-                                                                   const int lg) {
-    constexpr int NT = kDiffThreads, BM = 128, BN = kDiffBN;
-    constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
-    constexpr int HG = HD / 32;  // MFMA K steps of one map's channels
-    const fa_diff_fwd_args &a = p.a;
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+// A workgroup's work: gp = 2^lg heads of one GQA group at P = 128 / gp positions
+// from m0, which share the K / V tiles; a wave takes 32 rows of one head.
+struct DiffWork {
+    int b, h, hk, q_start, sq, sk, m0, P, causal_off, n_keys;  // n_keys: keys that some row sees
+    const f16 *kp, *vp;
+    bool live;
+};
 
-    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // The workgroup's rows: gp = 2^lg heads of one GQA group at P = 128 / gp
-    // positions from m0, which share the K / V tiles.
-    const int gp = 1 << lg, packs = a.nheads >> lg, P = BM >> lg;
-    int b, h, mb;
+template <bool CAUSAL, bool CACHE>
+__device__ __forceinline__ DiffWork diff_work(const DiffFwd &p, int num_m_blocks, int lg, int bid) {
+    const fa_diff_fwd_args &a = p.a;
+    DiffWork w;
+    const int gp = 1 << lg, packs = a.nheads >> lg;
+    int mb;
+    w.P = kDiffRows >> lg;
     if (a.work_order && a.cu_seqlens_q) {
-        const int it = a.work_order[blockIdx.x / packs];
-        b = __builtin_amdgcn_readfirstlane(it / num_m_blocks);
-        mb = __builtin_amdgcn_readfirstlane(it - b * num_m_blocks);
-        h = (blockIdx.x % packs) * gp;
+        const int it = a.work_order[bid / packs];
+        w.b = __builtin_amdgcn_readfirstlane(it / num_m_blocks);
+        mb = __builtin_amdgcn_readfirstlane(it - w.b * num_m_blocks);
+        w.h = (bid % packs) * gp;
     } else {
-        const int bp_count = a.batch * packs, bp = blockIdx.x % bp_count;
-        mb = blockIdx.x / bp_count;
+        const int bp_count = a.batch * packs, bp = bid % bp_count;
+        mb = bid / bp_count;
         if (CAUSAL) mb = num_m_blocks - 1 - mb;  // heaviest first
-        b = bp / packs;
-        h = (bp - b * packs) * gp;
+        w.b = bp / packs;
+        w.h = (bp - w.b * packs) * gp;
     }
-    const int hk = h / (a.nheads / a.nheads_k);
-    const bool packed_q = a.cu_seqlens_q != nullptr, packed_k = a.cu_seqlens_k != nullptr;
-    SeqInfo si = seq_info(b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
-    int kb = b;
+    w.hk = w.h / (a.nheads / a.nheads_k);
+    const bool packed_k = a.cu_seqlens_k != nullptr;
+    SeqInfo si = seq_info(w.b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
+    int kb = w.b;
     if constexpr (CACHE) {
         // A length or a cache row outside the cache leaves the sequence with no
         // keys, and the status word says so: no access leaves the cache.
-        const int used = p.cache_seqlens[b];
-        if (p.cache_batch_idx) kb = p.cache_batch_idx[b];
+        const int used = p.cache_seqlens[w.b];
+        if (p.cache_batch_idx) kb = p.cache_batch_idx[w.b];
         const int err = (used < 0 || int64_t(used) + p.seqlen_new > p.capacity ? 1 : 0) |
                         (p.cache_batch_idx && (kb < 0 || kb >= p.cache_batch) ? 2 : 0);
         si.sk = err ? 0 : used + p.seqlen_new;
         if (err) {
             kb = 0;
-            if (p.status && tid == 0) atomicOr(p.status, err);
+            if (p.status && threadIdx.x == 0) atomicOr(p.status, err);
         }
+        if (p.block_table) kb = 0;
     }
-    const int sq = si.sq, sk = si.sk, m0 = mb * P;
+    w.q_start = si.q_start;
+    w.sq = si.sq;
+    w.sk = si.sk;
+    w.m0 = mb * w.P;
+    w.causal_off = w.sk - w.sq;  // key j is visible to query i iff j <= i + causal_off
+    w.n_keys = CAUSAL ? max(0, min(w.sk, w.m0 + w.P + w.causal_off)) : w.sk;
+    w.kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, kb, si.k_start, w.hk);
+    w.vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, kb, si.k_start, w.hk);
+    w.live = w.m0 < w.sq;
+    return w;
+}
+
+// LSE rows of a block past its sequence: 0.
+__device__ __forceinline__ void diff_pad_lse(const fa_diff_fwd_args &a, const DiffWork &w, int lg) {
     const int64_t plane = int64_t(a.batch) * a.nheads * a.lse_seqlen;
-    float *lse_row = a.lse + (int64_t(b) * a.nheads + h) * a.lse_seqlen;
-    if (m0 >= sq) {  // past this sequence: LSE padding is 0
-        for (int i = tid; i < gp * P; i += NT) {
-            const int row = m0 + i % P;
-            if (row < a.lse_seqlen) {
-                lse_row[int64_t(i / P) * a.lse_seqlen + row] = 0.f;
-                lse_row[plane + int64_t(i / P) * a.lse_seqlen + row] = 0.f;
-            }
-        }
+    float *lse = a.lse + (int64_t(w.b) * a.nheads + w.h) * a.lse_seqlen;
+    for (int i = threadIdx.x; i < w.P << lg; i += blockDim.x) {
+        const int row = w.m0 + i % w.P;
+        if (row < a.lse_seqlen) lse[int64_t(i / w.P) * a.lse_seqlen + row] = lse[plane + int64_t(i / w.P) * a.lse_seqlen + row] = 0.f;
+    }
+}
+
+// Q^T of query qi of head h as B operands: lane (query, hh), K step g covers channels 16g + 8hh + 0..7.
+template <int HD>
+__device__ __forceinline__ void diff_load_q(const fa_diff_fwd_args &a, const DiffWork &w, int h, int qi, int hh,
+                                            f16x8 (&qB)[HD / 16]) {
+    const f16 *qp = (const f16 *)a.q.ptr + base_off(a.q, a.cu_seqlens_q != nullptr, w.b, w.q_start, h) +
+                    int64_t(qi < w.sq ? qi : 0) * a.q.row_stride + 8 * hh;
+#pragma unroll
+    for (int g = 0; g < HD / 16; ++g) {
+        u32x4 v = qi < w.sq ? ldg16(qp + 16 * g) : zero_u4();
+        if (a.softmax_scale < 0.f) v = neg_h8(v);
+        qB[g] = as_h8(v);
+    }
+}
+
+// Channel tiles [D0, D1) of a row of o (and o2), from both maps' O, maxima and
+// sums; the LSEs go with the first one.
+template <int HD, bool BF, int D0, int D1>
+__device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const DiffWork &w, int h, int qi, int hh,
+                                           const f32x16 (&o)[2][HD / 32], const float (&mx)[2], const float (&sum)[2]) {
+    const int64_t plane = int64_t(a.batch) * a.nheads * a.lse_seqlen;
+    float *lse_row = a.lse + (int64_t(w.b) * a.nheads + h) * a.lse_seqlen;
+    if (qi >= w.sq) {
+        if (D0 == 0 && hh == 0 && qi < a.lse_seqlen) lse_row[qi] = lse_row[plane + qi] = 0.f;
         return;
     }
-    const int causal_off = sk - sq;  // key j is visible to query i iff j <= i + causal_off
-    int n_end = sk;
-    if (CAUSAL) n_end = max(0, min(sk, m0 + P + causal_off));
-    const int n_blocks = (n_end + BN - 1) / BN;
-    const float cscale = fabsf(a.softmax_scale) * kLog2e;
-
-    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, CACHE && p.block_table ? 0 : kb, si.k_start, hk);
-    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, CACHE && p.block_table ? 0 : kb, si.k_start, hk);
-    const int64_t krs = a.k.row_stride, vrs = a.v.row_stride;
-    TileCopier<HD, BN, NT> kcp, vcp;
-    kcp.init(krs, wave, lane);
-    vcp.init(vrs, wave, lane);
-    // Copies of key block nb into stage st; a block past the sequence's end
-    // re-reads its last key (masked).  A page is a multiple of 64 tokens, so a
-    // block lies in one.
-    auto issue = [&](int nb, int st) FA_INLINE {
-        const int n0 = nb * BN;
-        int64_t koff = int64_t(n0) * krs, voff = int64_t(n0) * vrs;
-        if constexpr (CACHE) {
-            if (p.block_table) {
-                const int pg = n0 / p.page, in_page = n0 - pg * p.page;
-                const int blk = checked_page(p.block_table, p.block_table_stride, b, pg, p.num_pages, p.status);
-                koff = int64_t(blk) * a.k.batch_stride + int64_t(in_page) * krs;
-                voff = int64_t(blk) * a.v.batch_stride + int64_t(in_page) * vrs;
-            }
-        }
-        if (n0 + BN <= sk) {
-            kcp.copy_to(lds_addr(smem) + st * STAGE, kp + koff, krs);
-            vcp.copy_to(lds_addr(smem) + st * STAGE + TILE, vp + voff, vrs);
-        } else {
-            dma_tile<HD, BN, NT>(smem + st * STAGE, kp + koff, krs, 0, sk - 1 - n0, wave, lane);
-            dma_tile<HD, BN, NT>(smem + st * STAGE + TILE, vp + voff, vrs, 0, sk - 1 - n0, wave, lane);
-        }
-    };
-
-    // The wave's 32 rows: head h + wave / (P / 32), positions from q_lo.
-    h += wave >> (2 - lg);
-    const int q_lo = m0 + 32 * (wave & ((P >> 5) - 1));
-    const int qi = q_lo + (lane & 31);
-    f16x8 qB[HD / 16];  // B operands: lane (query, hh), K step g covers channels 16g + 8hh + 0..7
-    {
-        const f16 *qp = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, h) +
-                        int64_t(qi < sq ? qi : 0) * a.q.row_stride + 8 * hh;
+    const float l0 = sum[0], l1 = sum[1];
+    const bool packed_q = a.cu_seqlens_q != nullptr;
+    const float lam = diff_lam(a.lam, w.b, w.q_start + qi, h);
+    const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    f16 *orow = (f16 *)a.o.ptr + base_off(a.o, packed_q, w.b, w.q_start, h) + int64_t(qi) * a.o.row_stride + 4 * hh;
+    f16 *o2row = a.o2.ptr ? (f16 *)a.o2.ptr + base_off(a.o2, packed_q, w.b, w.q_start, h) +
+                                int64_t(qi) * a.o2.row_stride + 4 * hh
+                          : nullptr;
 #pragma unroll
-        for (int g = 0; g < HD / 16; ++g) {
-            u32x4 v = qi < sq ? ldg16(qp + 16 * g) : zero_u4();
-            if (a.softmax_scale < 0.f) v = neg_h8(v);
-            qB[g] = as_h8(v);
+    for (int dt = D0; dt < D1; ++dt)
+#pragma unroll
+        for (int a4 = 0; a4 < 4; ++a4) {
+            float x[4], y[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                y[t] = o[1][dt][4 * a4 + t] * i1;
+                x[t] = l0 > 0.f ? fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]) : 0.f;
+            }
+            *reinterpret_cast<f16x4 *>(orow + dt * 32 + 8 * a4) = pack4<BF>(x[0], x[1], x[2], x[3]);
+            if (o2row) *reinterpret_cast<f16x4 *>(o2row + dt * 32 + 8 * a4) = pack4<BF>(y[0], y[1], y[2], y[3]);
+        }
+    if (D0 == 0 && hh == 0) {
+        lse_row[qi] = l0 > 0.f ? (mx[0] + log2_fast(l0)) * kLn2 : 0.f;
+        lse_row[plane + qi] = l1 > 0.f ? (mx[1] + log2_fast(l1)) * kLn2 : 0.f;
+    }
+}
+
+// First rows of K and V tiles of a dense tensor or of the pages of a cache.  A
+// tile lies in one page; its page's id is read once a page.
+template <bool CACHE>
+struct DiffTiles {
+    int page = -1, blk = 0;
+    __device__ __forceinline__ void at(const DiffFwd &p, const DiffWork &w, int n0, const f16 *&k, const f16 *&v) {
+        const fa_diff_fwd_args &a = p.a;
+        if (CACHE && p.block_table) {
+            const int pg = n0 / p.page;
+            if (pg != page) {
+                page = pg;
+                blk = checked_page(p.block_table, p.block_table_stride, w.b, pg, p.num_pages, p.status);
+            }
+            const int64_t row = n0 - pg * p.page;
+            k = w.kp + int64_t(blk) * a.k.batch_stride + row * a.k.row_stride;
+            v = w.vp + int64_t(blk) * a.v.batch_stride + row * a.v.row_stride;
+        } else {
+            k = w.kp + int64_t(n0) * a.k.row_stride;
+            v = w.vp + int64_t(n0) * a.v.row_stride;
         }
     }
+};
+
+// NG = 1: four waves of 32 rows, two workgroups per CU, on grids that fill the
+// chip.  NG = 2: two groups of four waves over the same rows take the key blocks
+// in turn, each through LDS stages of its own, and merge through LDS; a workgroup
+// then has a CU to itself, with two waves on each SIMD and half the chain of
+// blocks.
+template <int HD, bool BF, bool CAUSAL, bool CACHE, int NG>
+__global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : 2) void diff_fwd_kernel(const DiffFwd p,
+                                                                                     const int num_m_blocks, const int lg) {
+    constexpr int NT = kDiffThreads, BN = kDiffBN;
+    constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
+    constexpr int HG = HD / 32;  // MFMA K steps of one map's channels
+    const fa_diff_fwd_args &a = p.a;
+    __shared__ __attribute__((aligned(16))) char smem[NG * 2 * STAGE];
+
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = NG == 1 ? wave8 : wave8 & 3, grp = NG == 1 ? 0 : wave8 >> 2;
+    const DiffWork w = diff_work<CAUSAL, CACHE>(p, num_m_blocks, lg, blockIdx.x);
+    if (!w.live) return diff_pad_lse(a, w, lg);
+    const int n_blocks = (w.n_keys + BN - 1) / BN;
+    const float cscale = uniform(fabsf(a.softmax_scale) * kLog2e);
+
+    DiffCopier<HD, BN, NT> cp;
+    cp.init(wave, lane);
+    DiffTiles<CACHE> tiles;
+    const int g0 = grp * 2 * STAGE;  // the group's stages
+    auto issue = [&](int nb, int st) FA_INLINE {
+        const f16 *k, *v;
+        tiles.at(p, w, nb * BN, k, v);
+        const uint32_t tile = lds_addr(smem) + g0 + st * STAGE;
+        cp.copy(tile, k, a.k.row_stride, w.sk - nb * BN);
+        cp.copy(tile + TILE, v, a.v.row_stride, w.sk - nb * BN);
+    };
+
+    // The wave's 32 rows: head h, positions from q_lo.
+    const int h = w.h + (wave >> (2 - lg));
+    const int q_lo = w.m0 + 32 * (wave & ((w.P >> 5) - 1));
+    const int qi = q_lo + (lane & 31);
+    f16x8 qB[HD / 16];
+    diff_load_q<HD>(a, w, h, qi, hh, qB);
     wait_vmem();  // only the tile copies are in flight inside the loop
 
     f32x16 o[2][HD / 32];
@@ -198,92 +273,125 @@ __global__ __launch_bounds__(kDiffThreads, 2) void diff_fwd_kernel(const DiffFwd
     TileReader<HD> rd;
     rd.init(lane);
 
-    auto block = [&](int nb, auto mask_tag) FA_INLINE {
+    // Iteration it: block NG * it + grp.
+    auto block = [&](int it, auto mask_tag) FA_INLINE {
         constexpr bool MASK = decltype(mask_tag)::value;
-        const int buf = nb & 1, n0 = nb * BN;
+        const int buf = it & 1, nb = NG * it + grp, n0 = nb * BN;
         wait_vmem();
         __syncthreads();  // block nb is in LDS; every wave is done with stage buf ^ 1
-        if (nb + 1 < n_blocks) issue(nb + 1, buf ^ 1);
-        if (CAUSAL && MASK && n0 > q_lo + 31 + causal_off) return;  // no visible key for this wave
-        if (q_lo >= sq) return;
+        if (nb + NG < n_blocks) issue(nb + NG, buf ^ 1);
+        if (NG > 1 && MASK && nb >= n_blocks) return;
+        if (CAUSAL && MASK && n0 > q_lo + 31 + w.causal_off) return;  // no visible key for this wave
+        if (q_lo >= w.sq) return;
+        // 32 keys at a time: the scores of both maps take as many registers as
+        // those of 64 keys of one, with the two O that is what fits.
         // Operand reads run PIPE - 1 steps ahead behind scheduling fences, from
         // the lane's bases with the stage added once per block (opaque, so that
         // no read address is held in registers through the loop).
-        constexpr int PIPE = 3, NPV = 4 * (HD / 32);
-        const int soff = buf * STAGE;
+        constexpr int PIPE = 3, NS = 2 * HG, NPV = 2 * (HD / 32);
+        const int soff = g0 + buf * STAGE;
         static_assert(STAGE % 512 == 0, "stage offsets must be multiples of 512 bytes");
         int ab = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff;
         asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
         f16x8 op[PIPE];
-        f16x8 pB[2][4];
-        const int lim = (CAUSAL ? min(sk - 1, qi + causal_off) : sk - 1) - n0;
+        const int lim = (CAUSAL ? min(w.sk - 1, qi + w.causal_off) : w.sk - 1) - n0;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            // Step u: key tile u % 2 (two independent chains), K step u / 2 of the map.
+        for (int sub = 0; sub < BN / 32; ++sub) {
+            // Step u: map u % 2, K step u / 2 of the map's channels.
             f32x16 s[2];
             auto rd_k = [&](int u) FA_INLINE {
-                op[u % PIPE] = rd.a_operand_at(smem + 32 * (u & 1) * (HD * 2), ab, m * HG + (u >> 1));
+                op[u % PIPE] = rd.a_operand_at(smem + 32 * sub * (HD * 2), ab, (u & 1) * HG + (u >> 1));
             };
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < PIPE - 1; ++u) rd_k(u);
 #pragma unroll
-            for (int u = 0; u < 2 * HG; ++u) {
-                if (u + PIPE - 1 < 2 * HG) rd_k(u + PIPE - 1);
-                s[u & 1] = mfma16<BF>(op[u % PIPE], qB[m * HG + (u >> 1)], u < 2 ? zero16() : s[u & 1]);
+            for (int u = 0; u < NS; ++u) {
+                if (u + PIPE - 1 < NS) rd_k(u + PIPE - 1);
+                s[u & 1] = mfma16<BF>(op[u % PIPE], qB[(u & 1) * HG + (u >> 1)], u < 2 ? zero16() : s[u & 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            diff_softmax<HD, BF, MASK>(s, pB[m], o[m], mx[m], sum[m], cscale, lim, hh);
-        }
-        auto rd_v = [&](int u) FA_INLINE {
-            op[u % PIPE] = rd.tr_operand_at(smem + TILE + 16 * (u & 3) * (HD * 2), tb0, tb1, u >> 2);
-        };
-        __builtin_amdgcn_sched_barrier(0);
+            // Step u: key step u % 2, channel tile u / 2; one V operand for both maps.
+            // The first reads go out before the softmax, which covers their latency.
+            auto rd_v = [&](int u) FA_INLINE {
+                op[u % PIPE] = rd.tr_operand_at(smem + TILE + 16 * (2 * sub + (u & 1)) * (HD * 2), tb0, tb1, u >> 1);
+            };
 #pragma unroll
-        for (int u = 0; u < PIPE - 1; ++u) rd_v(u);
+            for (int u = 0; u < PIPE - 1; ++u) rd_v(u);
+            f16x8 pB[2][2];
 #pragma unroll
-        for (int u = 0; u < NPV; ++u) {
-            if (u + PIPE - 1 < NPV) rd_v(u + PIPE - 1);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) o[m][u >> 2] = mfma16<BF>(op[u % PIPE], pB[m][u & 3], o[m][u >> 2]);
+            for (int m = 0; m < 2; ++m)
+                diff_softmax<HD, BF, MASK>(s[m], pB[m], o[m], mx[m], sum[m], cscale, lim - 32 * sub, hh);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < NPV; ++u) {
+                if (u + PIPE - 1 < NPV) rd_v(u + PIPE - 1);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) o[m][u >> 1] = mfma16<BF>(op[u % PIPE], pB[m][u & 1], o[m][u >> 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
 
-    // Blocks [0, n_full) need no mask for any wave of the workgroup.
-    int n_full = min(n_blocks, sk / BN);
-    if (CAUSAL) n_full = min(n_full, max(0, (m0 + causal_off + 1) / BN));
-    if (n_blocks > 0) issue(0, 0);
-    for (int nb = 0; nb < n_full; ++nb) block(nb, std::false_type{});
-    for (int nb = n_full; nb < n_blocks; ++nb) block(nb, std::true_type{});
+    // Iterations whose blocks need no mask for any wave of the workgroup come first.
+    int n_full = min(n_blocks, w.sk / BN);
+    if (CAUSAL) n_full = min(n_full, max(0, (w.m0 + w.causal_off + 1) / BN));
+    if (grp < n_blocks) issue(grp, 0);
+    const int it_full = n_full / NG, n_it = (n_blocks + NG - 1) / NG;
+    for (int it = 0; it < it_full; ++it) block(it, std::false_type{});
+    for (int it = it_full; it < n_it; ++it) block(it, std::true_type{});
 
-    lse_row = a.lse + (int64_t(b) * a.nheads + h) * a.lse_seqlen;
-    if (qi >= sq) {
-        if (hh == 0 && qi < a.lse_seqlen) lse_row[qi] = lse_row[plane + qi] = 0.f;
-        return;
-    }
-    const float l0 = sum_xor32(sum[0]), l1 = sum_xor32(sum[1]);
-    const float lam = diff_lam(a.lam, b, si.q_start + qi, h);
-    const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
-    f16 *orow = (f16 *)a.o.ptr + base_off(a.o, packed_q, b, si.q_start, h) + int64_t(qi) * a.o.row_stride;
-    f16 *o2row = a.o2.ptr ? (f16 *)a.o2.ptr + base_off(a.o2, packed_q, b, si.q_start, h) + int64_t(qi) * a.o2.row_stride
-                          : nullptr;
-#pragma unroll
-    for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-        for (int a4 = 0; a4 < 4; ++a4) {
-            float x[4], y[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                y[t] = o[1][dt][4 * a4 + t] * i1;
-                x[t] = l0 > 0.f ? fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]) : 0.f;
-            }
-            *reinterpret_cast<f16x4 *>(orow + dt * 32 + 8 * a4 + 4 * hh) = pack4<BF>(x[0], x[1], x[2], x[3]);
-            if (o2row) *reinterpret_cast<f16x4 *>(o2row + dt * 32 + 8 * a4 + 4 * hh) = pack4<BF>(y[0], y[1], y[2], y[3]);
+    sum[0] = sum_xor32(sum[0]);
+    sum[1] = sum_xor32(sum[1]);
+    if constexpr (NG == 1) {
+        diff_store<HD, BF, 0, HD / 32>(a, w, h, qi, hh, o, mx, sum);
+    } else {
+        // Each group finishes half of the channels of both maps: it hands the other
+        // half, and its maxima and sums, to the other group.
+        constexpr int H = HD / 64;  // 32-channel tiles of a half
+        __shared__ f32x2 ml[2][2][kDiffRows];
+        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);  // [group][2 maps * 4 H][NT threads]
+        const int t4 = tid & (NT - 1), r = 32 * wave + (lane & 31);
+        static_assert(2 * 2 * 4 * H * NT * 16 <= NG * 2 * STAGE, "the exchange fits the stages");
+        __syncthreads();  // every wave is done with the tiles
+        if (hh == 0) {
+            ml[grp][0][r] = f32x2{mx[0], sum[0]};
+            ml[grp][1][r] = f32x2{mx[1], sum[1]};
         }
-    if (hh == 0) {
-        lse_row[qi] = l0 > 0.f ? (mx[0] + log2_fast(l0)) * kLn2 : 0.f;
-        lse_row[plane + qi] = l1 > 0.f ? (mx[1] + log2_fast(l1)) * kLn2 : 0.f;
+        auto finish = [&](auto grp_tag) FA_INLINE {
+            constexpr int GRP = decltype(grp_tag)::value;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4 * H; ++i) {
+                    const f32x16 &t = o[m][(1 - GRP) * H + i / 4];
+                    const int e = 4 * (i & 3);
+                    xo[((GRP * 2 + m) * 4 * H + i) * NT + t4] = f32x4{t[e], t[e + 1], t[e + 2], t[e + 3]};
+                }
+            __syncthreads();
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const f32x2 other = ml[1 - GRP][m][r];
+                const float top = fmaxf(mx[m], other[0]);
+                const float f_own = mx[m] == -INFINITY ? 0.f : exp2_fast(mx[m] - top);
+                const float f_other = other[0] == -INFINITY ? 0.f : exp2_fast(other[0] - top);
+#pragma unroll
+                for (int i = 0; i < 4 * H; ++i) {
+                    const f32x4 x = xo[(((1 - GRP) * 2 + m) * 4 * H + i) * NT + t4];
+                    f32x16 &t = o[m][GRP * H + i / 4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[4 * (i & 3) + e] = fmaf(x[e], f_other, t[4 * (i & 3) + e] * f_own);
+                }
+                // In group order, so that both groups have the same bits.
+                sum[m] = GRP == 0 ? fmaf(other[1], f_other, sum[m] * f_own) : fmaf(sum[m], f_own, other[1] * f_other);
+                mx[m] = top;
+            }
+            diff_store<HD, BF, GRP * H, GRP * H + H>(a, w, h, qi, hh, o, mx, sum);
+        };
+        if (grp == 0)
+            finish(std::integral_constant<int, 0>{});
+        else
+            finish(std::integral_constant<int, 1>{});
     }
 }
 
@@ -310,11 +418,11 @@ __global__ __launch_bounds__(kOrderThreads) void diff_fwd_order_kernel(const fa_
     }, a.work_order, true);
 }
 
-// log2 of the heads of a GQA group that a workgroup's rows hold: the largest
+// log2 of the heads of a GQA group that a workgroup's BM rows hold: the largest
 // power of two that divides the group and leaves whole 32-row tiles per head.
-static int diff_pack_log2(int group) {
+static int diff_pack_log2(int group, int BM) {
     int lg = 0;
-    while (lg < 2 && group % (2 << lg) == 0) ++lg;
+    while ((64 << lg) <= BM && group % (2 << lg) == 0) ++lg;
     return lg;
 }
 
@@ -329,13 +437,15 @@ int check_diff_fwd(const fa_diff_fwd_args *p) {
     if (!a.lse || !a.lam.ptr) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.o})
         if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.k, &a.v})
+        if (t->row_stride < 0 || t->row_stride > kDiffMaxRowStride) return FA_ERR_INVALID_ARG;
     return check_tensor(a.o2, false);
 }
 
 template <int HD, bool BF, bool CACHE>
 static int launch_diff_fwd(const DiffFwd &p, hipStream_t s) {
     const fa_diff_fwd_args &a = p.a;
-    const int lg = diff_pack_log2(a.nheads / a.nheads_k), P = 128 >> lg;
+    const int lg = diff_pack_log2(a.nheads / a.nheads_k, kDiffRows), P = kDiffRows >> lg;
     const int nmb = (a.lse_seqlen + P - 1) / P;
     const int64_t grid = int64_t(nmb) * a.batch * (a.nheads >> lg);
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
@@ -347,12 +457,20 @@ static int launch_diff_fwd(const DiffFwd &p, hipStream_t s) {
         if (rc) return rc;
     }
     if (grid == 0) return FA_OK;
+    const int groups = grid <= device_cus() && a.seqlen_k > kDiffBN ? 2 : 1;
+    auto launch = [&](auto causal) {
+        constexpr bool C = decltype(causal)::value;
+        if (groups == 2)
+            hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, C, CACHE, 2>), dim3(unsigned(grid)), dim3(2 * kDiffThreads), 0, s,
+                               p, nmb, lg);
+        else
+            hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, C, CACHE, 1>), dim3(unsigned(grid)), dim3(kDiffThreads), 0, s, p,
+                               nmb, lg);
+    };
     if (a.causal)
-        hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, true, CACHE>), dim3(unsigned(grid)), dim3(kDiffThreads), 0, s, p,
-                           nmb, lg);
+        launch(std::true_type{});
     else
-        hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, false, CACHE>), dim3(unsigned(grid)), dim3(kDiffThreads), 0, s, p,
-                           nmb, lg);
+        launch(std::false_type{});
     return int(hipGetLastError());
 }
 
