@@ -46,6 +46,16 @@ inline void check_rc(int rc, const char *what) {
     TORCH_CHECK(rc == FA_OK, what, " failed: ", fa_error_string(rc));
 }
 
+// A workspace that a call is faster with but can do without: undefined where the
+// device has no memory left for it.
+inline at::Tensor optional_workspace(int64_t numel, const at::TensorOptions &options) {
+    try {
+        return at::empty({numel}, options);
+    } catch (const c10::OutOfMemoryError &) {
+        return at::Tensor();
+    }
+}
+
 // Bindings of the extension's other sources.
 void bind_diff(py::module_ &m);     // diff_api.cpp
 void bind_kvpages(py::module_ &m);  // kvpages_api.cpp

@@ -203,8 +203,16 @@ std::vector<std::optional<at::Tensor>> run_bwd(at::Tensor q, at::Tensor k, at::T
         order = at::empty({int64_t(std::max<size_t>(fa_diff_bwd_order_len(&a), 1))}, x->cu_q->options());
         a.work_order = order.data_ptr<int32_t>();
     }
+    // One allocation: the row planes and, where there is memory for it, the workspace of shared dK/dV items.
     a.dsum_bytes = int64_t(fa_diff_bwd_ws_bytes(&a));
-    at::Tensor ws = at::empty({a.dsum_bytes}, q.options().dtype(at::kByte));
+    const int64_t split = int64_t(fa_diff_bwd_split_bytes(&a)), at_split = (a.dsum_bytes + 255) / 256 * 256;
+    at::Tensor ws = split > 0 ? optional_workspace(at_split + split, q.options().dtype(at::kByte)) : at::Tensor();
+    if (ws.defined()) {
+        a.split_ws = static_cast<char *>(ws.data_ptr()) + at_split;
+        a.split_ws_bytes = split;
+    } else {
+        ws = at::empty({a.dsum_bytes}, q.options().dtype(at::kByte));
+    }
     a.dsum = static_cast<float *>(ws.data_ptr());
     check_rc(fa_diff_bwd(&a, current_stream()), "fa_diff_bwd");
     return got;

@@ -37,6 +37,14 @@ __host__ __device__ __forceinline__ int64_t diff_plane(const fa_diff_bwd_args &a
     return int64_t(a.batch) * a.nheads * a.lse_seqlen;
 }
 
+// Shared dK/dV items (diff_dkdv_kernel, SPLIT): split_ws starts with an int32
+// counter per (batch, key block, KV head), then, 256-byte aligned, come the fp32
+// partial sums.  The dQ kernel, which precedes it on the stream, clears the counters.
+__host__ __device__ __forceinline__ int64_t diff_dkdv_items(const fa_diff_bwd_args &a) {
+    return int64_t((a.seqlen_k + 127) / 128) * a.batch * a.nheads_k;
+}
+__host__ __device__ __forceinline__ int64_t diff_dkdv_count_bytes(int64_t items) { return (items * 4 + 255) & ~int64_t(255); }
+
 template <int HD, bool BF, bool CAUSAL>
 __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bwd_args a, const int num_m_blocks,
                                                                 const int lg) {
@@ -48,6 +56,11 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (a.split_ws) {
+        const int64_t n = diff_dkdv_items(a);
+        for (int64_t i = int64_t(blockIdx.x) * NT + tid; i < n; i += int64_t(gridDim.x) * NT)
+            static_cast<int32_t *>(a.split_ws)[i] = 0;
+    }
     const int packs = a.nheads >> lg, P = BM >> lg;
     int b, h, mb;
     if (a.work_order && a.cu_seqlens_q) {
@@ -277,19 +290,77 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
 // K rows live in registers (S's B operands), V rows in LDS (dP's), and every
 // 32-query block of Q, dO and the rows' D, LSE and lam goes HBM -> LDS in two
 // stages.  With lp = lam P_2: P = P_1 - lp feeds dV, dS_1 = P_1 (dP - D_1) and
-// lp (dP - D_2) feed dK; the latter's sign is applied at the end.
-template <int HD, bool BF, bool CAUSAL>
-__global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_bwd_args a, const int nnb) {
+// lp (dP - D_2) feed dK; the latter's sign is applied at the end.  SPLIT: S
+// workgroups share the steps (heads of the group x query blocks) of an item and
+// sum their dK / dV (diff_dkdv_sum).
+//
+// Of an item's S workgroups each stores its partial sums and then counts itself;
+// the one that counts last, or finds all others counted before it has stored
+// anything, adds them in the order of their shares: the sum does not depend on
+// who came last, and none waits.  Stores and loads at agent scope, 8 bytes a lane.
+template <int HD>
+__device__ __forceinline__ bool diff_dkdv_sum(const fa_diff_bwd_args &a, int item, int part, int S, int *ticket,
+                                              f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD / 32]) {
+    constexpr int N = HD / 2;  // pairs of floats a lane holds: dK, then dV
+    const int tid = threadIdx.x;
+    int32_t *count = static_cast<int32_t *>(a.split_ws) + item;
+    uint64_t *slots = reinterpret_cast<uint64_t *>(static_cast<char *>(a.split_ws) + diff_dkdv_count_bytes(diff_dkdv_items(a))) +
+                      int64_t(item) * S * N * kDbThreads + tid;
+    if (tid == 0) *ticket = part < 2 ? __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    __syncthreads();
+    if (*ticket != S - 1) {
+        uint64_t *own = slots + int64_t(part) * N * kDbThreads;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const f32x16 &t = i < N / 2 ? dk[i / 8] : dv[i / 8 - N / 16];
+            const f32x2 x = {t[2 * (i & 7)], t[2 * (i & 7) + 1]};
+            __hip_atomic_store(own + i * kDbThreads, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        }
+        wait_vmem();
+        __syncthreads();  // every wave's stores have completed
+        if (tid == 0) *ticket = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (*ticket != S - 1) return false;
+    }
+    // Its own share stays in registers when it is one of the first two (x0 + x1 = x1 + x0).
+    if (part >= 2) {
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) dk[i] = dv[i] = zero16();
+    }
+    for (int p = 0; p < S; ++p) {
+        if (p == part && part < 2) continue;
+        const uint64_t *slot = slots + int64_t(p) * N * kDbThreads;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const f32x2 x = __builtin_bit_cast(
+                f32x2, __hip_atomic_load(slot + i * kDbThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            f32x16 &t = i < N / 2 ? dk[i / 8] : dv[i / 8 - N / 16];
+            t[2 * (i & 7)] += x[0];
+            t[2 * (i & 7) + 1] += x[1];
+        }
+    }
+    return true;
+}
+
+template <int HD, bool BF, bool CAUSAL, bool SPLIT>
+__global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_bwd_args a, const int nnb, const int S) {
     constexpr int NT = kDbThreads, BN = 128, BM = 32;
     constexpr int QTILE = BM * HD * 2, STAGE = 2 * QTILE + 1024;  // Q, dO, 3 pairs of row planes
     constexpr int HG = HD / 32, DT = HD / 64;
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + BN * HD * 2];
+    __shared__ int ticket;
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int b, hk, nb;
+    int b, hk, nb, part = 0;
     if (a.work_order && a.cu_seqlens_k) {
-        const int it = a.work_order[blockIdx.x / a.nheads_k];
+        int slot = blockIdx.x / a.nheads_k;
+        if constexpr (SPLIT) {
+            part = slot % S;
+            slot /= S;
+        }
+        const int it = a.work_order[slot];
         if (it < 0) return;
         b = __builtin_amdgcn_readfirstlane(it / nnb);
         nb = __builtin_amdgcn_readfirstlane(it - b * nnb);
@@ -297,6 +368,10 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     } else {
         const int bh_count = a.batch * a.nheads_k, bhk = blockIdx.x % bh_count;
         nb = blockIdx.x / bh_count;  // the key blocks that most queries see first
+        if constexpr (SPLIT) {
+            part = nb % S;
+            nb /= S;
+        }
         b = bhk / a.nheads_k;
         hk = bhk - b * a.nheads_k;
     }
@@ -347,7 +422,20 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     const f16 *nq = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, hk * G);
     const f16 *ndo = (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, si.q_start, hk * G);
     const float *nd = a.dsum + (int64_t(b) * a.nheads + hk * G) * a.lse_seqlen;
-    int nh = 0, ni = 0;
+    // This workgroup's steps [t0, t1) of the G * n_qb (head slowest).
+    int t0 = 0, t1 = G * n_qb;
+    if constexpr (SPLIT) {
+        t0 = int(int64_t(G * n_qb) * part / S);
+        t1 = int(int64_t(G * n_qb) * (part + 1) / S);
+    }
+    int ni = 0, left = t1 - t0, i0 = 0;  // block of the next copy, steps not yet copied, first block
+    if (SPLIT && n_qb > 0) {
+        const int h0 = t0 / n_qb;
+        ni = i0 = t0 - h0 * n_qb;
+        nq += int64_t(h0) * a.q.head_stride;
+        ndo += int64_t(h0) * a.dout.head_stride;
+        nd += int64_t(h0) * a.lse_seqlen;
+    }
     const uint32_t smem_l = lds_addr(smem);
     auto issue_next = [&](int st) FA_INLINE {
         const int q0 = (m_first + ni) * BM;
@@ -363,9 +451,9 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
             const int64_t pl = min(2 * wave + hh, kDbPlanes - 1);
             g2l4_to(nd + pl * plane + min(q0 + col, sq - 1), smem_l + st * STAGE + 2 * QTILE + wave * 256);
         }
+        --left;
         if (++ni == n_qb) {
             ni = 0;
-            ++nh;
             nq += a.q.head_stride;
             ndo += a.dout.head_stride;
             nd += a.lse_seqlen;
@@ -464,7 +552,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     auto step = [&](int i, auto mask_tag, bool compute) FA_INLINE {
         wait_vmem();
         __syncthreads();
-        if (nh < G) issue_next((j & 1) ^ 1);
+        if (left > 0) issue_next((j & 1) ^ 1);
         if (compute) block(j, (m_first + i) * BM, mask_tag);
         ++j;
     };
@@ -473,16 +561,20 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     const int i1 = CAUSAL ? clampi(first_at(kw0 - 31 - causal_off), 0, n_qb) : 0;
     const int i2 = CAUSAL ? clampi(first_at(kw0 + 31 - causal_off), i1, n_qb) : 0;
     const int i3 = clampi(first_at(sq - 31), i2, n_qb);
-    if (n_qb > 0)
+    if (t1 > t0)
         issue_next(0);
     else
         wait_vmem();
-    for (int hidx = 0; hidx < G && n_qb > 0; ++hidx) {
-        for (int i = 0; i < i1; ++i) step(i, std::true_type{}, false);
-        for (int i = i1; i < i2; ++i) step(i, std::true_type{}, true);
-        for (int i = i2; i < i3; ++i) step(i, std::false_type{}, true);
-        for (int i = i3; i < n_qb; ++i) step(i, std::true_type{}, true);
+    for (int t = t0, i = i0; t < t1; i = 0) {
+        const int end = min(n_qb, i + t1 - t);
+        t += end - i;
+        for (const int e = min(i1, end); i < e; ++i) step(i, std::true_type{}, false);
+        for (const int e = min(i2, end); i < e; ++i) step(i, std::true_type{}, true);
+        for (const int e = min(i3, end); i < e; ++i) step(i, std::false_type{}, true);
+        for (; i < end; ++i) step(i, std::true_type{}, true);
     }
+    if constexpr (SPLIT)
+        if (!diff_dkdv_sum<HD>(a, (b * nnb + nb) * a.nheads_k + hk, part, S, &ticket, dk, dv)) return;
 
     if (key >= sk) return;
     f16 *dkrow = (f16 *)a.dk.ptr + base_off(a.dk, packed_k, b, si.k_start, hk) + int64_t(key) * a.dk.row_stride;
@@ -606,21 +698,72 @@ static int check_diff_bwd(const fa_diff_bwd_args *p) {
     if (!a.lse || !a.lam.ptr) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.o, &a.o2, &a.dout, &a.dq, &a.dk, &a.dv})
         if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
+    if (!split_ws_aligned(a.split_ws)) return FA_ERR_INVALID_ARG;
     if (!a.dsum || (reinterpret_cast<uintptr_t>(a.dsum) & 7u) || a.dsum_bytes < int64_t(fa_diff_bwd_ws_bytes(&a)))
         return FA_ERR_WORKSPACE;
     return FA_OK;
+}
+
+// Workgroups that share each (batch, key block, KV head) item of dK/dV.  One
+// where the grid fills the chip; with few items, or causal ones of very different
+// lengths, the longest item decides the kernel's time.  The estimate, in steps of
+// 32 queries (about 1.1 us at head_dim 128, two workgroups on a CU): the busiest
+// CU's steps (equal items in whole rounds; causal ones, longest first, leave about
+// half an item of imbalance), and the partials' traffic.  Packed batches are
+// taken as sequences of the mean length, which the packed tensors' rows tell, with
+// the longest one's longest item.
+static int diff_dkdv_splits(const fa_diff_bwd_args &a) {
+    constexpr int kMaxSplits = 16;
+    constexpr int64_t kMaxBytes = int64_t(256) << 20;  // of partials
+    const int64_t slots = diff_dkdv_items(a), cus = device_cus();
+    const int64_t cap = std::min<int64_t>(kMaxSplits, kMaxBytes / std::max<int64_t>(1, slots * 1024 * a.head_dim));
+    if (cap < 2 || a.seqlen_q <= 0) return 1;
+    const int G = a.nheads / a.nheads_k;
+    auto steps_of = [&](int64_t sq, int64_t sk, int64_t &items) {
+        const int64_t nnb = (sk + 127) / 128, n_qb = (sq + 31) / 32;
+        items += nnb;
+        if (!a.causal) return double(G) * n_qb * nnb;
+        double t = 0;
+        for (int64_t nb = 0; nb < nnb; ++nb) t += double(G) * std::max<int64_t>(0, n_qb - std::max<int64_t>(0, nb * 128 - (sk - sq)) / 32);
+        return t;
+    };
+    const double longest = double(G) * ((a.seqlen_q + 31) / 32);
+    int64_t items = 0;
+    const bool mean = a.cu_seqlens_q && a.dq_rows > 0 && a.dkv_rows > 0;
+    double total = steps_of(mean ? (a.dq_rows + a.batch - 1) / a.batch : a.seqlen_q,
+                            mean ? (a.dkv_rows + a.batch - 1) / a.batch : a.seqlen_k, items);
+    total *= double(a.batch) * a.nheads_k / cus;
+    items *= int64_t(a.batch) * a.nheads_k;
+    const bool uneven = a.causal || mean;
+    int best = 1;
+    double best_t = 0;
+    for (int S = 1; S <= cap; ++S) {
+        const int64_t wgs = items * S;
+        double t = uneven ? std::max(longest / S, total * (1 + 0.5 * cus / wgs))
+                          : double((wgs + cus - 1) / cus) * longest / S;
+        if (wgs <= cus) t *= 1.1;
+        if (S > 1) t += (2 * wgs <= cus ? 2 : 0) + (S - 1) * (0.025 * items + 3);
+        if (S == 1 || t < best_t) {
+            best = S;
+            best_t = t;
+        }
+    }
+    return best;
 }
 
 // Bytes of the planes, rounded so that the heads' fp64 sums, which follow, are aligned.
 static int64_t plane_bytes(const fa_diff_bwd_args &a) { return (kDbPlanes * diff_plane(a) * 4 + 7) & ~int64_t(7); }
 
 template <int HD, bool BF>
-static int launch_diff_bwd(const fa_diff_bwd_args &a, hipStream_t s) {
+static int launch_diff_bwd(fa_diff_bwd_args a, hipStream_t s) {
+    if (!a.split_ws || a.split_ws_bytes < int64_t(fa_diff_bwd_split_bytes(&a))) a.split_ws = nullptr;
+    const int S = a.split_ws ? diff_dkdv_splits(a) : 1;
+    if (S == 1) a.split_ws = nullptr;
     const int group = a.nheads / a.nheads_k;
     int lg = 0;  // heads of a GQA group in a dQ workgroup
     while (lg < 2 && group % (2 << lg) == 0) ++lg;
     const int P = 128 >> lg, nmb = (a.lse_seqlen + P - 1) / P, nnb = (a.seqlen_k + 127) / 128;
-    const int64_t q_grid = int64_t(nmb) * a.batch * (a.nheads >> lg), k_grid = int64_t(nnb) * a.batch * a.nheads_k;
+    const int64_t q_grid = int64_t(nmb) * a.batch * (a.nheads >> lg), k_grid = int64_t(nnb) * a.batch * a.nheads_k * S;
     if (q_grid > 0x7fffffff || k_grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     int rc;
     if (a.cu_seqlens_q && (a.work_order || a.dq_rows > 0)) {
@@ -643,10 +786,16 @@ static int launch_diff_bwd(const fa_diff_bwd_args &a, hipStream_t s) {
         if ((rc = int(hipGetLastError()))) return rc;
     }
     if (k_grid > 0) {
+        auto launch = [&](auto causal, auto split) {
+            hipLaunchKernelGGL((diff_dkdv_kernel<HD, BF, decltype(causal)::value, decltype(split)::value>),
+                               dim3(unsigned(k_grid)), dim3(kDbThreads), 0, s, a, nnb, S);
+        };
+        using T = std::true_type;
+        using F = std::false_type;
         if (a.causal)
-            hipLaunchKernelGGL((diff_dkdv_kernel<HD, BF, true>), dim3(unsigned(k_grid)), dim3(kDbThreads), 0, s, a, nnb);
+            S > 1 ? launch(T{}, T{}) : launch(T{}, F{});
         else
-            hipLaunchKernelGGL((diff_dkdv_kernel<HD, BF, false>), dim3(unsigned(k_grid)), dim3(kDbThreads), 0, s, a, nnb);
+            S > 1 ? launch(F{}, T{}) : launch(F{}, F{});
         if ((rc = int(hipGetLastError()))) return rc;
     }
     if (!a.dlam.ptr) return FA_OK;
@@ -671,6 +820,15 @@ static int launch_diff_bwd(const fa_diff_bwd_args &a, hipStream_t s) {
 extern "C" size_t fa_diff_bwd_ws_bytes(const fa_diff_bwd_args *a) {
     if (!a || a->batch < 0 || a->nheads <= 0 || a->lse_seqlen < 0) return 0;
     return size_t(fa::plane_bytes(*a) + 8 * int64_t(a->nheads));
+}
+
+extern "C" size_t fa_diff_bwd_split_bytes(const fa_diff_bwd_args *p) {
+    if (!p || p->batch <= 0 || p->seqlen_q <= 0 || p->seqlen_k <= 0 || p->nheads <= 0 || p->nheads_k <= 0 ||
+        (p->head_dim != 64 && p->head_dim != 128))
+        return 0;
+    const int S = fa::diff_dkdv_splits(*p);
+    const int64_t items = fa::diff_dkdv_items(*p);
+    return S > 1 ? size_t(fa::diff_dkdv_count_bytes(items) + items * S * 2 * 128 * p->head_dim * 4) : 0;
 }
 
 extern "C" size_t fa_diff_bwd_order_len(const fa_diff_bwd_args *a) {

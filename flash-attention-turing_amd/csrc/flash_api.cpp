@@ -66,16 +66,6 @@ int num_cus(int device) {
     return n;
 }
 
-// A workspace that a call is faster with but can do without: undefined where the
-// device has no memory left for it.
-at::Tensor optional_workspace(int64_t numel, const at::TensorOptions &options) {
-    try {
-        return at::empty({numel}, options);
-    } catch (const c10::OutOfMemoryError &) {
-        return at::Tensor();
-    }
-}
-
 // The workspace in which workgroups that share a query block sum their results
 // (undefined when the grid needs no sharing).
 at::Tensor fwd_workspace(fa_fwd_args &a, const at::Tensor &like) {
