@@ -143,6 +143,7 @@ std::vector<std::optional<at::Tensor>> run_fwd(at::Tensor q, at::Tensor k, at::T
     at::Tensor order;
     if (x) {
         a.o_rows = i32(q.size(0), "total_q");
+        a.k_rows = i32(k.size(0), "total_k");
         order = at::empty({int64_t(std::max<size_t>(fa_diff_fwd_order_len(&a), 1))}, x->cu_q->options());
         a.work_order = order.data_ptr<int32_t>();
     }

@@ -79,13 +79,13 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     }
     const int hk = h / (a.nheads / a.nheads_k);
     const bool packed_q = a.cu_seqlens_q != nullptr, packed_k = a.cu_seqlens_k != nullptr;
-    const SeqInfo si = seq_info(b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
-    const int sq = si.sq, sk = si.sk, m0 = mb * P;
+    const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows), rk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows);
+    const int sq = rq.n, sk = rk.n, m0 = mb * P;
     if (m0 >= sq) return;
     h += wave >> (2 - lg);
 
-    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, si.k_start, hk);
-    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, si.k_start, hk);
+    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, rk.start, hk);
+    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, rk.start, hk);
     const int64_t krs = a.k.row_stride, vrs = a.v.row_stride;
     const int causal_off = sk - sq;
     int n_end = sk;
@@ -117,12 +117,12 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     f16x8 qB[HD / 16], doB[HD / 16];
     float d1 = 0.f, d2 = 0.f;
     {
-        const f16 *qp = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, h) + qr * a.q.row_stride + 8 * hh;
+        const f16 *qp = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, rq.start, h) + qr * a.q.row_stride + 8 * hh;
         const f16 *dop =
-            (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, si.q_start, h) + qr * a.dout.row_stride + 8 * hh;
-        const f16 *op = (const f16 *)a.o.ptr + base_off(a.o, packed_q, b, si.q_start, h) + qr * a.o.row_stride + 8 * hh;
+            (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, rq.start, h) + qr * a.dout.row_stride + 8 * hh;
+        const f16 *op = (const f16 *)a.o.ptr + base_off(a.o, packed_q, b, rq.start, h) + qr * a.o.row_stride + 8 * hh;
         const f16 *o2p =
-            (const f16 *)a.o2.ptr + base_off(a.o2, packed_q, b, si.q_start, h) + qr * a.o2.row_stride + 8 * hh;
+            (const f16 *)a.o2.ptr + base_off(a.o2, packed_q, b, rq.start, h) + qr * a.o2.row_stride + 8 * hh;
 #pragma unroll
         for (int g = 0; g < HD / 16; ++g) {
             qB[g] = as_h8(qv ? ldg16(qp + 16 * g) : zero_u4());
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
             }
         }
     }
-    const float lam = qv ? diff_lam(a.lam, b, si.q_start + qi, h) : 0.f;
+    const float lam = qv ? diff_lam(a.lam, b, rq.start + qi, h) : 0.f;
     const int64_t lrow = (int64_t(b) * a.nheads + h) * a.lse_seqlen;
     const int64_t plane = diff_plane(a);
     const float lse1 = qv ? a.lse[lrow + qi] * kLog2e : 0.f, lse2 = qv ? a.lse[plane + lrow + qi] * kLog2e : 0.f;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     }
     int qo = qi;
     asm volatile("" : "+v"(qo));
-    f16 *row = (f16 *)a.dq.ptr + base_off(a.dq, packed_q, b, si.q_start, h) + int64_t(qo) * a.dq.row_stride;
+    f16 *row = (f16 *)a.dq.ptr + base_off(a.dq, packed_q, b, rq.start, h) + int64_t(qo) * a.dq.row_stride;
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt) {
         const float f = sgn * (dt < HD / 64 ? a.softmax_scale : -lam * a.softmax_scale);
@@ -377,12 +377,12 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     }
     const int G = a.nheads / a.nheads_k;
     const bool packed_q = a.cu_seqlens_q != nullptr, packed_k = a.cu_seqlens_k != nullptr;
-    const SeqInfo si = seq_info(b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
-    const int sq = si.sq, sk = si.sk, k0 = nb * BN;
+    const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows), rk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows);
+    const int sq = rq.n, sk = rk.n, k0 = nb * BN;
     if (k0 >= sk) return;
 
-    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, si.k_start, hk);
-    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, si.k_start, hk);
+    const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, rk.start, hk);
+    const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, rk.start, hk);
     const int causal_off = sk - sq;
     const float cs = a.softmax_scale * kLog2e;
     const int64_t qrs = a.q.row_stride, dors = a.dout.row_stride;
@@ -419,8 +419,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     ocp.init(dors, wave, lane);
     // Running pointers of the next (head, query block) to copy.
     const int64_t plane = diff_plane(a);
-    const f16 *nq = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, si.q_start, hk * G);
-    const f16 *ndo = (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, si.q_start, hk * G);
+    const f16 *nq = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, rq.start, hk * G);
+    const f16 *ndo = (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, rq.start, hk * G);
     const float *nd = a.dsum + (int64_t(b) * a.nheads + hk * G) * a.lse_seqlen;
     // This workgroup's steps [t0, t1) of the G * n_qb (head slowest).
     int t0 = 0, t1 = G * n_qb;
@@ -577,8 +577,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
         if (!diff_dkdv_sum<HD>(a, (b * nnb + nb) * a.nheads_k + hk, part, S, &ticket, dk, dv)) return;
 
     if (key >= sk) return;
-    f16 *dkrow = (f16 *)a.dk.ptr + base_off(a.dk, packed_k, b, si.k_start, hk) + int64_t(key) * a.dk.row_stride;
-    f16 *dvrow = (f16 *)a.dv.ptr + base_off(a.dv, packed_k, b, si.k_start, hk) + int64_t(key) * a.dv.row_stride;
+    f16 *dkrow = (f16 *)a.dk.ptr + base_off(a.dk, packed_k, b, rk.start, hk) + int64_t(key) * a.dk.row_stride;
+    f16 *dvrow = (f16 *)a.dv.ptr + base_off(a.dv, packed_k, b, rk.start, hk) + int64_t(key) * a.dv.row_stride;
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt) {
         const float f = dt < DT ? a.softmax_scale : -a.softmax_scale;
@@ -600,9 +600,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 // all heads the second launch sums the heads.
 __global__ __launch_bounds__(1024) void diff_dlam_rows_kernel(const fa_diff_bwd_args a) {
     const int b = blockIdx.y;
-    const int64_t start = a.cu_seqlens_q ? a.cu_seqlens_q[b] : 0;
-    const int sq = a.cu_seqlens_q ? min(a.cu_seqlens_q[b + 1] - int(start), a.lse_seqlen) : a.seqlen_q;
-    const int64_t n = int64_t(sq) * a.nheads;
+    const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows);
+    const int64_t start = rq.start, n = int64_t(rq.n) * a.nheads;
     for (int64_t i = int64_t(blockIdx.x) * 1024 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 1024) {
         const int64_t row = i / a.nheads;
         const int h = int(i - row * a.nheads);
@@ -629,8 +628,7 @@ __global__ __launch_bounds__(1024) void diff_dlam_head_kernel(const fa_diff_bwd_
     const float *nd2 = a.dsum + diff_plane(a);
     double x = 0;
     for (int b = 0; b < a.batch; ++b) {
-        const int sq =
-            a.cu_seqlens_q ? min(a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b], a.lse_seqlen) : a.seqlen_q;
+        const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
         const float *row = nd2 + (int64_t(b) * a.nheads + h) * a.lse_seqlen;
         for (int i = threadIdx.x; i < sq; i += 1024) x += row[i];
     }
@@ -661,7 +659,8 @@ __global__ __launch_bounds__(kOrderThreads) void diff_dkdv_order_kernel(const fa
     }
     order_items(a.batch * nnb, [&](int it) {
         const int b = it / nnb, nb = it - b * nnb;
-        const int sk = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b], sq = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b];
+        const int sk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows).n;
+        const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
         const int k0 = nb * 128;
         if (k0 >= sk) return -1;
         const int rows = a.causal ? max(0, min(sq, sk - k0)) : max(sq, 0);
@@ -678,7 +677,8 @@ __global__ __launch_bounds__(kOrderThreads) void diff_dq_order_kernel(const fa_d
     }
     order_items(a.batch * nmb, [&](int it) {
         const int b = it / nmb, mb = it - b * nmb;
-        const int sq = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b], sk = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b];
+        const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
+        const int sk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows).n;
         const int m0 = mb * P;
         if (m0 >= sq) return -1;
         const int keys = a.causal ? max(0, min(sk, m0 + P + sk - sq)) : sk;

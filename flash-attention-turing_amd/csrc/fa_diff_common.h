@@ -79,6 +79,23 @@ __device__ __forceinline__ float uniform(float x) {
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
+// Rows of sequence b of a dense or packed call.  A packed sequence is cut to the
+// call's maximum length, on which the LSE's rows, the grids and the work orders
+// go, and to the rows that its tensor has (rows; 0: not known), so that no access
+// leaves a tensor whatever cu holds.
+struct DiffRows {
+    int start, n;
+};
+__device__ __forceinline__ DiffRows diff_rows(const int32_t *cu, int b, int seqlen, int rows) {
+    DiffRows r{0, seqlen};
+    if (cu) {
+        const int most = rows > 0 ? rows : INT_MAX;
+        r.start = min(max(cu[b], 0), most);
+        r.n = min(max(min(cu[b + 1], most) - r.start, 0), seqlen);
+    }
+    return r;
+}
+
 // lam of (batch, row of the tensor, head); strides in elements, 0 where it is shared.
 __device__ __forceinline__ float diff_lam(const fa_diff_lam &l, int b, int64_t row, int h) {
     return l.ptr[int64_t(b) * l.batch_stride + row * l.row_stride + int64_t(h) * l.head_stride];

@@ -109,7 +109,8 @@ __device__ __forceinline__ DiffWork diff_work(const DiffFwd &p, int num_m_blocks
     }
     w.hk = w.h / (a.nheads / a.nheads_k);
     const bool packed_k = a.cu_seqlens_k != nullptr;
-    SeqInfo si = seq_info(w.b, a.seqlen_q, a.seqlen_k, a.cu_seqlens_q, a.cu_seqlens_k, nullptr, 0);
+    const DiffRows qr = diff_rows(a.cu_seqlens_q, w.b, a.seqlen_q, a.o_rows);
+    DiffRows kr = diff_rows(a.cu_seqlens_k, w.b, a.seqlen_k, a.k_rows);
     int kb = w.b;
     if constexpr (CACHE) {
         // A length or a cache row outside the cache leaves the sequence with no
@@ -118,21 +119,21 @@ __device__ __forceinline__ DiffWork diff_work(const DiffFwd &p, int num_m_blocks
         if (p.cache_batch_idx) kb = p.cache_batch_idx[w.b];
         const int err = (used < 0 || int64_t(used) + p.seqlen_new > p.capacity ? 1 : 0) |
                         (p.cache_batch_idx && (kb < 0 || kb >= p.cache_batch) ? 2 : 0);
-        si.sk = err ? 0 : used + p.seqlen_new;
+        kr.n = err ? 0 : used + p.seqlen_new;
         if (err) {
             kb = 0;
             if (p.status && threadIdx.x == 0) atomicOr(p.status, err);
         }
         if (p.block_table) kb = 0;
     }
-    w.q_start = si.q_start;
-    w.sq = si.sq;
-    w.sk = si.sk;
+    w.q_start = qr.start;
+    w.sq = qr.n;
+    w.sk = kr.n;
     w.m0 = mb * w.P;
     w.causal_off = w.sk - w.sq;  // key j is visible to query i iff j <= i + causal_off
     w.n_keys = CAUSAL ? max(0, min(w.sk, w.m0 + w.P + w.causal_off)) : w.sk;
-    w.kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, kb, si.k_start, w.hk);
-    w.vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, kb, si.k_start, w.hk);
+    w.kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, kb, kr.start, w.hk);
+    w.vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, kb, kr.start, w.hk);
     w.live = w.m0 < w.sq;
     return w;
 }
@@ -408,8 +409,8 @@ __global__ __launch_bounds__(kOrderThreads) void diff_fwd_order_kernel(const fa_
     }
     order_items(a.batch * nmb, [&](int it) {
         const int b = it / nmb, mb = it - b * nmb;
-        const int sq = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b];
-        const int sk = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b];
+        const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.o_rows).n;
+        const int sk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.k_rows).n;
         const int m0 = mb * P;
         if (m0 >= sq) return -1;
         const int64_t rows = min(P, sq - m0);

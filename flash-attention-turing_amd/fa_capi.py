@@ -76,6 +76,54 @@ class FaKvcacheArgs(ctypes.Structure):
     ]
 
 
+class FaDiffLam(ctypes.Structure):  # fa_diff_lam and fa_diff_dlam
+    _fields_ = [("ptr", _p), ("batch_stride", _i64), ("row_stride", _i64), ("head_stride", _i64)]
+
+
+class FaDiffFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", FaTensor), ("k", FaTensor), ("v", FaTensor), ("o", FaTensor), ("o2", FaTensor), ("lam", FaDiffLam),
+        ("lse", _p), ("cu_seqlens_q", _p), ("cu_seqlens_k", _p),
+        ("batch", _i32), ("seqlen_q", _i32), ("seqlen_k", _i32), ("nheads", _i32), ("nheads_k", _i32),
+        ("head_dim", _i32), ("lse_seqlen", _i32), ("softmax_scale", _f32), ("causal", _i32), ("dtype", _i32),
+        ("o_rows", _i32), ("k_rows", _i32), ("work_order", _p),
+    ]
+
+
+class FaDiffBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", FaTensor), ("k", FaTensor), ("v", FaTensor), ("o", FaTensor), ("o2", FaTensor), ("dout", FaTensor),
+        ("dq", FaTensor), ("dk", FaTensor), ("dv", FaTensor), ("lam", FaDiffLam), ("dlam", FaDiffLam),
+        ("lse", _p), ("cu_seqlens_q", _p), ("cu_seqlens_k", _p),
+        ("batch", _i32), ("seqlen_q", _i32), ("seqlen_k", _i32), ("nheads", _i32), ("nheads_k", _i32),
+        ("head_dim", _i32), ("lse_seqlen", _i32), ("softmax_scale", _f32), ("causal", _i32), ("dtype", _i32),
+        ("dq_rows", _i32), ("dkv_rows", _i32), ("work_order", _p), ("dsum", _p), ("dsum_bytes", _i64),
+        ("split_ws", _p), ("split_ws_bytes", _i64),
+    ]
+
+
+class FaDiffKvcacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", FaTensor), ("k_cache", FaTensor), ("v_cache", FaTensor), ("k_new", FaTensor), ("v_new", FaTensor),
+        ("o", FaTensor), ("lam", FaDiffLam), ("lse", _p), ("cache_seqlens", _p), ("cache_batch_idx", _p),
+        ("block_table", _p), ("block_table_stride", _i64),
+        ("batch", _i32), ("seqlen_q", _i32), ("nheads", _i32), ("nheads_k", _i32), ("head_dim", _i32),
+        ("seqlen_new", _i32), ("page_block_size", _i32), ("num_pages", _i32), ("num_splits", _i32),
+        ("softmax_scale", _f32), ("causal", _i32), ("dtype", _i32), ("cache_capacity", _i32), ("cache_batch", _i32),
+        ("status", _p), ("ws", _p), ("ws_bytes", _i64),
+    ]
+
+
+class FaKvpagesArgs(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", FaTensor), ("v_cache", FaTensor), ("nheads_k", _i32), ("head_bytes", _i32),
+        ("page_block_size", _i32), ("num_pages", _i32), ("block_table", _p), ("block_table_stride", _i64),
+        ("rows", _i32), ("max_pages", _i32), ("cache_seqlens", _p), ("page_refs", _p), ("from", _p), ("to", _p),
+        ("n", _i32), ("seqlen_new", _i32), ("seqlens_new", _p), ("out_table", _p), ("out_table_stride", _i64),
+        ("out_refs", _p), ("out_used", _p), ("status", _p), ("ws", _p), ("ws_bytes", _i64),
+    ]
+
+
 _ARGP = {
     "fa_fwd": FaFwdArgs,
     "fa_bwd_preprocess": FaBwdArgs,
@@ -87,6 +135,23 @@ _ARGP = {
     "fa_kv_combine": FaKvcacheArgs,
     "fa_fwd_kvcache": FaKvcacheArgs,
     "fa_fwd_kvcache_noalloc": FaKvcacheArgs,
+    "fa_diff_fwd": FaDiffFwdArgs,
+    "fa_diff_bwd": FaDiffBwdArgs,
+    "fa_diff_kvcache": FaDiffKvcacheArgs,
+    "fa_kvpages_alloc": FaKvpagesArgs,
+    "fa_kvpages_copy": FaKvpagesArgs,
+    "fa_kvpages_fork": FaKvpagesArgs,
+    "fa_kvpages_free": FaKvpagesArgs,
+    "fa_kvpages_compact": FaKvpagesArgs,
+}
+# Sizes of workspaces, of the same structs.
+_SIZES = {
+    "fa_diff_fwd_order_len": FaDiffFwdArgs,
+    "fa_diff_bwd_order_len": FaDiffBwdArgs,
+    "fa_diff_bwd_ws_bytes": FaDiffBwdArgs,
+    "fa_diff_bwd_split_bytes": FaDiffBwdArgs,
+    "fa_diff_kvcache_ws_bytes": FaDiffKvcacheArgs,
+    "fa_kvpages_ws_bytes": FaKvpagesArgs,
 }
 
 # FA_ABI_VERSION of include/fa_mi355x.h whose struct layouts the classes above mirror.
@@ -111,6 +176,10 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(st), _p]
         fn.restype = ctypes.c_int
+    for name, st in _SIZES.items():
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(st)]
+        fn.restype = ctypes.c_size_t
     lib.fa_kv_num_splits.argtypes = [ctypes.c_int] * 8
     lib.fa_kv_num_splits.restype = ctypes.c_int
     lib.fa_kv_args_num_splits.argtypes = [ctypes.POINTER(FaKvcacheArgs), ctypes.c_int, ctypes.c_int]

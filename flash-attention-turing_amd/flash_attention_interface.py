@@ -687,7 +687,7 @@ def flash_diff_attn_with_kvcache(
     if num_splits < 0:
         raise ValueError("num_splits must be non-negative")
     if validate and batch > 0:
-        lens = cache_seqlens.cpu()
+        lens = cache_seqlens.cpu().long()
         used = lens + (0 if k is None else k.shape[1])
         if int(lens.min()) < 0 or int(used.max()) > capacity:
             raise ValueError("cache capacity is insufficient for the requested append length")

@@ -303,7 +303,9 @@ typedef struct fa_diff_fwd_args {
     float softmax_scale;
     int32_t causal;                 /* bottom-right aligned                      */
     int32_t dtype;
-    int32_t o_rows;                 /* as fa_fwd_args.o_rows                     */
+    int32_t o_rows;                 /* rows of the packed q and o, as fa_fwd_args.o_rows */
+    int32_t k_rows;                 /* rows of the packed k and v, or 0; a packed sequence is cut to these
+                                       rows and to seqlen_q / seqlen_k, whatever cu_seqlens hold */
     int32_t *work_order;            /* fa_diff_fwd_order_len(args) int32s for packed batches, or NULL */
 } fa_diff_fwd_args;
 
@@ -328,7 +330,7 @@ typedef struct fa_diff_bwd_args {
     int32_t batch, seqlen_q, seqlen_k, nheads, nheads_k, head_dim, lse_seqlen;
     float softmax_scale;
     int32_t causal, dtype;
-    int32_t dq_rows, dkv_rows;      /* as in fa_bwd_args                          */
+    int32_t dq_rows, dkv_rows;      /* as o_rows and k_rows, and as in fa_bwd_args */
     int32_t *work_order;            /* fa_diff_bwd_order_len(args) int32s for packed batches, or NULL */
     float *dsum;                    /* workspace of dsum_bytes >= fa_diff_bwd_ws_bytes(args), 8-byte aligned */
     int64_t dsum_bytes;
