@@ -299,7 +299,7 @@ def test_refusals(device):
 def test_serving_loop(device, dtype):
     """Prompts, forks, decode steps, ends and compaction together: every step's output against the definition over
     the row's own token history, and in fp16 ordinary attention on the same cache against itself on a
-    contiguous copy of the tokens."""
+    contiguous copy of the tokens (whose keys it may split and sum in another order)."""
     h, hk, d, page, rows, width = 4, 2, 64, 256, 6, 4
     g = torch.Generator().manual_seed(5)
     mk = lambda *s: torch.randn(*s, generator=g).to(dtype).to(device)  # noqa: E731
@@ -325,9 +325,12 @@ def test_serving_loop(device, dtype):
             assert_within(f"row {r}", out[i:i + 1], diff_attention(q[i:i + 1], ks, vs, lam, None, True)["out"])
             if dtype == torch.float16 and n == 1:
                 a = fai.flash_attn_with_kvcache(q[i:i + 1], k_cache, v_cache, cache_seqlens=lens[r:r + 1],
-                                                block_table=table[r:r + 1].clamp_min(0), causal=True, num_splits=1)
-                same = torch.equal(a, fai.flash_attn_with_kvcache(q[i:i + 1], ks, vs, causal=True, num_splits=1))
-                assert same, f"ordinary attention, row {r}"
+                                                block_table=table[r:r + 1].clamp_min(0), causal=True)
+                b = fai.flash_attn_with_kvcache(q[i:i + 1], ks, vs, causal=True)
+                # Two roundings to fp16 (2^-11 each) and twice the fp32 error of 350 keys' scores and sums with
+                # |v| < 5: (350 + 16) * 2^-23 * 5 and 2^-21 * 20 * 5.
+                worst = float(((a - b).float().abs() - 2.0 ** -10 * a.float().abs()).max())
+                assert worst <= 2 * (366 * 2.0 ** -23 * 5 + 2.0 ** -21 * 100), f"ordinary attention, row {r}: {worst}"
 
     step([0], 300)
     step([1], 256)
