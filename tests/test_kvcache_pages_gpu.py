@@ -342,7 +342,8 @@ def test_serving_loop(device, dtype):
     history[0], history[1] = [], []
     step([2, 3, 4], 3)
     table, refs, used = fai.flash_attn_kvcache_compact(k_cache, v_cache, table, refs)
-    assert int(used) == int((refs > 0).sum()) == 7 and int(table.max()) == 6
+    # Rows 2 and 3 share the old row 0's full page and have one of their own, row 4 has two.
+    assert int(used) == int((refs > 0).sum()) == 5 and int(table.max()) == 4
     step([3, 4], 1)
     step([0], 40)
     fai.flash_attn_kvcache_fork(k_cache, v_cache, table, lens, refs, ints([3]), ints([1]))
