@@ -31,11 +31,52 @@
 namespace fa {
 
 constexpr int kDbThreads = 256;
-constexpr int kDbPlanes = 5;  // fp32 planes of the workspace: -D1, -D2, LSE1 * log2(e), LSE2 * log2(e), lam
+// The workspace: -D_2 of every row in fp32 (for dlam), then DiffRowOps of every row.
+//
+// What the dK/dV kernel needs of a query row (its LSEs, D_m and lam) belongs to
+// the M dimension of its products, so a lane would need all 16 rows' values of
+// its accumulators: 24 16-byte LDS reads per 32 x 32 tile, a quarter of the LDS
+// time that bounded the kernel.  Instead the row's values enter the products, as
+// one more K step: a value v is the sum of three 16-bit numbers times the powers
+// of two in row_weights, which is exact to 2^-24 of it or 2^-36, whichever is
+// larger.  The scores so come out as S_m - LSE_m / scale, with log2 |lam| taken off
+// LSE_2, and dP as dP - D_1 and, by one more product, dP - D_2.  The sign of lam
+// goes in the fourth place, whose weight is 0.
+struct DiffRowOps {
+    f16x4 lse1, lse2, nd1, e;  // of -LSE_1 / scale, -(LSE_2 - log |lam|) / scale, -D_1, D_1 - D_2
+};
+static_assert(sizeof(DiffRowOps) == 32, "copied as 32 rows a KiB");
+constexpr float kRowHi = 256.f, kRowLo = 1.f / 4096.f;
+
+template <bool BF>
+__device__ __forceinline__ float round16(float x) {
+    if constexpr (BF)
+        return float((__bf16)x);
+    else
+        return float((f16)x);
+}
+template <bool BF>
+__device__ __forceinline__ f16x4 row_op(float v, float fourth) {
+    const float hi = round16<BF>(fminf(fmaxf(v * (1.f / kRowHi), -65504.f), 65504.f));
+    const float r = fmaf(-kRowHi, hi, v);
+    const float mid = round16<BF>(fminf(fmaxf(r, -65504.f), 65504.f));
+    return pack4<BF>(hi, mid, fminf(fmaxf((r - mid) * (1.f / kRowLo), -65504.f), 65504.f), fourth);
+}
+// B operand that weighs the first (which = 0) or second of two row_ops in an A
+// operand: K slots 0..3 and 4..7 of the lower lane half, the upper half's are 0.
+template <bool BF>
+__device__ __forceinline__ f16x8 row_weights(int which, int hh) {
+    const f16x4 w = pack4<BF>(hh ? 0.f : kRowHi, hh ? 0.f : 1.f, hh ? 0.f : kRowLo, 0.f);
+    const f16x4 z = pack4<BF>(0.f, 0.f, 0.f, 0.f);
+    return which ? __builtin_shufflevector(z, w, 0, 1, 2, 3, 4, 5, 6, 7) : __builtin_shufflevector(w, z, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 __host__ __device__ __forceinline__ int64_t diff_plane(const fa_diff_bwd_args &a) {
     return int64_t(a.batch) * a.nheads * a.lse_seqlen;
 }
+
+// Floats from the start of the workspace to the row operands (32-byte aligned from a 32-byte aligned start).
+__host__ __device__ __forceinline__ int64_t diff_ops_at(const fa_diff_bwd_args &a) { return (diff_plane(a) + 7) & ~int64_t(7); }
 
 // Shared dK/dV items (diff_dkdv_kernel, SPLIT): split_ws starts with an int32
 // counter per (batch, key block, KV head), then, 256-byte aligned, come the fp32
@@ -91,20 +132,15 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     int n_end = sk;
     if (CAUSAL) n_end = max(0, min(sk, m0 + P + causal_off));
     const int n_blocks = (n_end + BN - 1) / BN;
-    const float cs = a.softmax_scale * kLog2e;
+    const float cs = uniform(a.softmax_scale * kLog2e);
 
-    TileCopier<HD, BN, NT> kcp, vcp;
-    kcp.init(krs, wave, lane);
-    vcp.init(vrs, wave, lane);
+    DiffCopier<HD, BN, NT> cp;
+    cp.init(wave, lane);
     auto issue = [&](int nb, int st) FA_INLINE {
         const int n0 = nb * BN;
-        if (n0 + BN <= sk) {
-            kcp.template copy_to<true>(lds_addr(smem) + st * STAGE, kp + int64_t(n0) * krs, krs);
-            vcp.template copy_to<true>(lds_addr(smem) + st * STAGE + TILE, vp + int64_t(n0) * vrs, vrs);
-        } else {
-            dma_tile<HD, BN, NT>(smem + st * STAGE, kp, krs, n0, sk - 1, wave, lane);
-            dma_tile<HD, BN, NT>(smem + st * STAGE + TILE, vp, vrs, n0, sk - 1, wave, lane);
-        }
+        const uint32_t tile = lds_addr(smem) + st * STAGE;
+        cp.copy(tile, kp + int64_t(n0) * krs, krs, sk - n0);
+        cp.copy(tile + TILE, vp + int64_t(n0) * vrs, vrs, sk - n0);
     };
     if (n_blocks > 0) issue(0, 0);
 
@@ -230,10 +266,14 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[t][r] *= dp[t][r] + e;
-                    if (m == 1) sum += s[t][r];
+                    if (m == 0 && !MASK) {
+                        s[t][r] *= dp[t][r];
+                    } else {
+                        s[t][r] *= dp[t][r] + e;
+                        if (m == 1) sum += s[t][r];
+                    }
                 }
-            ds2_sum += sum;
+            if (m == 1) ds2_sum += sum;
             f16x8 dsB[4];
 #pragma unroll
             for (int gg = 0; gg < 4; ++gg) dsB[gg] = pack16<BF>(s[gg >> 1], 8 * (gg & 1));
@@ -265,12 +305,14 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     ds2_sum = sum_xor32(ds2_sum);
     if (!qv) return;
     if (hh == 0) {
-        float *w = a.dsum + lrow + qi;
-        w[0] = -sgn * d1;
-        w[plane] = -sgn * (d2 + ds2_sum);
-        w[2 * plane] = lse1;
-        w[3 * plane] = lse2;
-        w[4 * plane] = lam;
+        const float D1 = sgn * d1, D2 = sgn * (d2 + ds2_sum);
+        // exp2(cs (S - LSE / cs)); with a scale of 0 the dK/dV kernel takes scores of 0 and cs = 1.
+        const float per = a.softmax_scale != 0.f ? -1.f / cs : -1.f;
+        const float l2 = lam != 0.f ? lse2 - log2_fast(fabsf(lam)) : lse2 + 1000.f;  // 2^-1000 is 0
+        a.dsum[lrow + qi] = -D2;
+        DiffRowOps *ops = reinterpret_cast<DiffRowOps *>(a.dsum + diff_ops_at(a)) + lrow + qi;
+        *ops = DiffRowOps{row_op<BF>(lse1 * per, 0.f), row_op<BF>(l2 * per, lam < 0.f ? -1.f : 1.f), row_op<BF>(-D1, 0.f),
+                          row_op<BF>(D1 - D2, 0.f)};
     }
     int qo = qi;
     asm volatile("" : "+v"(qo));
@@ -290,7 +332,9 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
 // K rows live in registers (S's B operands), V rows in LDS (dP's), and every
 // 32-query block of Q, dO and the rows' D, LSE and lam goes HBM -> LDS in two
 // stages.  With lp = lam P_2: P = P_1 - lp feeds dV, dS_1 = P_1 (dP - D_1) and
-// lp (dP - D_2) feed dK; the latter's sign is applied at the end.  SPLIT: S
+// lp (dP - D_2) feed dK; the latter's sign is applied at the end.  The LDS bounds
+// it: per 32 x 32 tile 26 plain operand reads (5.7 cycles of the CU) and 32
+// transposed ones (8.1) against 36 MFMAs, with eight waves on a CU.  SPLIT: S
 // workgroups share the steps (heads of the group x query blocks) of an item and
 // sum their dK / dV (diff_dkdv_sum).
 //
@@ -346,7 +390,7 @@ __device__ __forceinline__ bool diff_dkdv_sum(const fa_diff_bwd_args &a, int ite
 template <int HD, bool BF, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_bwd_args a, const int nnb, const int S) {
     constexpr int NT = kDbThreads, BN = 128, BM = 32;
-    constexpr int QTILE = BM * HD * 2, STAGE = 2 * QTILE + 1024;  // Q, dO, 3 pairs of row planes
+    constexpr int QTILE = BM * HD * 2, STAGE = 2 * QTILE + 1024;  // Q, dO, row operands
     constexpr int HG = HD / 32, DT = HD / 64;
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + BN * HD * 2];
     __shared__ int ticket;
@@ -384,7 +428,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, rk.start, hk);
     const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, rk.start, hk);
     const int causal_off = sk - sq;
-    const float cs = a.softmax_scale * kLog2e;
+    const bool flat = a.softmax_scale == 0.f;  // scores of 0: see the dQ kernel
+    const float cs = uniform(flat ? 1.f : a.softmax_scale * kLog2e);
     const int64_t qrs = a.q.row_stride, dors = a.dout.row_stride;
     const int kw0 = k0 + wave * 32, key = kw0 + col;
     TileReader<HD> rd;
@@ -406,7 +451,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     {
         const f16 *kr = kp + int64_t(min(key, sk - 1)) * a.k.row_stride + 8 * hh;
 #pragma unroll
-        for (int g = 0; g < HD / 16; ++g) kreg[g] = *reinterpret_cast<const f16x8 *>(kr + 16 * g);
+        for (int g = 0; g < HD / 16; ++g) kreg[g] = flat ? as_h8(zero_u4()) : *reinterpret_cast<const f16x8 *>(kr + 16 * g);
     }
     f32x16 dk[HD / 32], dv[HD / 32];
 #pragma unroll
@@ -414,14 +459,13 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 
     const int m_first = CAUSAL ? max(0, k0 - causal_off) / BM : 0;
     const int n_qb = max(0, (sq + BM - 1) / BM - m_first);
-    TileCopier<HD, BM, NT> qcp, ocp;
-    qcp.init(qrs, wave, lane);
-    ocp.init(dors, wave, lane);
+    DiffCopier<HD, BM, NT> cp;
+    cp.init(wave, lane);
     // Running pointers of the next (head, query block) to copy.
-    const int64_t plane = diff_plane(a);
     const f16 *nq = (const f16 *)a.q.ptr + base_off(a.q, packed_q, b, rq.start, hk * G);
     const f16 *ndo = (const f16 *)a.dout.ptr + base_off(a.dout, packed_q, b, rq.start, hk * G);
-    const float *nd = a.dsum + (int64_t(b) * a.nheads + hk * G) * a.lse_seqlen;
+    const DiffRowOps *ops =
+        reinterpret_cast<const DiffRowOps *>(a.dsum + diff_ops_at(a)) + (int64_t(b) * a.nheads + hk * G) * a.lse_seqlen;
     // This workgroup's steps [t0, t1) of the G * n_qb (head slowest).
     int t0 = 0, t1 = G * n_qb;
     if constexpr (SPLIT) {
@@ -434,29 +478,23 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
         ni = i0 = t0 - h0 * n_qb;
         nq += int64_t(h0) * a.q.head_stride;
         ndo += int64_t(h0) * a.dout.head_stride;
-        nd += int64_t(h0) * a.lse_seqlen;
+        ops += int64_t(h0) * a.lse_seqlen;
     }
     const uint32_t smem_l = lds_addr(smem);
     auto issue_next = [&](int st) FA_INLINE {
         const int q0 = (m_first + ni) * BM;
-        if (q0 + BM <= sq) {
-            qcp.copy_to(smem_l + st * STAGE, nq + int64_t(q0) * qrs, qrs);
-            ocp.copy_to(smem_l + st * STAGE + QTILE, ndo + int64_t(q0) * dors, dors);
-        } else {
-            dma_tile<HD, BM, NT>(smem + st * STAGE, nq, qrs, q0, sq - 1, wave, lane);
-            dma_tile<HD, BM, NT>(smem + st * STAGE + QTILE, ndo, dors, q0, sq - 1, wave, lane);
-        }
-        // Planes 2w and 2w + 1 of the 32 rows by wave w (lanes 0..31 and 32..63).
-        if (wave < 3) {
-            const int64_t pl = min(2 * wave + hh, kDbPlanes - 1);
-            g2l4_to(nd + pl * plane + min(q0 + col, sq - 1), smem_l + st * STAGE + 2 * QTILE + wave * 256);
-        }
+        const uint32_t tile = smem_l + st * STAGE;
+        cp.copy(tile, nq + int64_t(q0) * qrs, qrs, sq - q0);
+        cp.copy(tile + QTILE, ndo + int64_t(q0) * dors, dors, sq - q0);
+        if (wave == 0)  // 32 rows of 32 bytes, two lanes a row
+            g2l16_at(reinterpret_cast<const f16 *>(uniform(ops + q0)), min(lane >> 1, sq - 1 - q0) * 32 + (lane & 1) * 16,
+                     __builtin_amdgcn_readfirstlane(tile + 2 * QTILE));
         --left;
         if (++ni == n_qb) {
             ni = 0;
             nq += a.q.head_stride;
             ndo += a.dout.head_stride;
-            nd += a.lse_seqlen;
+            ops += a.lse_seqlen;
         }
     };
     const int vb0 = rd.a_base + 2 * STAGE + 32 * wave * (HD * 2);
@@ -465,7 +503,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     auto block = [&](int j, int qh0, auto mask_tag) FA_INLINE {
         constexpr bool MASK = decltype(mask_tag)::value;
         const int soff = (j & 1) * STAGE;
-        const float *lf = reinterpret_cast<const float *>(smem + soff + 2 * QTILE);  // planes of 32 rows
+        const char *lf = smem + soff + 2 * QTILE;  // 32 rows' DiffRowOps
         int qb = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff, vb = vb0;
         asm volatile("" : "+v"(qb), "+v"(tb0), "+v"(tb1), "+v"(vb));
         constexpr int PIPE = 2, NG = HD / 16;
@@ -476,56 +514,78 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
             va[g % PIPE] = rd.a_operand_at(smem, vb, g);
         };
         __builtin_amdgcn_sched_barrier(0);
+        // The A operands of the products take row sigma(col) of the tile.
+        int ro = sigma(col) * 32 + soff + 2 * QTILE;
+        asm volatile("" : "+v"(ro));
 #pragma unroll
         for (int g = 0; g < PIPE - 1; ++g) ld(g);
         f32x16 s[2], dp;
-#pragma unroll
-        for (int r8 = 0; r8 < 2; ++r8)  // accumulators 8 r8 + u: row 16 r8 + 8 hh + u
-#pragma unroll
-            for (int u = 0; u < 8; u += 4) {
-                const f32x4 d = *reinterpret_cast<const f32x4 *>(lf + 16 * r8 + 8 * hh + u);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) dp[8 * r8 + u + t] = d[t];
-            }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g + PIPE - 1 < NG) ld(g + PIPE - 1);
-            const int m = g / HG;
-            s[m] = mfma16<BF>(qa[g % PIPE], kreg[g], g % HG == 0 ? zero16() : s[m]);
-            dp = mfma16<BF>(oa[g % PIPE], va[g % PIPE], dp);
+        {
+            int h0 = hh;
+            asm volatile("" : "+v"(h0));  // formed per block, not held
+            const f16x8 w0 = row_weights<BF>(0, h0), w1 = row_weights<BF>(1, h0);
+            const f16x8 lses = lds_ld16(smem, ro), ds = lds_ld16(smem + 16, ro);
+            s[0] = mfma16<BF>(lses, w0, zero16());
+            s[1] = mfma16<BF>(lses, w1, zero16());
+            dp = mfma16<BF>(ds, w0, zero16());
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (g + PIPE - 1 < NG) ld(g + PIPE - 1);
+                const int m = g / HG;
+                s[m] = mfma16<BF>(qa[g % PIPE], kreg[g], s[m]);
+                dp = mfma16<BF>(oa[g % PIPE], va[g % PIPE], dp);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        // lam's sign, where some row of the block has a negative one.
+        const bool neg = __builtin_amdgcn_ballot_w64(*reinterpret_cast<const int16_t *>(smem + 14 + ro) < 0) != 0;
         // Query row c = 16 r8 + u (from qh0 + 8 hh) is live for m_lo <= c < m_hi.
         const int mbase = qh0 + 8 * hh;
         const int m_lo = CAUSAL ? key - causal_off - mbase : -(1 << 30), m_hi = sq - mbase;
         f16x8 pB[2], d1B[2], d2B[2];
 #pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[0][r] = exp2_fast(s[0][r] * cs);
+            s[1][r] = exp2_fast(s[1][r] * cs);
+        }
+        if (neg) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint16_t sign = *reinterpret_cast<const uint16_t *>(lf + (16 * (r >> 3) + 8 * hh + (r & 7)) * 32 + 14);
+                s[1][r] = __uint_as_float(__float_as_uint(s[1][r]) | uint32_t(sign & 0x8000) << 16);
+            }
+        }
+        if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int c = 16 * (r >> 3) + (r & 7);
+                const bool off = c < m_lo || c >= m_hi;
+                s[0][r] = off ? 0.f : s[0][r];
+                s[1][r] = off ? 0.f : s[1][r];
+            }
+        }
+#pragma unroll
+        for (int r8 = 0; r8 < 2; ++r8) {
+            f32x16 mix;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) mix[u] = s[0][8 * r8 + u] - s[1][8 * r8 + u];
+            pB[r8] = pack16<BF>(mix, 0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[0][8 * r8 + u] *= dp[8 * r8 + u];
+            d1B[r8] = pack16<BF>(s[0], 8 * r8);
+        }
+        // dP - D_1 is used up: dP - D_2 takes its place.
+        asm volatile("" : "+v"(d1B[0]), "+v"(d1B[1]), "+v"(pB[0]), "+v"(pB[1]));
+        {
+            int h0 = hh;
+            asm volatile("" : "+v"(h0));
+            dp = mfma16<BF>(lds_ld16(smem + 16, ro), row_weights<BF>(1, h0), dp);
+        }
+#pragma unroll
         for (int r8 = 0; r8 < 2; ++r8) {
 #pragma unroll
-            for (int u4 = 0; u4 < 8; u4 += 4) {
-                const float *row = lf + 16 * r8 + 8 * hh + u4;
-                const f32x4 nd1 = *reinterpret_cast<const f32x4 *>(row), nd2 = *reinterpret_cast<const f32x4 *>(row + 32);
-                const f32x4 l1 = *reinterpret_cast<const f32x4 *>(row + 64), l2 = *reinterpret_cast<const f32x4 *>(row + 96);
-                const f32x4 lam = *reinterpret_cast<const f32x4 *>(row + 128);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int r = 8 * r8 + u4 + t;
-                    float p1 = exp2_fast(fmaf(s[0][r], cs, -l1[t]));
-                    float p2 = exp2_fast(fmaf(s[1][r], cs, -l2[t])) * lam[t];
-                    if constexpr (MASK) {
-                        const int c = 16 * r8 + u4 + t;
-                        const bool off = c < m_lo || c >= m_hi;
-                        p1 = off ? 0.f : p1;
-                        p2 = off ? 0.f : p2;
-                    }
-                    const float x = dp[r];
-                    s[0][r] = p1 - p2;
-                    dp[r] = p1 * x;
-                    s[1][r] = p2 * (x + (nd2[t] - nd1[t]));
-                }
-            }
-            pB[r8] = pack16<BF>(s[0], 8 * r8);
-            d1B[r8] = pack16<BF>(dp, 8 * r8);
+            for (int u = 0; u < 8; ++u) s[1][8 * r8 + u] *= dp[8 * r8 + u];
             d2B[r8] = pack16<BF>(s[1], 8 * r8);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -594,7 +654,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 }
 
 // ---------------------------------------------------------------------------
-// dlam from the rows' -D_2 (plane 1 of the workspace, written by the dQ kernel).
+// dlam from the rows' -D_2 (the start of the workspace, written by the dQ kernel).
 // A lam for each row: one value each, transposed.  One that rows share: one
 // workgroup per head sums its rows in fp64 in a fixed order, and for a lam of
 // all heads the second launch sums the heads.
@@ -606,7 +666,7 @@ __global__ __launch_bounds__(1024) void diff_dlam_rows_kernel(const fa_diff_bwd_
         const int64_t row = i / a.nheads;
         const int h = int(i - row * a.nheads);
         a.dlam.ptr[b * a.dlam.batch_stride + (start + row) * a.dlam.row_stride + h * a.dlam.head_stride] =
-            a.dsum[diff_plane(a) + (int64_t(b) * a.nheads + h) * a.lse_seqlen + row];
+            a.dsum[(int64_t(b) * a.nheads + h) * a.lse_seqlen + row];
     }
 }
 
@@ -622,10 +682,10 @@ __device__ __forceinline__ double block_sum(double x) {
 }
 
 // Head blockIdx.x; the sum goes to dlam (a lam for each head) or, for a lam of
-// all heads, to plane 0 of the workspace, which nothing reads any more.
+// all heads, to sums.
 __global__ __launch_bounds__(1024) void diff_dlam_head_kernel(const fa_diff_bwd_args a, double *const sums) {
     const int h = blockIdx.x;
-    const float *nd2 = a.dsum + diff_plane(a);
+    const float *nd2 = a.dsum;
     double x = 0;
     for (int b = 0; b < a.batch; ++b) {
         const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
@@ -698,8 +758,10 @@ static int check_diff_bwd(const fa_diff_bwd_args *p) {
     if (!a.lse || !a.lam.ptr) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.o, &a.o2, &a.dout, &a.dq, &a.dk, &a.dv})
         if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.dout})
+        if (t->row_stride < 0 || t->row_stride > kDiffMaxRowStride) return FA_ERR_INVALID_ARG;
     if (!split_ws_aligned(a.split_ws)) return FA_ERR_INVALID_ARG;
-    if (!a.dsum || (reinterpret_cast<uintptr_t>(a.dsum) & 7u) || a.dsum_bytes < int64_t(fa_diff_bwd_ws_bytes(&a)))
+    if (!a.dsum || (reinterpret_cast<uintptr_t>(a.dsum) & 31u) || a.dsum_bytes < int64_t(fa_diff_bwd_ws_bytes(&a)))
         return FA_ERR_WORKSPACE;
     return FA_OK;
 }
@@ -751,8 +813,10 @@ static int diff_dkdv_splits(const fa_diff_bwd_args &a) {
     return best;
 }
 
-// Bytes of the planes, rounded so that the heads' fp64 sums, which follow, are aligned.
-static int64_t plane_bytes(const fa_diff_bwd_args &a) { return (kDbPlanes * diff_plane(a) * 4 + 7) & ~int64_t(7); }
+// Bytes of the rows' parts; the heads' fp64 sums follow.
+static int64_t plane_bytes(const fa_diff_bwd_args &a) {
+    return diff_ops_at(a) * 4 + diff_plane(a) * int64_t(sizeof(DiffRowOps));
+}
 
 template <int HD, bool BF>
 static int launch_diff_bwd(fa_diff_bwd_args a, hipStream_t s) {

@@ -332,7 +332,7 @@ typedef struct fa_diff_bwd_args {
     int32_t causal, dtype;
     int32_t dq_rows, dkv_rows;      /* as o_rows and k_rows, and as in fa_bwd_args */
     int32_t *work_order;            /* fa_diff_bwd_order_len(args) int32s for packed batches, or NULL */
-    float *dsum;                    /* workspace of dsum_bytes >= fa_diff_bwd_ws_bytes(args), 8-byte aligned */
+    float *dsum;                    /* workspace of dsum_bytes >= fa_diff_bwd_ws_bytes(args), 32-byte aligned */
     int64_t dsum_bytes;
     void *split_ws;                 /* fa_diff_bwd_split_bytes(args) bytes, 256-byte aligned, as fa_bwd_args.split_ws, or NULL */
     int64_t split_ws_bytes;
