@@ -392,8 +392,12 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     constexpr int NT = kDbThreads, BN = 128, BM = 32;
     constexpr int QTILE = BM * HD * 2, STAGE = 2 * QTILE + 1024;  // Q, dO, row operands
     constexpr int HG = HD / 32, DT = HD / 64;
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + BN * HD * 2];
+    // The last KL of a wave's K operands wait in LDS: with all of them the registers
+    // do not hold what the interleaved block below needs.
+    constexpr int KL = HD == 128 ? 2 : 0, KR = HD / 16 - KL, KAT = 2 * STAGE + BN * HD * 2;
+    __shared__ __attribute__((aligned(16))) char smem[KAT + 4 * KL * 1024];
     __shared__ int ticket;
+    static_assert(2 * (KAT + 4 * KL * 1024) <= 160 * 1024, "two workgroups per CU");
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -447,11 +451,19 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
             g2l16(vp + r * a.v.row_stride + 8 * (c ^ swz<KCH>(pos)), tile + base * 16);
         }
     }
-    f16x8 kreg[HD / 16];
+    f16x8 kreg[KR];
+    const int kat = KAT + wave * KL * 1024 + lane * 16;
     {
         const f16 *kr = kp + int64_t(min(key, sk - 1)) * a.k.row_stride + 8 * hh;
+        const uint32_t keep = flat ? 0u : ~0u;
 #pragma unroll
-        for (int g = 0; g < HD / 16; ++g) kreg[g] = flat ? as_h8(zero_u4()) : *reinterpret_cast<const f16x8 *>(kr + 16 * g);
+        for (int g = 0; g < HD / 16; ++g) {
+            const f16x8 x = as_h8(ldg16(kr + 16 * g) & keep);
+            if (g < KR)
+                kreg[g] = x;
+            else
+                *reinterpret_cast<f16x8 *>(smem + kat + (g - KR) * 1024) = x;
+        }
     }
     f32x16 dk[HD / 32], dv[HD / 32];
 #pragma unroll
@@ -506,102 +518,133 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
         const char *lf = smem + soff + 2 * QTILE;  // 32 rows' DiffRowOps
         int qb = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff, vb = vb0;
         asm volatile("" : "+v"(qb), "+v"(tb0), "+v"(tb1), "+v"(vb));
-        constexpr int PIPE = 2, NG = HD / 16;
-        f16x8 qa[PIPE], oa[PIPE], va[PIPE];
-        auto ld = [&](int g) FA_INLINE {
-            qa[g % PIPE] = rd.a_operand_at(smem, qb, g);
-            oa[g % PIPE] = rd.a_operand_at(smem + QTILE, qb, g);
-            va[g % PIPE] = rd.a_operand_at(smem, vb, g);
-        };
-        __builtin_amdgcn_sched_barrier(0);
+        constexpr int PIPE = 2, PS = 4, PT = 3, NG = HD / 16;  // operands read ahead: dP, scores, dK and dV
         // The A operands of the products take row sigma(col) of the tile.
         int ro = sigma(col) * 32 + soff + 2 * QTILE;
         asm volatile("" : "+v"(ro));
-#pragma unroll
-        for (int g = 0; g < PIPE - 1; ++g) ld(g);
         f32x16 s[2], dp;
+        // Query row c = 16 r8 + u (from qh0 + 8 hh) is live for m_lo <= c < m_hi.
+        const int mbase = qh0 + 8 * hh;
+        const int m_lo = CAUSAL ? key - causal_off - mbase : -(1 << 30), m_hi = sq - mbase;
+        // Rows with a negative lam: bit l for the row of lane l, sigma(l); row 16 r8 + 8 hh + u is lane's
+        // 16 r8 + 8 (u / 4) + 4 hh + u % 4.
+        const uint64_t neg = __builtin_amdgcn_ballot_w64(*reinterpret_cast<const int16_t *>(smem + 14 + ro) < 0);
+        auto exps = [&](int m, int r0, int n) FA_INLINE {
+#pragma unroll
+            for (int r = r0; r < r0 + n; ++r) {
+                s[m][r] = exp2_fast(s[m][r] * cs);
+                if constexpr (MASK) {
+                    const int c = 16 * (r >> 3) + (r & 7);
+                    s[m][r] = c < m_lo || c >= m_hi ? 0.f : s[m][r];
+                }
+            }
+        };
         {
             int h0 = hh;
             asm volatile("" : "+v"(h0));  // formed per block, not held
             const f16x8 w0 = row_weights<BF>(0, h0), w1 = row_weights<BF>(1, h0);
-            const f16x8 lses = lds_ld16(smem, ro), ds = lds_ld16(smem + 16, ro);
+            const f16x8 lses = lds_ld16(smem, ro);
+            // Step u of the scores: map u % 2, K step u / 2 of its channels.
+            f16x8 op[PS];
+            auto ldq = [&](int u) FA_INLINE { op[u % PS] = rd.a_operand_at(smem, qb, (u & 1) * HG + (u >> 1)); };
+#pragma unroll
+            for (int u = 0; u < PS - 1; ++u) ldq(u);
+            f16x8 kl[KL > 0 ? KL : 1];
+#pragma unroll
+            for (int i = 0; i < KL; ++i) kl[i] = lds_ld16(smem + i * 1024, kat);
             s[0] = mfma16<BF>(lses, w0, zero16());
             s[1] = mfma16<BF>(lses, w1, zero16());
-            dp = mfma16<BF>(ds, w0, zero16());
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                if (u + PS - 1 < NG) ldq(u + PS - 1);
+                const int g = (u & 1) * HG + (u >> 1);
+                s[u & 1] = mfma16<BF>(op[u % PS], g < KR ? kreg[g < KR ? g : 0] : kl[g < KR ? 0 : g - KR], s[u & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // dP, with the exponentials beside its products.
+            f16x8 oa[PIPE], va[PIPE];
+            auto ldo = [&](int g) FA_INLINE {
+                oa[g % PIPE] = rd.a_operand_at(smem + QTILE, qb, g);
+                va[g % PIPE] = rd.a_operand_at(smem, vb, g);
+            };
+#pragma unroll
+            for (int g = 0; g < PIPE - 1; ++g) ldo(g);
+            asm volatile("" : "+v"(h0));
+            dp = mfma16<BF>(lds_ld16(smem + 16, ro), row_weights<BF>(0, h0), zero16());
+#pragma unroll
             for (int g = 0; g < NG; ++g) {
-                if (g + PIPE - 1 < NG) ld(g + PIPE - 1);
-                const int m = g / HG;
-                s[m] = mfma16<BF>(qa[g % PIPE], kreg[g], s[m]);
+                if (g + PIPE - 1 < NG) ldo(g + PIPE - 1);
                 dp = mfma16<BF>(oa[g % PIPE], va[g % PIPE], dp);
+                exps(g * 2 / NG, 32 / NG * (g % (NG / 2)), 32 / NG);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // lam's sign, where some row of the block has a negative one.
-        const bool neg = __builtin_amdgcn_ballot_w64(*reinterpret_cast<const int16_t *>(smem + 14 + ro) < 0) != 0;
-        // Query row c = 16 r8 + u (from qh0 + 8 hh) is live for m_lo <= c < m_hi.
-        const int mbase = qh0 + 8 * hh;
-        const int m_lo = CAUSAL ? key - causal_off - mbase : -(1 << 30), m_hi = sq - mbase;
-        f16x8 pB[2], d1B[2], d2B[2];
+        f16x8 pB[2], d1B[2], d2B[2], tr[PT];
+        // Transposed operand u of dV (Q = 0) or dK: channel tile u / 2, query step u % 2.
+        auto ldt = [&](int n, int q, int u) FA_INLINE {
+            tr[n % PT] = rd.tr_operand_at(smem + (q ? 0 : QTILE) + 16 * (u & 1) * (HD * 2), tb0, tb1, u >> 1);
+        };
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[0][r] = exp2_fast(s[0][r] * cs);
-            s[1][r] = exp2_fast(s[1][r] * cs);
-        }
-        if (neg) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const uint16_t sign = *reinterpret_cast<const uint16_t *>(lf + (16 * (r >> 3) + 8 * hh + (r & 7)) * 32 + 14);
-                s[1][r] = __uint_as_float(__float_as_uint(s[1][r]) | uint32_t(sign & 0x8000) << 16);
-            }
-        }
-        if constexpr (MASK) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int c = 16 * (r >> 3) + (r & 7);
-                const bool off = c < m_lo || c >= m_hi;
-                s[0][r] = off ? 0.f : s[0][r];
-                s[1][r] = off ? 0.f : s[1][r];
-            }
-        }
+        for (int n = 0; n < PT - 1; ++n) ldt(n, 1, n);
 #pragma unroll
         for (int r8 = 0; r8 < 2; ++r8) {
-            f32x16 mix;
+            f32x16 x;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) mix[u] = s[0][8 * r8 + u] - s[1][8 * r8 + u];
-            pB[r8] = pack16<BF>(mix, 0);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s[0][8 * r8 + u] *= dp[8 * r8 + u];
-            d1B[r8] = pack16<BF>(s[0], 8 * r8);
+            for (int u = 0; u < 8; ++u) x[u] = s[0][8 * r8 + u] * dp[8 * r8 + u];
+            d1B[r8] = pack16<BF>(x, 0);
+            asm volatile("" : "+v"(d1B[r8]));
         }
         // dP - D_1 is used up: dP - D_2 takes its place.
-        asm volatile("" : "+v"(d1B[0]), "+v"(d1B[1]), "+v"(pB[0]), "+v"(pB[1]));
         {
             int h0 = hh;
             asm volatile("" : "+v"(h0));
             dp = mfma16<BF>(lds_ld16(smem + 16, ro), row_weights<BF>(1, h0), dp);
         }
-#pragma unroll
-        for (int r8 = 0; r8 < 2; ++r8) {
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s[1][8 * r8 + u] *= dp[8 * r8 + u];
-            d2B[r8] = pack16<BF>(s[1], 8 * r8);
-        }
         __builtin_amdgcn_sched_barrier(0);
-        constexpr int NT2 = 2 * (HD / 32);
-        f16x8 ta[PIPE], tq[PIPE];
-        auto ldt = [&](int t) FA_INLINE {
-            ta[t % PIPE] = rd.tr_operand_at(smem + QTILE + 16 * (t & 1) * (HD * 2), tb0, tb1, t >> 1);
-            tq[t % PIPE] = rd.tr_operand_at(smem + 16 * (t & 1) * (HD * 2), tb0, tb1, t >> 1);
+        // dK of map 1 beside P, dV beside dS_2, dK of map 2.
+        constexpr int N1 = 2 * DT, N2 = N1 + 2 * (HD / 32), N3 = N2 + 2 * DT;
+        auto ldn = [&](int n) FA_INLINE {
+            if (n < N1)
+                ldt(n, 1, n);
+            else if (n < N2)
+                ldt(n, 0, n - N1);
+            else
+                ldt(n, 1, n - N2 + N1);
         };
+        if (neg != 0) {
+            const uint32_t m = uint32_t(neg) >> (4 * hh);
 #pragma unroll
-        for (int t = 0; t < PIPE - 1; ++t) ldt(t);
+            for (int r = 0; r < 16; ++r)
+                s[1][r] = __uint_as_float(__float_as_uint(s[1][r]) |
+                                          (m << (31 - 16 * (r >> 3) - 8 * (r >> 2 & 1) - (r & 3)) & 0x80000000u));
+        }
 #pragma unroll
-        for (int t = 0; t < NT2; ++t) {
-            if (t + PIPE - 1 < NT2) ldt(t + PIPE - 1);
-            dv[t >> 1] = mfma16<BF>(ta[t % PIPE], pB[t & 1], dv[t >> 1]);
-            dk[t >> 1] = mfma16<BF>(tq[t % PIPE], (t >> 1) < DT ? d1B[t & 1] : d2B[t & 1], dk[t >> 1]);
+        for (int n = 0; n < N1; ++n) {
+            if (n + PT - 1 < N3) ldn(n + PT - 1);
+            dk[n >> 1] = mfma16<BF>(tr[n % PT], d1B[n & 1], dk[n >> 1]);
+            constexpr int E = 16 / N1;
+#pragma unroll
+            for (int r = E * n; r < E * n + E; ++r) s[0][r] -= s[1][r];
+            if (E * (n + 1) % 8 == 0) pB[E * (n + 1) / 8 - 1] = pack16<BF>(s[0], E * (n + 1) - 8);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = N1; n < N2; ++n) {
+            if (n + PT - 1 < N3) ldn(n + PT - 1);
+            const int u = n - N1;
+            dv[u >> 1] = mfma16<BF>(tr[n % PT], pB[u & 1], dv[u >> 1]);
+            constexpr int E = 16 / (N2 - N1);
+#pragma unroll
+            for (int r = E * u; r < E * u + E; ++r) s[1][r] *= dp[r];
+            if (E * (u + 1) % 8 == 0) d2B[E * (u + 1) / 8 - 1] = pack16<BF>(s[1], E * (u + 1) - 8);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = N2; n < N3; ++n) {
+            if (n + PT - 1 < N3) ldn(n + PT - 1);
+            const int u = n - N2 + N1;
+            dk[u >> 1] = mfma16<BF>(tr[n % PT], d2B[u & 1], dk[u >> 1]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };

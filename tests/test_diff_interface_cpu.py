@@ -193,7 +193,8 @@ def test_workspace_sizes(lib):
     assert size(num_splits=2, cache_capacity=256) == 256 + 4 * 2 * 4 * (8 + 512)
     assert lib.fa_diff_kvcache_ws_bytes(None) == 0 and lib.fa_kvpages_ws_bytes(None) == 0
     b = _bwd()
-    assert lib.fa_diff_bwd_ws_bytes(ctypes.byref(b)) == 5 * 4 * 8 * 4 + 4 * 8
+    # 4 bytes (-D_2) and 32 (the products' operands) a row of 4 heads x 8 queries, 8 a head.
+    assert lib.fa_diff_bwd_ws_bytes(ctypes.byref(b)) == 4 * 8 * (4 + 32) + 4 * 8
     assert lib.fa_diff_bwd_split_bytes(ctypes.byref(b)) == 0
 
 
