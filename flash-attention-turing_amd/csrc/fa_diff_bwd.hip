@@ -87,12 +87,13 @@ __host__ __device__ __forceinline__ int64_t diff_dkdv_items(const fa_diff_bwd_ar
 __host__ __device__ __forceinline__ int64_t diff_dkdv_count_bytes(int64_t items) { return (items * 4 + 255) & ~int64_t(255); }
 
 template <int HD, bool BF, bool CAUSAL>
-__global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bwd_args a, const int num_m_blocks,
+__global__ __launch_bounds__(kDbThreads, HD == 64 ? 3 : 2) void diff_dq_kernel(const fa_diff_bwd_args a, const int num_m_blocks,
                                                                 const int lg) {
     constexpr int NT = kDbThreads, BM = 128, BN = 64;
     constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
     constexpr int HG = HD / 32;  // MFMA K steps of one map's channels
     constexpr int PIPE = 3;
+    constexpr int KT = HD == 64 ? 1 : 2;  // 32-key tiles at a time
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     d2 = sum_xor32(d2);
     d1 = fmaf(lam, d2, sum_xor32(d1));
     // All keys of the wave's rows in block 0: D_m from that block.
-    const bool one = (CAUSAL ? min(sk, q_lo + 32 + causal_off) : sk) <= BN;
+    const bool one = (CAUSAL ? min(sk, q_lo + 32 + causal_off) : sk) <= 32 * KT;
     if (one) d1 = d2 = 0.f;
     float ds2_sum = 0.f;  // this lane half's sum of P_2 (dP - D_2)
 
@@ -205,91 +206,97 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
         asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
         const int lim = (CAUSAL ? min(sk - 1, qi + causal_off) : sk - 1) - n0;
         f16x8 op[PIPE];
-        f32x16 dp[2];
-        // dP^T from -D_1 on, so that the product comes out as dP - D_1.
-        {
-            float nd = -d1;
-            asm volatile("" : "+v"(nd));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[0][i] = dp[1][i] = nd;
-        }
-        auto rd_dp = [&](int u) FA_INLINE {
-            op[u % PIPE] = rd.a_operand_at(smem + TILE + 32 * (u & 1) * (HD * 2), ab, u >> 1);
-        };
-        __builtin_amdgcn_sched_barrier(0);
+        for (int sub = 0; sub < BN / 32; sub += KT) {
+            f32x16 dp[KT];
+            // dP^T from -D_1 on, so that the product comes out as dP - D_1.
+            {
+                float nd = -d1;
+                asm volatile("" : "+v"(nd));
 #pragma unroll
-        for (int u = 0; u < PIPE - 1; ++u) rd_dp(u);
+                for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int u = 0; u < HD / 8; ++u) {
-            if (u + PIPE - 1 < HD / 8) rd_dp(u + PIPE - 1);
-            dp[u & 1] = mfma16<BF>(op[u % PIPE], doB[u >> 1], dp[u & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f32x16 s[2];
-            auto rd_k = [&](int u) FA_INLINE {
-                op[u % PIPE] = rd.a_operand_at(smem + 32 * (u & 1) * (HD * 2), ab, m * HG + (u >> 1));
+                    for (int i = 0; i < 16; ++i) dp[t][i] = nd;
+            }
+            auto rd_dp = [&](int u) FA_INLINE {
+                op[u % PIPE] = rd.a_operand_at(smem + TILE + 32 * (sub + u % KT) * (HD * 2), ab, u / KT);
             };
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < PIPE - 1; ++u) rd_k(u);
+            for (int u = 0; u < PIPE - 1; ++u) rd_dp(u);
 #pragma unroll
-            for (int u = 0; u < 2 * HG; ++u) {
-                if (u + PIPE - 1 < 2 * HG) rd_k(u + PIPE - 1);
-                s[u & 1] = mfma16<BF>(op[u % PIPE], qB[m * HG + (u >> 1)], u < 2 ? zero16() : s[u & 1]);
+            for (int u = 0; u < KT * HD / 16; ++u) {
+                if (u + PIPE - 1 < KT * HD / 16) rd_dp(u + PIPE - 1);
+                dp[u % KT] = mfma16<BF>(op[u % PIPE], doB[u / KT], dp[u % KT]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const float lse = m == 0 ? lse1 : lse2;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int m = 0; m < 2; ++m) {
+                f32x16 s[KT];
+                auto rd_k = [&](int u) FA_INLINE {
+                    op[u % PIPE] = rd.a_operand_at(smem + 32 * (sub + u % KT) * (HD * 2), ab, m * HG + u / KT);
+                };
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float x = exp2_fast(fmaf(s[t][r], cs, -lse));
-                    if constexpr (MASK) x = t * 32 + acc_lrow(r, hh) > lim ? 0.f : x;
-                    s[t][r] = x;
+                for (int u = 0; u < PIPE - 1 && u < KT * HG; ++u) rd_k(u);
+#pragma unroll
+                for (int u = 0; u < KT * HG; ++u) {
+                    if (u + PIPE - 1 < KT * HG) rd_k(u + PIPE - 1);
+                    s[u % KT] = mfma16<BF>(op[u % PIPE], qB[m * HG + u / KT], u < KT ? zero16() : s[u % KT]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            float e = m == 0 ? 0.f : d1 - d2;
-            if constexpr (MASK) {
-                if (one) {
-                    float d = 0.f;
+                // dQ_m^T += K_m^T dS_m^T: step u is key step u / DT, channel tile u % DT of the map;
+                // the first reads go out before the exponentials, which cover their latency.
+                constexpr int DT = HD / 64;  // 32-channel tiles of a map
+                auto rd_dq = [&](int u) FA_INLINE {
+                    op[u % PIPE] = rd.tr_operand_at(smem + 16 * (2 * sub + u / DT) * (HD * 2), tb0, tb1, m * DT + u % DT);
+                };
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int u = 0; u < PIPE - 1; ++u) rd_dq(u);
+                const float lse = m == 0 ? lse1 : lse2;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) d = fmaf(s[t][r], dp[t][r], d);
-                    d = sum_xor32(d);
-                    e = -d;
-                    (m == 0 ? d1 : d2) = d;
-                }
-            }
-            float sum = 0.f;
+                for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                    for (int r = 0; r < 16; ++r) {
+                        float x = exp2_fast(fmaf(s[t][r], cs, -lse));
+                        if constexpr (MASK) x = (sub + t) * 32 + acc_lrow(r, hh) > lim ? 0.f : x;
+                        s[t][r] = x;
+                    }
+                float e = m == 0 ? 0.f : d1 - d2;
+                if constexpr (MASK) {
+                    if (one && sub == 0) {
+                        float d = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    if (m == 0 && !MASK) {
-                        s[t][r] *= dp[t][r];
-                    } else {
-                        s[t][r] *= dp[t][r] + e;
-                        if (m == 1) sum += s[t][r];
+                        for (int t = 0; t < KT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) d = fmaf(s[t][r], dp[t][r], d);
+                        d = sum_xor32(d);
+                        e = -d;
+                        (m == 0 ? d1 : d2) = d;
                     }
                 }
-            if (m == 1) ds2_sum += sum;
-            f16x8 dsB[4];
+                float sum = 0.f;
 #pragma unroll
-            for (int gg = 0; gg < 4; ++gg) dsB[gg] = pack16<BF>(s[gg >> 1], 8 * (gg & 1));
-            // dQ_m^T += K_m^T dS_m^T: step u is key step u / HG, channel tile u % (HG / 1) of the map.
-            constexpr int DT = HD / 64;  // 32-channel tiles of a map
-            auto rd_dq = [&](int u) FA_INLINE {
-                op[u % PIPE] = rd.tr_operand_at(smem + 16 * (u / DT) * (HD * 2), tb0, tb1, m * DT + u % DT);
-            };
-            __builtin_amdgcn_sched_barrier(0);
+                for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int u = 0; u < PIPE - 1; ++u) rd_dq(u);
+                    for (int r = 0; r < 16; ++r) {
+                        if (m == 0 && !MASK) {
+                            s[t][r] *= dp[t][r];
+                        } else {
+                            s[t][r] *= dp[t][r] + e;
+                            if (m == 1) sum += s[t][r];
+                        }
+                    }
+                if (m == 1) ds2_sum += sum;
+                f16x8 dsB[2 * KT];
 #pragma unroll
-            for (int u = 0; u < 4 * DT; ++u) {
-                if (u + PIPE - 1 < 4 * DT) rd_dq(u + PIPE - 1);
-                dq[m * DT + u % DT] = mfma16<BF>(op[u % PIPE], dsB[u / DT], dq[m * DT + u % DT]);
+                for (int gg = 0; gg < 2 * KT; ++gg) dsB[gg] = pack16<BF>(s[gg >> 1], 8 * (gg & 1));
                 __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2 * KT * DT; ++u) {
+                    if (u + PIPE - 1 < 2 * KT * DT) rd_dq(u + PIPE - 1);
+                    dq[m * DT + u % DT] = mfma16<BF>(op[u % PIPE], dsB[u / DT], dq[m * DT + u % DT]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     };
@@ -298,7 +305,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dq_kernel(const fa_diff_bw
     // a wave's rows see block 0 alone, that block is taken as a masked one.
     int n_full = min(n_blocks, sk / BN);
     if (CAUSAL) n_full = min(n_full, max(0, (m0 + causal_off + 1) / BN));
-    if (n_full == 1 && (CAUSAL ? min(sk, m0 + 32 + causal_off) : sk) <= BN) n_full = 0;
+    if (n_full == 1 && (CAUSAL ? min(sk, m0 + 32 + causal_off) : sk) <= 32 * KT) n_full = 0;
     for (int nb = 0; nb < n_full; ++nb) block(nb, std::false_type{});
     for (int nb = n_full; nb < n_blocks; ++nb) block(nb, std::true_type{});
 

@@ -229,7 +229,7 @@ struct DiffTiles {
 // then has a CU to itself, with two waves on each SIMD and half the chain of
 // blocks.
 template <int HD, bool BF, bool CAUSAL, bool CACHE, int NG>
-__global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : 2) void diff_fwd_kernel(const DiffFwd p,
+__global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) void diff_fwd_kernel(const DiffFwd p,
                                                                                      const int num_m_blocks, const int lg) {
     constexpr int NT = kDiffThreads, BN = kDiffBN;
     constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
