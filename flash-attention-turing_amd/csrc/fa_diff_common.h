@@ -118,6 +118,12 @@ __device__ __forceinline__ int scalar_load(const int32_t *p) {
     return v;
 }
 
+// The same through the compiler, which waits where the value is used; for memory
+// that nothing writes while the kernel runs.
+__device__ __forceinline__ int scalar_load_ahead(const int32_t *p) {
+    return *(const __attribute__((address_space(4))) int32_t *)uniform(p);
+}
+
 // g2l16 (fa_common.h) with the address as a wave-uniform base and a 32-bit byte
 // offset per lane: no 64-bit address is formed or held per lane and copy.  Same
 // waiting rules.
@@ -169,14 +175,12 @@ struct DiffCopier {
     }
 };
 
-// Page at table entry pg of sequence b, checked: one outside the cache becomes
-// page 0 and is reported, so that no access leaves the cache.
-__device__ __forceinline__ int checked_page(const int32_t *table, int64_t stride, int b, int pg, int num_pages,
-                                            int32_t *status) {
-    const int blk = scalar_load(table + int64_t(b) * stride + pg);
-    if (blk >= 0 && blk < num_pages) return blk;
-    if (status && (threadIdx.x & 63) == 0) atomicOr(status, FA_KV_BAD_PAGE);
-    return 0;
+// A table's entry, checked: a page outside the cache becomes page 0 and is
+// reported, so that no access leaves the cache.
+__device__ __forceinline__ int checked_page(int blk, int num_pages, int32_t *status) {
+    const bool ok = blk >= 0 && blk < num_pages;
+    if (!ok && status && (threadIdx.x & 63) == 0) atomicOr(status, FA_KV_BAD_PAGE);
+    return __builtin_amdgcn_readfirstlane(ok ? blk : 0);
 }
 
 }  // namespace fa

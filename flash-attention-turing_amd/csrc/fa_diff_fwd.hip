@@ -88,18 +88,37 @@ struct DiffWork {
     bool live;
 };
 
-template <bool CAUSAL, bool CACHE>
+// The sequence of rank r when a cache's sequences are sorted by length, longest
+// first (as they come where a wave has no lane for each).
+__device__ __forceinline__ int diff_nth_longest(const int32_t *lens, int batch, int r) {
+    if (batch == 1 || batch > 64) return r;
+    const int lane = threadIdx.x & 63, mine = lens[min(lane, batch - 1)];
+    int rank = 0;
+    for (int j = 0; j < batch; ++j) {
+        const int other = __builtin_amdgcn_readlane(mine, j);
+        rank += other > mine || (other == mine && j < lane);
+    }
+    return __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(lane < batch && rank == r)) - 1;
+}
+
+template <bool CAUSAL, bool CACHE, int NG>
 __device__ __forceinline__ DiffWork diff_work(const DiffFwd &p, int num_m_blocks, int lg, int bid) {
     const fa_diff_fwd_args &a = p.a;
     DiffWork w;
     const int gp = 1 << lg, packs = a.nheads >> lg;
     int mb;
-    w.P = kDiffRows >> lg;
+    w.P = kDiffRows / NG >> lg;
     if (a.work_order && a.cu_seqlens_q) {
         const int it = a.work_order[bid / packs];
         w.b = __builtin_amdgcn_readfirstlane(it / num_m_blocks);
         mb = __builtin_amdgcn_readfirstlane(it - w.b * num_m_blocks);
         w.h = (bid % packs) * gp;
+    } else if (CACHE && NG == 2) {
+        const int per = num_m_blocks * packs, r = bid / per;
+        w.b = __builtin_amdgcn_readfirstlane(diff_nth_longest(p.cache_seqlens, a.batch, r));
+        mb = (bid - r * per) / packs;
+        w.h = (bid - r * per - mb * packs) * gp;
+        if (CAUSAL) mb = num_m_blocks - 1 - mb;
     } else {
         const int bp_count = a.batch * packs, bp = bid % bp_count;
         mb = bid / bp_count;
@@ -200,65 +219,74 @@ __device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const Diff
     }
 }
 
-// First rows of K and V tiles of a dense tensor or of the pages of a cache.  A
-// tile lies in one page; its page's id is read once a page.
+// First rows of K and V tiles of a dense tensor or of the pages of a cache, block
+// after block.  A tile lies in one page (pages are multiples of 64 tokens).
 template <bool CACHE>
 struct DiffTiles {
-    int page = -1, blk = 0;
-    __device__ __forceinline__ void at(const DiffFwd &p, const DiffWork &w, int n0, const f16 *&k, const f16 *&v) {
+    const f16 *k, *v;  // the next block
+    int left = 0;      // blocks left in its page
+    int next = 0;      // the table's entry after that page
+    __device__ __forceinline__ void init(const DiffFwd &p, const DiffWork &w) {
+        k = w.kp;
+        v = w.vp;
+        if (CACHE && p.block_table) next = scalar_load_ahead(p.block_table + int64_t(w.b) * p.block_table_stride);
+    }
+    // Goes to block n0 / kDiffBN, which follows the one before.
+    __device__ __forceinline__ void step(const DiffFwd &p, const DiffWork &w, int n0) {
         const fa_diff_fwd_args &a = p.a;
-        if (CACHE && p.block_table) {
-            const int pg = n0 / p.page;
-            if (pg != page) {
-                page = pg;
-                blk = checked_page(p.block_table, p.block_table_stride, w.b, pg, p.num_pages, p.status);
-            }
-            const int64_t row = n0 - pg * p.page;
-            k = w.kp + int64_t(blk) * a.k.batch_stride + row * a.k.row_stride;
-            v = w.vp + int64_t(blk) * a.v.batch_stride + row * a.v.row_stride;
-        } else {
-            k = w.kp + int64_t(n0) * a.k.row_stride;
-            v = w.vp + int64_t(n0) * a.v.row_stride;
+        if (CACHE && p.block_table && left-- == 0) {
+            const int blk = checked_page(next, p.num_pages, p.status);
+            k = w.kp + int64_t(blk) * a.k.batch_stride;
+            v = w.vp + int64_t(blk) * a.v.batch_stride;
+            left = p.page / kDiffBN - 1;
+            // Loaded a page ahead: its latency would stall every wave once a page.
+            const int last = (w.n_keys - 1) / p.page;
+            next = scalar_load_ahead(p.block_table + int64_t(w.b) * p.block_table_stride + min(n0 / p.page + 1, last));
+        } else if (n0 > 0) {
+            k += kDiffBN * a.k.row_stride;
+            v += kDiffBN * a.v.row_stride;
         }
     }
 };
 
-// NG = 1: four waves of 32 rows, two workgroups per CU, on grids that fill the
-// chip.  NG = 2: two groups of four waves over the same rows take the key blocks
-// in turn, each through LDS stages of its own, and merge through LDS; a workgroup
-// then has a CU to itself, with two waves on each SIMD and half the chain of
-// blocks.
+// NG = 1: four waves of 32 rows each.  NG = 2, for grids that do not fill the chip:
+// 64 rows, and the two pairs of waves take the two halves of each key block and
+// merge through LDS, so that there are twice the workgroups with half the chain
+// of products each.  Of these the first workgroup on a CU gets one of the longest
+// items and the second one of the shortest; a cache's sequences are sorted by
+// length for it.  launch_diff_fwd has what both measured.
 template <int HD, bool BF, bool CAUSAL, bool CACHE, int NG>
-__global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) void diff_fwd_kernel(const DiffFwd p,
-                                                                                     const int num_m_blocks, const int lg) {
+__global__ __launch_bounds__(kDiffThreads, HD == 64 ? 3 : 2) void diff_fwd_kernel(const DiffFwd p, const int num_m_blocks,
+                                                                                    const int lg, const int cus) {
     constexpr int NT = kDiffThreads, BN = kDiffBN;
     constexpr int TILE = BN * HD * 2, STAGE = 2 * TILE;
     constexpr int HG = HD / 32;  // MFMA K steps of one map's channels
     const fa_diff_fwd_args &a = p.a;
-    __shared__ __attribute__((aligned(16))) char smem[NG * 2 * STAGE];
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
-    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wave = NG == 1 ? wave8 : wave8 & 3, grp = NG == 1 ? 0 : wave8 >> 2;
-    const DiffWork w = diff_work<CAUSAL, CACHE>(p, num_m_blocks, lg, blockIdx.x);
+    const int wave4 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = NG == 1 ? wave4 : wave4 & 1, grp = NG == 1 ? 0 : wave4 >> 1;
+    int bid = blockIdx.x;
+    if (NG == 2 && int(gridDim.x) <= 2 * cus && bid >= cus) bid = gridDim.x - 1 - (bid - cus);
+    const DiffWork w = diff_work<CAUSAL, CACHE, NG>(p, num_m_blocks, lg, bid);
     if (!w.live) return diff_pad_lse(a, w, lg);
     const int n_blocks = (w.n_keys + BN - 1) / BN;
     const float cscale = uniform(fabsf(a.softmax_scale) * kLog2e);
 
     DiffCopier<HD, BN, NT> cp;
-    cp.init(wave, lane);
+    cp.init(wave4, lane);
     DiffTiles<CACHE> tiles;
-    const int g0 = grp * 2 * STAGE;  // the group's stages
+    tiles.init(p, w);
     auto issue = [&](int nb, int st) FA_INLINE {
-        const f16 *k, *v;
-        tiles.at(p, w, nb * BN, k, v);
-        const uint32_t tile = lds_addr(smem) + g0 + st * STAGE;
-        cp.copy(tile, k, a.k.row_stride, w.sk - nb * BN);
-        cp.copy(tile + TILE, v, a.v.row_stride, w.sk - nb * BN);
+        tiles.step(p, w, nb * BN);
+        const uint32_t tile = lds_addr(smem) + st * STAGE;
+        cp.copy(tile, tiles.k, a.k.row_stride, w.sk - nb * BN);
+        cp.copy(tile + TILE, tiles.v, a.v.row_stride, w.sk - nb * BN);
     };
 
     // The wave's 32 rows: head h, positions from q_lo.
-    const int h = w.h + (wave >> (2 - lg));
+    const int h = w.h + (wave >> (3 - NG - lg));
     const int q_lo = w.m0 + 32 * (wave & ((w.P >> 5) - 1));
     const int qi = q_lo + (lane & 31);
     f16x8 qB[HD / 16];
@@ -274,14 +302,13 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
     TileReader<HD> rd;
     rd.init(lane);
 
-    // Iteration it: block NG * it + grp.
-    auto block = [&](int it, auto mask_tag) FA_INLINE {
+    auto block = [&](int nb, auto mask_tag) FA_INLINE {
         constexpr bool MASK = decltype(mask_tag)::value;
-        const int buf = it & 1, nb = NG * it + grp, n0 = nb * BN;
+        const int buf = nb & 1, n0 = nb * BN + 32 * grp;
         wait_vmem();
         __syncthreads();  // block nb is in LDS; every wave is done with stage buf ^ 1
-        if (nb + NG < n_blocks) issue(nb + NG, buf ^ 1);
-        if (NG > 1 && MASK && nb >= n_blocks) return;
+        if (nb + 1 < n_blocks) issue(nb + 1, buf ^ 1);
+        if (NG > 1 && MASK && n0 >= w.sk) return;
         if (CAUSAL && MASK && n0 > q_lo + 31 + w.causal_off) return;  // no visible key for this wave
         if (q_lo >= w.sq) return;
         // 32 keys at a time: the scores of both maps take as many registers as
@@ -290,14 +317,14 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
         // the lane's bases with the stage added once per block (opaque, so that
         // no read address is held in registers through the loop).
         constexpr int PIPE = 3, NS = 2 * HG, NPV = 2 * (HD / 32);
-        const int soff = g0 + buf * STAGE;
+        const int soff = buf * STAGE + 32 * grp * (HD * 2);
         static_assert(STAGE % 512 == 0, "stage offsets must be multiples of 512 bytes");
         int ab = rd.a_base + soff, tb0 = rd.tr_base[0] + soff, tb1 = rd.tr_base[1] + soff;
         asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
         f16x8 op[PIPE];
         const int lim = (CAUSAL ? min(w.sk - 1, qi + w.causal_off) : w.sk - 1) - n0;
 #pragma unroll
-        for (int sub = 0; sub < BN / 32; ++sub) {
+        for (int sub = 0; sub < BN / 32 / NG; ++sub) {
             // Step u: map u % 2, K step u / 2 of the map's channels.
             f32x16 s[2];
             auto rd_k = [&](int u) FA_INLINE {
@@ -337,10 +364,9 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
     // Iterations whose blocks need no mask for any wave of the workgroup come first.
     int n_full = min(n_blocks, w.sk / BN);
     if (CAUSAL) n_full = min(n_full, max(0, (w.m0 + w.causal_off + 1) / BN));
-    if (grp < n_blocks) issue(grp, 0);
-    const int it_full = n_full / NG, n_it = (n_blocks + NG - 1) / NG;
-    for (int it = 0; it < it_full; ++it) block(it, std::false_type{});
-    for (int it = it_full; it < n_it; ++it) block(it, std::true_type{});
+    if (n_blocks > 0) issue(0, 0);
+    for (int nb = 0; nb < n_full; ++nb) block(nb, std::false_type{});
+    for (int nb = n_full; nb < n_blocks; ++nb) block(nb, std::true_type{});
 
     sum[0] = sum_xor32(sum[0]);
     sum[1] = sum_xor32(sum[1]);
@@ -350,10 +376,11 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
         // Each group finishes half of the channels of both maps: it hands the other
         // half, and its maxima and sums, to the other group.
         constexpr int H = HD / 64;  // 32-channel tiles of a half
-        __shared__ f32x2 ml[2][2][kDiffRows];
-        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);  // [group][2 maps * 4 H][NT threads]
-        const int t4 = tid & (NT - 1), r = 32 * wave + (lane & 31);
-        static_assert(2 * 2 * 4 * H * NT * 16 <= NG * 2 * STAGE, "the exchange fits the stages");
+        __shared__ f32x2 ml[2][2][kDiffRows / 2];
+        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);  // [group][2 maps * 4 H][GT threads]
+        constexpr int GT = NT / 2;
+        const int t4 = tid & (GT - 1), r = 32 * wave + (lane & 31);
+        static_assert(2 * 2 * 4 * H * GT * 16 <= 2 * STAGE, "the exchange fits the stages");
         __syncthreads();  // every wave is done with the tiles
         if (hh == 0) {
             ml[grp][0][r] = f32x2{mx[0], sum[0]};
@@ -367,7 +394,7 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
                 for (int i = 0; i < 4 * H; ++i) {
                     const f32x16 &t = o[m][(1 - GRP) * H + i / 4];
                     const int e = 4 * (i & 3);
-                    xo[((GRP * 2 + m) * 4 * H + i) * NT + t4] = f32x4{t[e], t[e + 1], t[e + 2], t[e + 3]};
+                    xo[((GRP * 2 + m) * 4 * H + i) * GT + t4] = f32x4{t[e], t[e + 1], t[e + 2], t[e + 3]};
                 }
             __syncthreads();
 #pragma unroll
@@ -378,7 +405,7 @@ __global__ __launch_bounds__(kDiffThreads * NG, NG == 2 ? 1 : HD == 64 ? 3 : 2) 
                 const float f_other = other[0] == -INFINITY ? 0.f : exp2_fast(other[0] - top);
 #pragma unroll
                 for (int i = 0; i < 4 * H; ++i) {
-                    const f32x4 x = xo[(((1 - GRP) * 2 + m) * 4 * H + i) * NT + t4];
+                    const f32x4 x = xo[(((1 - GRP) * 2 + m) * 4 * H + i) * GT + t4];
                     f32x16 &t = o[m][GRP * H + i / 4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) t[4 * (i & 3) + e] = fmaf(x[e], f_other, t[4 * (i & 3) + e] * f_own);
@@ -446,9 +473,24 @@ int check_diff_fwd(const fa_diff_fwd_args *p) {
 template <int HD, bool BF, bool CACHE>
 static int launch_diff_fwd(const DiffFwd &p, hipStream_t s) {
     const fa_diff_fwd_args &a = p.a;
-    const int lg = diff_pack_log2(a.nheads / a.nheads_k, kDiffRows), P = kDiffRows >> lg;
-    const int nmb = (a.lse_seqlen + P - 1) / P;
-    const int64_t grid = int64_t(nmb) * a.batch * (a.nheads >> lg);
+    int lg, P, nmb;
+    int64_t grid;
+    auto rows = [&](int BM) {
+        lg = diff_pack_log2(a.nheads / a.nheads_k, BM);
+        P = BM >> lg;
+        nmb = (a.lse_seqlen + P - 1) / P;
+        grid = int64_t(nmb) * a.batch * (a.nheads >> lg);
+    };
+    rows(kDiffRows);
+    const int cus = device_cus();
+    // Measured with NG = 1 and NG = 2 (fp16, 128 channels, us): 128 tokens, batch 4, 16/4
+    // heads 10.8 and 9.2; 16 heads, 1024 tokens 36 and 27; 2048 tokens (grid = CUs) 74 and 67,
+    // causal 67 and 47; 20 heads, 2048 tokens, causal (1.25 of the CUs) 72 and 51; batch 3,
+    // 1024 tokens, causal 43 and 39; two paged chunks of 512 queries over 4 k and 12 k
+    // tokens 401 and 289.  Twice the CUs, 2048 tokens: 118 and 129, causal 79 and 81.
+    const bool uneven = a.causal || CACHE;
+    const int groups = 2 * grid <= (uneven ? 3 : 2) * cus && a.seqlen_k > 32 ? 2 : 1;
+    if (groups == 2) rows(kDiffRows / 2);
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     if (a.cu_seqlens_q && (a.work_order || a.o_rows > 0)) {
         const int order_wgs = a.work_order ? 1 : 0;
@@ -458,15 +500,14 @@ static int launch_diff_fwd(const DiffFwd &p, hipStream_t s) {
         if (rc) return rc;
     }
     if (grid == 0) return FA_OK;
-    const int groups = grid <= device_cus() && a.seqlen_k > kDiffBN ? 2 : 1;
     auto launch = [&](auto causal) {
         constexpr bool C = decltype(causal)::value;
         if (groups == 2)
-            hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, C, CACHE, 2>), dim3(unsigned(grid)), dim3(2 * kDiffThreads), 0, s,
-                               p, nmb, lg);
+            hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, C, CACHE, 2>), dim3(unsigned(grid)), dim3(kDiffThreads), 0, s, p,
+                               nmb, lg, cus);
         else
             hipLaunchKernelGGL((diff_fwd_kernel<HD, BF, C, CACHE, 1>), dim3(unsigned(grid)), dim3(kDiffThreads), 0, s, p,
-                               nmb, lg);
+                               nmb, lg, cus);
     };
     if (a.causal)
         launch(std::true_type{});

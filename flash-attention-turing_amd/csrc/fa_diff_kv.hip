@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
         int at = p0;
         if (a.block_table) {
             const int pg = p0 / a.page_block_size;
-            line = checked_page(a.block_table, a.block_table_stride, b, pg, a.num_pages, a.status);
+            line = checked_page(scalar_load(a.block_table + int64_t(b) * a.block_table_stride + pg), a.num_pages, a.status);
             at = p0 - pg * a.page_block_size;
         }
         const f16 *kb = (const f16 *)a.k_cache.ptr + line * a.k_cache.batch_stride + int64_t(at) * krs +
