@@ -758,42 +758,34 @@ __global__ __launch_bounds__(64) void diff_dlam_all_kernel(const fa_diff_bwd_arg
     if (threadIdx.x == 0) a.dlam.ptr[0] = float(x);
 }
 
-// Packed batches: work orders and zeros in the gradients of rows of no sequence.
-__global__ __launch_bounds__(kOrderThreads) void diff_dkdv_order_kernel(const fa_diff_bwd_args a, const int nnb,
-                                                                        const int order_wgs) {
+// Packed batches: work orders (workgroup 0 for dK/dV, 1 for dQ) and zeros in the
+// gradients of rows of no sequence.
+__global__ __launch_bounds__(kOrderThreads) void diff_bwd_order_kernel(const fa_diff_bwd_args a, const int nnb,
+                                                                       const int nmb, const int P, const int order_wgs) {
     if (int(blockIdx.x) >= order_wgs) {
-        for (const fa_tensor *t : {&a.dk, &a.dv})
-            zero_gaps(*t, a.cu_seqlens_k, a.batch, a.seqlen_k, a.dkv_rows, a.nheads_k, a.head_dim,
-                      blockIdx.x - order_wgs, gridDim.x - order_wgs);
+        const int i = blockIdx.x - order_wgs, n = gridDim.x - order_wgs;
+        if (a.dq_rows > 0)
+            zero_gaps(a.dq, a.cu_seqlens_q, a.batch, a.lse_seqlen, a.dq_rows, a.nheads, a.head_dim, i, n);
+        if (a.dkv_rows > 0)
+            for (const fa_tensor *t : {&a.dk, &a.dv})
+                zero_gaps(*t, a.cu_seqlens_k, a.batch, a.seqlen_k, a.dkv_rows, a.nheads_k, a.head_dim, i, n);
         return;
     }
-    order_items(a.batch * nnb, [&](int it) {
-        const int b = it / nnb, nb = it - b * nnb;
-        const int sk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows).n;
-        const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
-        const int k0 = nb * 128;
-        if (k0 >= sk) return -1;
-        const int rows = a.causal ? max(0, min(sq, sk - k0)) : max(sq, 0);
-        return min(rows >> 6, kOrderBuckets - 1);
-    }, a.work_order, false);
-}
-
-__global__ __launch_bounds__(kOrderThreads) void diff_dq_order_kernel(const fa_diff_bwd_args a, const int nnb,
-                                                                      const int nmb, const int P, const int order_wgs) {
-    if (int(blockIdx.x) >= order_wgs) {
-        zero_gaps(a.dq, a.cu_seqlens_q, a.batch, a.lse_seqlen, a.dq_rows, a.nheads, a.head_dim, blockIdx.x - order_wgs,
-                  gridDim.x - order_wgs);
-        return;
-    }
-    order_items(a.batch * nmb, [&](int it) {
-        const int b = it / nmb, mb = it - b * nmb;
+    const bool dq = blockIdx.x == 1;
+    const int per = dq ? nmb : nnb;
+    order_items(a.batch * per, [&](int it) {
+        const int b = it / per, blk = it - b * per;
         const int sq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows).n;
         const int sk = diff_rows(a.cu_seqlens_k, b, a.seqlen_k, a.dkv_rows).n;
-        const int m0 = mb * P;
-        if (m0 >= sq) return -1;
-        const int keys = a.causal ? max(0, min(sk, m0 + P + sk - sq)) : sk;
-        return min(keys >> 6, kOrderBuckets - 1);
-    }, a.work_order + int64_t(a.batch) * nnb, false);
+        const int at = blk * (dq ? P : 128);
+        if (at >= (dq ? sq : sk)) return -1;
+        int n;  // keys of a dQ item, queries of a dK/dV item
+        if (dq)
+            n = a.causal ? min(sk, at + P + sk - sq) : sk;
+        else
+            n = a.causal ? min(sq, sk - at) : sq;
+        return min(max(0, n) >> 6, kOrderBuckets - 1);
+    }, a.work_order + (dq ? int64_t(a.batch) * nnb : 0), false);
 }
 
 static int check_diff_bwd(const fa_diff_bwd_args *p) {
@@ -880,10 +872,10 @@ static int launch_diff_bwd(fa_diff_bwd_args a, hipStream_t s) {
     const int64_t q_grid = int64_t(nmb) * a.batch * (a.nheads >> lg), k_grid = int64_t(nnb) * a.batch * a.nheads_k * S;
     if (q_grid > 0x7fffffff || k_grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     int rc;
-    if (a.cu_seqlens_q && (a.work_order || a.dq_rows > 0)) {
-        const int order_wgs = a.work_order ? 1 : 0;
-        hipLaunchKernelGGL(diff_dq_order_kernel, dim3(order_wgs + (a.dq_rows > 0 ? kZeroBlocks : 0)),
-                           dim3(kOrderThreads), 0, s, a, nnb, nmb, P, order_wgs);
+    if (a.cu_seqlens_q && (a.work_order || a.dq_rows > 0 || a.dkv_rows > 0)) {
+        const int order_wgs = a.work_order ? 2 : 0, zero_wgs = a.dq_rows > 0 || a.dkv_rows > 0 ? kZeroBlocks : 0;
+        hipLaunchKernelGGL(diff_bwd_order_kernel, dim3(order_wgs + zero_wgs), dim3(kOrderThreads), 0, s, a, nnb, nmb, P,
+                           order_wgs);
         if ((rc = int(hipGetLastError()))) return rc;
     }
     if (q_grid > 0) {
@@ -891,12 +883,6 @@ static int launch_diff_bwd(fa_diff_bwd_args a, hipStream_t s) {
             hipLaunchKernelGGL((diff_dq_kernel<HD, BF, true>), dim3(unsigned(q_grid)), dim3(kDbThreads), 0, s, a, nmb, lg);
         else
             hipLaunchKernelGGL((diff_dq_kernel<HD, BF, false>), dim3(unsigned(q_grid)), dim3(kDbThreads), 0, s, a, nmb, lg);
-        if ((rc = int(hipGetLastError()))) return rc;
-    }
-    if (a.cu_seqlens_k && (a.work_order || a.dkv_rows > 0)) {
-        const int order_wgs = a.work_order ? 1 : 0;
-        hipLaunchKernelGGL(diff_dkdv_order_kernel, dim3(order_wgs + (a.dkv_rows > 0 ? kZeroBlocks : 0)),
-                           dim3(kOrderThreads), 0, s, a, nnb, order_wgs);
         if ((rc = int(hipGetLastError()))) return rc;
     }
     if (k_grid > 0) {

@@ -126,18 +126,6 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
     const int qpos = row_ok ? row / G : 0, hq = hk * G + (row_ok ? row - qpos * G : 0);
     const int lim = a.causal ? qpos + L - a.seqlen_q : L - 1;                     // last visible key
     const int lim_min = a.causal ? (rt * kDkRows) / G + L - a.seqlen_q : L - 1;  // ... of the tile's first row
-    f16x8 qB[HD / 16];
-    {
-        const f16 *qp = (const f16 *)a.q.ptr + int64_t(b) * a.q.batch_stride + int64_t(qpos) * a.q.row_stride +
-                        int64_t(hq) * a.q.head_stride + 8 * hh;
-#pragma unroll
-        for (int g = 0; g < HD / 16; ++g) {
-            u32x4 v = row_ok && g / HG == map ? ldg16(qp + 16 * g) : zero_u4();
-            if (a.softmax_scale < 0.f) v = neg_h8(v);
-            qB[g] = as_h8(v);
-        }
-    }
-    wait_vmem();
     const float cscale = fabsf(a.softmax_scale) * kLog2e;
     f32x16 o[HD / 32];
 #pragma unroll
@@ -170,6 +158,19 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
     rd.init(lane);
     if (n_my > 0) issue(my_first, 0);
     if (NST > 1 && n_my > 1) issue(my_first + 4, 1);
+    // Q^T as B operands, behind the first copies: the two latencies run together.
+    f16x8 qB[HD / 16];
+    {
+        const f16 *qp = (const f16 *)a.q.ptr + int64_t(b) * a.q.batch_stride + int64_t(qpos) * a.q.row_stride +
+                        int64_t(hq) * a.q.head_stride + 8 * hh;
+#pragma unroll
+        for (int g = 0; g < HD / 16; ++g) {
+            u32x4 v = row_ok && g / HG == map ? ldg16(qp + 16 * g) : zero_u4();
+            if (a.softmax_scale < 0.f) v = neg_h8(v);
+            qB[g] = as_h8(v);
+        }
+    }
+    wait_vmem();  // only tile copies are in flight inside the loop
     for (int k = 0; k < n_my; ++k) {
         const int st = k % NST, p0 = (my_first + 4 * k) * kDkTile;
         if (k + 1 < n_my)
@@ -307,35 +308,51 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
     };
     const int d2 = lane % (HD / 2);
     for (int r = wave; r < rows; r += 4) {
-        float mm[2], ll[2];
-        f32x2 x[2];
+        // Lane i holds chunk i's maxima and sums; both maps' loads, and eight chunks', are in flight together.
+        float mm[2] = {-INFINITY, -INFINITY}, ll[2] = {0.f, 0.f};
+        f32x2 x[2] = {}, own[2];
+        for (int i0 = 0; i0 < live_chunks; i0 += 64)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int c = k * rows + r;
-            float mt = -INFINITY;
-            for (int i = lane; i < live_chunks; i += 64) mt = fmaxf(mt, load(mls + i * 2 * R16 + c)[0]);
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor(mt, d));
-            float lt = 0.f;
-            f32x2 acc = {0.f, 0.f};
-            for (int i0 = 0; i0 < live_chunks; i0 += 64) {
-                const int n = min(64, live_chunks - i0);
-                const f32x2 own = load(mls + (i0 + min(lane, n - 1)) * 2 * R16 + c);
-                const float f = lane < n && own[0] != -INFINITY ? exp2_fast(own[0] - mt) : 0.f;
-                lt = fmaf(own[1], f, lt);
-                for (int i = 0; i < n; ++i) {
-                    const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
-                    const f32x2 y = load(os + (int64_t(i0 + i) * 2 * R16 + c) * (HD / 2) + d2);
-                    acc[0] = fmaf(w, y[0], acc[0]);
-                    acc[1] = fmaf(w, y[1], acc[1]);
-                }
+            for (int k = 0; k < 2; ++k) {
+                const f32x2 y = load(mls + min(i0 + lane, live_chunks - 1) * 2 * R16 + k * rows + r);
+                if (i0 == 0) own[k] = y;
+                mm[k] = fmaxf(mm[k], y[0]);
             }
 #pragma unroll
-            for (int d = 32; d > 0; d >>= 1) lt += __shfl_xor(lt, d);
-            mm[k] = mt;
-            ll[k] = lt;
-            x[k] = acc;
+        for (int d = 32; d > 0; d >>= 1)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) mm[k] = fmaxf(mm[k], __shfl_xor(mm[k], d));
+        for (int i0 = 0; i0 < live_chunks; i0 += 64) {
+            const int n = min(64, live_chunks - i0);
+            float f[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (i0 > 0) own[k] = load(mls + (i0 + min(lane, n - 1)) * 2 * R16 + k * rows + r);
+                f[k] = lane < n && own[k][0] != -INFINITY ? exp2_fast(own[k][0] - mm[k]) : 0.f;
+                ll[k] = fmaf(own[k][1], f[k], ll[k]);
+            }
+            for (int i = 0; i < n; i += 8) {
+                f32x2 y[8][2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        y[j][k] = i + j < n ? load(os + (int64_t(i0 + i + j) * 2 * R16 + k * rows + r) * (HD / 2) + d2)
+                                            : f32x2{0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[k]), i + j));
+                        x[k][0] = fmaf(w, y[j][k][0], x[k][0]);
+                        x[k][1] = fmaf(w, y[j][k][1], x[k][1]);
+                    }
+            }
         }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) ll[k] += __shfl_xor(ll[k], d);
         if (lane < HD / 2) store(r, 2 * d2, x[0], mm[0], ll[0], x[1], mm[1], ll[1]);
     }
 }
