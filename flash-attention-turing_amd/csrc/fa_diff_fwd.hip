@@ -229,7 +229,7 @@ struct DiffTiles {
     __device__ __forceinline__ void init(const DiffFwd &p, const DiffWork &w) {
         k = w.kp;
         v = w.vp;
-        if (CACHE && p.block_table) next = scalar_load_ahead(p.block_table + int64_t(w.b) * p.block_table_stride);
+        if (CACHE && p.block_table && w.n_keys > 0) next = scalar_load_ahead(p.block_table + int64_t(w.b) * p.block_table_stride);
     }
     // Goes to block n0 / kDiffBN, which follows the one before.
     __device__ __forceinline__ void step(const DiffFwd &p, const DiffWork &w, int n0) {

@@ -64,6 +64,19 @@ def test_forward_and_gradients(device, b, sq, sk, h, hk, d, causal, kind, dtype)
     _check(*_inputs(device, b, sq, sk, h, hk, d, kind, dtype, 11), causal)
 
 
+# More workgroups than the chip has places for, with and without a mask, so that every one of them has whole rows,
+# ragged ones and a row of its own (one group of waves); and causal grids between one and two workgroups on a CU.
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,causal,dtype", [
+    (13, 150, 170, 32, 32, 128, True, torch.float16),
+    (13, 129, 129, 32, 32, 64, True, torch.bfloat16),
+    (9, 150, 97, 32, 32, 128, False, torch.bfloat16),
+    (10, 200, 200, 32, 16, 64, True, torch.float16),
+    (5, 129, 260, 32, 32, 128, True, torch.bfloat16),
+])
+def test_grids_that_fill_the_chip(device, b, sq, sk, h, hk, d, causal, dtype):
+    _check(*_inputs(device, b, sq, sk, h, hk, d, "head", dtype, 23), causal)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 2.0])
 def test_scales(device, scale):
     _check(*_inputs(device, 1, 100, 140, 4, 2, 64, "token", torch.float16, 5), True, scale)
@@ -266,6 +279,37 @@ def test_captured_training_step(device, kind):
         got = [x.clone() for x in captured]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_captured_autograd_step(device):
+    """The public function's forward and backward in one graph, with an eager step of the same leaves before (its graph
+    gone), eager work between the replays and an eager step after."""
+    g = torch.Generator().manual_seed(31)
+    q, k, v, lam, do = _inputs(device, 2, 150, 150, 8, 2, 64, "head", torch.bfloat16, 31)
+    leaves = [x.requires_grad_() for x in (q, k, v, lam)]
+
+    def step():
+        out = fai.flash_diff_attn_func(*leaves, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for turn in range(3):
+        with torch.no_grad():
+            for x in (*leaves, do):
+                x.copy_(torch.randn(x.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        for a, b in zip(captured, eager):
+            assert torch.equal(a, b), turn
 
 
 def test_refusals(device):

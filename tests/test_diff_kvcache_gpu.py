@@ -116,6 +116,17 @@ def test_page_sizes(device, page):
         _check(_setup(device, [page - 1, page, 3 * page + 5], sq, 1, 4, 2, 128, torch.float16, "paged", "head", page=page))
 
 
+@pytest.mark.parametrize("layout", ["paged", "contiguous"])
+@pytest.mark.parametrize("b,h,hk,d,dtype", [
+    (5, 8, 2, 128, torch.float16),    # the longest sequences first
+    (70, 3, 3, 64, torch.bfloat16),   # more sequences than a wave has lanes: as they come
+    (13, 32, 32, 64, torch.float16),  # more workgroups than the chip has places for
+])
+def test_chunks_of_many_sequences(device, layout, b, h, hk, d, dtype):
+    lens = [(37 * i * i + 11 * i) % 500 for i in range(b)]
+    _check(_setup(device, lens, 66, 66, h, hk, d, dtype, layout, "head"))
+
+
 def test_full_cache(device):
     s = _setup(device, [255, 100], 1, 1, 4, 2, 64, torch.float16, "contiguous", "head", cap=256)
     _check(s)
