@@ -357,20 +357,38 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
     }
 }
 
-// Rows per KV head from which the forward kernel's 128-row tiles take the call.
-constexpr int kDkMostRows = 64;
+// Whether the forward kernel takes the call: more rows than one tile (with one,
+// this kernel reads the cache once, which nothing beats), and less time by these
+// estimates in us, the tokens counted as the capacity.  This kernel: its launches
+// and the join, and the chip's rate of 32-key tiles.  The forward kernel: one
+// workgroup's walk over the keys, longer with a second one on its CU.
+// Measured (128 channels, 4 heads a KV head, bf16; this kernel, the forward one):
+//   1 x 1000 tokens, 8 KV heads,  32 / 64 / 128 rows   20 / 20 / 25      27 / 27 / 29 us
+//   1 x 8192                                           37 / 43 / 59      150 / 151 / 152
+//   16 x 4096                                          99 / 178 / 335    94 / 96 / 97
 static bool diff_kv_many_rows(const fa_diff_kvcache_args &a) {
-    return int64_t(a.nheads / a.nheads_k) * a.seqlen_q > kDkMostRows;
+    const int G = a.nheads / a.nheads_k;
+    if (int64_t(G) * a.seqlen_q <= kDkRows) return false;
+    const int heads = G % 2 == 0 ? 2 : 1, P = 64 / heads;  // of a forward workgroup of 64 rows
+    const double cus = device_cus(), cap = a.cache_capacity;
+    const double w = double(a.batch) * (a.nheads / heads) * ((a.seqlen_q + P - 1) / P) / cus;
+    return 8 + cap / 64 * std::max(1 + 0.5 * w, w) < 15 + cap * double(diff_kv_items(a)) / (50 * cus);
 }
 
-// Keys of a chunk, a multiple of the 128 that four waves take at a time.
+// Keys of a chunk, a multiple of the 128 that four waves take at a time.  Chunks of
+// one sequence are equal: as many as find room on the chip at once.  With more
+// sequences, whose lengths differ, half as many again, so that the rounds fill.
+// Under 256 keys a chunk's start and the join cost more than its keys.  Measured
+// (decode, 32/8 heads of 128 channels; 2 or 3 chunks per CU, us): 1 x 32 k
+// tokens 38 and 46; 32 sequences of 500 to 5000 78 and 66; at least 128, 256 or 512
+// keys: 1 x 8192 30, 21 and 20.5, 1 x 1500 13.2, 13.2 and 15.4.
 static int diff_kv_chunk(const fa_diff_kvcache_args &a) {
-    const int64_t cap = std::max(a.cache_capacity, 1);
+    const int64_t cap = std::max(a.cache_capacity, 1), items = diff_kv_items(a);
     int64_t chunk;
     if (a.num_splits > 0)
         chunk = (cap + a.num_splits - 1) / a.num_splits;
     else
-        chunk = std::min<int64_t>(std::max<int64_t>(cap * diff_kv_items(a) / (4 * device_cus()), 128), 2048);
+        chunk = std::min<int64_t>(std::max<int64_t>(cap * items / ((a.batch == 1 ? 2 : 3) * device_cus()), 256), 4096);
     return int((chunk + 127) / 128 * 128);
 }
 

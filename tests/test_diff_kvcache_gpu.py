@@ -83,8 +83,10 @@ def _check(s, causal=True, scale=None, **more):
     ([5, 255, 256, 257], 1, 1, 4, 4, 64, torch.bfloat16, "token"),
     ([1500], 1, 1, 32, 8, 128, torch.bfloat16, "layer"),
     ([10, 900], 5, 5, 6, 2, 64, torch.float16, "token"),
-    ([33, 400, 1], 17, 17, 4, 1, 128, torch.float16, "head"),   # 68 rows a KV head: the forward kernel
+    ([33, 400, 1], 17, 17, 4, 1, 128, torch.float16, "head"),   # 68 rows a KV head
     ([0, 300], 130, 130, 4, 4, 64, torch.bfloat16, "token"),
+    ([90, 400, 1], 300, 300, 4, 1, 128, torch.float16, "head"),  # 1200 rows a KV head: the forward kernel
+    ([0, 290], 400, 310, 4, 4, 64, torch.bfloat16, "token"),
     ([200, 64, 100], 4, 0, 4, 2, 128, torch.float16, "layer"),  # no append
     ([40, 3], 3, 7, 12, 4, 128, torch.bfloat16, "head"),        # more new tokens than queries
 ])
@@ -99,11 +101,11 @@ def test_split_counts(device, splits):
 
 def test_fewer_keys_than_queries(device):
     # Causal rows without a key give 0.
-    for rows in (8, 40):
+    for rows in (8, 40, 300):
         _check(_setup(device, [0, 2], rows, 3, 4, 2, 64, torch.float16, "paged", "token"))
 
 
-@pytest.mark.parametrize("sq", [1, 40])
+@pytest.mark.parametrize("sq", [1, 40, 300])
 def test_no_mask_and_scales(device, sq):
     s = _setup(device, [100, 300], sq, 1, 4, 2, 64, torch.bfloat16, "paged", "head")
     _check(s, causal=False)
@@ -112,7 +114,7 @@ def test_no_mask_and_scales(device, sq):
 
 @pytest.mark.parametrize("page", [64, 128, 320])
 def test_page_sizes(device, page):
-    for sq in (1, 40):
+    for sq in (1, 40, 300):
         _check(_setup(device, [page - 1, page, 3 * page + 5], sq, 1, 4, 2, 128, torch.float16, "paged", "head", page=page))
 
 
@@ -134,7 +136,7 @@ def test_full_cache(device):
 
 def test_garbage_past_the_length(device):
     for layout in ("paged", "contiguous"):
-        for sq in (1, 40):
+        for sq in (1, 40, 300):
             s = _setup(device, [70, 130], sq, 1, 4, 2, 64, torch.float16, layout, "head")
             clean = _call({**s, "kc": s["kc"].clone(), "vc": s["vc"].clone()})
             keep = torch.zeros(s["kc"].shape[:2], dtype=torch.bool, device=device)
@@ -162,12 +164,12 @@ def test_offsets_past_32_bits(device):
     n_pages, page, hk, d = 9000, 256, 8, 128
     kc = torch.empty(n_pages, page, hk, d, dtype=torch.float16, device=device)
     vc = torch.empty_like(kc)
-    pages = [n_pages - 1, 0, n_pages - 2]
+    pages = [n_pages - 1, 0, n_pages - 2, 1]
     g = torch.Generator().manual_seed(1)
     for p in pages:
         kc[p] = torch.randn(page, hk, d, generator=g).half().to(device)
         vc[p] = torch.randn(page, hk, d, generator=g).half().to(device)
-    for sq in (1, 40):
+    for sq in (1, 40, 300):
         mk = lambda h: torch.randn(1, sq, h, d, generator=g).half().to(device)  # noqa: E731
         s = {"q": mk(8), "k": mk(hk), "v": mk(hk), "lam": torch.rand(8, generator=g).to(device), "index": None,
              "lens": torch.tensor([600], dtype=torch.int32, device=device),
@@ -179,7 +181,7 @@ def test_offsets_past_32_bits(device):
         assert torch.equal(_rows(kc, places[600:]), s["k"][0])
 
 
-@pytest.mark.parametrize("sq", [1, 40])
+@pytest.mark.parametrize("sq", [1, 40, 300])
 def test_bad_sequences_are_reported_and_left_alone(device, sq):
     fai.flash_attn_kvcache_check()
     good = _setup(device, [50, 60, 70], sq, 1, 4, 2, 64, torch.float16, "paged", "head")
