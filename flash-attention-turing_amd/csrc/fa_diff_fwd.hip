@@ -32,52 +32,52 @@ struct DiffFwd {
     int32_t *status;
 };
 
-// One map's 32 keys of S^T -> P^T operands: mask (keys past lim, relative to the
-// first), running maximum, rescale of O, exponentials, row sum.  P is
-// rounded to 16 bits for the product with V, as in ordinary attention; O and
-// the LSE are normalised by the fp32 sum of the unrounded P.
-// The maximum m that P is taken against is raised, and O and the sum rescaled,
-// only when some row of the wave finds a score more than kDiffSlack doublings
-// above it: with scores of unit variance an exact maximum rises in every second
-// block of a row of 4096 keys, and the 128 multiplications were a third of the
-// VALU work that bounds the kernel.  P stays below 2^kDiffSlack; its rounding is
-// relative and as large as elsewhere (only a row's largest P, 1 against an exact
-// maximum, is no longer free of it).
-constexpr float kDiffSlack = 4.f;
+// The softmax of one map's 32 keys of S^T: exponentials against a maximum m that is
+// not looked for.  P and the sum are right against any m near a row's maximum, so m
+// stays what it is until a lane's sum of 16 P passes kDiffTop (or is infinite or NaN:
+// at first m is -infinity), which 16-bit P would not hold much longer; then the
+// tile's scores are taken once more, and m is raised to their maximum and O and the
+// sum rescaled.  m is never above the row's maximum, so small P lose nothing either.
+// The running maximum that this replaces, kept up lazily, was a quarter of the VALU
+// work that bounds the kernel beside its MFMAs, and the exponentials waited for it:
+// b 4, s 4096, 16 heads of 128, causal, bf16 505 -> 455 us; 64 channels, s 4096,
+// fp16 672 -> 605 us; an exact maximum had cost 15 % more.
+// P is rounded to 16 bits for the product with V, as in ordinary attention (its 2^-9
+// in bf16 weighs as the output's own rounding does; carrying the remainder would take
+// 32 MFMAs more beside 48); O and the LSE are normalised by the fp32 sum of the
+// unrounded P.
+constexpr float kDiffTop = 32768.f;
 
-template <int HD, bool BF, bool MASK>
-__device__ __forceinline__ void diff_softmax(f32x16 &s, f16x8 (&pB)[2], f32x16 (&o)[HD / 32], float &m, float &l,
-                                             float cscale, int lim, int hh) {
-    if constexpr (MASK) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (acc_lrow(e, hh) > lim) s[e] = -INFINITY;
-    }
-    const float mx = max2_xor32(max16(s));
-    const float mx_t = MASK && mx == -INFINITY ? -INFINITY : mx * cscale;
-    if (__builtin_amdgcn_ballot_w64(mx_t > m + kDiffSlack) != 0) {
-        const float m_new = fmaxf(m, mx_t);
-        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-        l *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-        m = m_new;
-    }
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float rs = 0.f;
+// P of keys up to lim (relative to the first) in place of their scores; returns their sum.
+template <bool MASK>
+__device__ __forceinline__ float diff_exps(f32x16 &s, float m, float cscale, int lim, int hh) {
+    float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const float x = s[e];
-        float p = exp2_fast(fmaf(x, cscale, -m_use));
-        if constexpr (MASK) p = x == -INFINITY ? 0.f : p;
-        s[e] = p;
-        rs += p;
+        float x = fmaf(s[e], cscale, -m);
+        if constexpr (MASK) x = acc_lrow(e, hh) > lim ? -INFINITY : x;
+        s[e] = exp2_fast(x);
+        sum += s[e];
     }
-    l += rs;
-    pB[0] = pack16<BF>(s, 0);
-    pB[1] = pack16<BF>(s, 8);
+    return sum;
+}
+
+// Raises m to the maximum of the visible scores, O and the sum l with it.
+template <int HD, bool MASK>
+__device__ __forceinline__ void diff_raise(const f32x16 &s, f32x16 (&o)[HD / 32], float &m, float &l, float cscale,
+                                           int lim, int hh) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, MASK && acc_lrow(e, hh) > lim ? -INFINITY : s[e]);
+    mx = max2_xor32(mx);
+    const float m_new = fmaxf(m, mx == -INFINITY ? mx : mx * cscale);
+    const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    m = m_new;
 }
 
 // A workgroup's work: gp = 2^lg heads of one GQA group at P = 128 / gp positions
@@ -346,10 +346,28 @@ __global__ __launch_bounds__(kDiffThreads, HD == 64 ? 3 : 2) void diff_fwd_kerne
             };
 #pragma unroll
             for (int u = 0; u < PIPE - 1; ++u) rd_v(u);
+            float part[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) part[m] = diff_exps<MASK>(s[m], mx[m], cscale, lim - 32 * sub, hh);
+            if (__builtin_amdgcn_ballot_w64(!(fmaxf(part[0], part[1]) <= kDiffTop)) != 0) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    f32x16 t = zero16();
+#pragma unroll
+                    for (int g = 0; g < HG; ++g)
+                        t = mfma16<BF>(rd.a_operand_at(smem + 32 * sub * (HD * 2), ab, m * HG + g), qB[m * HG + g], t);
+                    diff_raise<HD, MASK>(t, o[m], mx[m], sum[m], cscale, lim - 32 * sub, hh);
+                    part[m] = diff_exps<MASK>(t, mx[m] == -INFINITY ? 0.f : mx[m], cscale, lim - 32 * sub, hh);
+                    s[m] = t;
+                }
+            }
             f16x8 pB[2][2];
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-                diff_softmax<HD, BF, MASK>(s[m], pB[m], o[m], mx[m], sum[m], cscale, lim - 32 * sub, hh);
+            for (int m = 0; m < 2; ++m) {
+                sum[m] += part[m];
+                pB[m][0] = pack16<BF>(s[m], 0);
+                pB[m][1] = pack16<BF>(s[m], 8);
+            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < NPV; ++u) {

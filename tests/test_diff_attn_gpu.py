@@ -99,6 +99,22 @@ def test_rising_and_large_scores(device, dtype):
     _check(q, k, v, lam, do, True, names=("out", "dv", "dlam"))
 
 
+@pytest.mark.parametrize("jump", [9.0, 10.5, 25.0, 300.0, -60.0])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_scores_that_jump(device, d, dtype, jump):
+    # Keys from 130 on score `jump` above the ones before, in one map for even queries and in both for odd ones: short
+    # of what the forward kernel's maximum lets pass (2^15, 10.4), past it, far past it, and below.
+    q, k, v, lam, do = _inputs(device, 2, 200, 260, 4, 2, d, "head", dtype, 17)
+    scale = (d // 2) ** -0.5
+    for half in (0, d // 2):
+        q[..., half] = 8.0
+        k[..., half] = 0.0
+        k[:, 130:, :, half] = jump / (8.0 * scale)
+    q[:, ::2, :, d // 2] = 0.0
+    for causal in (False, True):
+        _check(q, k, v, lam, do, causal)
+
+
 def test_a_dlam_that_many_rows_share(device):
     # 2 x 1024 rows x 8 heads: the terms' signs vary and the sum is small, so a common leaning of the terms shows
     # (they were once 3e-8 low each).  Bound: 16384 terms of at most 4e-7 each that do not lean add up to
