@@ -23,6 +23,14 @@
 //
 // dK/dV kernel: 4 waves x 32 keys of one KV head, S and dP with queries on M.
 // It loops over the heads of the GQA group and sums them in fp32 registers.
+//
+// What bounds both is the matrix cores beside the VALU: dQ takes 48 MFMAs and 290
+// VALU instructions (64 exponentials) for 32 queries x 64 keys at 128 channels,
+// dK/dV 36 (4 of them for the row operands) and 210 for 32 x 32.  Counters: MFMA 48
+// to 55 and 58 to 61 % of dQ's and dK/dV's cycles, VALU 60 to 64 and 56 to 58 %.
+// b 4, s 4096, 16 heads of 128, causal, bf16: dQ 520 us, dK/dV 655 us (793 and 839
+// TFLOP/s of the formulas' products); b 1, s 8192, 32/8 heads, fp16: 925 and 1215 us
+// (892 and 905); a library product of 8192^3 runs at 1224 to 1280.
 #include <algorithm>
 #include <type_traits>
 
