@@ -333,6 +333,7 @@ std::vector<at::Tensor> diff_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::T
     at::Tensor out = at::empty(q.sizes(), q.options());
     at::Tensor lse = at::empty({2, batch, q.size(2), seqlen_q}, q.options().dtype(at::kFloat));
     if (k_cache.numel() == 0) {
+        TORCH_CHECK(a.seqlen_new == 0, "cache capacity is insufficient for the requested append length");
         out.zero_();
         lse.zero_();
         return {out, lse};

@@ -36,6 +36,7 @@ struct Call {
                         c.stride(0) * e % 16 == 0 && c.stride(1) * e % 16 == 0 && c.stride(2) * e % 16 == 0 &&
                         (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0,
                     name, " must have a contiguous last dimension and 16-byte aligned rows");
+        TORCH_CHECK(c.size(0) == 1 || c.stride(0) > 0, "pages of ", name, " must not overlap");
         return fa_tensor{c.data_ptr(), c.stride(0) * e, c.stride(1) * e, c.stride(2) * e};
     }
     void cache(const at::Tensor &k, const at::Tensor &v) {
@@ -49,6 +50,7 @@ struct Call {
     void table(const at::Tensor &t, const std::optional<at::Tensor> &lens, const at::Tensor &refs) {
         check_ints(t, device, 2, "block_table");
         check_ints(refs, device, 1, "page_refs");
+        TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), "rows of block_table must not overlap");
         TORCH_CHECK(a.num_pages == 0 || refs.size(0) == a.num_pages, "page_refs must have one entry a page");
         a.num_pages = i32(refs.size(0), "num_blocks");
         a.block_table = t.data_ptr<int32_t>();

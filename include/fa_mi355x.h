@@ -360,7 +360,7 @@ typedef struct fa_diff_kvcache_args {
     int32_t page_block_size;        /* paged: a multiple of 64                    */
     int32_t num_pages;              /* paged: pages of the cache; a table entry in use outside them reads page
                                        0, is not appended to and ORs FA_KV_BAD_PAGE into *status */
-    int32_t num_splits;             /* pieces of cache_capacity, 0: chosen        */
+    int32_t num_splits;             /* pieces of cache_capacity, 0: chosen (calls of few query rows) */
     float softmax_scale;
     int32_t causal, dtype;
     int32_t cache_capacity;         /* tokens one sequence's cache holds          */

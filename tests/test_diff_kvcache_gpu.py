@@ -260,3 +260,16 @@ def test_refusals(device):
         _call({**s, "k": s["k"][:, :, :1], "v": s["v"][:, :, :1]})
     with pytest.raises(RuntimeError, match="batch size must match"):
         _call({**s, "table": None, "kc": s["kc"][:1], "vc": s["vc"][:1]})
+    with pytest.raises(RuntimeError, match="capacity is insufficient"):  # also without the host's checks
+        _call({**s, "kc": s["kc"][:0], "vc": s["vc"][:0]}, validate=False)
+
+
+@pytest.mark.parametrize("sq", [1, 300])
+def test_no_pages_and_no_keys(device, sq):
+    # A table of no columns, an empty pool, and sequences of no token: rows without keys are 0.
+    s = _setup(device, [0, 0], sq, 0, 4, 2, 64, torch.float16, "paged", "head", cap=256)
+    for x in (s, {**s, "table": s["table"][:, :0]}, {**s, "kc": s["kc"][:0], "vc": s["vc"][:0]}):
+        for validate in (True, False):
+            fai.flash_attn_kvcache_check()
+            out, lse = _call(x, validate=validate)
+            assert not out.any() and not lse.any()

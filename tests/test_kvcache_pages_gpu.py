@@ -293,6 +293,10 @@ def test_refusals(device):
         fai.flash_attn_kvcache_fork(c.k, c.v, c.table, c.lens, c.refs[:5], c.ints([0]), c.ints([2]))
     with pytest.raises(RuntimeError, match="one entry a row"):
         fai.flash_attn_kvcache_free(c.table, c.lens[:2], c.refs, c.ints([0]))
+    with pytest.raises(RuntimeError, match="rows of block_table must not overlap"):
+        fai.flash_attn_kvcache_free(c.table[:1].expand(c.lens.shape[0], -1), c.lens, c.refs, c.ints([0]))
+    with pytest.raises(RuntimeError, match="pages of k_cache must not overlap"):
+        fai.flash_attn_kvcache_copy_pages(c.k[:1].expand(4, -1, -1, -1), c.v[:4], c.ints([0]), c.ints([1]))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
