@@ -615,7 +615,10 @@ def flash_diff_attn_func(q, k, v, lam, softmax_scale: Optional[float] = None, ca
     headdim / 2 channels of q and k are the first map's, the others the second's; headdim is 64 or 128 and
     softmax_scale defaults to (headdim / 2) ** -0.5.  lam is fp32: a scalar tensor, (nheads,), or one value for each
     query and head, (batch, seqlen_q, nheads).  causal, grouped heads and rows without a visible key are as in
-    flash_attn_func.  Returns out (batch, seqlen_q, nheads, headdim); q, k, v and lam get gradients."""
+    flash_attn_func.  Returns out (batch, seqlen_q, nheads, headdim); q, k, v and lam get gradients.
+
+    A backward pass is captured into a graph with torch.autograd.grad, or when no eager graph of the same leaves is
+    alive: torch ties the accumulation into a leaf's grad to the stream of its first live graph."""
     softmax_scale = _check_diff_args(q, lam, softmax_scale)
     return FlashDiffAttnFunc.apply(q, k, v, lam, softmax_scale, causal, torch.is_grad_enabled())
 

@@ -328,6 +328,42 @@ def test_captured_autograd_step(device):
             assert torch.equal(a, b), turn
 
 
+def test_two_at_once(device):
+    """Steps on two streams at once, eager and as two graphs, give the bits that each gives alone (small grids, whose
+    key blocks several workgroups share through workspaces)."""
+    sets = [_inputs(device, 1, 400, 400, 8, 2, 128, kind, torch.bfloat16, seed) for kind, seed in (("layer", 41), ("token", 42))]
+
+    def step(q, k, v, lam, do):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, lam)]
+        out = fai.flash_diff_attn_func(*leaves, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    alone = [step(*x) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            captured.append(step(*sets[i]))
+        graphs.append(g)
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for one in (*got[i], captured[i]):
+                for a, b in zip(one, alone[i]):
+                    assert torch.equal(a, b)
+
+
 def test_refusals(device):
     q, k, v, lam, _ = _inputs(device, 2, 8, 8, 4, 2, 64, "head", torch.float16, 1)
     f = fai.flash_diff_attn_func
