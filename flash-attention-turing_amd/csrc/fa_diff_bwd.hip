@@ -717,14 +717,15 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 // workgroup per head sums its rows in fp64 in a fixed order, and for a lam of
 // all heads the second launch sums the heads.
 __global__ __launch_bounds__(1024) void diff_dlam_rows_kernel(const fa_diff_bwd_args a) {
-    const int b = blockIdx.y;
-    const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows);
-    const int64_t start = rq.start, n = int64_t(rq.n) * a.nheads;
-    for (int64_t i = int64_t(blockIdx.x) * 1024 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 1024) {
-        const int64_t row = i / a.nheads;
-        const int h = int(i - row * a.nheads);
-        a.dlam.ptr[b * a.dlam.batch_stride + (start + row) * a.dlam.row_stride + h * a.dlam.head_stride] =
-            a.dsum[(int64_t(b) * a.nheads + h) * a.lse_seqlen + row];
+    for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+        const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows);
+        const int64_t start = rq.start, n = int64_t(rq.n) * a.nheads;
+        for (int64_t i = int64_t(blockIdx.x) * 1024 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 1024) {
+            const int64_t row = i / a.nheads;
+            const int h = int(i - row * a.nheads);
+            a.dlam.ptr[b * a.dlam.batch_stride + (start + row) * a.dlam.row_stride + h * a.dlam.head_stride] =
+                a.dsum[(int64_t(b) * a.nheads + h) * a.lse_seqlen + row];
+        }
     }
 }
 
@@ -802,8 +803,7 @@ static int check_diff_bwd(const fa_diff_bwd_args *p) {
     if (a.head_dim != 64 && a.head_dim != 128) return FA_ERR_UNSUPPORTED;
     if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
     if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_k < 0 || a.nheads <= 0 || a.nheads_k <= 0 ||
-        a.nheads % a.nheads_k != 0 || a.lse_seqlen < a.seqlen_q || (!a.cu_seqlens_q) != (!a.cu_seqlens_k) ||
-        a.batch > 65535)
+        a.nheads % a.nheads_k != 0 || a.lse_seqlen < a.seqlen_q || (!a.cu_seqlens_q) != (!a.cu_seqlens_k))
         return FA_ERR_INVALID_ARG;
     if (!a.lse || !a.lam.ptr) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.q, &a.k, &a.v, &a.o, &a.o2, &a.dout, &a.dq, &a.dk, &a.dv})
@@ -910,7 +910,7 @@ static int launch_diff_bwd(fa_diff_bwd_args a, hipStream_t s) {
     if (a.dlam.row_stride != 0) {
         if (a.batch == 0 || a.lse_seqlen == 0) return FA_OK;
         const int64_t n = int64_t(a.lse_seqlen) * a.nheads;
-        hipLaunchKernelGGL(diff_dlam_rows_kernel, dim3(unsigned(std::min<int64_t>((n + 1023) / 1024, 1024)), a.batch),
+        hipLaunchKernelGGL(diff_dlam_rows_kernel, dim3(unsigned(std::min<int64_t>((n + 1023) / 1024, 1024)), std::min(a.batch, 65535)),
                            dim3(1024), 0, s, a);
         return int(hipGetLastError());
     }

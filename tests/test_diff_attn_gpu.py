@@ -162,6 +162,19 @@ def test_broadcast_lam_gets_its_summed_gradient(device):
     assert_within("dlam", torch.autograd.grad(out, lam, do)[0], want["dlam"])
 
 
+def test_a_batch_past_the_grids_second_dimension(device):
+    # 65536 sequences and more, a lam for each row, the last sequences checked.
+    b = 65540
+    q, k, v, lam, do = _inputs(device, b, 2, 3, 1, 1, 64, "token", torch.float16, 29)
+    leaves = [x.requires_grad_() for x in (q, k, v, lam)]
+    out = fai.flash_diff_attn_func(*leaves, causal=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    tail = slice(b - 8, b)
+    want = diff_attention(q[tail], k[tail], v[tail], lam[tail], None, True, do[tail])
+    for name, x in zip(("out", "dq", "dk", "dv", "dlam"), (out, *grads)):
+        assert_within(name, x[tail], want[name])
+
+
 def test_no_rows_and_no_keys(device):
     for b, sq, sk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
         q, k, v, lam, do = _inputs(device, b, sq, sk, 2, 1, 64, "head", torch.float16, 1)

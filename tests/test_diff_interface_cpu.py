@@ -157,7 +157,7 @@ def _bwd(**more):
 @pytest.mark.parametrize("want,change", [
     (-2, {"head_dim": 32}), (-2, {"dtype": -1}), (-1, {"nheads_k": 3}), (-1, {"o2": _tensor(None)}), (-1, {"lse": None}),
     (-1, {"dq": _tensor(P + 2)}), (-3, {"dsum": None}), (-3, {"dsum": P + 4}), (-3, {"dsum_bytes": 16}),
-    (-1, {"split_ws": P + 128, "split_ws_bytes": 1 << 30}), (-1, {"batch": 70000}),
+    (-1, {"split_ws": P + 128, "split_ws_bytes": 1 << 30}), (-3, {"batch": 70000}),
 ])
 def test_backward_refusals(lib, want, change):
     assert lib.fa_diff_bwd(ctypes.byref(_bwd(**change)), None) == want
