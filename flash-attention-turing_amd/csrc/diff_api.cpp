@@ -65,6 +65,11 @@ fa_diff_dlam dlam_of(const at::Tensor &dlam) {
     return l;
 }
 
+// Rows further apart than the kernels' 32-bit tile offsets reach (8 M elements) are copied, as misaligned ones are.
+constexpr int64_t kMostRowStride = int64_t(1) << 23;
+bool rows_near(const at::Tensor &t) { return t.size(-3) <= 1 || t.stride(-3) <= kMostRowStride; }
+at::Tensor usable(const at::Tensor &t) { return rows_near(t) ? aligned(t) : t.clone(at::MemoryFormat::Contiguous); }
+
 struct Varlen {
     const at::Tensor *cu_q, *cu_k;
     int max_q, max_k;
@@ -117,9 +122,9 @@ std::vector<std::optional<at::Tensor>> run_fwd(at::Tensor q, at::Tensor k, at::T
     fa_diff_fwd_args a{};
     set_sizes(a, q, k, x);
     a.lam = lam_of(lam, q);
-    q = aligned(q);
-    k = aligned(k);
-    v = aligned(v);
+    q = usable(q);
+    k = usable(k);
+    v = usable(v);
     at::Tensor out = at::empty(q.sizes(), q.options()), o2;
     if (save) o2 = at::empty(q.sizes(), q.options());
     at::Tensor lse = at::empty({2, a.batch, a.nheads, a.lse_seqlen}, q.options().dtype(at::kFloat));
@@ -165,12 +170,12 @@ std::vector<std::optional<at::Tensor>> run_bwd(at::Tensor q, at::Tensor k, at::T
     TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 4 &&
                     lse.size(0) == 2 && lse.size(1) == a.batch && lse.size(2) == a.nheads && lse.size(3) == a.lse_seqlen,
                 "lse must be a contiguous float32 tensor of shape [2, batch_size, nheads, seqlen_q]");
-    q = aligned(q);
-    k = aligned(k);
-    v = aligned(v);
+    q = usable(q);
+    k = usable(k);
+    v = usable(v);
     out = aligned(out);
     o2 = aligned(o2);
-    dout = aligned(dout);
+    dout = usable(dout);
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                dv = at::empty(v.sizes(), v.options()), dlam;
     const bool none = q.numel() == 0 || k.numel() == 0;
@@ -266,6 +271,7 @@ void check_cache(const at::Tensor &c, const at::Tensor &q, const char *name) {
     check_like(c, q, name);
     TORCH_CHECK(c.dim() == 4, name, " must be a rank-4 tensor");
     TORCH_CHECK(is_aligned(c), name, " must have a contiguous last dimension and 16-byte aligned rows");
+    TORCH_CHECK(rows_near(c), name, " must have tokens at most 2^23 elements apart");
 }
 
 std::vector<at::Tensor> diff_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor lam,

@@ -411,6 +411,8 @@ static int check_diff_kv(const fa_diff_kvcache_args *p) {
         return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.q, &a.k_cache, &a.v_cache, &a.o})
         if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.k_cache, &a.v_cache})
+        if (t->row_stride < 0 || t->row_stride > kDiffMaxRowStride) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.k_new, &a.v_new})
         if (check_tensor(*t, a.seqlen_new > 0)) return FA_ERR_INVALID_ARG;
     if (a.ws_bytes < int64_t(fa_diff_kvcache_ws_bytes(&a)) || (reinterpret_cast<uintptr_t>(a.ws) & 255u) ||

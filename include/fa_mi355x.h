@@ -278,8 +278,9 @@ int fa_fwd_kvcache_noalloc(const fa_kvcache_args *args, void *stream);
  * their head_dim channels (map 1 the first half, map 2 the second), v has
  * head_dim channels:
  *   o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v.
- * All tensors are laid out as those of fa_fwd / fa_bwd; dtype is FA_FP16 or
- * FA_BF16 for all of them.  No counterpart in the reference.
+ * All tensors are laid out as those of fa_fwd / fa_bwd, with row strides of 0 to
+ * 2^23 elements (o, o2 and the gradients: any); dtype is FA_FP16 or FA_BF16 for
+ * all of them.  No counterpart in the reference.
  */
 enum { FA_FP16 = 0, FA_BF16 = 1 };
 

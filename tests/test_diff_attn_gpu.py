@@ -154,6 +154,28 @@ def test_layouts(device):
         assert_within(name, x.grad, want[name])
 
 
+def test_rows_far_apart(device):
+    # Rows 2^23 + 64 elements apart, past the tiles' 32-bit offsets, are copied; 2^23 apart they are read in place.
+    q, k, v, lam, do = _inputs(device, 1, 70, 70, 2, 2, 64, "head", torch.float16, 10)
+    want = _check(q, k, v, lam, do, True)
+    for far in ((1 << 23) + 64, 1 << 23):
+        pool = torch.zeros(70 * far, dtype=torch.float16, device=device)
+        x = pool.as_strided(q.shape, (0, far, 64, 1))
+        for i in range(3):
+            x.copy_((q, k, v)[i])
+            leaves = [y.detach().requires_grad_() for y in (q, k, v)]
+            leaves[i] = x.detach().requires_grad_()
+            out = fai.flash_diff_attn_func(*leaves, lam, causal=True)
+            assert torch.equal(out, want["out"])
+            for name, y in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)):
+                assert torch.equal(y, want[name])
+        x.copy_(do)
+        leaves = [y.detach().requires_grad_() for y in (q, k, v)]
+        out = fai.flash_diff_attn_func(*leaves, lam, causal=True)
+        for name, y in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, x)):
+            assert torch.equal(y, want[name])
+
+
 def test_broadcast_lam_gets_its_summed_gradient(device):
     q, k, v, _, do = _inputs(device, 2, 40, 40, 4, 2, 64, "layer", torch.float16, 9)
     lam = torch.tensor([0.3, 0.5, 0.7, 0.9], device=device).requires_grad_()

@@ -178,7 +178,8 @@ def _kv(**more):
     (-2, {"head_dim": 96}), (-2, {"dtype": 7}), (-1, {"nheads_k": 3}), (-1, {"num_splits": -1}), (-1, {"cache_seqlens": None}),
     (-1, {"block_table": P, "page_block_size": 100, "num_pages": 4}), (-1, {"block_table": P, "page_block_size": 64}),
     (-1, {"block_table": P, "page_block_size": 64, "num_pages": 4, "cache_batch_idx": P}),
-    (-1, {"seqlen_new": 1}), (-1, {"k_cache": _tensor(P + 8)}), (-3, {"cache_capacity": 100000}),
+    (-1, {"seqlen_new": 1}), (-1, {"k_cache": _tensor(P + 8)}), (-1, {"v_cache": _tensor(rs=(1 << 23) + 8)}),
+    (-3, {"cache_capacity": 100000}),
     (-3, {"cache_capacity": 100000, "ws": P + 16, "ws_bytes": 1 << 30}),
 ])
 def test_kvcache_refusals(lib, want, change):
