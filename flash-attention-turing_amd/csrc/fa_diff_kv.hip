@@ -19,7 +19,7 @@
 // last adds all partial results in the order of the chunks; none waits.
 //
 // Measured (32/8 heads of 128): 64 sequences of 1 k to 16 k tokens, paged, bf16,
-// one query each: 331 us for 1.73 GB, 5.2 TB/s (a large copy reaches 4.7); one
+// one query each: 305 us for 1.73 GB, 5.7 TB/s (a large copy reaches 4.7); one
 // sequence of 1500 tokens, where the chain of latencies counts (arguments, length,
 // tiles, partial results, counter, join): 11 us, 3 more for the append.
 #include <algorithm>
@@ -29,6 +29,40 @@
 namespace fa {
 
 constexpr int kDkThreads = 256, kDkTile = 32, kDkRows = 16;
+
+// g2l16 (fa_common.h) for bytes that are read once (one row tile): the caches are
+// asked not to keep them, and so evict nothing for them.  64 sequences of 1 k to
+// 16 k tokens, 32/8 heads of 128: 335 -> 305 us.  After other work has filled the
+// 256 MB memory-side cache: 404 -> 327, 32 x 500 to 5000 tokens 128 -> 81, 16 x 500
+// to 12000 120 -> 79 us; the last one repeated with nothing between, so that its
+// 240 MB stay there, 54 -> 67 us.
+__device__ __forceinline__ void g2l16_once(const void *g, char *lds_base) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off nt\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(g), "s"(__builtin_amdgcn_readfirstlane(lds_addr(lds_base)))
+        : "memory");
+}
+
+// A wave's copy of kDkTile rows of K or V, swizzled as TileReader reads them; rows past last_row re-read it.
+template <int HD, bool ONCE>
+__device__ __forceinline__ void diff_kv_tile(char *tile, const f16 *src, int64_t rs, int last_row, int lane) {
+    constexpr int KCH = HD / 8;
+#pragma unroll
+    for (int i = 0; i < kDkTile * KCH / 64; ++i) {
+        const int p = i * 64 + lane, row = p / KCH, c = p % KCH;
+        const f16 *g = src + min(row, last_row) * rs + 8 * (c ^ swz<KCH>(row));
+        if constexpr (ONCE)
+            g2l16_once(g, tile + i * 1024);
+        else
+            g2l16(g, tile + i * 1024);
+    }
+}
 
 __device__ __forceinline__ int diff_kv_err(const fa_diff_kvcache_args &a, int b, int &L0, int &row) {
     L0 = a.cache_seqlens[b];
@@ -156,8 +190,14 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
                         int64_t(hk) * a.k_cache.head_stride;
         const f16 *vb = (const f16 *)a.v_cache.ptr + line * a.v_cache.batch_stride + int64_t(at) * vrs +
                         int64_t(hk) * a.v_cache.head_stride;
-        dma_tile<HD, kDkTile, 64>(slot + st * STAGE, kb, krs, 0, L - 1 - p0, 0, lane);
-        dma_tile<HD, kDkTile, 64>(slot + st * STAGE + TILE, vb, vrs, 0, L - 1 - p0, 0, lane);
+        char *const ks = slot + st * STAGE;
+        if (row_tiles == 1) {
+            diff_kv_tile<HD, true>(ks, kb, krs, L - 1 - p0, lane);
+            diff_kv_tile<HD, true>(ks + TILE, vb, vrs, L - 1 - p0, lane);
+        } else {
+            diff_kv_tile<HD, false>(ks, kb, krs, L - 1 - p0, lane);
+            diff_kv_tile<HD, false>(ks + TILE, vb, vrs, L - 1 - p0, lane);
+        }
     };
     TileReader<HD> rd;
     rd.init(lane);
