@@ -15,7 +15,7 @@
 // plans are a few dependent reads in one workgroup, which is latency.  Measured:
 // 256 rows forked from 16 parents (half a page of 8 heads of 128, K and V, each):
 // copies 32 us for 233 MB, plan 9, alloc and free 4 each; 796 of a pool's 1600
-// pages compacted: moves 161 us, plan 7; a pool of 64 pages: 5 and 4.
+// pages compacted: moves 155 us, plan 7; a pool of 64 pages: 5 and 4.
 #include <algorithm>
 
 #include "fa_common.h"
@@ -113,7 +113,11 @@ __global__ __launch_bounds__(kPgThreads) void pg_alloc_kernel(const fa_kvpages_a
 }
 
 // Copies pieces [piece0, piece0 + kPgSlice) of the first `tokens` tokens of page
-// src to page dst, of K (which = 0) or V.
+// src to page dst, of K (which = 0) or V.  ONCE: the source is in no other copy, so
+// the caches are asked to keep neither side (a pool of 1600 pages, half in use,
+// compacted: 161 -> 155 us, 192 -> 168 after other work; a fork's sources, 16 children
+// each, are better kept: 60 us against 73).
+template <bool ONCE>
 __device__ __forceinline__ void pg_copy(const fa_kvpages_args &a, int which, int64_t src, int64_t dst, int tokens,
                                         int piece0) {
     const fa_tensor &t = which ? a.v_cache : a.k_cache;
@@ -132,10 +136,19 @@ __device__ __forceinline__ void pg_copy(const fa_kvpages_args &a, int which, int
         u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * kPgCopyThreads < n) v[u] = *reinterpret_cast<const u32x4 *>(s + at(i + u * kPgCopyThreads));
+            if (i + u * kPgCopyThreads < n) {
+                const u32x4 *p = reinterpret_cast<const u32x4 *>(s + at(i + u * kPgCopyThreads));
+                v[u] = ONCE ? __builtin_nontemporal_load(p) : *p;
+            }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * kPgCopyThreads < n) *reinterpret_cast<u32x4 *>(d + at(i + u * kPgCopyThreads)) = v[u];
+            if (i + u * kPgCopyThreads < n) {
+                u32x4 *p = reinterpret_cast<u32x4 *>(d + at(i + u * kPgCopyThreads));
+                if constexpr (ONCE)
+                    __builtin_nontemporal_store(v[u], p);
+                else
+                    *p = v[u];
+            }
     }
 }
 
@@ -152,7 +165,7 @@ __global__ __launch_bounds__(kPgCopyThreads) void pg_copy_kernel(const fa_kvpage
         if (part == 0) pg_report(a, FA_KV_BAD_LIST);
         return;
     }
-    pg_copy(a, part / slices, src, dst, a.page_block_size, part % slices * kPgSlice);
+    pg_copy<false>(a, part / slices, src, dst, a.page_block_size, part % slices * kPgSlice);
 }
 
 // Fork, the plan: checks the list and gives each child whose parent's last page
@@ -231,7 +244,7 @@ __global__ __launch_bounds__(kPgCopyThreads) void pg_fork_kernel(const fa_kvpage
     const int L = a.cache_seqlens[parent], full = L / a.page_block_size, rest = L - full * a.page_block_size;
     const int32_t *row = a.block_table + parent * a.block_table_stride;
     if (part >= 0) {
-        if (fresh >= 0) pg_copy(a, part / slices, row[full], fresh, rest, part % slices * kPgSlice);
+        if (fresh >= 0) pg_copy<false>(a, part / slices, row[full], fresh, rest, part % slices * kPgSlice);
         return;
     }
     int32_t *own = a.block_table + child * a.block_table_stride;
@@ -311,7 +324,7 @@ __global__ __launch_bounds__(kPgCopyThreads) void pg_compact_kernel(const fa_kvp
     const int64_t n = int64_t(ws[0]) * 2 * slices;
     for (int64_t w = blockIdx.x - table_wgs; w < n; w += gridDim.x - table_wgs) {
         const int k = int(w / (2 * slices)), part = int(w - int64_t(k) * 2 * slices);
-        pg_copy(a, part / slices, src[k], dst[k], a.page_block_size, part % slices * kPgSlice);
+        pg_copy<true>(a, part / slices, src[k], dst[k], a.page_block_size, part % slices * kPgSlice);
     }
 }
 
