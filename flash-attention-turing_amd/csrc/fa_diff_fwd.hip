@@ -195,7 +195,8 @@ __device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const Diff
     const float l0 = sum[0], l1 = sum[1];
     const bool packed_q = a.cu_seqlens_q != nullptr;
     const float lam = diff_lam(a.lam, w.b, w.q_start + qi, h);
-    const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    // A sum of 0 is that of a row without a visible key; one that is NaN goes on to the outputs.
+    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
     f16 *orow = (f16 *)a.o.ptr + base_off(a.o, packed_q, w.b, w.q_start, h) + int64_t(qi) * a.o.row_stride + 4 * hh;
     f16 *o2row = a.o2.ptr ? (f16 *)a.o2.ptr + base_off(a.o2, packed_q, w.b, w.q_start, h) +
                                 int64_t(qi) * a.o2.row_stride + 4 * hh
@@ -208,14 +209,14 @@ __device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const Diff
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 y[t] = o[1][dt][4 * a4 + t] * i1;
-                x[t] = l0 > 0.f ? fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]) : 0.f;
+                x[t] = l0 == 0.f ? 0.f : fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]);
             }
             *reinterpret_cast<f16x4 *>(orow + dt * 32 + 8 * a4) = pack4<BF>(x[0], x[1], x[2], x[3]);
             if (o2row) *reinterpret_cast<f16x4 *>(o2row + dt * 32 + 8 * a4) = pack4<BF>(y[0], y[1], y[2], y[3]);
         }
     if (D0 == 0 && hh == 0) {
-        lse_row[qi] = l0 > 0.f ? (mx[0] + log2_fast(l0)) * kLn2 : 0.f;
-        lse_row[plane + qi] = l1 > 0.f ? (mx[1] + log2_fast(l1)) * kLn2 : 0.f;
+        lse_row[qi] = l0 == 0.f ? 0.f : (mx[0] + log2_fast(l0)) * kLn2;
+        lse_row[plane + qi] = l1 == 0.f ? 0.f : (mx[1] + log2_fast(l1)) * kLn2;
     }
 }
 

@@ -1,0 +1,96 @@
+"""Differential attention at the ends of its types' ranges: NaN and infinite scores reach
+every output that the definition gives them.  Bounds are those of oracle/diff.py."""
+
+import pytest
+import torch
+
+import flash_attention_interface as fai
+from oracle.diff import assert_within, diff_attention
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"1": 0, "2": 1}  # the map whose scores a value spoils
+
+
+def _inputs(device, b, sq, sk, h, hk, d, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda *s: torch.randn(*s, generator=g).to(dtype).to(device)  # noqa: E731
+    lam = (torch.rand(h, generator=g) * 0.6 + 0.2).to(device)
+    return mk(b, sq, h, d), mk(b, sk, hk, d), mk(b, sk, hk, d), lam
+
+
+def _check_rows(name, got, want, bad):
+    """got NaN throughout where bad (of got's leading sizes), within its bound elsewhere."""
+    assert torch.isnan(got[bad]).all(), f"{name}: {int((~torch.isnan(got[bad])).sum())} elements hide a NaN"
+    assert_within(name, torch.where(bad[(...,) + (None,) * (got.dim() - bad.dim())], 0.0, got.double()),
+                  tuple(torch.where(bad[(...,) + (None,) * (x.dim() - bad.dim())], 0.0, x) for x in want))
+
+
+# Grids of one and of two wave groups; a key and a query in the middle of a tile, in its first and its last row.
+@pytest.mark.parametrize("which", ["k1", "k2", "q1", "q2", "inf1", "inf2"])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,causal,dtype", [
+    (1, 70, 90, 4, 2, 64, True, torch.float16),
+    (2, 40, 200, 2, 2, 128, False, torch.bfloat16),
+    (5, 130, 140, 64, 64, 64, True, torch.bfloat16),
+    (5, 33, 70, 64, 64, 128, False, torch.float16),
+])
+def test_a_nan_reaches_every_row_that_sees_it(device, b, sq, sk, h, hk, d, causal, dtype, which):
+    q, k, v, lam = _inputs(device, b, sq, sk, h, hk, d, dtype, 3)
+    m = HALF[which[-1]]
+    i, c = b - 1, m * (d // 2) + 5
+    if which.startswith("inf"):
+        q[..., c] = q[..., c].abs() + 0.25  # scores of +infinity: their softmax is NaN
+    want = diff_attention(q, k, v, lam, None, causal)
+    see = torch.ones(sq, sk, dtype=torch.bool, device=device)
+    if causal:
+        see = see.tril(sk - sq)
+    for at in (0, sk // 2, sk - 1) if which[0] != "q" else (0, sq // 2, sq - 1):
+        q1, k1 = q.clone(), k.clone()
+        rows = torch.zeros(b, sq, h, dtype=torch.bool, device=device)
+        if which[0] == "q":
+            q1[i, at, h - 1, c] = float("nan")
+            rows[i, at, h - 1] = bool(see[at].any())
+        else:
+            k1[i, at, hk - 1, c] = float("inf" if which.startswith("inf") else "nan")
+            rows[i, :, h - h // hk:] = see[:, at, None]
+        out = fai.flash_diff_attn_func(q1, k1, v, lam, causal=causal)
+        _check_rows("out", out, want["out"], rows)
+
+
+@pytest.mark.parametrize("which", ["k1", "k2", "q1", "q2", "inf1", "inf2"])
+@pytest.mark.parametrize("lens,sq,h,hk,d,dtype,splits", [
+    ([40, 20], 1, 8, 2, 128, torch.float16, 0),       # one piece
+    ([700, 1200], 3, 4, 2, 64, torch.bfloat16, 0),    # several, joined
+    ([900, 100], 1, 32, 8, 128, torch.bfloat16, 7),
+    ([300, 640], 40, 4, 1, 64, torch.float16, 0),     # several row tiles
+    ([350, 640], 300, 4, 4, 128, torch.float16, 0),   # the forward kernel
+])
+def test_a_nan_in_a_cache(device, lens, sq, h, hk, d, dtype, splits, which):
+    cap = 1280
+    q, kc, vc, lam = _inputs(device, 2, sq, cap, h, hk, d, dtype, 4)
+    m = HALF[which[-1]]
+    c = m * (d // 2) + 7
+    if which.startswith("inf"):
+        q[..., c] = q[..., c].abs() + 0.25
+    used = torch.tensor(lens, dtype=torch.int32, device=device)
+
+    def want(n, i):
+        return diff_attention(q[i:i + 1], kc[i:i + 1, :n], vc[i:i + 1, :n], lam, None, True)
+
+    n = lens[1]
+    for at in (0, n // 2, n - sq) if which[0] != "q" else (0, sq - 1):
+        q1, k1 = q.clone(), kc.clone()
+        rows = torch.zeros(2, sq, h, dtype=torch.bool, device=device)
+        if which[0] == "q":
+            q1[1, at, h - 1, c] = float("nan")
+            rows[1, at, h - 1] = True
+        else:
+            k1[1, at, hk - 1, c] = float("inf" if which.startswith("inf") else "nan")
+            rows[1, :, h - h // hk:] = (torch.arange(sq, device=device) + n - sq >= at)[:, None]
+        out, lse = fai.flash_diff_attn_with_kvcache(q1, k1, vc, lam, cache_seqlens=used, causal=True, num_splits=splits,
+                                                    return_softmax_lse=True)
+        for j in (0, 1):
+            w = want(lens[j], j)
+            _check_rows("out", out[j:j + 1], w["out"], rows[j:j + 1])
+            spoilt = rows[j:j + 1].transpose(1, 2)
+            _check_rows("lse", lse[m, j:j + 1], tuple(x[m] for x in w["lse"]), spoilt)
