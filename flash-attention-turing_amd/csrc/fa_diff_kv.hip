@@ -5,9 +5,9 @@
 // head.  The rows of a KV head are its query heads times the query positions;
 // a tile of 16 of them fills the 32 columns of one MFMA with both maps: column
 // c < 16 is row c's map 1, whose query operand is 0 on map 2's channels,
-// column 16 + c its map 2.  So the scores of both maps are one product with the
-// whole K row, and both products with V are one as well; the waste is in MFMA
-// slots, which wait for memory here.
+// column 16 + c its map 2.  So the scores of both maps take the products of one
+// whole K row, and both products with V are one; the waste is in MFMA slots, which
+// wait for memory here.
 //
 // A workgroup takes one chunk of the keys of one (sequence, KV head, row tile);
 // chunks have the same length for all sequences, so the items are of equal work
@@ -232,9 +232,16 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
             for (int gg = 0; gg < 2; ++gg) va[dt][gg] = rd.tr_operand(vs, 16 * gg, dt);
         wait_lds();
         if (k + NST < n_my) issue(my_first + 4 * (k + NST), st);
-        f32x16 s = mfma16<BF>(ka[0], qB[0], zero16());
+        // Each map's channels apart, of which a column takes its own map's: a key's infinity or NaN in the other
+        // map's channels, times the query operand's 0, would be NaN.
+        f32x16 s = mfma16<BF>(ka[0], qB[0], zero16()), s2 = mfma16<BF>(ka[HG], qB[HG], zero16());
 #pragma unroll
-        for (int g = 1; g < HD / 16; ++g) s = mfma16<BF>(ka[g], qB[g], s);
+        for (int g = 1; g < HG; ++g) {
+            s = mfma16<BF>(ka[g], qB[g], s);
+            s2 = mfma16<BF>(ka[HG + g], qB[HG + g], s2);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = map ? s2[r] : s[r];
         if (p0 + kDkTile > s1 || p0 + kDkTile - 1 > lim_min) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {

@@ -94,3 +94,16 @@ def test_a_nan_in_a_cache(device, lens, sq, h, hk, d, dtype, splits, which):
             _check_rows("out", out[j:j + 1], w["out"], rows[j:j + 1])
             spoilt = rows[j:j + 1].transpose(1, 2)
             _check_rows("lse", lse[m, j:j + 1], tuple(x[m] for x in w["lse"]), spoilt)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("m", [0, 1])
+@pytest.mark.parametrize("sq,d,dtype", [(1, 64, torch.bfloat16), (3, 128, torch.float16), (40, 128, torch.bfloat16)])
+def test_a_key_of_one_map_does_not_reach_the_other(device, sq, d, dtype, m, value):
+    h, hk, n = 4, 2, 700
+    q, kc, vc, lam = _inputs(device, 1, sq, 1024, h, hk, d, dtype, 6)
+    want = diff_attention(q, kc[:, :n], vc[:, :n], lam, None, True)["lse"]
+    kc[0, 300, :, m * (d // 2) + 1] = value
+    used = torch.tensor([n], dtype=torch.int32, device=device)
+    _, lse = fai.flash_diff_attn_with_kvcache(q, kc, vc, lam, cache_seqlens=used, causal=True, return_softmax_lse=True)
+    assert_within("lse", lse[1 - m], tuple(x[1 - m] for x in want))
