@@ -195,7 +195,9 @@ __device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const Diff
     const float l0 = sum[0], l1 = sum[1];
     const bool packed_q = a.cu_seqlens_q != nullptr;
     const float lam = diff_lam(a.lam, w.b, w.q_start + qi, h);
-    // A sum of 0 is that of a row without a visible key; one that is NaN goes on to the outputs.
+    // A sum of 0 is that of a map without a visible key (or with scores of -infinity alone); one that is NaN goes on
+    // to the outputs.
+    const bool none = l0 == 0.f && l1 == 0.f;
     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
     f16 *orow = (f16 *)a.o.ptr + base_off(a.o, packed_q, w.b, w.q_start, h) + int64_t(qi) * a.o.row_stride + 4 * hh;
     f16 *o2row = a.o2.ptr ? (f16 *)a.o2.ptr + base_off(a.o2, packed_q, w.b, w.q_start, h) +
@@ -209,7 +211,7 @@ __device__ __forceinline__ void diff_store(const fa_diff_fwd_args &a, const Diff
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 y[t] = o[1][dt][4 * a4 + t] * i1;
-                x[t] = l0 == 0.f ? 0.f : fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]);
+                x[t] = none ? 0.f : fmaf(o[0][dt][4 * a4 + t], i0, -lam * y[t]);
             }
             *reinterpret_cast<f16x4 *>(orow + dt * 32 + 8 * a4) = pack4<BF>(x[0], x[1], x[2], x[3]);
             if (o2row) *reinterpret_cast<f16x4 *>(o2row + dt * 32 + 8 * a4) = pack4<BF>(y[0], y[1], y[2], y[3]);
@@ -350,7 +352,8 @@ __global__ __launch_bounds__(kDiffThreads, HD == 64 ? 3 : 2) void diff_fwd_kerne
             float part[2];
 #pragma unroll
             for (int m = 0; m < 2; ++m) part[m] = diff_exps<MASK>(s[m], mx[m], cscale, lim - 32 * sub, hh);
-            if (__builtin_amdgcn_ballot_w64(!(fmaxf(part[0], part[1]) <= kDiffTop)) != 0) {
+            // (Each by itself: a maximum of both would pass over a NaN, which scores of -infinity give while m is -infinity.)
+            if (__builtin_amdgcn_ballot_w64(!(part[0] <= kDiffTop) || !(part[1] <= kDiffTop)) != 0) {
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     f32x16 t = zero16();

@@ -310,12 +310,14 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
     auto store = [&](int r, int d, f32x2 x1, float m1, float l1, f32x2 x2, float m2, float l2) FA_INLINE {
         const int row = rt * kDkRows + r, qp = row / G, h = hk * G + row - qp * G;
         const float lam = diff_lam(a.lam, b, qp, h);
-        // A sum of 0 is that of a row without a visible key; one that is NaN goes on to the outputs.
+        // A sum of 0 is that of a map without a visible key (or with scores of -infinity alone); one that is NaN goes
+        // on to the outputs.
         const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : lam / l2;
         f16 *out = (f16 *)a.o.ptr + int64_t(b) * a.o.batch_stride + int64_t(qp) * a.o.row_stride +
                    int64_t(h) * a.o.head_stride + d;
-        const f16x4 y = l1 == 0.f ? pack4<BF>(0.f, 0.f, 0.f, 0.f)
-                                  : pack4<BF>(x1[0] * i1 - x2[0] * i2, x1[1] * i1 - x2[1] * i2, 0.f, 0.f);
+        const f16x4 y = l1 == 0.f && l2 == 0.f
+                            ? pack4<BF>(0.f, 0.f, 0.f, 0.f)
+                            : pack4<BF>(x1[0] * i1 - x2[0] * i2, x1[1] * i1 - x2[1] * i2, 0.f, 0.f);
         *reinterpret_cast<uint32_t *>(out) = __builtin_bit_cast(u32x2, y)[0];
         if (d == 0) {
             float *lse = a.lse + (int64_t(b) * a.nheads + h) * a.seqlen_q + qp;

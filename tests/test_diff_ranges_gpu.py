@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import flash_attention_interface as fai
-from oracle.diff import assert_within, diff_attention
+from oracle.diff import _steps, assert_within, diff_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,32 @@ def test_a_key_of_one_map_does_not_reach_the_other(device, sq, d, dtype, m, valu
     used = torch.tensor([n], dtype=torch.int32, device=device)
     _, lse = fai.flash_diff_attn_with_kvcache(q, kc, vc, lam, cache_seqlens=used, causal=True, return_softmax_lse=True)
     assert_within("lse", lse[1 - m], tuple(x[1 - m] for x in want))
+
+
+# Scores of -infinity are keys that the map does not see.  Each wave group meets whole tiles of them in one map before
+# a tile that mixes them with finite ones.
+@pytest.mark.parametrize("m", [0, 1])
+@pytest.mark.parametrize("lead", [64, 128, None])  # None: all of them
+@pytest.mark.parametrize("b,h,d,dtype", [(1, 2, 64, torch.float16), (5, 64, 64, torch.bfloat16), (5, 64, 128, torch.float16)])
+def test_scores_of_minus_infinity(device, b, h, d, dtype, lead, m):
+    sq, sk = 40, (lead or 64) + 96
+    q, k, v, lam = _inputs(device, b, sq, sk, h, h, d, dtype, 5)
+    c = m * (d // 2)
+    q[..., c] = 1.0
+    hidden = torch.zeros(sk, dtype=torch.bool, device=device)
+    hidden[:lead] = True
+    if lead:
+        hidden[[lead + 6, lead + 36, lead + 66, lead + 95]] = True
+    low = k.clone()
+    low[:, hidden, :, c] = -float("inf")
+    out = fai.flash_diff_attn_func(q, low, v, lam)
+    # O_1 - lam O_2 from two calls of the definition without a second map, the first map's channels in front.
+    none = torch.zeros_like(lam)
+    swap = lambda x: torch.cat((x[..., d // 2:], x[..., : d // 2]), -1)  # noqa: E731
+    seen = (k[:, ~hidden], v[:, ~hidden])
+    sides = [seen if m == 0 else (k, v), seen if m == 1 else (k, v)]
+    o1, o2 = (diff_attention(f(q), f(x), y, none, None, False)["out"] for f, (x, y) in zip((lambda x: x, swap), sides))
+    u, t = _steps(dtype)
+    val = o1[0] - lam.double()[:, None] * o2[0]
+    bound = o1[1] + lam.double()[:, None] * o2[1]
+    assert_within("out", out, (val, bound + u * (val.abs() + bound) + t))
