@@ -45,37 +45,31 @@ constexpr int kDbThreads = 256;
 // the M dimension of its products, so a lane would need all 16 rows' values of
 // its accumulators: 24 16-byte LDS reads per 32 x 32 tile, a quarter of the LDS
 // time that bounded the kernel.  Instead the row's values enter the products, as
-// one more K step: a value v is the sum of three 16-bit numbers times the powers
-// of two in row_weights, which is exact to 2^-24 of it or 2^-36, whichever is
-// larger.  The scores so come out as S_m - LSE_m / scale, with log2 |lam| taken off
-// LSE_2, and dP as dP - D_1 and, by one more product, dP - D_2.  The sign of lam
-// goes in the fourth place, whose weight is 0.
+// one more K step, of bf16 whatever the tensors' type: a value v is the sum of three
+// bf16 numbers, each the rounding of what the ones before leave, which is v to 2^-27
+// of it (fp32 itself holds 2^-24) over all of fp32's range, and NaN if v is.  (fp16
+// pieces with weights held v up to 1.7e7 only, which D passes with a large dO, and
+// LSE / scale with a small scale.)  The scores so come out as S_m - LSE_m / scale, with
+// log2 |lam| taken off LSE_2, and dP as dP - D_1 and, by one more product, dP - D_2.
+// The sign of lam goes in the fourth place, whose weight is 0.
 struct DiffRowOps {
-    f16x4 lse1, lse2, nd1, e;  // of -LSE_1 / scale, -(LSE_2 - log |lam|) / scale, -D_1, D_1 - D_2
+    f16x4 lse1, lse2, nd1, e;  // bf16 bits of -LSE_1 / scale, -(LSE_2 - log |lam|) / scale, -D_1, D_1 - D_2
 };
 static_assert(sizeof(DiffRowOps) == 32, "copied as 32 rows a KiB");
-constexpr float kRowHi = 256.f, kRowLo = 1.f / 4096.f;
 
-template <bool BF>
-__device__ __forceinline__ float round16(float x) {
-    if constexpr (BF)
-        return float((__bf16)x);
-    else
-        return float((f16)x);
-}
-template <bool BF>
+// Scales below this count as 0 in the dK/dV kernel's scores, so that LSE / scale stays within fp32: they
+// move the exponent of a raw score up to 2^75 by less than 2^-25 (fp16 products are below 2^39).
+constexpr float kDiffFlatScale = 0x1p-100f;
+
 __device__ __forceinline__ f16x4 row_op(float v, float fourth) {
-    const float hi = round16<BF>(fminf(fmaxf(v * (1.f / kRowHi), -65504.f), 65504.f));
-    const float r = fmaf(-kRowHi, hi, v);
-    const float mid = round16<BF>(fminf(fmaxf(r, -65504.f), 65504.f));
-    return pack4<BF>(hi, mid, fminf(fmaxf((r - mid) * (1.f / kRowLo), -65504.f), 65504.f), fourth);
+    const float hi = float((__bf16)v), mid = float((__bf16)(v - hi));
+    return pack4<true>(hi, mid, (v - hi) - mid, fourth);
 }
-// B operand that weighs the first (which = 0) or second of two row_ops in an A
+// B operand that takes the first (which = 0) or second of two row_ops in an A
 // operand: K slots 0..3 and 4..7 of the lower lane half, the upper half's are 0.
-template <bool BF>
 __device__ __forceinline__ f16x8 row_weights(int which, int hh) {
-    const f16x4 w = pack4<BF>(hh ? 0.f : kRowHi, hh ? 0.f : 1.f, hh ? 0.f : kRowLo, 0.f);
-    const f16x4 z = pack4<BF>(0.f, 0.f, 0.f, 0.f);
+    const float one = hh ? 0.f : 1.f;
+    const f16x4 w = pack4<true>(one, one, one, 0.f), z = pack4<true>(0.f, 0.f, 0.f, 0.f);
     return which ? __builtin_shufflevector(z, w, 0, 1, 2, 3, 4, 5, 6, 7) : __builtin_shufflevector(w, z, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -322,12 +316,12 @@ __global__ __launch_bounds__(kDbThreads, HD == 64 ? 3 : 2) void diff_dq_kernel(c
     if (hh == 0) {
         const float D1 = sgn * d1, D2 = sgn * (d2 + ds2_sum);
         // exp2(cs (S - LSE / cs)); with a scale of 0 the dK/dV kernel takes scores of 0 and cs = 1.
-        const float per = a.softmax_scale != 0.f ? -1.f / cs : -1.f;
-        const float l2 = lam != 0.f ? lse2 - log2_fast(fabsf(lam)) : lse2 + 1000.f;  // 2^-1000 is 0
+        const float per = fabsf(a.softmax_scale) < kDiffFlatScale ? -1.f : -1.f / cs;
+        // A lam of 0 (or subnormal, which the logarithm does not take): 2^-1000 is 0.  (A NaN is neither.)
+        const float l2 = fabsf(lam) < 0x1p-126f ? lse2 + 1000.f : lse2 - log2_fast(fabsf(lam));
         a.dsum[lrow + qi] = -D2;
         DiffRowOps *ops = reinterpret_cast<DiffRowOps *>(a.dsum + diff_ops_at(a)) + lrow + qi;
-        *ops = DiffRowOps{row_op<BF>(lse1 * per, 0.f), row_op<BF>(l2 * per, lam < 0.f ? -1.f : 1.f), row_op<BF>(-D1, 0.f),
-                          row_op<BF>(D1 - D2, 0.f)};
+        *ops = DiffRowOps{row_op(lse1 * per, 0.f), row_op(l2 * per, lam < 0.f ? -1.f : 1.f), row_op(-D1, 0.f), row_op(D1 - D2, 0.f)};
     }
     int qo = qi;
     asm volatile("" : "+v"(qo));
@@ -447,7 +441,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
     const f16 *kp = (const f16 *)a.k.ptr + base_off(a.k, packed_k, b, rk.start, hk);
     const f16 *vp = (const f16 *)a.v.ptr + base_off(a.v, packed_k, b, rk.start, hk);
     const int causal_off = sk - sq;
-    const bool flat = a.softmax_scale == 0.f;  // scores of 0: see the dQ kernel
+    const bool flat = fabsf(a.softmax_scale) < kDiffFlatScale;  // scores of 0: see the dQ kernel
     const float cs = uniform(flat ? 1.f : a.softmax_scale * kLog2e);
     const int64_t qrs = a.q.row_stride, dors = a.dout.row_stride;
     const int kw0 = k0 + wave * 32, key = kw0 + col;
@@ -557,7 +551,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
         {
             int h0 = hh;
             asm volatile("" : "+v"(h0));  // formed per block, not held
-            const f16x8 w0 = row_weights<BF>(0, h0), w1 = row_weights<BF>(1, h0);
+            const f16x8 w0 = row_weights(0, h0), w1 = row_weights(1, h0);
             const f16x8 lses = lds_ld16(smem, ro);
             // Step u of the scores: map u % 2, K step u / 2 of its channels.
             f16x8 op[PS];
@@ -567,8 +561,8 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
             f16x8 kl[KL > 0 ? KL : 1];
 #pragma unroll
             for (int i = 0; i < KL; ++i) kl[i] = lds_ld16(smem + i * 1024, kat);
-            s[0] = mfma16<BF>(lses, w0, zero16());
-            s[1] = mfma16<BF>(lses, w1, zero16());
+            s[0] = mfma16<true>(lses, w0, zero16());
+            s[1] = mfma16<true>(lses, w1, zero16());
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
@@ -586,7 +580,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 #pragma unroll
             for (int g = 0; g < PIPE - 1; ++g) ldo(g);
             asm volatile("" : "+v"(h0));
-            dp = mfma16<BF>(lds_ld16(smem + 16, ro), row_weights<BF>(0, h0), zero16());
+            dp = mfma16<true>(lds_ld16(smem + 16, ro), row_weights(0, h0), zero16());
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 if (g + PIPE - 1 < NG) ldo(g + PIPE - 1);
@@ -614,7 +608,7 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
         {
             int h0 = hh;
             asm volatile("" : "+v"(h0));
-            dp = mfma16<BF>(lds_ld16(smem + 16, ro), row_weights<BF>(1, h0), dp);
+            dp = mfma16<true>(lds_ld16(smem + 16, ro), row_weights(1, h0), dp);
         }
         __builtin_amdgcn_sched_barrier(0);
         // dK of map 1 beside P, dV beside dS_2, dK of map 2.

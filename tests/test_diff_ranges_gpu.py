@@ -1,5 +1,9 @@
 """Differential attention at the ends of its types' ranges: NaN and infinite scores reach
-every output that the definition gives them.  Bounds are those of oracle/diff.py."""
+every output that the definition gives them, gradients of any finite size, scales and
+scores of any size.
+
+Bounds are those of oracle/diff.py, and exact equality where a power of two scales
+everything that is rounded."""
 
 import pytest
 import torch
@@ -136,3 +140,79 @@ def test_scores_of_minus_infinity(device, b, h, d, dtype, lead, m):
     val = o1[0] - lam.double()[:, None] * o2[0]
     bound = o1[1] + lam.double()[:, None] * o2[1]
     assert_within("out", out, (val, bound + u * (val.abs() + bound) + t))
+
+
+# ---------------------------------------------------------------------------
+# Gradients.
+
+
+def _inputs_and_dout(device, b, sq, sk, h, hk, d, dtype, seed):
+    do = torch.randn(b, sq, h, d, generator=torch.Generator().manual_seed(seed + 100)).to(dtype).to(device)
+    return *_inputs(device, b, sq, sk, h, hk, d, dtype, seed), do
+
+
+def _grads(q, k, v, lam, do, causal, scale=None):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, lam)]
+    return torch.autograd.grad(fai.flash_diff_attn_func(*leaves, softmax_scale=scale, causal=causal), leaves, do)
+
+
+@pytest.mark.parametrize("power", [23, 60, 100])
+@pytest.mark.parametrize("sq,sk,d,causal", [(70, 90, 64, True), (140, 140, 128, True), (40, 200, 128, False)])
+def test_gradients_scale_with_dout(device, sq, sk, d, causal, power):
+    """bf16: dO times a power of two gives every gradient times that power, bit for bit."""
+    q, k, v, lam, do = _inputs_and_dout(device, 1, sq, sk, 4, 2, d, torch.bfloat16, 7)
+    one = _grads(q, k, v, lam, do, causal)
+    much = _grads(q, k, v, lam, do * 2.0 ** power, causal)
+    for name, x, y in zip(("dq", "dk", "dv", "dlam"), one, much):
+        assert torch.equal(x * 2.0 ** power, y), f"{name}: off by up to {float((y / 2.0 ** power - x).abs().max())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [64.0, 2000.0])
+def test_large_dout(device, dtype, size):
+    q, k, v, lam, do = _inputs_and_dout(device, 1, 100, 120, 4, 2, 64, dtype, 8)
+    do = do * size
+    want = diff_attention(q, k, v, lam, None, True, do)
+    for name, x in zip(("dq", "dk", "dv", "dlam"), _grads(q, k, v, lam, do, True)):
+        assert_within(name, x, want[name])
+
+
+# |scale| down to where every score is 0 to fp32, and on both sides of 2^-100; a lam of 0 and a negative one.
+@pytest.mark.parametrize("scale", [1e-5, 3e-7, -1e-7, 1e-8, 1e-20, -1e-29, 2.0 ** -99, 2.0 ** -101, 1e-36])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_small_scales(device, d, dtype, scale):
+    q, k, v, lam, do = _inputs_and_dout(device, 1, 70, 300, 4, 2, d, dtype, 9)
+    lam = torch.tensor([0.0, 0.7, -1.5, 1e-40], device=device)
+    want = diff_attention(q, k, v, lam, scale, True, do)
+    out = fai.flash_diff_attn_func(q, k, v, lam, softmax_scale=scale, causal=True)
+    assert_within("out", out, want["out"])
+    for name, x in zip(("dq", "dk", "dv", "dlam"), _grads(q, k, v, lam, do, True, scale)):
+        assert_within(name, x, want[name])
+
+
+@pytest.mark.parametrize("dtype,size,scale", [
+    (torch.float16, 1500.0, 1e-7),
+    (torch.bfloat16, 1e4, 3e-9),
+    (torch.bfloat16, 1e10, -2e-21),
+])
+def test_large_scores_with_a_small_scale(device, dtype, size, scale):
+    """Scores near 1 from products that pass 2^24."""
+    q, k, v, lam, do = _inputs_and_dout(device, 1, 90, 150, 4, 2, 64, dtype, 10)
+    q, k = q * size, k * size
+    assert float((q[0, :, 0, :32].float() @ k[0, :, 0, :32].float().T).abs().max()) > 2.0 ** 24
+    want = diff_attention(q, k, v, lam, scale, True, do)
+    for name, x in zip(("dq", "dk", "dv", "dlam"), _grads(q, k, v, lam, do, True, scale)):
+        assert_within(name, x, want[name])
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_a_nan_in_the_gradients(device, d, dtype):
+    """A value that is NaN makes D NaN in every row that sees it, and with it dK of every key that those rows see, also
+    of the keys whose own products are finite."""
+    q, k, v, lam, do = _inputs_and_dout(device, 1, 150, 150, 2, 2, d, dtype, 11)
+    want = diff_attention(q, k, v, lam, None, True, do)
+    v[0, 0, 1, 3] = float("nan")
+    dq, dk, dv, dlam = _grads(q, k, v, lam, do, True)
+    assert torch.isnan(dk[:, :, 1]).all() and torch.isnan(dq[:, :, 1]).all() and torch.isnan(dlam[1])
+    for name, x in (("dq", dq), ("dk", dk), ("dv", dv)):  # the other head is as it was
+        assert_within(name, x[:, :, :1], tuple(y[:, :, :1] for y in want[name]))
