@@ -49,18 +49,17 @@ constexpr int kKvThreads = 256;
 constexpr int kKvWaves = 4;
 constexpr int kTile = 32;  // keys per wave tile
 
-__device__ __forceinline__ const f16 *kv_row_ptr(const fa_tensor &t, const fa_kvcache_args &a, int b, int cache_row,
-                                                 int hk, int pos) {
-    // Element pointer of token `pos` (logical) of sequence b, head hk.
-    int64_t off;
-    if (a.block_table) {
-        const int page = a.page_block_size;
-        const int blk = a.block_table[int64_t(b) * a.block_table_stride + pos / page];
-        off = int64_t(blk) * t.batch_stride + int64_t(pos % page) * t.row_stride;
-    } else {
-        off = int64_t(cache_row) * t.batch_stride + int64_t(pos) * t.row_stride;
-    }
-    return (const f16 *)t.ptr + off + int64_t(hk) * t.head_stride;
+// Whether a table entry names no page of the cache (cache_batch pages; 0: not checked).
+// Such an entry is reported; page 0 is read in its place and nothing is appended to it,
+// so that no access leaves the cache whatever the table holds: a table that
+// fa_kvpages_alloc could not fill for want of pages holds -1.
+__device__ __forceinline__ bool kv_bad_page(const fa_kvcache_args &a, int blk) {
+    return a.cache_batch > 0 && uint32_t(blk) >= uint32_t(a.cache_batch);
+}
+__device__ __forceinline__ int kv_page(const fa_kvcache_args &a, int blk) {
+    const bool bad = kv_bad_page(a, blk);
+    if (bad && a.status) atomicOr(a.status, FA_KV_BAD_PAGE);
+    return bad ? 0 : blk;
 }
 
 // Cache length and cache row of sequence b, checked against the cache: a
@@ -151,13 +150,24 @@ __device__ __forceinline__ void append_chunk(const fa_kvcache_args &a, const int
         return;
     }
     const int pos = sq.L0 + t;
-    const int cache_row = sq.row;
+    int line = sq.row, at = pos;  // cache row or page, and the token's place in it
+    if (a.block_table) {
+        const int pi = pos / a.page_block_size;
+        line = a.block_table[int64_t(b) * a.block_table_stride + pi];
+        at = pos - pi * a.page_block_size;
+        if (kv_bad_page(a, line)) {
+            if (a.status && hk == 0 && c == 0) atomicOr(a.status, FA_KV_BAD_PAGE);
+            return;
+        }
+    }
     const f16 *ks = (const f16 *)a.k_new.ptr + int64_t(b) * a.k_new.batch_stride + int64_t(t) * a.k_new.row_stride +
                     int64_t(hk) * a.k_new.head_stride + 8 * c;
     const f16 *vs = (const f16 *)a.v_new.ptr + int64_t(b) * a.v_new.batch_stride + int64_t(t) * a.v_new.row_stride +
                     int64_t(hk) * a.v_new.head_stride + 8 * c;
-    f16 *kd = const_cast<f16 *>(kv_row_ptr(a.k_cache, a, b, cache_row, hk, pos)) + 8 * c;
-    f16 *vd = const_cast<f16 *>(kv_row_ptr(a.v_cache, a, b, cache_row, hk, pos)) + 8 * c;
+    auto dst = [&](const fa_tensor &x) {
+        return (f16 *)x.ptr + int64_t(line) * x.batch_stride + int64_t(at) * x.row_stride + int64_t(hk) * x.head_stride + 8 * c;
+    };
+    f16 *kd = dst(a.k_cache), *vd = dst(a.v_cache);
     u32x4 kx = ldg16(ks);
     if (8 * c < a.rotary_dim) kx = rotary8(a, kx, ks - 8 * c, 8 * c, pos);
     *reinterpret_cast<u32x4 *>(kd) = kx;
@@ -499,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void kv_splitkv_kernel(const fa_kvcache_arg
             // hoisted out of the item loop (and spilled in the options instance).
             int i0 = tid;
             asm volatile("" : "+v"(i0));
-            for (int i = i0; i < n_pages; i += kKvThreads) pages[i] = bt[i];
+            for (int i = i0; i < n_pages; i += kKvThreads) pages[i] = kv_page(a, bt[i]);
         }
         __syncthreads();
 
@@ -521,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void kv_splitkv_kernel(const fa_kvcache_arg
                 if constexpr (LDS_PAGES)
                     blk = pages[pi - pg_first];
                 else
-                    blk = a.block_table[int64_t(b) * a.block_table_stride + pi];
+                    blk = kv_page(a, a.block_table[int64_t(b) * a.block_table_stride + pi]);
                 const int in_page = p0 - pi * page;
                 koff = int64_t(blk) * a.k_cache.batch_stride + int64_t(in_page) * krs;
                 voff = int64_t(blk) * a.v_cache.batch_stride + int64_t(in_page) * vrs;
@@ -923,7 +933,7 @@ __global__ __launch_bounds__(kKvThreads, 2) void kv_chunk_kernel(const fa_kvcach
     if (a.block_table && nb1 > nb0) {
         const int32_t *bt = a.block_table + int64_t(b) * a.block_table_stride + pg0;
         const int n_pages = (nb1 * BN - 1) / page - pg0 + 1;
-        for (int i = tid; i < n_pages; i += kKvThreads) pages[i] = bt[i];
+        for (int i = tid; i < n_pages; i += kKvThreads) pages[i] = kv_page(a, bt[i]);
     }
     wait_vmem();  // only the tile copies are in flight in the loop
     __syncthreads();

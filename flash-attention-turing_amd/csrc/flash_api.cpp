@@ -22,6 +22,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <vector>
@@ -347,7 +348,8 @@ std::vector<at::Tensor> mha_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::Te
     // the reference's arguments): an int32 device word; when given, the cache
     // capacity and cache_batch_idx bounds are checked on the device instead of
     // by host reads (no synchronisation, so the call can be graph-captured):
-    // 1 (capacity) / 2 (cache row) are ORed into it for the caller to report.
+    // 1 (capacity) / 2 (cache row) are ORed into it for the caller to report,
+    // and FA_KV_BAD_PAGE for a table entry in use that is no page of the cache.
     // lengths_checked (likewise): the caller has read cache_seqlens and checked
     // the capacity, so it is not read (and waited for) a second time.
     TORCH_CHECK(!out_opt.has_value(), "Turing KV-cache does not support a preallocated output tensor yet");
@@ -491,7 +493,8 @@ std::vector<at::Tensor> mha_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::Te
     a.causal = is_causal ? 1 : 0;
     a.num_splits = 1;
     a.cache_capacity = int32_t(seqlen_cache);
-    a.cache_batch = has_block_table ? 0 : i32(batch_size_cache, "cache batch size");
+    a.cache_batch = has_block_table ? i32(std::min(k_cache.size(0), v_cache.size(0)), "num_blocks")
+                                    : i32(batch_size_cache, "cache batch size");
     a.status = status;
     // Upstream's normalisation: a bound at least the cache capacity is no bound.
     if (window_size_left >= seqlen_cache) window_size_left = -1;

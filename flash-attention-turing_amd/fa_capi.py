@@ -300,7 +300,7 @@ def kvcache_args(q, k_cache, v_cache, o, lse, cache_seqlens, softmax_scale: floa
     a.out_accum, a.lse_accum = ptr(out_accum), ptr(lse_accum)
     a.batch_order = ptr(batch_order)
     a.cache_capacity = k_cache.shape[1] * (block_table.shape[1] if block_table is not None else 1)
-    a.cache_batch = k_cache.shape[0] if block_table is None else 0
+    a.cache_batch = k_cache.shape[0]
     a.status = ptr(status)
     a.local_window = int(tuple(window) != (-1, -1))
     a.window_left, a.window_right = window

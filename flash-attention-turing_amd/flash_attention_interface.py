@@ -405,7 +405,8 @@ def _kv_status(device: torch.device) -> torch.Tensor:
 
 def flash_attn_kvcache_check(device: Optional[Union[torch.device, int]] = None) -> None:
     """Report what earlier flash_attn_with_kvcache(validate=False) calls on a
-    device found wrong, then clear it.
+    device found wrong, then clear it.  Entries of a block_table that are in use
+    and name no page of the cache are reported here whatever validate was.
 
     Such calls read neither cache_seqlens nor cache_batch_idx on the host; the
     kernels check them instead.  A sequence that would overflow its cache, or
@@ -471,6 +472,12 @@ def flash_attn_with_kvcache(
     check every sequence themselves (an out-of-range one is neither appended to
     nor attended over) and record the error for flash_attn_kvcache_check(),
     so a decode step can be captured in a HIP graph.
+
+    The entries of block_table are checked by the kernels in both modes (reading
+    the table on the host would be a second wait): one that is in use and names
+    no page of the cache, such as the -1 that flash_attn_kvcache_alloc leaves
+    when the pages run out, is not appended to, page 0 is read in its place, and
+    flash_attn_kvcache_check() raises the error.
     """
     # Validation order of interface.py:807-867.
     _validate_unsupported_kvcache_args(rotary_cos, rotary_sin, cache_leftpad, window_size, softcap, alibi_slopes)
@@ -540,7 +547,11 @@ def flash_attn_with_kvcache(
             raise RuntimeError("k and v must be float16 tensors")
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
-    status = None if validate else _kv_status(q.device)
+    status = None
+    if not validate:
+        status = _kv_status(q.device)
+    elif block_table is not None and not (q.device.index not in _KV_STATUS and torch.cuda.is_current_stream_capturing()):
+        status = _kv_status(q.device)  # for the table's entries
     out, lse = _flash_attn_kvcache_forward(
         q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, causal, num_splits,
         status, tuple(window_size), softcap, cache_leftpad, alibi_slopes, rotary_cos, rotary_sin, rotary_interleaved,

@@ -190,7 +190,9 @@ typedef struct fa_kvcache_args {
      * appended to and is attended over no keys (O = 0, LSE = 0); with status
      * set, 1 (capacity) or 2 (cache row) is ORed into *status.  0 = unchecked. */
     int32_t cache_capacity;         /* tokens one sequence's cache holds (paged: pages * page size) */
-    int32_t cache_batch;            /* rows of a contiguous cache (bounds cache_batch_idx)         */
+    int32_t cache_batch;            /* rows of a contiguous cache (bounds cache_batch_idx); paged: pages of the
+                                       cache (a table entry in use outside them reads page 0, is not appended to
+                                       and ORs FA_KV_BAD_PAGE into *status), or 0: the table is not checked */
     int32_t *status;                /* device int32 error word, or NULL                            */
     /* Upstream FlashAttention options the reference's signature takes but rejects
      * (flash_attention_interface.py:617-634), with upstream's semantics: query i
