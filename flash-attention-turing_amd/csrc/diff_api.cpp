@@ -338,13 +338,13 @@ std::vector<at::Tensor> diff_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::T
     }
     at::Tensor out = at::empty(q.sizes(), q.options());
     at::Tensor lse = at::empty({2, batch, q.size(2), seqlen_q}, q.options().dtype(at::kFloat));
+    if (batch == 0 || (q.numel() == 0 && a.seqlen_new == 0)) return {out, lse};
     if (k_cache.numel() == 0) {
         TORCH_CHECK(a.seqlen_new == 0, "cache capacity is insufficient for the requested append length");
         out.zero_();
         lse.zero_();
         return {out, lse};
     }
-    if (q.numel() == 0 && a.seqlen_new == 0) return {out, lse};
     a.q = desc(q);
     a.o = desc(out);
     a.k_cache = desc(k_cache);

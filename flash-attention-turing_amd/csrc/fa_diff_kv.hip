@@ -455,11 +455,16 @@ static int check_diff_kv(const fa_diff_kvcache_args *p) {
     if (a.head_dim != 64 && a.head_dim != 128) return FA_ERR_UNSUPPORTED;
     if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
     if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_new < 0 || a.nheads <= 0 || a.nheads_k <= 0 ||
-        a.nheads % a.nheads_k != 0 || a.num_splits < 0 || a.cache_capacity < 0 || !a.lse || !a.lam.ptr || !a.cache_seqlens)
+        a.nheads % a.nheads_k != 0 || a.num_splits < 0 || a.cache_capacity < 0)
         return FA_ERR_INVALID_ARG;
+    if (a.batch == 0) return FA_OK;  // tensors of no sequences have no address
+    const bool queries = a.seqlen_q > 0;  // none: an append alone
+    if (!a.cache_seqlens || (queries && (!a.lse || !a.lam.ptr))) return FA_ERR_INVALID_ARG;
     if (a.block_table && (a.cache_batch_idx || a.page_block_size <= 0 || a.page_block_size % 64 != 0 || a.num_pages <= 0))
         return FA_ERR_INVALID_ARG;
-    for (const fa_tensor *t : {&a.q, &a.k_cache, &a.v_cache, &a.o})
+    for (const fa_tensor *t : {&a.q, &a.o})
+        if (check_tensor(*t, queries)) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.k_cache, &a.v_cache})
         if (check_tensor(*t, true)) return FA_ERR_INVALID_ARG;
     for (const fa_tensor *t : {&a.k_cache, &a.v_cache})
         if (t->row_stride < 0 || t->row_stride > kDiffMaxRowStride) return FA_ERR_INVALID_ARG;

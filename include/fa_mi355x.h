@@ -349,7 +349,8 @@ int fa_diff_bwd(const fa_diff_bwd_args *args, void *stream);
 /*
  * Differential attention over a key-value cache, laid out and checked on the
  * device as in fa_kvcache_args: k_new / v_new are appended at cache_seqlens,
- * then seqlen_q queries attend over L = cache_seqlens + seqlen_new keys.
+ * then seqlen_q queries attend over L = cache_seqlens + seqlen_new keys.  With
+ * seqlen_q 0 the append alone runs (q, o, lam and lse may be NULL).
  */
 typedef struct fa_diff_kvcache_args {
     fa_tensor q, k_cache, v_cache, k_new, v_new, o;
