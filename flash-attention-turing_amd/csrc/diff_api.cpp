@@ -106,6 +106,12 @@ void set_sizes(Args &a, const at::Tensor &q, const at::Tensor &k, const Varlen *
     a.dtype = dtype_of(q);
 }
 
+// Whether no row sees a key: empty tensors, or maxima of 0, to which packed sequences are cut.
+template <class Args>
+bool no_pairs(const Args &a, const at::Tensor &q, const at::Tensor &k) {
+    return q.numel() == 0 || k.numel() == 0 || a.seqlen_q == 0 || a.seqlen_k == 0;
+}
+
 // The descriptor of a rank-3 or rank-4 tensor; a size of 1 has no stride (torch leaves any number there).
 fa_tensor desc(const at::Tensor &t) {
     fa_tensor d = t.dim() == 3 ? desc3(t) : desc4(t);
@@ -131,7 +137,7 @@ std::vector<std::optional<at::Tensor>> run_fwd(at::Tensor q, at::Tensor k, at::T
     auto got = [&]() {
         return std::vector<std::optional<at::Tensor>>{out, save ? std::optional<at::Tensor>(o2) : std::nullopt, lse};
     };
-    if (q.numel() == 0 || k.numel() == 0) {  // no row sees a key
+    if (no_pairs(a, q, k)) {
         out.zero_();
         if (save) o2.zero_();
         lse.zero_();
@@ -178,7 +184,7 @@ std::vector<std::optional<at::Tensor>> run_bwd(at::Tensor q, at::Tensor k, at::T
     dout = usable(dout);
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                dv = at::empty(v.sizes(), v.options()), dlam;
-    const bool none = q.numel() == 0 || k.numel() == 0;
+    const bool none = no_pairs(a, q, k);
     if (need_dlam)  // packed rows of no sequence read 0
         dlam = none || (x && lam.dim() == 2) ? at::zeros(lam.sizes(), lam.options().memory_format(at::MemoryFormat::Contiguous))
                                              : at::empty(lam.sizes(), lam.options().memory_format(at::MemoryFormat::Contiguous));

@@ -1,4 +1,4 @@
-"""Calls of differential attention with nothing to attend from."""
+"""Calls of differential attention with nothing to attend from or over."""
 
 import pytest
 import torch
@@ -47,3 +47,18 @@ def test_append_without_sequences(device, sq):
         out, lse = fai.flash_diff_attn_with_kvcache(q, c, c.clone(), torch.zeros(4, device=device), k, k,
                                                     cache_seqlens=lens, block_table=table, return_softmax_lse=True)
         assert out.shape == q.shape and lse.shape == (2, 0, 4, sq)
+
+
+@pytest.mark.parametrize("max_q,max_k", [(0, 8), (8, 0), (0, 0)])
+@pytest.mark.parametrize("kind", ["layer", "head", "token"])
+def test_packed_maxima_of_zero(device, max_q, max_k, kind):
+    # Sequences are cut to the call's maxima: no row sees a key, and outputs and gradients are 0.
+    rows, h, hk, d = 9, 4, 2, 128
+    lam = torch.rand({"layer": (), "head": (h,), "token": (rows, h)}[kind]).to(device)
+    leaves = [x.requires_grad_() for x in (_mk(device, rows, h, d), _mk(device, rows, hk, d), _mk(device, rows, hk, d), lam)]
+    for cu in ([0, 0, 0], [0, 4, 9]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=device)
+        out = fai.flash_diff_attn_varlen_func(*leaves, cu, cu, max_q, max_k, causal=True)
+        assert out.shape == (rows, h, d) and not out.any()
+        for x, g in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
+            assert g.shape == x.shape and not g.any()
