@@ -567,8 +567,9 @@ def flash_attn_with_kvcache(
 class FlashDiffAttnFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, softmax_scale, causal, is_grad_enabled):
-        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        # (Before the copies of strided channels, which require no gradient here.)
         save = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
         out, o2, lse = flash_attn_gpu.diff_fwd(q, k, v, lam, softmax_scale, causal, save)
         if save:
             ctx.save_for_backward(q, k, v, lam, out, o2, lse)
@@ -588,8 +589,9 @@ class FlashDiffAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
                 is_grad_enabled):
-        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        # (Before the copies of strided channels, which require no gradient here.)
         save = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
         out, o2, lse = flash_attn_gpu.diff_varlen_fwd(
             q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal, save
         )

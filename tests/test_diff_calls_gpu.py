@@ -1,9 +1,11 @@
-"""Calls of differential attention with nothing to attend from or over."""
+"""Calls of differential attention with nothing to attend from or over, and with layouts that
+need a copy."""
 
 import pytest
 import torch
 
 import flash_attention_interface as fai
+from oracle.diff import assert_within, diff_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +64,24 @@ def test_packed_maxima_of_zero(device, max_q, max_k, kind):
         assert out.shape == (rows, h, d) and not out.any()
         for x, g in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
             assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradients_of_strided_channels(device, packed):
+    # q, k and v whose last dimension is strided are copied; all of them get gradients, lam none.
+    b, s, h, d = 2, 50, 2, 64
+    base = [_mk(device, b, s, d, h, seed=i).transpose(2, 3) for i in range(3)]
+    do, lam = _mk(device, b, s, h, d, seed=5), torch.rand(h).to(device)
+    want = diff_attention(*(x.contiguous() for x in base), lam, None, True, do)
+    leaves = [x.detach().requires_grad_() for x in base]
+    assert all(x.stride(-1) != 1 for x in leaves)
+    if packed:
+        cu = torch.tensor([0, s, 2 * s], dtype=torch.int32, device=device)
+        flat = [x.flatten(0, 1) for x in leaves]
+        assert all(x.stride(-1) != 1 for x in flat)
+        out = fai.flash_diff_attn_varlen_func(*flat, lam, cu, cu, s, s, causal=True).view(b, s, h, d)
+    else:
+        out = fai.flash_diff_attn_func(*leaves, lam, causal=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        assert_within(name, x, want[name])
