@@ -4,6 +4,8 @@
 #include <algorithm>
 #include <optional>
 #include <tuple>
+#include <utility>
+#include <vector>
 
 #include "api_common.h"
 
@@ -13,6 +15,22 @@ void check_ints(const at::Tensor &t, const at::Device &device, int64_t dim, cons
     TORCH_CHECK(t.is_cuda() && t.device() == device, name, " must be on the device of the cache");
     TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && (t.numel() == 0 || dim == 0 || t.stride(-1) == 1 || t.size(-1) == 1),
                 name, " must be an int32 tensor of rank ", dim, " with a contiguous last dimension");
+}
+
+// Whether two of a cache's elements may share a place: of the sizes over 1, in the order of their strides, each
+// stride has to pass what those before it span, as in any slice and order of a dense tensor.  Tokens or heads that a
+// stride of 0 repeats within a page are one place.
+bool may_overlap(const at::Tensor &c) {
+    std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+    for (int64_t i = 0; i < c.dim(); ++i)
+        if (c.size(i) > 1 && (i == 0 || c.stride(i) != 0)) dims.emplace_back(c.stride(i), c.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t span = 1;
+    for (const auto &[stride, size] : dims) {
+        if (stride < span) return true;
+        span += (size - 1) * stride;
+    }
+    return false;
 }
 
 int32_t *ints(const std::optional<at::Tensor> &t) { return t.has_value() ? t->data_ptr<int32_t>() : nullptr; }
@@ -36,7 +54,7 @@ struct Call {
                         c.stride(0) * e % 16 == 0 && c.stride(1) * e % 16 == 0 && c.stride(2) * e % 16 == 0 &&
                         (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0,
                     name, " must have a contiguous last dimension and 16-byte aligned rows");
-        TORCH_CHECK(c.size(0) == 1 || c.stride(0) > 0, "pages of ", name, " must not overlap");
+        TORCH_CHECK(!may_overlap(c), "pages of ", name, " must not overlap");
         return fa_tensor{c.data_ptr(), c.stride(0) * e, c.stride(1) * e, c.stride(2) * e};
     }
     void cache(const at::Tensor &k, const at::Tensor &v) {
