@@ -341,11 +341,12 @@ __global__ __launch_bounds__(kDbThreads, HD == 64 ? 3 : 2) void diff_dq_kernel(c
 // K rows live in registers (S's B operands), V rows in LDS (dP's), and every
 // 32-query block of Q, dO and the rows' D, LSE and lam goes HBM -> LDS in two
 // stages.  With lp = lam P_2: P = P_1 - lp feeds dV, dS_1 = P_1 (dP - D_1) and
-// lp (dP - D_2) feed dK; the latter's sign is applied at the end.  The LDS bounds
-// it: per 32 x 32 tile 26 plain operand reads (5.7 cycles of the CU) and 32
-// transposed ones (8.1) against 36 MFMAs, with eight waves on a CU.  SPLIT: S
-// workgroups share the steps (heads of the group x query blocks) of an item and
-// sum their dK / dV (diff_dkdv_sum).
+// lp (dP - D_2) feed dK; the latter's sign is applied at the end.  At 128 channels
+// MFMA and VALU bound it (58 to 61 and 56 to 58 % of the cycles; LDS issue 12 to 13
+// %).  At 64 channels neither does (37 and 59 %): its waves wait 30 % of the time, two
+// workgroups a CU being too few to fill in, and three spill.  SPLIT: S workgroups
+// share the steps (heads of the group x query blocks) of an item and sum their
+// dK / dV (diff_dkdv_sum).
 //
 // Of an item's S workgroups each stores its partial sums and then counts itself;
 // the one that counts last, or finds all others counted before it has stored
@@ -709,7 +710,9 @@ __global__ __launch_bounds__(kDbThreads, 2) void diff_dkdv_kernel(const fa_diff_
 // dlam from the rows' -D_2 (the start of the workspace, written by the dQ kernel).
 // A lam for each row: one value each, transposed.  One that rows share: one
 // workgroup per head sums its rows in fp64 in a fixed order, and for a lam of
-// all heads the second launch sums the heads.
+// all heads the second launch sums the heads.  It takes a batch's sequences one
+// after the other: 10 us for 16 of them, but 1.8 ms for 4096 of 8 tokens (16 heads)
+// beside 1.0 ms for the rest of the step.
 __global__ __launch_bounds__(1024) void diff_dlam_rows_kernel(const fa_diff_bwd_args a) {
     for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
         const DiffRows rq = diff_rows(a.cu_seqlens_q, b, a.seqlen_q, a.dq_rows);

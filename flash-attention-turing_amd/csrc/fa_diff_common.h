@@ -60,14 +60,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-__device__ __forceinline__ float max16(const f32x16 &s) {
-    float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]);
-    a = max3(a, s[6], s[7]);
-    b = max3(b, s[8], s[9]);
-    a = max3(a, s[10], s[11]);
-    b = max3(b, s[12], s[13]);
-    return max3(max3(a, s[14], s[15]), b, b);
-}
 // max_xor32 (fa_common.h) without the canonicalisations.
 __device__ __forceinline__ float max2_xor32(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

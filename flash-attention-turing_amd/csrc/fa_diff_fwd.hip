@@ -5,8 +5,9 @@
 //   o = (P_1 - lam P_2) v
 //
 // Each wave owns 32 queries of one head and walks 64-key blocks, keeping for
-// both maps a running maximum, a sum and an fp32 O_m of its own (the sums that
-// would join them are known at the end only).  S_m^T = K_m Q_m^T puts keys on
+// both maps a sum and an fp32 O_m of its own against a maximum that is raised only
+// when it must be (diff_exps, below; the sums that would join the maps are known at
+// the end only).  S_m^T = K_m Q_m^T puts keys on
 // the MFMA M dimension, so a lane owns one query column, and P_m^T feeds
 // O_m^T += V^T P_m^T from the accumulators.  One transposed read of V serves
 // the products of both maps, which two calls of ordinary attention would read

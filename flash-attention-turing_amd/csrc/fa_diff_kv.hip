@@ -11,8 +11,9 @@
 //
 // A workgroup takes one chunk of the keys of one (sequence, KV head, row tile);
 // chunks have the same length for all sequences, so the items are of equal work
-// whatever the lengths, and a row's sum does not depend on the rest of the
-// batch.  Its four waves walk 32-key tiles (tile t to wave t % 4), each through
+// whatever the lengths.  That length follows from num_splits and the capacity, and
+// a row's sum does not depend on the rest of the batch; with num_splits 0 it is
+// chosen by the batch's items too (diff_kv_chunk).  Its four waves walk 32-key tiles (tile t to wave t % 4), each through
 // LDS slots of its own: operands go to registers, the next copy into the same
 // slot goes out, then the tile is computed, with no barrier in the loop.  The
 // waves merge through LDS.  Of a sequence's chunks, the workgroup that counts
@@ -21,7 +22,11 @@
 // Measured (32/8 heads of 128): 64 sequences of 1 k to 16 k tokens, paged, bf16,
 // one query each: 305 us for 1.73 GB, 5.7 TB/s (a large copy reaches 4.7); one
 // sequence of 1500 tokens, where the chain of latencies counts (arguments, length,
-// tiles, partial results, counter, join): 11 us, 3 more for the append.
+// tiles, partial results, counter, join): 11 us, 3 more for the append.  Both in
+// tables no wider than the longest sequence.  The host knows the capacity only, not
+// the lengths, so a wider table means longer chunks and fewer of them: the one
+// sequence in a table of 131072 tokens 25 us a call against 15, eight of 8000 tokens
+// 69 against 59, the 64 sequences 300 against 299.
 #include <algorithm>
 
 #include "fa_diff_common.h"
@@ -73,7 +78,7 @@ __device__ __forceinline__ int diff_kv_err(const fa_diff_kvcache_args &a, int b,
     return err;
 }
 
-// Append (one 16-byte chunk of K and of V a thread) after order_wgs workgroups
+// Append (one 16-byte chunk of K and of V a thread) after clear_wgs workgroups
 // that clear the split counters.
 __global__ __launch_bounds__(256) void diff_kv_prep_kernel(const fa_diff_kvcache_args a, int32_t *const count,
                                                            const int n_count, const int clear_wgs) {

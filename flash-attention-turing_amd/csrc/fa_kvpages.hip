@@ -153,7 +153,9 @@ __device__ __forceinline__ void pg_copy(const fa_kvpages_args &a, int which, int
 }
 
 // Copy: workgroup (pair, K or V, slice).  All pairs copy at once, so a pair whose
-// source another writes, or whose destination is another's, is not copied.
+// source another writes, or whose destination is another's, is not copied.  (Every
+// workgroup looks through the list for that: 500 pairs of 512 KB pages 208 us, 5.0
+// TB/s; 1000 pairs of 32 KB 22 us; with 10000 such pairs it shows, 333 us, 3.9 TB/s.)
 __global__ __launch_bounds__(kPgCopyThreads) void pg_copy_kernel(const fa_kvpages_args a, const int slices) {
     const int i = blockIdx.x / (2 * slices), part = blockIdx.x % (2 * slices);
     const int src = a.from[i], dst = a.to[i];

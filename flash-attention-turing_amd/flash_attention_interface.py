@@ -671,8 +671,9 @@ def flash_diff_attn_with_kvcache(
     The caches, k, v, cache_seqlens, cache_batch_idx and block_table are those of flash_attn_with_kvcache (fp16 or
     bf16; both maps' keys are the halves of a key's channels, so the two functions take the same caches; pages are a
     multiple of 64 tokens here); lam is a scalar, (nheads,) or (batch, seqlen_q, nheads).  num_splits > 0 cuts the
-    cache's capacity into that many pieces (calls of few query rows).  return_softmax_lse adds the log-sum-exp of both maps, fp32 (2, batch,
-    nheads, seqlen_q).
+    cache's capacity into that many pieces (calls of few query rows), and a row's bits then do not depend on the batch.
+    return_softmax_lse adds the log-sum-exp of both maps, fp32 (2, batch, nheads, seqlen_q).  A q without rows
+    (seqlen_q 0) appends alone.
 
     validate as there: True checks lengths, rows and pages on the host; False leaves that to the kernels, which
     record what is wrong for flash_attn_kvcache_check(): a sequence with a bad length or row is neither appended to
