@@ -43,10 +43,12 @@ struct DiffFwd {
 // work that bounds the kernel beside its MFMAs, and the exponentials waited for it:
 // b 4, s 4096, 16 heads of 128, causal, bf16 505 -> 455 us; 64 channels, s 4096,
 // fp16 672 -> 605 us; an exact maximum had cost 15 % more.
-// P is rounded to 16 bits for the product with V, as in ordinary attention (its 2^-9
-// in bf16 weighs as the output's own rounding does; carrying the remainder would take
-// 32 MFMAs more beside 48); O and the LSE are normalised by the fp32 sum of the
-// unrounded P.
+// P is rounded to 16 bits for the product with V, as in ordinary attention's forward (its
+// 2^-9 in bf16 weighs as the output's own rounding does).  Carrying the remainder, as
+// ordinary attention's prompt chunks over a cache and the decode kernel here do, takes 32
+// MFMAs more beside 48: two paged chunks of 512 queries over 4 k and 12 k tokens 256 ->
+// 361 us, for an error of 1.0 times a plain form's instead of 1.5 (bf16; fp16 1.3).  O
+// and the LSE are normalised by the fp32 sum of the unrounded P.
 constexpr float kDiffTop = 32768.f;
 
 // P of keys up to lim (relative to the first) in place of their scores; returns their sum.
