@@ -161,3 +161,26 @@ def test_a_serving_loop_that_runs_out_of_pages(device, diff):
         assert table.tolist() == model.table and refs.tolist() == model.refs
     for w in (kw, vw):
         assert torch.isnan(w[:GUARD]).all() and torch.isnan(w[GUARD + n:]).all()
+
+
+def test_a_checked_call_inside_a_capture(device, monkeypatch):
+    """A length that the host knows needs no read, so such a call can be captured with validate=True, also where no
+    status word was ever made; the table's entries are bounded without one."""
+    s = _setup(device, [700, 300, 900], 1, 4, 2, 64, 2, {})
+    table = s["table"].clone()
+    table[1, 1] = -1
+    call = lambda: fai.flash_attn_with_kvcache(s["q"], s["kp"], s["vp"], cache_seqlens=300, block_table=table,  # noqa: E731
+                                               causal=True, num_splits=2)
+    want = call()
+    with pytest.raises(RuntimeError, match="block_table entries in use"):
+        fai.flash_attn_kvcache_check()
+    torch.cuda.synchronize()
+    monkeypatch.setattr(fai, "_KV_STATUS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.isfinite(got).all()
+        assert torch.equal(call(), want)
