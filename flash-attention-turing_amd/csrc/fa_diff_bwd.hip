@@ -27,7 +27,7 @@
 // What bounds both is the matrix cores beside the VALU: dQ takes 48 MFMAs and 290
 // VALU instructions (64 exponentials) for 32 queries x 64 keys at 128 channels,
 // dK/dV 36 (4 of them for the row operands) and 210 for 32 x 32.  Counters: MFMA 48
-// to 55 and 58 to 61 % of dQ's and dK/dV's cycles, VALU 60 to 64 and 56 to 58 %.
+// to 55 and 58 to 61 % of dQ's and dK/dV's cycles, VALU 60 to 64 and 54 to 57 %.
 // b 4, s 4096, 16 heads of 128, causal, bf16: dQ 520 us, dK/dV 655 us (793 and 839
 // TFLOP/s of the formulas' products); b 1, s 8192, 32/8 heads, fp16: 925 and 1215 us
 // (892 and 905); a library product of 8192^3 runs at 1224 to 1280.
@@ -342,8 +342,8 @@ __global__ __launch_bounds__(kDbThreads, HD == 64 ? 3 : 2) void diff_dq_kernel(c
 // 32-query block of Q, dO and the rows' D, LSE and lam goes HBM -> LDS in two
 // stages.  With lp = lam P_2: P = P_1 - lp feeds dV, dS_1 = P_1 (dP - D_1) and
 // lp (dP - D_2) feed dK; the latter's sign is applied at the end.  At 128 channels
-// MFMA and VALU bound it (58 to 61 and 56 to 58 % of the cycles; LDS issue 12 to 13
-// %).  At 64 channels neither does (37 and 59 %): its waves wait 30 % of the time, two
+// MFMA and VALU bound it (58 to 61 and 54 to 57 % of the cycles; LDS issue 12 to 13
+// %).  At 64 channels neither does (37 and 58 %): its waves wait 31 % of the time, two
 // workgroups a CU being too few to fill in, and three spill.  SPLIT: S workgroups
 // share the steps (heads of the group x query blocks) of an item and sum their
 // dK / dV (diff_dkdv_sum).

@@ -20,7 +20,7 @@
 // last adds all partial results in the order of the chunks; none waits.
 //
 // Measured (32/8 heads of 128): 64 sequences of 1 k to 16 k tokens, paged, bf16,
-// one query each: 305 us for 1.73 GB, 5.7 TB/s (a large copy reaches 4.7); one
+// one query each: 307 us for 1.73 GB, 5.6 TB/s (a large copy reaches 4.7); one
 // sequence of 1500 tokens, where the chain of latencies counts (arguments, length,
 // tiles, partial results, counter, join): 11 us, 3 more for the append.  Both in
 // tables no wider than the longest sequence.  The host knows the capacity only, not
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kDkThreads, 2) void diff_kv_kernel(const fa_diff_kv
         l += rs;
         // P keeps 32 bits through the product, as hi + lo in the tensors' type: the matrix cores wait for memory here
         // (64 sequences of 1 k to 16 k tokens, bf16: 306.5 -> 307.3 us, and 1.4 times a plain form's error -> the same;
-        // one of 1500: 13.4 -> 13.6).
+        // one of 1500: 13.4 -> 13.6; four of 4096, 4 queries each, fp16: 31 -> 33).
 #pragma unroll
         for (int gg = 0; gg < 2; ++gg) {
             const f16x8 hi = pack16<BF>(s, 8 * gg);

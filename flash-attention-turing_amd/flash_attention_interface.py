@@ -406,7 +406,8 @@ def _kv_status(device: torch.device) -> torch.Tensor:
 def flash_attn_kvcache_check(device: Optional[Union[torch.device, int]] = None) -> None:
     """Report what earlier flash_attn_with_kvcache(validate=False) calls on a
     device found wrong, then clear it.  Entries of a block_table that are in use
-    and name no page of the cache are reported here whatever validate was.
+    and name no page of the cache, and negative lengths beside a block_table, are
+    reported here whatever validate was.
 
     Such calls read neither cache_seqlens nor cache_batch_idx on the host; the
     kernels check them instead.  A sequence that would overflow its cache, or
