@@ -13,11 +13,12 @@
 // chunks have the same length for all sequences, so the items are of equal work
 // whatever the lengths.  That length follows from num_splits and the capacity, and
 // a row's sum does not depend on the rest of the batch; with num_splits 0 it is
-// chosen by the batch's items too (diff_kv_chunk).  Its four waves walk 32-key tiles (tile t to wave t % 4), each through
-// LDS slots of its own: operands go to registers, the next copy into the same
-// slot goes out, then the tile is computed, with no barrier in the loop.  The
-// waves merge through LDS.  Of a sequence's chunks, the workgroup that counts
-// last adds all partial results in the order of the chunks; none waits.
+// chosen by the batch's items too (diff_kv_chunk).  A workgroup's four waves walk
+// 32-key tiles (tile t to wave t % 4), each through LDS slots of its own: operands
+// go to registers, the next copy into the same slot goes out, then the tile is
+// computed, with no barrier in the loop.  The waves merge through LDS.  Of a
+// sequence's chunks, the workgroup that counts last adds all partial results in
+// the order of the chunks; none waits.
 //
 // Measured (32/8 heads of 128): 64 sequences of 1 k to 16 k tokens, paged, bf16,
 // one query each: 307 us for 1.73 GB, 5.6 TB/s (a large copy reaches 4.7); one
