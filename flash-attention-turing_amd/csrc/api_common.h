@@ -59,3 +59,4 @@ inline at::Tensor optional_workspace(int64_t numel, const at::TensorOptions &opt
 // Bindings of the extension's other sources.
 void bind_diff(py::module_ &m);     // diff_api.cpp
 void bind_kvpages(py::module_ &m);  // kvpages_api.cpp
+void bind_rotary(py::module_ &m);   // rotary_api.cpp

@@ -633,4 +633,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("lengths_checked") = false);
     bind_diff(m);
     bind_kvpages(m);
+    bind_rotary(m);
 }

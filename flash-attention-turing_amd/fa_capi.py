@@ -30,6 +30,7 @@ FA_ERR_SCRATCH = -4
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _p = ctypes.c_void_p
 
 
@@ -124,6 +125,24 @@ class FaKvpagesArgs(ctypes.Structure):
     ]
 
 
+class FaRotaryTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("cos", _p), ("sin", _p), ("seqlen", _i32), ("rotary_dim", _i32), ("dtype", _i32), ("offset", _i64),
+        ("base", _f64), ("factor", _f64), ("original_seqlen", _f64), ("low_turns", _f64), ("high_turns", _f64),
+        ("attention_factor", _f64),
+    ]
+
+
+class FaRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", FaTensor), ("k", FaTensor), ("q_out", FaTensor), ("k_out", FaTensor), ("cos", _p), ("sin", _p),
+        ("cos_stride", _i64), ("sin_stride", _i64), ("positions", _p), ("positions_stride", _i64),
+        ("seqlen_offsets", _p), ("cu_seqlens", _p), ("batch", _i32), ("seqlen", _i32), ("nheads", _i32),
+        ("nheads_k", _i32), ("head_dim", _i32), ("rotary_dim", _i32), ("table_rows", _i32), ("offset", _i32),
+        ("interleaved", _i32), ("inverse", _i32), ("dtype", _i32), ("table_dtype", _i32),
+    ]
+
+
 _ARGP = {
     "fa_fwd": FaFwdArgs,
     "fa_bwd_preprocess": FaBwdArgs,
@@ -143,6 +162,8 @@ _ARGP = {
     "fa_kvpages_fork": FaKvpagesArgs,
     "fa_kvpages_free": FaKvpagesArgs,
     "fa_kvpages_compact": FaKvpagesArgs,
+    "fa_rotary_tables": FaRotaryTablesArgs,
+    "fa_rotary": FaRotaryArgs,
 }
 # Sizes of workspaces, of the same structs.
 _SIZES = {

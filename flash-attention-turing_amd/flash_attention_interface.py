@@ -17,6 +17,10 @@ and the pages of a paged cache
     flash_attn_kvcache_alloc, flash_attn_kvcache_copy_pages, flash_attn_kvcache_fork,
     flash_attn_kvcache_free, flash_attn_kvcache_compact
 
+and rotary positions
+
+    flash_attn_rotary_tables, flash_attn_rotary_func
+
 and the autograd classes FlashAttnFunc, FlashAttnQKVPackedFunc,
 FlashAttnKVPackedFunc, FlashAttnVarlenFunc, FlashAttnVarlenQKVPackedFunc,
 FlashAttnVarlenKVPackedFunc (:172-445).  Every call goes to the native
@@ -806,3 +810,101 @@ def flash_attn_kvcache_compact(k_cache, v_cache, block_table, page_refs) -> Tupl
     queued, until those pages are given out again."""
     _check_pages(block_table, page_refs=page_refs)
     return flash_attn_gpu.kvpages_compact(k_cache, v_cache, block_table, page_refs)
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions (no counterpart in the reference).
+
+
+def flash_attn_rotary_tables(
+    seqlen: int, rotary_dim: int, base: float = 10000.0, factor: float = 1.0, original_seqlen: Optional[int] = None,
+    low_turns: float = 1.0, high_turns: float = 32.0, attention_factor: float = 1.0, offset: int = 0,
+    dtype: torch.dtype = torch.float32, device: Union[torch.device, str, int, None] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin (seqlen, rotary_dim / 2) of the angles (offset + i) * f_j, f_j = base ** (-2 j / rotary_dim), computed
+    in 64 bits and rounded once to dtype (float32, float16 or bfloat16); rotary_dim is a multiple of 16.
+
+    For contexts longer than those of the training by a factor: f_j / factor, or, with original_seqlen (the training's
+    length), by the turns t that a pair makes in it: f_j for t >= high_turns, f_j / factor for t <= low_turns, and
+    f_j (keep + (1 - keep) / factor), keep = (t - low_turns) / (high_turns - low_turns), in between.  attention_factor
+    multiplies both tables, so that scores of rotated q and k grow by its square.
+
+    flash_attn_rotary_func takes them in any of the types, flash_attn_with_kvcache in float16."""
+    if rotary_dim <= 0 or rotary_dim % 16 != 0 or rotary_dim > 256:
+        raise ValueError("rotary_dim must be a multiple of 16 up to 256")
+    if seqlen < 0:
+        raise ValueError("seqlen must be non-negative")
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError("dtype must be torch.float32, torch.float16 or torch.bfloat16")
+    if not all(math.isfinite(x) for x in (base, factor, attention_factor)) or base <= 0 or factor <= 0:
+        raise ValueError("base and factor must be positive and finite, attention_factor finite")
+    if original_seqlen is not None and (original_seqlen <= 0 or not high_turns > low_turns):
+        raise ValueError("original_seqlen must be positive and high_turns larger than low_turns")
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise RuntimeError("rotary tables are made on a CUDA device")
+    cos, sin = (torch.empty((seqlen, rotary_dim // 2), dtype=dtype, device=device) for _ in range(2))
+    flash_attn_gpu.rotary_tables(cos, sin, offset, base, factor, original_seqlen or 0.0, low_turns, high_turns,
+                                 attention_factor)
+    return cos, sin
+
+
+class FlashAttnRotaryFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, *rest):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*(x for x in rest if isinstance(x, torch.Tensor)))
+        ctx.rest = tuple(None if isinstance(x, torch.Tensor) else (x,) for x in rest)
+        return tuple(flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest, False))
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        tensors = iter(ctx.saved_tensors)
+        rest = tuple(next(tensors) if x is None else x[0] for x in ctx.rest)
+        dq, dk = maybe_contiguous(dq), maybe_contiguous(dk)
+        if dq is None and dk is not None:  # a gradient of k alone
+            dk = flash_attn_gpu.rotary(dk, None, *rest, True)[0]
+        elif dq is not None:
+            dq, dk = flash_attn_gpu.rotary(dq, dk, *rest, True)
+        return (dq, dk) + (None,) * len(rest)
+
+
+def flash_attn_rotary_func(
+    q, k, rotary_cos, rotary_sin, rotary_interleaved: bool = True, positions: Optional[torch.Tensor] = None,
+    seqlen_offsets: Union[int, torch.Tensor] = 0, cu_seqlens: Optional[torch.Tensor] = None,
+):
+    """Rotate the first rotary_dim channels of q and k by their positions, as flash_attn_with_kvcache does.
+
+    q (batch, seqlen, nheads, headdim) and k (batch, seqlen, nheads_k, headdim), fp16 or bf16, headdim 64 or 128; with
+    cu_seqlens (int32 (batch_size + 1,)) packed: (total, nheads, headdim), and rows that no sequence covers become 0.
+    k may be None.  rotary_cos and rotary_sin (rows, rotary_dim / 2) are float32, float16 or bfloat16 (as
+    flash_attn_rotary_tables makes them); pairs are channels (2j, 2j + 1) if rotary_interleaved, else (j, j + rotary_dim / 2).
+
+    Row i of a sequence is at position seqlen_offsets + i (an int, or int32 (batch_size,): the tokens before it), or, with
+    positions (int32, (batch, seqlen) or (total,)), where they say.  A row whose position the tables do not have becomes
+    NaN in the rotated channels.
+
+    Returns q and k rotated, new tensors (q alone where k is None); q and k get gradients, the tables none."""
+    for name, t in (("rotary_cos", rotary_cos), ("rotary_sin", rotary_sin)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise TypeError(f"{name} must be a 2-D tensor (rows, rotary_dim / 2)")
+    for name, t in (("positions", positions), ("cu_seqlens", cu_seqlens)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32):
+            raise TypeError(f"{name} must be a torch.int32 tensor")
+    offsets, offset = None, seqlen_offsets
+    if isinstance(seqlen_offsets, torch.Tensor):
+        offsets, offset = seqlen_offsets, 0
+        if offsets.dtype != torch.int32:
+            raise TypeError("seqlen_offsets must be an int or a torch.int32 tensor")
+    elif not isinstance(seqlen_offsets, int):
+        raise TypeError("seqlen_offsets must be an int or a torch.int32 tensor")
+    rest = (maybe_contiguous(rotary_cos), maybe_contiguous(rotary_sin), rotary_interleaved, positions,
+            maybe_contiguous(offsets), offset, maybe_contiguous(cu_seqlens))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
+                                    or rotary_cos.requires_grad or rotary_sin.requires_grad):
+        if rotary_cos.requires_grad or rotary_sin.requires_grad:
+            raise RuntimeError("rotary_cos and rotary_sin get no gradient")
+        q, k = FlashAttnRotaryFunc.apply(q, k, *rest)
+    else:
+        q, k = flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest, False)
+    return q if k is None else (q, k)

@@ -284,7 +284,7 @@ int fa_fwd_kvcache_noalloc(const fa_kvcache_args *args, void *stream);
  * 2^23 elements (o, o2 and the gradients: any); dtype is FA_FP16 or FA_BF16 for
  * all of them.  No counterpart in the reference.
  */
-enum { FA_FP16 = 0, FA_BF16 = 1 };
+enum { FA_FP16 = 0, FA_BF16 = 1, FA_FP32 = 2 /* rotary tables alone */ };
 
 /* lam, fp32: element [batch b][row i][head h] at ptr + b * batch_stride + i *
  * row_stride + h * head_stride (strides in elements, 0 where it is shared; for
@@ -423,6 +423,52 @@ int fa_kvpages_fork(const fa_kvpages_args *args, void *stream);
 int fa_kvpages_free(const fa_kvpages_args *args, void *stream);
 /* The used pages move to the front of the pool: out_table and out_refs are the table and the counts afterwards. */
 int fa_kvpages_compact(const fa_kvpages_args *args, void *stream);
+
+/*
+ * Rotary positions: cosines and sines of angles, and q and k rotated by them.  A pair
+ * (x1, x2) of channels of a row at position p becomes (x1 c - x2 s, x2 c + x1 s), in
+ * fp32 and rounded once.  fa_kvcache_args has the same rotation for fp16 caches; here it is
+ * for training (inverse is the gradient), packed batches, bf16 and tables of 32 bits.
+ * No counterpart in the reference.
+ */
+#define FA_ROTARY_MAX_DIM 256
+
+/* cos and sin, [seqlen][rotary_dim / 2] of dtype: entry (i, j) is attention_factor times the
+ * cosine / sine of (offset + i) * f_j, computed in 64 bits, f_j = base ^ (-2 j / rotary_dim).
+ * factor != 1 divides the frequencies: all of them (original_seqlen 0), or, by the turns t that
+ * a pair makes in original_seqlen tokens, f_j (keep + (1 - keep) / factor) with
+ * keep = (t - low_turns) / (high_turns - low_turns) cut to [0, 1]. */
+typedef struct fa_rotary_tables_args {
+    void *cos, *sin;                /* 16-byte aligned                           */
+    int32_t seqlen, rotary_dim;     /* rotary_dim: a multiple of 16 up to FA_ROTARY_MAX_DIM */
+    int32_t dtype;                  /* FA_FP16, FA_BF16 or FA_FP32               */
+    int64_t offset;
+    double base, factor, original_seqlen, low_turns, high_turns, attention_factor;
+} fa_rotary_tables_args;
+
+int fa_rotary_tables(const fa_rotary_tables_args *args, void *stream);
+
+/* q and k (ptr NULL: none) to q_out and k_out, apart from them.  Row i of sequence b is at position
+ * positions[b * positions_stride + i], or else offset + seqlen_offsets[b] + i; packed (cu_seqlens): i
+ * counts from the sequence's first row, and rows of no sequence become 0.  A row whose
+ * position is outside the tables gets NaN in the rotated channels. */
+typedef struct fa_rotary_args {
+    fa_tensor q, k, q_out, k_out;   /* fp16 or bf16                              */
+    const void *cos, *sin;          /* [table_rows][rotary_dim / 2], 16-byte aligned rows */
+    int64_t cos_stride, sin_stride; /* between their rows, elements              */
+    const int32_t *positions;       /* [batch][seqlen], packed [seqlen], or NULL */
+    int64_t positions_stride;
+    const int32_t *seqlen_offsets;  /* [batch] or NULL                           */
+    const int32_t *cu_seqlens;      /* [batch + 1]: packed, or NULL              */
+    int32_t batch, seqlen;          /* seqlen: rows a sequence, or all packed rows */
+    int32_t nheads, nheads_k, head_dim, rotary_dim, table_rows;
+    int32_t offset;
+    int32_t interleaved;            /* pairs (2j, 2j + 1), else (j, j + rotary_dim / 2) */
+    int32_t inverse;                /* rotates back: the gradient of q and k from those of q_out and k_out */
+    int32_t dtype, table_dtype;
+} fa_rotary_args;
+
+int fa_rotary(const fa_rotary_args *args, void *stream);
 
 /* Human-readable text for a return code (FA_* or hipError_t). */
 const char *fa_error_string(int code);
