@@ -60,3 +60,4 @@ inline at::Tensor optional_workspace(int64_t numel, const at::TensorOptions &opt
 void bind_diff(py::module_ &m);     // diff_api.cpp
 void bind_kvpages(py::module_ &m);  // kvpages_api.cpp
 void bind_rotary(py::module_ &m);   // rotary_api.cpp
+void bind_kv8(py::module_ &m);      // kv8_api.cpp

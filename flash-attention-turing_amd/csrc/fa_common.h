@@ -516,6 +516,24 @@ __device__ __forceinline__ SeqInfo seq_info(int b, int seqlen_q, int seqlen_k, c
     return s;
 }
 
+// The last packed sequence that starts at or before the row (-1: none), by the whole wave: 64 starts are compared at a
+// time.  cu is not read outside [0, batch], whatever it holds.
+__device__ __forceinline__ int packed_sequence(const int32_t *cu, int batch, int row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = batch + 1;
+    while (n > 0) {
+        const int step = (n + 63) / 64, i = lo + lane * step;
+        const bool starts = lane * step < n && cu[i] <= row;
+        const int k = __popcll(__builtin_amdgcn_ballot_w64(starts));
+        if (k == 0) return lo - 1;
+        lo += (k - 1) * step;
+        if (step == 1) return lo;
+        n = min(step, n - (k - 1) * step);
+        // lo itself starts at or before the row; what follows it is looked at next.
+    }
+    return lo;
+}
+
 // Element offset of (batch b / packed row start, head) in a strided tensor.
 __device__ __forceinline__ int64_t base_off(const fa_tensor &t, bool packed, int b, int row_start, int head) {
     return (packed ? int64_t(row_start) * t.row_stride : int64_t(b) * t.batch_stride) +

@@ -1,0 +1,629 @@
+// A key-value cache in 8 bits: quantising as it is written, reading back, and attention of few query rows
+// (decode steps, drafted tokens) split over the cache's length.
+#include <algorithm>
+
+#include "fa_kv8_common.h"
+
+namespace fa {
+
+// ---------------------------------------------------------------------------
+// Append.
+//
+// A workgroup takes one block of tokens of one head of K or V: it reads the new rows into registers, finds their largest
+// magnitude as an integer (the bits of |x|, in which infinities and NaN come out on top), settles the block's scale, and
+// writes codes.  Only where the scale grows are the block's earlier codes read and written again.  Scales are powers of
+// two: the quotients are exact, codes that stay in e4m3's normal range keep their bits when a scale grows, and a block is
+// raised at most a few times however many appends fill it.
+
+constexpr int kKv8Threads = 256;
+
+// The smallest power of two s >= 2^-126 with x <= most * s, from the bits of |x| in the tensors' type; NaN if x is not finite.
+template <bool BF, bool INT8>
+__device__ __forceinline__ float kv8_scale_for(uint32_t bits) {
+    if (bits >= (BF ? 0x7f80u : 0x7c00u)) return __builtin_nanf("");
+    const float x = BF ? __uint_as_float(bits << 16) : float(__builtin_bit_cast(f16, uint16_t(bits)));
+    const uint32_t u = __float_as_uint(x);
+    // x = (1 + f) 2^e; 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6.
+    const int e = int(u >> 23) - 127 - (INT8 ? 6 : 8) + ((u & 0x7fffffu) > (INT8 ? 0x7e0000u : 0x600000u) ? 1 : 0);
+    return e <= -126 ? kKv8MinScale : __uint_as_float(uint32_t(e + 127) << 23);
+}
+
+// x / s for eight values, as codes.  A power of two divides by its reciprocal, exactly.
+template <bool INT8>
+__device__ __forceinline__ u32x2 kv8_encode(const float (&x)[8], float s) {
+    f32x4 v[2];
+    if ((__float_as_uint(s) & 0x7fffffu) == 0) {
+        const float inv = 1.f / s;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = x[i] * inv;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = __fdiv_rn(x[i], s);
+    }
+    return u32x2{kv8_codes<INT8>(v[0]), kv8_codes<INT8>(v[1])};
+}
+
+template <int HD, bool BF, bool INT8, int U>
+__global__ __launch_bounds__(kKv8Threads) void kv8_append_kernel(const fa_kv8_args a, const Kv8Plan plan, const int plan_wgs,
+                                                                 const int clear_wgs, const int blocks) {
+    if (int(blockIdx.x) < plan_wgs) return kv8_make_plan(a, plan);
+    if (int(blockIdx.x) < plan_wgs + clear_wgs) {
+        const int64_t i = int64_t(blockIdx.x - plan_wgs) * kKv8Threads + threadIdx.x;
+        if (i < plan.items) static_cast<int32_t *>(a.ws)[i] = 0;
+        return;
+    }
+    constexpr int KCH = HD / 8;  // units of a row: 8 elements
+    __shared__ uint32_t part[kKv8Threads / 64];
+    const fa_kv8_cache &c = a.cache;
+    int64_t rest = blockIdx.x - plan_wgs - clear_wgs;
+    const bool is_v = rest & 1;
+    rest >>= 1;
+    const int hk = int(rest % c.nheads_k);
+    rest /= c.nheads_k;
+    const int j = int(rest % blocks), b = int(rest / blocks);
+    const int L0 = a.cache_seqlens[b], n = a.seqlens_new ? a.seqlens_new[b] : a.seqlen_new;
+    int row;
+    const int err = kv8_err(c, b, L0, n, a.seqlen_new, row);
+    if (err) {
+        if (c.status && rest % blocks == 0 && hk == 0 && !is_v && threadIdx.x == 0) atomicOr(c.status, err);
+        return;
+    }
+    const int p0 = (L0 / c.scale_block + j) * c.scale_block;  // the block's first token; a capacity's blocks are whole
+    const int end = min(L0 + n, p0 + c.scale_block), first = max(L0, p0);
+    if (first >= end) return;
+    int64_t line = row;
+    int at = p0;
+    if (c.block_table) {
+        const int pg = p0 / c.page_block_size;
+        line = c.block_table[int64_t(b) * c.block_table_stride + pg];
+        at = p0 - pg * c.page_block_size;
+        if (line < 0 || line >= c.num_pages) {
+            if (c.status && hk == 0 && !is_v && threadIdx.x == 0) atomicOr(c.status, FA_KV_BAD_PAGE);
+            return;
+        }
+    }
+    const fa_tensor &src_t = is_v ? a.v_new : a.k_new, &dst_t = is_v ? c.v : c.k;
+    const fa_kv8_scales &sc = is_v ? c.v_scale : c.k_scale;
+    const f16 *src = (const f16 *)src_t.ptr + int64_t(b) * src_t.batch_stride + int64_t(hk) * src_t.head_stride;
+    char *dst = (char *)dst_t.ptr + line * dst_t.batch_stride + int64_t(at) * dst_t.row_stride + int64_t(hk) * dst_t.head_stride;
+    float *scale = sc.ptr + line * sc.batch_stride + int64_t(at / c.scale_block) * sc.row_stride + int64_t(hk) * sc.head_stride;
+
+    const int units = (end - first) * KCH;
+    u32x4 v[U];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int e = i * kKv8Threads + threadIdx.x;
+        v[i] = e < units ? ldg16(src + int64_t(first - L0 + e / KCH) * src_t.row_stride + 8 * (e % KCH)) : zero_u4();
+    }
+    const bool held = p0 < L0;
+    const float old = held ? *scale : kKv8MinScale;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = max(top, max(v[i][w] & 0x7fffu, v[i][w] >> 16 & 0x7fffu));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), d)));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();  // every thread has read the old scale, too
+#pragma unroll
+    for (int w = 0; w < kKv8Threads / 64; ++w) top = max(top, part[w]);
+    float s = kv8_scale_for<BF, INT8>(top);
+    const bool bad = !(s == s) || !(old == old);  // such a block reads as NaN; its codes are finite, so that no masked
+    if (bad)                                      // key's turns up in a product
+        s = __builtin_nanf("");
+    else
+        s = fmaxf(s, old);
+    if (threadIdx.x == 0) *scale = s;
+    if (held && !bad && s != old) {
+        const int olds = (L0 - p0) * KCH;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < olds; e += kKv8Threads) {
+            u32x2 *p = reinterpret_cast<u32x2 *>(dst + int64_t(e / KCH) * dst_t.row_stride + 8 * (e % KCH));
+            const u32x2 q = *p;
+            const f32x4 lo = kv8_values<INT8>(q[0]), hi = kv8_values<INT8>(q[1]);
+            const float x[8] = {lo[0] * old, lo[1] * old, lo[2] * old, lo[3] * old,
+                                hi[0] * old, hi[1] * old, hi[2] * old, hi[3] * old};
+            *p = kv8_encode<INT8>(x, s);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int e = i * kKv8Threads + threadIdx.x;
+        if (e >= units) continue;
+        float x[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) x[t] = elem<BF>(as_h8(v[i]), t);
+        u32x2 q = {0u, 0u};
+        if (!bad) q = kv8_encode<INT8>(x, s);
+        *reinterpret_cast<u32x2 *>(dst + int64_t(first - p0 + e / KCH) * dst_t.row_stride + 8 * (e % KCH)) = q;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Read back: a wave takes kKv8Rows packed rows, all heads of K and of V, 16 codes a lane.
+
+constexpr int kKv8Rows = 4;
+
+template <int HD, bool BF, bool INT8>
+__global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read_args a) {
+    constexpr int CH = HD / 16;
+    const fa_kv8_cache &c = a.cache;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t r0 = (int64_t(blockIdx.x) * (kKv8Threads / 64) + wave) * kKv8Rows;
+    if (r0 >= a.total) return;
+    for (int64_t r = r0; r < min(r0 + kKv8Rows, int64_t(a.total)); ++r) {
+        const int b = packed_sequence(a.cu_seqlens, c.batch, int(r));
+        bool ok = b >= 0 && b < c.batch;
+        int64_t line = 0;
+        int at = 0;
+        if (ok) {
+            const int start = a.cu_seqlens[b];
+            int row;
+            const int n = a.cu_seqlens[b + 1] - start, err = kv8_err(c, b, 0, n, INT_MAX, row);
+            if (err && c.status && lane == 0) atomicOr(c.status, err);
+            ok = !err && r - start < n;
+            at = ok ? int(r) - start : 0;
+            line = row;
+            if (ok && c.block_table) {
+                const int pg = at / c.page_block_size;
+                line = c.block_table[int64_t(b) * c.block_table_stride + pg];
+                at -= pg * c.page_block_size;
+                if (line < 0 || line >= c.num_pages) {
+                    if (c.status && lane == 0) atomicOr(c.status, FA_KV_BAD_PAGE);
+                    line = 0;
+                }
+            }
+        }
+        for (int u = lane; u < 2 * c.nheads_k * CH; u += 64) {
+            const bool is_v = u >= c.nheads_k * CH;
+            const int x = is_v ? u - c.nheads_k * CH : u, h = x / CH, ch = x % CH;
+            const fa_tensor &t = is_v ? c.v : c.k, &o = is_v ? a.v_out : a.k_out;
+            const fa_kv8_scales &sc = is_v ? c.v_scale : c.k_scale;
+            u32x4 lo = zero_u4(), hi = zero_u4();
+            if (ok) {
+                const u32x4 q = *reinterpret_cast<const u32x4 *>((const char *)t.ptr + line * t.batch_stride +
+                                                                 int64_t(at) * t.row_stride + int64_t(h) * t.head_stride + 16 * ch);
+                const float s = sc.ptr[line * sc.batch_stride + int64_t(at / c.scale_block) * sc.row_stride + int64_t(h) * sc.head_stride];
+                f16x4 y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = kv8_values<INT8>(q[i]);
+                    y[i] = pack4<BF>(v[0] * s, v[1] * s, v[2] * s, v[3] * s);
+                }
+                lo = __builtin_bit_cast(u32x4, f16x8(__builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7)));
+                hi = __builtin_bit_cast(u32x4, f16x8(__builtin_shufflevector(y[2], y[3], 0, 1, 2, 3, 4, 5, 6, 7)));
+            }
+            u32x4 *p = reinterpret_cast<u32x4 *>((f16 *)o.ptr + r * o.row_stride + int64_t(h) * o.head_stride + 16 * ch);
+            p[0] = lo;
+            p[1] = hi;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Attention of few rows.
+//
+// S^T = K Q^T in 16 x 16 x 32 MFMAs: 16 keys by 16 rows, the rows of a KV head being its query heads times the query
+// positions.  A lane's 16-byte LDS read holds the codes of two K steps (which channels a step takes is free, as long as Q's
+// operand takes the same), and keys are dealt to the two MFMAs of a tile so that a lane ends up with the eight consecutive
+// keys that it supplies to the product with V, whose codes come transposed from LDS, eight keys of a channel a lane.
+//
+// A workgroup's four waves walk the 32-key tiles of its piece (tile t to wave t % 4), each through LDS slots of its own with
+// no barrier in the loop; codes go from memory to LDS without passing registers.
+
+constexpr int kKdTile = 32, kKdRows = 16;
+
+// Chunk c of row r of a 32-row tile of codes sits at chunk c ^ kd_swz(r): the K reads (16 rows that differ in bits 0, 1, 3 and
+// 4, one chunk) and the transposed V reads (16 rows that differ in bits 0 to 3) then take each bank once.
+template <int HD>
+__device__ __forceinline__ int kd_swz(int r) {
+    if constexpr (HD == 128)
+        return (r >> 1 & 1) | (r >> 3 & 1) << 1 | ((r >> 4 ^ r >> 2) & 1) << 2;
+    else
+        return (r >> 3 & 1) | ((r >> 4 ^ r >> 2) & 1) << 1;
+}
+
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
+
+// ds_read_b64_tr_b8: within 16 lanes, lane i gets byte i % 8 of the 8-byte words at the addresses of lanes 2 j + i / 8,
+// j = 0..7.  With lane 2 j + h at row j, bytes 8 h, lane i so holds column i of 8 rows.
+__device__ __forceinline__ u32x2 lds_tr8(const char *base, int off) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t *)(base + off)));
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x4 kd_mfma(const f16x8 a, const f16x8 b, const f32x4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Maximum / sum over the four lanes l % 16 + 16 i.
+__device__ __forceinline__ float kd_max4(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
+__device__ __forceinline__ float kd_sum4(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+template <int HD, bool BF, bool INT8>
+__global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8_args a, const Kv8Plan plan) {
+    constexpr int CH = HD / 16, TILE = kKdTile * HD, STAGE = 2 * TILE, NST = 2;
+    constexpr int CPW = TILE / 1024;  // copies a lane for K or V of a tile
+    constexpr int MERGE = 17;         // row stride of the waves' O^T at the merge
+    constexpr int WAVE_LDS = NST * STAGE > HD * MERGE * 4 ? NST * STAGE : HD * MERGE * 4;
+    constexpr int STEPS = HD / 32;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * WAVE_LDS];
+    __shared__ f32x2 ml[4][16];
+    __shared__ int ticket;
+    static_assert(4 * WAVE_LDS >= 16 * (kKv8Join + 2) * 4, "the join's scratch");
+
+    const fa_kv8_cache &c = a.cache;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int HI = c.nheads_k * plan.row_tiles;
+    const int slot_i = blockIdx.x / HI, hi_i = blockIdx.x % HI, hk = hi_i / plan.row_tiles, rt = hi_i % plan.row_tiles;
+    const Kv8Slot sl = kv8_slot(a, plan, slot_i);
+    if (sl.b < 0) return;
+    const int G = a.nheads / c.nheads_k, R = G * a.seqlen_q, L = sl.keys;
+    const int row = rt * kKdRows + col;
+    const bool row_ok = row < R;
+    const int qpos = row_ok ? row / G : 0, hq = hk * G + (row_ok ? row - qpos * G : 0);
+    const int shift = L - a.seqlen_q;  // position of query 0
+    const int first = kv8_first(a, qpos + shift), last = kv8_last(a, qpos + shift, L);
+    // Keys that every row of the tile sees, and that any does.
+    const int q_lo = rt * kKdRows / G, q_hi = min(rt * kKdRows + kKdRows - 1, R - 1) / G;
+    const int all_first = kv8_first(a, q_hi + shift), all_last = kv8_last(a, q_lo + shift, L);
+    const int s0 = max(sl.begin, kv8_first(a, q_lo + shift)) / kKdTile * kKdTile, s1 = min(sl.end, kv8_last(a, q_hi + shift, L) + 1);
+    const int t_first = s0 / kKdTile, t_end = (s1 + kKdTile - 1) / kKdTile;
+    const int my_first = t_first + wave;
+    const int n_my = my_first < t_end ? (t_end - my_first + 3) / 4 : 0;
+
+    const int krs = int(c.k.row_stride), vrs = int(c.v.row_stride);
+    char *const slot = smem + wave * WAVE_LDS;
+    const int p_row = lane / CH, p_ch = lane % CH;  // of copy 0; copy i: rows 64 / CH further
+    const float cscale = a.softmax_scale * kLog2e;
+    float ks[NST], vs[NST];
+    auto issue = [&](int t, int st) FA_INLINE {
+        const int p0 = t * kKdTile;
+        int64_t line = sl.row;
+        int at = p0;
+        if (c.block_table) {
+            const int pg = p0 / c.page_block_size;
+            line = checked_page(scalar_load(c.block_table + int64_t(sl.b) * c.block_table_stride + pg), c.num_pages, c.status);
+            at = p0 - pg * c.page_block_size;
+        }
+        const char *kb = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * krs + int64_t(hk) * c.k.head_stride;
+        const char *vb = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * vrs + int64_t(hk) * c.v.head_stride;
+        const int blk = at / c.scale_block;
+        ks[st] = scalar_float(c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride +
+                              int64_t(hk) * c.k_scale.head_stride);
+        vs[st] = scalar_float(c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride +
+                              int64_t(hk) * c.v_scale.head_stride);
+        // Rows past the sequence re-read its last one, so that no stale code reaches a product.
+        const int most = min(L - 1 - p0, kKdTile - 1);
+        char *const base = slot + st * STAGE;
+#pragma unroll
+        for (int i = 0; i < CPW; ++i) {
+            const int r = i * (64 / CH) + p_row, rc = min(r, most), ch = 16 * (p_ch ^ kd_swz<HD>(r));
+            g2l16(kb + int64_t(rc) * krs + ch, base + i * 1024);
+            g2l16(vb + int64_t(rc) * vrs + ch, base + TILE + i * 1024);
+        }
+    };
+#pragma unroll
+    for (int st = 0; st < NST; ++st)
+        if (st < n_my) issue(my_first + 4 * st, st);
+    // Q^T as B operands: step st takes channels 64 (st / 2) + 16 g + 8 (st % 2) + 0..7.
+    f16x8 qB[STEPS];
+    {
+        const f16 *qp = (const f16 *)a.q.ptr + int64_t(sl.b) * a.q.batch_stride + int64_t(qpos) * a.q.row_stride +
+                        int64_t(hq) * a.q.head_stride + 16 * g;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) qB[st] = as_h8(row_ok ? ldg16(qp + 64 * (st / 2) + 8 * (st % 2)) : zero_u4());
+    }
+    wait_vmem();  // only tile copies are in flight inside the loop
+    f32x4 o[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    // LDS addresses: K rows of the tile's two MFMAs, and the transposed V reads.
+    const int k_row0 = 8 * (col >> 2) + (col & 3), v_row = 8 * g + (col >> 1), v_half = 8 * (col & 1);
+
+    for (int k0 = 0; k0 < n_my; k0 += NST) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st) {
+            const int k = k0 + st;
+            if (k >= n_my) break;
+            const int p0 = (my_first + 4 * k) * kKdTile;
+            if (k + 1 < n_my)
+                wait_vmem_n<(NST - 1) * 2 * CPW>();
+            else
+                wait_vmem();
+            const char *kt = slot + st * STAGE, *vt = kt + TILE;
+            u32x4 kc[2][HD / 64];
+            u32x2 vc[CH];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) {
+                    const int r = k_row0 + 4 * t;
+                    kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kd_swz<HD>(r)));
+                }
+#pragma unroll
+            for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kd_swz<HD>(v_row)) + v_half);
+            // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
+            const float sk = ks[st] * cscale, sv0 = vs[st] * 0.f, sv = sv0 == 0.f ? vs[st] : 0.f;
+            wait_lds();
+            if (k + NST < n_my) issue(my_first + 4 * (k + NST), st);
+            f32x4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const u32x4 q = kc[t][i / 2];
+                    s[t] = kd_mfma<BF>(kv8_decode<INT8, BF>(i % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[i], s[t]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], sk, sv0);
+            }
+            if (p0 < all_first || p0 + kKdTile - 1 > all_last) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int key = p0 + 8 * g + 4 * t + r;
+                        if (key < first || key > last) s[t][r] = -INFINITY;
+                    }
+            }
+            // The maximum is raised only when a score passes it by 2^8: sums and products keep 32 bits.
+            const float top = max3(max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]), max3(s[1][1], s[1][2], s[1][3]), -INFINITY);
+            if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
+                const float m_new = fmaxf(m, kd_max4(top));
+                const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < CH; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
+                m = m_new;
+            }
+            const float m_use = m == -INFINITY ? 0.f : m;
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = exp2_fast(s[i / 4][i % 4] - m_use);
+                l += e[i];
+            }
+            // P times V's scale in bf16, which has fp32's range, as hi + lo: 16 bits.
+            bf16x8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = e[i] * sv;
+                hi[i] = (__bf16)w;
+                lo[i] = (__bf16)(w - float(hi[i]));
+            }
+#pragma unroll
+            for (int d = 0; d < CH; ++d) {
+                const f16x8 v = kv8_decode<INT8, true>(vc[d]);
+                o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, hi), o[d]);
+                o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, lo), o[d]);
+            }
+        }
+    }
+
+    // Merge the four waves: O^T to LDS, then every thread sums pairs of channels of a row.
+    l = kd_sum4(l);
+    float *ow = reinterpret_cast<float *>(slot);
+#pragma unroll
+    for (int d = 0; d < CH; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ow[(16 * d + 4 * g + r) * MERGE + col] = o[d][r];
+    if (g == 0) ml[wave][col] = f32x2{m, l};
+    __syncthreads();
+    const int rows = min(kKdRows, R - rt * kKdRows);
+    auto merged = [&](int r, int d, float &mm, float &ll) FA_INLINE {
+        mm = fmaxf(fmaxf(ml[0][r][0], ml[1][r][0]), fmaxf(ml[2][r][0], ml[3][r][0]));
+        ll = 0.f;
+        f32x2 x = {0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = ml[w][r][0] == -INFINITY ? 0.f : exp2_fast(ml[w][r][0] - mm);
+            const float *q = reinterpret_cast<const float *>(smem + w * WAVE_LDS);
+            ll = fmaf(ml[w][r][1], f, ll);
+            x[0] = fmaf(q[d * MERGE + r], f, x[0]);
+            x[1] = fmaf(q[(d + 1) * MERGE + r], f, x[1]);
+        }
+        return x;
+    };
+    if (sl.n_pieces == 1) {
+        for (int e = tid; e < rows * (HD / 2); e += kKv8Threads) {
+            const int r = e / (HD / 2), d = 2 * (e % (HD / 2));
+            float mm, ll;
+            const f32x2 x = merged(r, d, mm, ll);
+            kv8_store<HD, BF>(a, sl.b, hk, rt * kKdRows + r, d, x, mm, ll);
+        }
+        return;
+    }
+    const int64_t part = int64_t(slot_i) * HI + hi_i;
+    for (int e = tid; e < rows * (HD / 2); e += kKv8Threads) {
+        const int r = e / (HD / 2), d2 = e % (HD / 2);
+        float mm, ll;
+        const f32x2 x = merged(r, 2 * d2, mm, ll);
+        kv8_put(kv8_o<HD>(a, plan, part) + e, x);
+        if (d2 == 0) kv8_put(kv8_ml(a, plan, part) + r, f32x2{mm, ll});
+    }
+    int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
+    if (!kv8_count(count, sl.n_pieces, &ticket)) return;
+    kv8_join<HD, BF, kKdRows>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, reinterpret_cast<float *>(smem),
+                              [&](int i) { return part + int64_t(i - sl.ch) * HI; });
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+
+static Kv8Plan kv8_plan(const fa_kv8_args &a) {
+    Kv8Plan p{};
+    const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q, cap = std::max(a.cache.cache_capacity, 1);
+    const int tile = kKdRows;
+    p.row_tiles = int((rows + tile - 1) / tile);
+    p.rows_max = int(std::min<int64_t>(rows, tile));
+    const int64_t heads = int64_t(a.cache.nheads_k) * p.row_tiles;
+    p.items = a.cache.batch * heads;
+    p.round = 128;
+    p.least = 256;
+    p.want = int(std::max<int64_t>(3 * device_cus() / heads, 1));
+    int64_t slots;
+    if (a.num_splits > 0) {
+        p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + p.round - 1) / p.round * p.round);
+        slots = a.cache.batch * ((cap + p.fixed - 1) / p.fixed);
+    } else {
+        // Pieces of at least total / want keys: a sequence has at most one short piece.
+        slots = std::min<int64_t>(int64_t(p.want) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
+    }
+    p.slots = int(std::min<int64_t>(slots, INT32_MAX));
+    const bool parts = slots > a.cache.batch;
+    auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    p.at_slots = up(p.items * 4);
+    p.at_ml = p.at_slots + up(slots * int64_t(sizeof(Kv8Slot)));
+    p.at_o = p.at_ml + (parts ? up(slots * heads * p.rows_max * 8) : 0);
+    p.bytes = p.at_o + (parts ? slots * heads * p.rows_max * a.cache.head_dim * 4 : 0);
+    return p;
+}
+
+// Descriptors of a cache; tokens: of a page or row.
+static int check_kv8_cache(const fa_kv8_cache &c) {
+    if (c.head_dim != 64 && c.head_dim != 128) return FA_ERR_UNSUPPORTED;
+    if (c.kind != FA_KV8_E4M3 && c.kind != FA_KV8_INT8) return FA_ERR_UNSUPPORTED;
+    if (c.batch < 0 || c.nheads_k <= 0 || c.cache_capacity < 0) return FA_ERR_INVALID_ARG;
+    if (c.scale_block != 32 && c.scale_block != 64 && c.scale_block != 128 && c.scale_block != 256) return FA_ERR_INVALID_ARG;
+    if (c.block_table ? c.cache_batch_idx || c.page_block_size <= 0 || c.page_block_size % c.scale_block || c.num_pages <= 0
+                      : c.cache_capacity % c.scale_block != 0)
+        return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&c.k, &c.v}) {
+        if (!t->ptr || ((reinterpret_cast<uintptr_t>(t->ptr) | uint64_t(t->batch_stride) | uint64_t(t->row_stride) |
+                         uint64_t(t->head_stride)) & 15u))
+            return FA_ERR_INVALID_ARG;
+        if (t->row_stride < 0 || t->row_stride > kDiffMaxRowStride) return FA_ERR_INVALID_ARG;
+    }
+    for (const fa_kv8_scales *s : {&c.k_scale, &c.v_scale})
+        if (!s->ptr || (reinterpret_cast<uintptr_t>(s->ptr) & 3u)) return FA_ERR_INVALID_ARG;
+    return FA_OK;
+}
+
+static int check_kv8_new(const fa_kv8_args &a) {
+    if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
+    if (a.seqlen_new < 0 || !a.cache_seqlens) return FA_ERR_INVALID_ARG;
+    for (const fa_tensor *t : {&a.k_new, &a.v_new})
+        if (check_tensor(*t, a.seqlen_new > 0)) return FA_ERR_INVALID_ARG;
+    return FA_OK;
+}
+
+// The call with its sizes as types: f(head_dim, bf16, int8).
+template <class F>
+static int kv8_by_type(int head_dim, int dtype, int kind, F f) {
+    auto by_kind = [&](auto hd, auto bf) {
+        return kind == FA_KV8_INT8 ? f(hd, bf, std::true_type{}) : f(hd, bf, std::false_type{});
+    };
+    auto by_dtype = [&](auto hd) { return dtype == FA_BF16 ? by_kind(hd, std::true_type{}) : by_kind(hd, std::false_type{}); };
+    return head_dim == 128 ? by_dtype(std::integral_constant<int, 128>{}) : by_dtype(std::integral_constant<int, 64>{});
+}
+
+// Workgroups that plan and clear (plan NULL: none) and those that append, in one launch.
+static int launch_kv8_append(const fa_kv8_args &a, const Kv8Plan *plan, hipStream_t s) {
+    const fa_kv8_cache &c = a.cache;
+    const int blocks = a.seqlen_new > 0 ? int((int64_t(a.seqlen_new) + 2 * c.scale_block - 2) / c.scale_block) : 0;
+    const int64_t clear = plan ? (plan->items + kKv8Threads - 1) / kKv8Threads : 0;
+    const int64_t grid = (plan ? 1 : 0) + clear + int64_t(c.batch) * blocks * c.nheads_k * 2;
+    if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    if (grid == 0) return FA_OK;
+    const int most = std::min(c.scale_block, std::max(a.seqlen_new, 1)) * (c.head_dim / 8);  // units of a workgroup
+    return kv8_by_type(c.head_dim, a.dtype, c.kind, [&](auto hd, auto bf, auto int8) {
+        constexpr int HD = decltype(hd)::value;
+        constexpr bool BF = decltype(bf)::value, INT8 = decltype(int8)::value;
+        auto go = [&](auto u) {
+            hipLaunchKernelGGL((kv8_append_kernel<HD, BF, INT8, decltype(u)::value>), dim3(unsigned(grid)), dim3(kKv8Threads), 0,
+                               s, a, plan ? *plan : Kv8Plan{}, plan ? 1 : 0, int(clear), std::max(blocks, 1));
+            return int(hipGetLastError());
+        };
+        if (most <= kKv8Threads) return go(std::integral_constant<int, 1>{});
+        if (most <= 4 * kKv8Threads) return go(std::integral_constant<int, 4>{});
+        return go(std::integral_constant<int, 256 * HD / 8 / kKv8Threads>{});
+    });
+}
+
+static int check_kv8(const fa_kv8_args *p) {
+    if (!p) return FA_ERR_INVALID_ARG;
+    const fa_kv8_args &a = *p;
+    if (a.cache.batch == 0) return FA_OK;  // tensors of no sequences have no address
+    int rc = check_kv8_cache(a.cache);
+    if (rc == FA_OK) rc = check_kv8_new(a);
+    if (rc) return rc;
+    if (a.seqlen_q < 0 || a.nheads <= 0 || a.nheads % a.cache.nheads_k || a.num_splits < 0 || a.window_left < -1 ||
+        a.window_right < -1 || a.seqlens_new)
+        return FA_ERR_INVALID_ARG;
+    if (a.seqlen_q == 0) return FA_OK;
+    if (!a.lse || check_tensor(a.q, true) || check_tensor(a.o, true)) return FA_ERR_INVALID_ARG;
+    const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q;
+    if (rows > INT32_MAX / 2) return FA_ERR_INVALID_ARG;
+    if (!a.ws || a.ws_bytes < int64_t(fa_kv8_ws_bytes(&a)) || (reinterpret_cast<uintptr_t>(a.ws) & 255u)) return FA_ERR_WORKSPACE;
+    return FA_OK;
+}
+
+}  // namespace fa
+
+extern "C" int fa_kv8_append(const fa_kv8_args *args, void *stream) {
+    using namespace fa;
+    if (!args) return FA_ERR_INVALID_ARG;
+    if (args->cache.batch == 0) return FA_OK;
+    int rc = check_kv8_cache(args->cache);
+    if (rc == FA_OK) rc = check_kv8_new(*args);
+    if (rc) return rc;
+    return launch_kv8_append(*args, nullptr, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t fa_kv8_ws_bytes(const fa_kv8_args *a) {
+    if (!a || a->cache.batch <= 0 || a->seqlen_q <= 0 || a->nheads <= 0 || a->cache.nheads_k <= 0) return 0;
+    return size_t(fa::kv8_plan(*a).bytes);
+}
+
+extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
+    using namespace fa;
+    int rc = check_kv8(args);
+    if (rc) return rc;
+    const fa_kv8_args &a = *args;
+    if (a.cache.batch == 0) return FA_OK;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (a.seqlen_q == 0) return launch_kv8_append(a, nullptr, s);
+    const Kv8Plan plan = kv8_plan(a);
+    const int64_t grid = int64_t(plan.slots) * a.cache.nheads_k * plan.row_tiles;
+    if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    if ((rc = launch_kv8_append(a, &plan, s))) return rc;
+    return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
+        hipLaunchKernelGGL((kv8_decode_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),
+                           dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, plan);
+        return int(hipGetLastError());
+    });
+}
+
+extern "C" int fa_kv8_read(const fa_kv8_read_args *args, void *stream) {
+    using namespace fa;
+    if (!args) return FA_ERR_INVALID_ARG;
+    const fa_kv8_read_args &a = *args;
+    if (a.total < 0 || a.cache.batch < 0) return FA_ERR_INVALID_ARG;
+    if (a.total == 0) return FA_OK;
+    const int rc = check_kv8_cache(a.cache);
+    if (rc) return rc;
+    if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
+    if (!a.cu_seqlens || check_tensor(a.k_out, true) || check_tensor(a.v_out, true)) return FA_ERR_INVALID_ARG;
+    const int64_t per = kKv8Rows * (kKv8Threads / 64), grid = (int64_t(a.total) + per - 1) / per;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
+        hipLaunchKernelGGL((kv8_read_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),
+                           dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a);
+        return int(hipGetLastError());
+    });
+}

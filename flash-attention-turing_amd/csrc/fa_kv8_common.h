@@ -1,0 +1,315 @@
+// Shared by the kernels of a key-value cache in 8 bits: codes, places in the cache, and the plan of an attention call.
+//
+// A value is code * scale, one scale for each block of tokens of a head.  A tile of 32 keys lies in one block, so
+// its scales are two numbers of the wave: k's multiplies scores, v's probabilities, and no element is
+// ever scaled.  Codes of both types are exact in fp16 and in bf16.
+#pragma once
+
+#include "fa_diff_common.h"
+
+namespace fa {
+
+constexpr float kKv8MinScale = 1.17549435e-38f;  // 2^-126
+
+// Eight codes as MFMA operand elements: fp16 (BF: bf16).
+template <bool INT8, bool BF>
+__device__ __forceinline__ f16x8 kv8_decode(const u32x2 c) {
+    u32x4 r;
+    if constexpr (!INT8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (BF) {
+                r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.f, false));
+                r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.f, true));
+            } else {
+                r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, false));
+                r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, true));
+            }
+        }
+    } else if constexpr (BF) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float lo = float(int8_t(c[i] >> 16 * h)), hi = float(int8_t(c[i] >> (16 * h + 8)));
+                // At most 7 bits: the upper halves of the fp32 words are the bf16 values.
+                r[2 * i + h] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+            }
+    } else {
+        // 0x6400 | u is 1024 + u in fp16, u = code + 128.
+        const _Float16 off = _Float16(-1152.f);
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = c[i] ^ 0x80808080u;
+            const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(u, 0x64646464u, 0x00050004u)) + h2{off, off};
+            const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(u, 0x64646464u, 0x00070006u)) + h2{off, off};
+            r[2 * i] = __builtin_bit_cast(uint32_t, a);
+            r[2 * i + 1] = __builtin_bit_cast(uint32_t, b);
+        }
+    }
+    return as_h8(r);
+}
+
+// Four codes from and to fp32 values in the codes' own units.
+template <bool INT8>
+__device__ __forceinline__ f32x4 kv8_values(uint32_t c) {
+    f32x4 v;
+    if constexpr (INT8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = float(int8_t(c >> 8 * i));
+    } else {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+        v = f32x4{a[0], a[1], b[0], b[1]};
+    }
+    return v;
+}
+template <bool INT8>
+__device__ __forceinline__ uint32_t kv8_codes(const f32x4 v) {
+    if constexpr (INT8) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c |= uint32_t(uint8_t(int8_t(int(rintf(v[i]))))) << 8 * i;
+        return c;
+    } else {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], c, true));
+    }
+}
+
+// A wave-uniform float of memory that no kernel in flight writes, through the scalar cache.
+__device__ __forceinline__ float scalar_float(const float *p) {
+    return *(const __attribute__((address_space(4))) float *)uniform(p);
+}
+
+// Cache row of sequence b, and what is wrong with it and with its lengths (0: nothing).
+__device__ __forceinline__ int kv8_err(const fa_kv8_cache &c, int b, int L0, int n, int most_new, int &row) {
+    row = c.cache_batch_idx ? c.cache_batch_idx[b] : b;
+    const int err = (L0 < 0 || n < 0 || n > most_new || int64_t(L0) + n > c.cache_capacity ? 1 : 0) |
+                    (c.cache_batch_idx && (row < 0 || row >= c.cache_batch) ? 2 : 0);
+    if (err) row = 0;
+    return err;
+}
+
+// Attention's plan, made by one workgroup of the launch before: the keys of each sequence cut into equal pieces, so
+// many that the chip has work for all its places.  All pieces have `piece` keys (the last ones of a
+// sequence fewer), whatever the capacity is; a sequence without keys has one empty piece.
+struct Kv8Slot {
+    int b, row;         // sequence, its cache row
+    int begin, end;     // keys
+    int keys;           // of the sequence
+    int ch, n_pieces;   // this piece, and how many the sequence has
+    int pad;
+};
+static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
+
+// Workspace: counters of the (sequence, KV head, row tile) items, the slots, then the partial results.
+struct Kv8Plan {
+    int row_tiles;      // of a KV head
+    int rows_max;       // rows of a tile whose partial results are kept
+    int slots;          // at most
+    int round;          // piece lengths are multiples of it
+    int fixed;          // keys of a piece, where the call says so, or 0
+    int want;           // slots that fill the chip
+    int least;          // keys of a piece at least
+    int64_t items;      // batch * nheads_k * row_tiles
+    int64_t at_slots, at_ml, at_o, bytes;
+};
+
+// First key that a row at position p sees, and its last one.
+__device__ __forceinline__ int kv8_first(const fa_kv8_args &a, int p) { return a.window_left >= 0 ? max(p - a.window_left, 0) : 0; }
+__device__ __forceinline__ int kv8_last(const fa_kv8_args &a, int p, int L) {
+    const int64_t r = a.causal ? p : a.window_right >= 0 ? int64_t(p) + a.window_right : L - 1;
+    return int(min(r, int64_t(L - 1)));
+}
+
+// Sum of x over the 256 threads of a workgroup and the sum over those before this one.
+__device__ __forceinline__ int64_t kv8_scan(int64_t x, int64_t &total) {
+    __shared__ int64_t part[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t inc = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(inc, d);
+        if (lane >= d) inc += y;
+    }
+    __syncthreads();  // the last call's reads are done
+    if (lane == 63) part[wave] = inc;
+    __syncthreads();
+    int64_t base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        base += w < wave ? part[w] : 0;
+        total += part[w];
+    }
+    return base + inc - x;
+}
+
+// One workgroup: the slots of an attention call.
+__device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Plan &plan) {
+    __shared__ int64_t before[257];
+    __shared__ int keys_of[256], begin_of[256], row_of[256];
+    const int tid = threadIdx.x;
+    Kv8Slot *slots = reinterpret_cast<Kv8Slot *>(static_cast<char *>(a.ws) + plan.at_slots);
+    auto sequence = [&](int b, int &begin, int &L, int &row) {
+        const int L0 = a.cache_seqlens[b], err = kv8_err(a.cache, b, L0, a.seqlen_new, a.seqlen_new, row);
+        if (err && a.cache.status) atomicOr(a.cache.status, err);
+        L = err ? 0 : L0 + a.seqlen_new;
+        begin = min(kv8_first(a, max(L - a.seqlen_q, 0)), L) / 32 * 32;
+    };
+    int piece = plan.fixed;
+    if (piece == 0) {
+        int64_t sum = 0, total;
+        for (int b = tid; b < a.cache.batch; b += 256) {
+            int begin, L, row;
+            sequence(b, begin, L, row);
+            sum += L - begin;
+        }
+        kv8_scan(sum, total);
+        const int64_t c = (total + plan.want - 1) / plan.want;
+        piece = int(max(int64_t(plan.least), (c + plan.round - 1) / plan.round * plan.round));
+    }
+    int64_t done = 0;
+    for (int b0 = 0; b0 < a.cache.batch; b0 += 256) {
+        const int b = b0 + tid;
+        int begin = 0, L = 0, row = 0, n = 0;
+        if (b < a.cache.batch) {
+            sequence(b, begin, L, row);
+            n = max(1, int((int64_t(L) - begin + piece - 1) / piece));
+        }
+        int64_t total;
+        const int64_t at = kv8_scan(n, total);
+        before[tid] = at;
+        keys_of[tid] = L;
+        begin_of[tid] = begin;
+        row_of[tid] = row;
+        if (tid == 0) before[256] = total;
+        __syncthreads();
+        for (int64_t s = tid; s < total && done + s < plan.slots; s += 256) {
+            int lo = 0;  // the last sequence whose first slot is at or before s
+#pragma unroll
+            for (int d = 128; d > 0; d >>= 1)
+                if (before[lo + d] <= s) lo += d;
+            Kv8Slot x;
+            x.b = b0 + lo;
+            x.row = row_of[lo];
+            x.ch = int(s - before[lo]);
+            x.keys = keys_of[lo];
+            x.n_pieces = int(before[lo + 1] - before[lo]);
+            x.begin = begin_of[lo] + x.ch * piece;
+            x.end = min(x.keys, x.begin + piece);
+            x.pad = 0;
+            slots[done + s] = x;
+        }
+        done += total;
+        __syncthreads();
+    }
+    for (int64_t s = done + tid; s < plan.slots; s += 256) slots[s].b = -1;
+}
+
+// A wave-uniform slot, through the scalar cache.
+__device__ __forceinline__ Kv8Slot kv8_slot(const fa_kv8_args &a, const Kv8Plan &plan, int i) {
+    typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+    const i32x8 *s = reinterpret_cast<const i32x8 *>(static_cast<const char *>(a.ws) + plan.at_slots) + i;
+    return __builtin_bit_cast(Kv8Slot, i32x8(*(const __attribute__((address_space(4))) i32x8 *)uniform(s)));
+}
+
+// Writes one row of the output: x holds channels d and d + 1 over the sum l.
+template <int HD, bool BF>
+__device__ __forceinline__ void kv8_store(const fa_kv8_args &a, int b, int hk, int row, int d, f32x2 x, float m, float l) {
+    const int G = a.nheads / a.cache.nheads_k, qp = row / G, h = hk * G + row - qp * G;
+    // A sum of 0 is that of a row without a visible key (or with scores of -infinity alone); NaN goes on to the output.
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const f16x4 y = l == 0.f ? pack4<BF>(0.f, 0.f, 0.f, 0.f) : pack4<BF>(x[0] * inv, x[1] * inv, 0.f, 0.f);
+    f16 *out = (f16 *)a.o.ptr + int64_t(b) * a.o.batch_stride + int64_t(qp) * a.o.row_stride + int64_t(h) * a.o.head_stride + d;
+    *reinterpret_cast<uint32_t *>(out) = __builtin_bit_cast(u32x2, y)[0];
+    if (d == 0) a.lse[(int64_t(b) * a.nheads + h) * a.seqlen_q + qp] = l == 0.f ? 0.f : (m + log2_fast(l)) * kLn2;
+}
+
+// Partial results of a piece: rows_max (maximum, sum) pairs and rows_max x HD / 2 pairs of unnormalised fp32 O.
+__device__ __forceinline__ uint64_t *kv8_ml(const fa_kv8_args &a, const Kv8Plan &p, int64_t part) {
+    return reinterpret_cast<uint64_t *>(static_cast<char *>(a.ws) + p.at_ml) + part * p.rows_max;
+}
+template <int HD>
+__device__ __forceinline__ uint64_t *kv8_o(const fa_kv8_args &a, const Kv8Plan &p, int64_t part) {
+    return reinterpret_cast<uint64_t *>(static_cast<char *>(a.ws) + p.at_o) + part * p.rows_max * (HD / 2);
+}
+__device__ __forceinline__ void kv8_put(uint64_t *p, f32x2 x) {
+    __hip_atomic_store(p, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 kv8_get(const uint64_t *p) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Counts a piece whose partial results are stored; true in the workgroup that counts last, which joins them all.
+__device__ __forceinline__ bool kv8_count(int32_t *count, int n_pieces, int *ticket) {
+    wait_vmem();
+    __syncthreads();  // every wave's stores have completed
+    if (threadIdx.x == 0) *ticket = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return *ticket == n_pieces - 1;
+}
+
+// Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels).  scratch: LDS of
+// ROWS * (kKv8Join + 2) floats.  part(i) is the place of piece i's partial results.
+constexpr int kKv8Join = 32;  // pieces whose weights are in LDS at a time
+template <int HD, bool BF, int ROWS, class Part>
+__device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &plan, int b, int hk, int row0, int rows, int n,
+                                         float *scratch, Part part) {
+    constexpr int UNITS = ROWS * (HD / 2) / 256, T = 256 / ROWS < 1 ? 1 : 256 / ROWS;  // T threads a row look for its maximum
+    float *top = scratch, *sum = scratch + ROWS, *weight = scratch + 2 * ROWS;
+    const int tid = threadIdx.x, r = tid / T, t = tid % T;
+    float mm = -INFINITY, ll = 0.f;
+    if (r < rows)
+        for (int i = t; i < n; i += T) mm = fmaxf(mm, kv8_get(kv8_ml(a, plan, part(i)) + r)[0]);
+#pragma unroll
+    for (int d = 1; d < T; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+    f32x2 x[UNITS] = {};
+    for (int i0 = 0; i0 < n; i0 += kKv8Join) {
+        const int k = min(kKv8Join, n - i0);
+        __syncthreads();  // the weights before are used up
+        if (r < rows)
+            for (int i = t; i < k; i += T) {
+                const f32x2 ml = kv8_get(kv8_ml(a, plan, part(i0 + i)) + r);
+                const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - mm);
+                weight[i * ROWS + r] = f;
+                ll = fmaf(ml[1], f, ll);
+            }
+        __syncthreads();
+        constexpr int AHEAD = UNITS >= 16 ? 1 : 8;
+        for (int i = 0; i < k; i += AHEAD) {
+            f32x2 y[AHEAD][UNITS];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    const int e = u * 256 + tid, row = e / (HD / 2);
+                    y[j][u] = i + j < k && row < rows ? kv8_get(kv8_o<HD>(a, plan, part(i0 + i + j)) + e) : f32x2{0.f, 0.f};
+                }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    const int row = (u * 256 + tid) / (HD / 2);
+                    const float f = i + j < k && row < rows ? weight[(i + j) * ROWS + row] : 0.f;
+                    x[u][0] = fmaf(f, y[j][u][0], x[u][0]);
+                    x[u][1] = fmaf(f, y[j][u][1], x[u][1]);
+                }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < T; d <<= 1) ll += __shfl_xor(ll, d);
+    if (t == 0 && r < ROWS) {
+        top[r] = mm;
+        sum[r] = ll;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int e = u * 256 + tid, row = e / (HD / 2);
+        if (row < rows) kv8_store<HD, BF>(a, b, hk, row0 + row, 2 * (e % (HD / 2)), x[u], top[row], sum[row]);
+    }
+}
+
+}  // namespace fa

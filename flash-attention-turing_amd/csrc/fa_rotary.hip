@@ -14,23 +14,6 @@ namespace fa {
 
 constexpr int kRtThreads = 256, kRtHeads = 4;  // heads a lane has in flight
 
-// The last sequence that starts at or before the row (-1: none), by the whole wave: 64 starts are compared at a time.
-__device__ __forceinline__ int rt_sequence(const int32_t *cu, int batch, int row) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = batch + 1;
-    while (n > 0) {
-        const int step = (n + 63) / 64, i = lo + lane * step;
-        const bool starts = lane * step < n && cu[i] <= row;
-        const int k = __popcll(__builtin_amdgcn_ballot_w64(starts));
-        if (k == 0) return lo - 1;
-        lo += (k - 1) * step;
-        if (step == 1) return lo;
-        n = min(step, n - (k - 1) * step);
-        // lo itself starts at or before the row; what follows it is looked at next.
-    }
-    return lo;
-}
-
 template <bool BF>
 __device__ __forceinline__ void rt_unpack(const u32x4 v, float (&x)[8]) {
 #pragma unroll
@@ -79,7 +62,7 @@ __global__ __launch_bounds__(kRtThreads) void rotary_kernel(const fa_rotary_args
     int b = 0, i = int(r), seq = 0;
     bool covered = true;
     if (a.cu_seqlens) {
-        seq = rt_sequence(a.cu_seqlens, a.batch, i);
+        seq = packed_sequence(a.cu_seqlens, a.batch, i);
         covered = seq >= 0 && seq < a.batch;
     } else {
         b = seq = int(r / a.seqlen);

@@ -634,4 +634,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_diff(m);
     bind_kvpages(m);
     bind_rotary(m);
+    bind_kv8(m);
 }

@@ -143,6 +143,33 @@ class FaRotaryArgs(ctypes.Structure):
     ]
 
 
+class FaKv8Scales(ctypes.Structure):
+    _fields_ = [("ptr", _p), ("batch_stride", _i64), ("row_stride", _i64), ("head_stride", _i64)]
+
+
+class FaKv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", FaTensor), ("v", FaTensor), ("k_scale", FaKv8Scales), ("v_scale", FaKv8Scales), ("cache_batch_idx", _p),
+        ("block_table", _p), ("block_table_stride", _i64), ("batch", _i32), ("nheads_k", _i32), ("head_dim", _i32),
+        ("scale_block", _i32), ("kind", _i32), ("page_block_size", _i32), ("num_pages", _i32), ("cache_capacity", _i32),
+        ("cache_batch", _i32), ("status", _p),
+    ]
+
+
+class FaKv8Args(ctypes.Structure):
+    _fields_ = [
+        ("cache", FaKv8Cache), ("k_new", FaTensor), ("v_new", FaTensor), ("cache_seqlens", _p), ("seqlens_new", _p),
+        ("seqlen_new", _i32), ("dtype", _i32), ("q", FaTensor), ("o", FaTensor), ("lse", _p), ("seqlen_q", _i32),
+        ("nheads", _i32), ("causal", _i32), ("window_left", _i32), ("window_right", _i32), ("num_splits", _i32),
+        ("softmax_scale", _f32), ("ws", _p), ("ws_bytes", _i64),
+    ]
+
+
+class FaKv8ReadArgs(ctypes.Structure):
+    _fields_ = [("cache", FaKv8Cache), ("k_out", FaTensor), ("v_out", FaTensor), ("cu_seqlens", _p), ("total", _i32),
+                ("dtype", _i32)]
+
+
 _ARGP = {
     "fa_fwd": FaFwdArgs,
     "fa_bwd_preprocess": FaBwdArgs,
@@ -164,6 +191,9 @@ _ARGP = {
     "fa_kvpages_compact": FaKvpagesArgs,
     "fa_rotary_tables": FaRotaryTablesArgs,
     "fa_rotary": FaRotaryArgs,
+    "fa_kv8_append": FaKv8Args,
+    "fa_kv8_attention": FaKv8Args,
+    "fa_kv8_read": FaKv8ReadArgs,
 }
 # Sizes of workspaces, of the same structs.
 _SIZES = {
@@ -173,6 +203,7 @@ _SIZES = {
     "fa_diff_bwd_split_bytes": FaDiffBwdArgs,
     "fa_diff_kvcache_ws_bytes": FaDiffKvcacheArgs,
     "fa_kvpages_ws_bytes": FaKvpagesArgs,
+    "fa_kv8_ws_bytes": FaKv8Args,
 }
 
 # FA_ABI_VERSION of include/fa_mi355x.h whose struct layouts the classes above mirror.

@@ -21,6 +21,10 @@ and rotary positions
 
     flash_attn_rotary_tables, flash_attn_rotary_func
 
+and a KV cache in 8 bits
+
+    flash_attn_kvcache_append_q8, flash_attn_kvcache_read_q8, flash_attn_with_kvcache_q8
+
 and the autograd classes FlashAttnFunc, FlashAttnQKVPackedFunc,
 FlashAttnKVPackedFunc, FlashAttnVarlenFunc, FlashAttnVarlenQKVPackedFunc,
 FlashAttnVarlenKVPackedFunc (:172-445).  Every call goes to the native
@@ -908,3 +912,167 @@ def flash_attn_rotary_func(
     else:
         q, k = flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest, False)
     return q if k is None else (q, k)
+
+
+# ---------------------------------------------------------------------------
+# A KV cache in 8 bits (no counterpart in the reference).
+#
+# The caches are those of flash_attn_with_kvcache with codes of one byte: k_cache and v_cache [num_blocks, page_block_size,
+# nheads_k, headdim] with a block_table, or [rows, capacity, nheads_k, headdim], torch.float8_e4m3fn or torch.int8, and
+# k_scale and v_scale fp32 [num_blocks or rows, page_block_size or capacity / block, nheads_k]: a value is its code times
+# the scale of its block of tokens and head.  block (32, 64, 128 or 256 tokens) follows from the shapes.  New caches need no
+# clearing.  The appends make scales powers of two: the smallest s >= 2 ** -126 with max|x| <= most * s (most is 448 for
+# e4m3, 127 for int8), or the old one where the block holds earlier tokens and that is larger; codes are x / s, rounded to
+# nearest even, and earlier tokens' codes are rounded again where a scale grows.  A NaN or an infinity among a block's new
+# values makes its scale NaN.  The readers take any scales that are not negative.
+
+
+def _q8_places(batch, k_cache, lens, seqlen_new, cache_batch_idx, block_table, validate):
+    """What is wrong with lengths (int32 [batch] tokens before the new ones), rows and pages; validate reads them."""
+    for name, t, dim in (("cache_batch_idx", cache_batch_idx, 1), ("block_table", block_table, 2)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise TypeError(f"{name} must be a torch.int32 tensor")
+        if t.dim() != dim or t.shape[0] != batch:
+            raise ValueError(f"{name} must have batch_size rows")
+    if block_table is not None and cache_batch_idx is not None:
+        raise NotImplementedError("Paged KV cache does not support cache_batch_idx")
+    if not validate or batch == 0:
+        return
+    capacity, before = _cache_capacity(k_cache, block_table), lens.cpu().long()
+    used = before + (seqlen_new.cpu().long() if isinstance(seqlen_new, torch.Tensor) else seqlen_new)
+    if int(before.min()) < 0 or int(used.max()) > capacity or int((used - before).min()) < 0:
+        raise ValueError("cache capacity is insufficient for the requested append length")
+    if cache_batch_idx is not None:
+        rows = cache_batch_idx.cpu()
+        if int(rows.min()) < 0 or int(rows.max()) >= k_cache.shape[0]:
+            raise RuntimeError("cache_batch_idx entries must be within cache batch bounds")
+    if block_table is not None and block_table.shape[1] > 0:
+        pages = block_table.cpu()
+        needed = torch.arange(pages.shape[1]) * k_cache.shape[1] < used[:, None]
+        if bool((needed & ((pages < 0) | (pages >= k_cache.shape[0]))).any()):
+            raise RuntimeError("block_table entries in use must be pages of the cache")
+
+
+def _q8_lengths(cache_seqlens, batch):
+    if not isinstance(cache_seqlens, torch.Tensor) or cache_seqlens.dtype != torch.int32:
+        raise TypeError("cache_seqlens must be a torch.int32 tensor")
+    if cache_seqlens.dim() != 1 or cache_seqlens.shape[0] != batch:
+        raise ValueError("cache_seqlens must have batch_size rows")
+
+
+def flash_attn_kvcache_append_q8(
+    k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+    v_scale: torch.Tensor, cache_seqlens: torch.Tensor, cache_batch_idx: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None, seqlens_new: Optional[torch.Tensor] = None, validate: bool = True,
+) -> None:
+    """Quantise k and v (batch, seqlen_new, nheads_k, headdim; fp16 or bf16) into a cache in 8 bits at cache_seqlens
+    (int32 (batch,), which the caller advances).  seqlens_new (int32 (batch,)): new tokens of each sequence of a padded
+    batch, the rows of k and v behind them are not looked at; None: all of them.
+
+    validate as in flash_diff_attn_with_kvcache: True checks lengths, rows and pages on the host; False leaves that to the
+    kernels, which append nothing where something is wrong and record it for flash_attn_kvcache_check()."""
+    batch = k.shape[0]
+    _q8_lengths(cache_seqlens, batch)
+    if seqlens_new is not None:
+        if not isinstance(seqlens_new, torch.Tensor) or seqlens_new.dtype != torch.int32:
+            raise TypeError("seqlens_new must be a torch.int32 tensor")
+        if seqlens_new.dim() != 1 or seqlens_new.shape[0] != batch:
+            raise ValueError("seqlens_new must have batch_size rows")
+        if validate and batch > 0 and int(seqlens_new.max()) > k.shape[1]:
+            raise ValueError("seqlens_new must not be larger than the sequence length of k and v")
+    _q8_places(batch, k_cache, cache_seqlens, k.shape[1] if seqlens_new is None else seqlens_new, cache_batch_idx,
+               block_table, validate)
+    status = None if validate or not k.is_cuda else _kv_status(k.device)
+    flash_attn_gpu.kv8_append(
+        maybe_contiguous(k), maybe_contiguous(v), k_cache, v_cache, k_scale, v_scale, maybe_contiguous(cache_seqlens),
+        maybe_contiguous(cache_batch_idx), maybe_contiguous(block_table), maybe_contiguous(seqlens_new), status,
+    )
+
+
+def flash_attn_kvcache_read_q8(
+    k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, cu_seqlens_k: torch.Tensor,
+    total_k: int, cache_batch_idx: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
+    dtype: torch.dtype = torch.float16, validate: bool = True,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The first tokens of every sequence of a cache in 8 bits, packed for flash_attn_varlen_func: k and v (total_k,
+    nheads_k, headdim) of dtype (float16 or bfloat16), cu_seqlens_k[b + 1] - cu_seqlens_k[b] tokens of sequence b in rows
+    cu_seqlens_k[b] and on.  Values are rounded once (those of float16 may overflow).  Rows that no sequence covers are 0.
+
+    validate as in flash_attn_kvcache_append_q8; with False, a sequence that is longer than the cache's capacity is 0."""
+    if not isinstance(cu_seqlens_k, torch.Tensor) or cu_seqlens_k.dtype != torch.int32:
+        raise TypeError("cu_seqlens_k must be a torch.int32 tensor")
+    if cu_seqlens_k.dim() != 1 or cu_seqlens_k.shape[0] < 1:
+        raise ValueError("cu_seqlens_k must have batch_size + 1 elements")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("dtype must be torch.float16 or torch.bfloat16")
+    if total_k < 0:
+        raise ValueError("total_k must be non-negative")
+    batch = cu_seqlens_k.shape[0] - 1
+    if validate:
+        cu = cu_seqlens_k.cpu()
+        if int(cu[0]) < 0 or int(cu[-1]) > total_k or bool((cu[1:] < cu[:-1]).any()):
+            raise ValueError("cu_seqlens_k must not decrease and end at total_k at most")
+        _q8_places(batch, k_cache, torch.zeros_like(cu[1:]), cu[1:] - cu[:-1], cache_batch_idx, block_table, True)
+    else:
+        _q8_places(batch, k_cache, None, 0, cache_batch_idx, block_table, False)
+    status = None if validate or not k_cache.is_cuda else _kv_status(k_cache.device)
+    return flash_attn_gpu.kv8_read(
+        k_cache, v_cache, k_scale, v_scale, maybe_contiguous(cu_seqlens_k), total_k, maybe_contiguous(cache_batch_idx),
+        maybe_contiguous(block_table), dtype == torch.bfloat16, status,
+    )
+
+
+def flash_attn_with_kvcache_q8(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    k: Optional[torch.Tensor] = None,
+    v: Optional[torch.Tensor] = None,
+    cache_seqlens: Optional[Union[torch.Tensor, int]] = None,
+    cache_batch_idx: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    causal: bool = False,
+    window_size: Tuple[int, int] = (-1, -1),
+    num_splits: int = 0,
+    return_softmax_lse: bool = False,
+    validate: bool = True,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """flash_attn_with_kvcache over a cache in 8 bits, for inference: k and v are quantised into it as by
+    flash_attn_kvcache_append_q8, then q (batch, seqlen_q, nheads, headdim; fp16 or bf16, headdim 64 or 128) attends over
+    cache_seqlens + seqlen_new keys.  Masks, window_size, grouped heads and rows without a visible key (0, LSE 0) as there.
+
+    The keys are cut into pieces on the device by the lengths of the whole batch; num_splits > 0 cuts the cache's capacity
+    into that many instead, and a row's bits then do not depend on the batch.  return_softmax_lse adds the log-sum-exp,
+    fp32 (batch, nheads, seqlen_q).  A q without rows (seqlen_q 0) appends alone.  For rotary positions rotate q and k by
+    flash_attn_rotary_func(..., seqlen_offsets=cache_seqlens) first.
+
+    validate as in flash_attn_kvcache_append_q8; with False a call can be captured in a graph, a sequence with a bad length
+    or row is neither appended to nor attended over, a page outside the cache is not written and page 0 is read in its place."""
+    _validate_supported_head_dim(q.shape[-1])
+    if (k is None) != (v is None):
+        raise ValueError("k and v must either both be provided or both be None")
+    if len(tuple(window_size)) != 2 or not all(isinstance(w, int) for w in window_size):
+        raise TypeError("window_size must be a pair of ints")
+    batch = q.shape[0]
+    if cache_seqlens is None:
+        if k is not None:
+            raise ValueError("cache_seqlens is required when appending k and v")
+        cache_seqlens = _cache_capacity(k_cache, block_table)
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((batch,), cache_seqlens, dtype=torch.int32, device=k_cache.device)
+    _q8_lengths(cache_seqlens, batch)
+    if num_splits < 0:
+        raise ValueError("num_splits must be non-negative")
+    _q8_places(batch, k_cache, cache_seqlens, 0 if k is None else k.shape[1], cache_batch_idx, block_table, validate)
+    status = None if validate or not q.is_cuda else _kv_status(q.device)
+    out, lse = flash_attn_gpu.kv8_fwd_kvcache(
+        maybe_contiguous(q), k_cache, v_cache, k_scale, v_scale, maybe_contiguous(k), maybe_contiguous(v),
+        maybe_contiguous(cache_seqlens), maybe_contiguous(cache_batch_idx), maybe_contiguous(block_table),
+        _default_scale(q, softmax_scale), causal, max(window_size[0], -1), max(window_size[1], -1), num_splits, status,
+    )
+    return (out, lse) if return_softmax_lse else out

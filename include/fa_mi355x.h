@@ -470,6 +470,77 @@ typedef struct fa_rotary_args {
 
 int fa_rotary(const fa_rotary_args *args, void *stream);
 
+/*
+ * A key-value cache in 8 bits: codes of one byte and one fp32 scale for each block of
+ * scale_block tokens of a head; a value is code * scale.  fa_kv8_append quantises k_new and v_new
+ * as it writes them at cache_seqlens: a block's scale becomes the smallest power of two s >= 2^-126
+ * with max|x| <= most * s over the block's new values (most: 448 for e4m3, 127 for int8), or
+ * the old scale where the block holds earlier tokens and that is larger, and codes are x / s rounded to
+ * nearest even; earlier tokens' codes are rounded again where the scale grows.  A NaN or an
+ * infinity among the new values makes the scale NaN, and so every value of the block.
+ * Attention takes any scales >= 0.  Lengths, rows and pages are checked on the device as in
+ * fa_diff_kvcache_args.  No counterpart in the reference.
+ */
+enum { FA_KV8_E4M3 = 0, FA_KV8_INT8 = 1 };
+
+/* Scale of (page or cache row, block of tokens, head) at ptr + row * batch_stride + block *
+ * row_stride + head * head_stride (strides in elements). */
+typedef struct fa_kv8_scales {
+    float *ptr;
+    int64_t batch_stride, row_stride, head_stride;
+} fa_kv8_scales;
+
+typedef struct fa_kv8_cache {
+    fa_tensor k, v;                 /* codes [pages or rows][tokens][nheads_k][head_dim], strides multiples of 16 bytes, tokens at most 2^23 apart */
+    fa_kv8_scales k_scale, v_scale; /* [pages or rows][tokens / scale_block][nheads_k] */
+    const int32_t *cache_batch_idx; /* [batch] or NULL (contiguous caches)        */
+    const int32_t *block_table;     /* [batch][block_table_stride] or NULL        */
+    int64_t block_table_stride;
+    int32_t batch, nheads_k, head_dim;
+    int32_t scale_block;            /* 32, 64, 128 or 256; divides the tokens of a page or row */
+    int32_t kind;                   /* FA_KV8_E4M3 or FA_KV8_INT8                 */
+    int32_t page_block_size, num_pages;
+    int32_t cache_capacity;         /* tokens one sequence's cache holds          */
+    int32_t cache_batch;            /* rows of a contiguous cache                 */
+    int32_t *status;                /* device error word, or NULL                 */
+} fa_kv8_cache;
+
+typedef struct fa_kv8_args {
+    fa_kv8_cache cache;
+    fa_tensor k_new, v_new;         /* [batch][seqlen_new][nheads_k][head_dim] of dtype */
+    const int32_t *cache_seqlens;   /* [batch] tokens before the append           */
+    const int32_t *seqlens_new;     /* [batch] new tokens of each sequence, 0 to seqlen_new, or NULL: all of them (fa_kv8_append alone) */
+    int32_t seqlen_new;
+    int32_t dtype;                  /* FA_FP16 or FA_BF16: q, o, k_new and v_new  */
+    /* Attention alone. */
+    fa_tensor q, o;                 /* [batch][seqlen_q][nheads][head_dim]        */
+    float *lse;                     /* fp32 [batch][nheads][seqlen_q]             */
+    int32_t seqlen_q, nheads;
+    int32_t causal;                 /* bottom-right aligned                       */
+    int32_t window_left, window_right; /* keys that a query sees to either side of its own position, -1: all */
+    int32_t num_splits;             /* pieces of cache_capacity, 0: chosen        */
+    float softmax_scale;
+    void *ws;                       /* fa_kv8_ws_bytes(args) bytes, 256-byte aligned */
+    int64_t ws_bytes;
+} fa_kv8_args;
+
+int fa_kv8_append(const fa_kv8_args *args, void *stream);
+size_t fa_kv8_ws_bytes(const fa_kv8_args *args);
+/* The append (seqlen_new > 0), then seqlen_q queries over cache_seqlens + seqlen_new keys. */
+int fa_kv8_attention(const fa_kv8_args *args, void *stream);
+
+/* The first cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence b as values of dtype, in rows cu_seqlens[b]
+ * and on of k_out and v_out; rows that no sequence covers, and those of a sequence that is longer than the cache's
+ * capacity, become 0. */
+typedef struct fa_kv8_read_args {
+    fa_kv8_cache cache;
+    fa_tensor k_out, v_out;         /* packed [total][nheads_k][head_dim]         */
+    const int32_t *cu_seqlens;      /* [batch + 1]                                */
+    int32_t total, dtype;
+} fa_kv8_read_args;
+
+int fa_kv8_read(const fa_kv8_read_args *args, void *stream);
+
 /* Human-readable text for a return code (FA_* or hipError_t). */
 const char *fa_error_string(int code);
 

@@ -50,10 +50,11 @@ setup(
     ext_modules=[
         Extension(
             "flash_attn_turing",
-            sources=[f"{PKG_DIR}/csrc/{f}" for f in ("flash_api.cpp", "diff_api.cpp", "kvpages_api.cpp", "rotary_api.cpp")]
+            sources=[f"{PKG_DIR}/csrc/{f}" for f in ("flash_api.cpp", "diff_api.cpp", "kvpages_api.cpp", "rotary_api.cpp",
+                                              "kv8_api.cpp")]
             + [f"{PKG_DIR}/csrc/{f}" for f in ("fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip",
                                                "fa_diff_fwd.hip", "fa_diff_bwd.hip", "fa_diff_kv.hip",
-                                               "fa_kvpages.hip", "fa_rotary.hip")],
+                                               "fa_kvpages.hip", "fa_rotary.hip", "fa_kv8.hip")],
         )
     ],
     cmdclass={"build_ext": HipBuild},
