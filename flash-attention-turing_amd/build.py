@@ -26,7 +26,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 KERNEL_SOURCES = ["fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip", "fa_diff_fwd.hip", "fa_diff_bwd.hip",
-                  "fa_diff_kv.hip", "fa_kvpages.hip", "fa_rotary.hip", "fa_kv8.hip"]
+                  "fa_diff_kv.hip", "fa_kvpages.hip", "fa_rotary.hip", "fa_kv8.hip", "fa_kv8_fwd.hip"]
 EXTENSION_SOURCES = ["flash_api.cpp", "diff_api.cpp", "kvpages_api.cpp", "rotary_api.cpp", "kv8_api.cpp"]
 LIB_NAME = "libfa_mi355x.so"
 

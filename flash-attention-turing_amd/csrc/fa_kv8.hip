@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read
 // A workgroup's four waves walk the 32-key tiles of its piece (tile t to wave t % 4), each through LDS slots of its own with
 // no barrier in the loop; codes go from memory to LDS without passing registers.
 
-constexpr int kKdTile = 32, kKdRows = 16;
+constexpr int kKdTile = 32;
 
 // Chunk c of row r of a 32-row tile of codes sits at chunk c ^ kd_swz(r): the K reads (16 rows that differ in bits 0, 1, 3 and
 // 4, one chunk) and the transposed V reads (16 rows that differ in bits 0 to 3) then take each bank once.
@@ -465,17 +465,20 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
 // ---------------------------------------------------------------------------
 // Host.
 
+int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s);  // fa_kv8_fwd.hip
+
 static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     Kv8Plan p{};
     const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q, cap = std::max(a.cache.cache_capacity, 1);
-    const int tile = kKdRows;
+    p.many = rows >= 64;
+    const int tile = p.many ? kKcRows : kKdRows;
     p.row_tiles = int((rows + tile - 1) / tile);
-    p.rows_max = int(std::min<int64_t>(rows, tile));
+    p.rows_max = p.many ? tile : int(std::min<int64_t>(rows, tile));
     const int64_t heads = int64_t(a.cache.nheads_k) * p.row_tiles;
     p.items = a.cache.batch * heads;
     p.round = 128;
     p.least = 256;
-    p.want = int(std::max<int64_t>(3 * device_cus() / heads, 1));
+    p.want = int(std::max<int64_t>((p.many ? 2 : 3) * device_cus() / heads, 1));
     int64_t slots;
     if (a.num_splits > 0) {
         p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + p.round - 1) / p.round * p.round);
@@ -520,16 +523,6 @@ static int check_kv8_new(const fa_kv8_args &a) {
     for (const fa_tensor *t : {&a.k_new, &a.v_new})
         if (check_tensor(*t, a.seqlen_new > 0)) return FA_ERR_INVALID_ARG;
     return FA_OK;
-}
-
-// The call with its sizes as types: f(head_dim, bf16, int8).
-template <class F>
-static int kv8_by_type(int head_dim, int dtype, int kind, F f) {
-    auto by_kind = [&](auto hd, auto bf) {
-        return kind == FA_KV8_INT8 ? f(hd, bf, std::true_type{}) : f(hd, bf, std::false_type{});
-    };
-    auto by_dtype = [&](auto hd) { return dtype == FA_BF16 ? by_kind(hd, std::true_type{}) : by_kind(hd, std::false_type{}); };
-    return head_dim == 128 ? by_dtype(std::integral_constant<int, 128>{}) : by_dtype(std::integral_constant<int, 64>{});
 }
 
 // Workgroups that plan and clear (plan NULL: none) and those that append, in one launch.
@@ -602,6 +595,7 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
     const int64_t grid = int64_t(plan.slots) * a.cache.nheads_k * plan.row_tiles;
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     if ((rc = launch_kv8_append(a, &plan, s))) return rc;
+    if (plan.many) return kv8_chunk(a, plan, s);
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
         hipLaunchKernelGGL((kv8_decode_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),
                            dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, plan);

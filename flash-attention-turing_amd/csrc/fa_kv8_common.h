@@ -5,6 +5,8 @@
 // ever scaled.  Codes of both types are exact in fp16 and in bf16.
 #pragma once
 
+#include <type_traits>
+
 #include "fa_diff_common.h"
 
 namespace fa {
@@ -104,7 +106,9 @@ struct Kv8Slot {
 static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
 
 // Workspace: counters of the (sequence, KV head, row tile) items, the slots, then the partial results.
+constexpr int kKdRows = 16, kKcRows = 128;  // rows of a tile: few rows, many
 struct Kv8Plan {
+    bool many;          // the kernel of many rows (fa_kv8_fwd.hip)
     int row_tiles;      // of a KV head
     int rows_max;       // rows of a tile whose partial results are kept
     int slots;          // at most
@@ -310,6 +314,16 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
         const int e = u * 256 + tid, row = e / (HD / 2);
         if (row < rows) kv8_store<HD, BF>(a, b, hk, row0 + row, 2 * (e % (HD / 2)), x[u], top[row], sum[row]);
     }
+}
+
+// The call with its sizes as types: f(head_dim, bf16, int8).
+template <class F>
+static int kv8_by_type(int head_dim, int dtype, int kind, F f) {
+    auto by_kind = [&](auto hd, auto bf) {
+        return kind == FA_KV8_INT8 ? f(hd, bf, std::true_type{}) : f(hd, bf, std::false_type{});
+    };
+    auto by_dtype = [&](auto hd) { return dtype == FA_BF16 ? by_kind(hd, std::true_type{}) : by_kind(hd, std::false_type{}); };
+    return head_dim == 128 ? by_dtype(std::integral_constant<int, 128>{}) : by_dtype(std::integral_constant<int, 64>{});
 }
 
 }  // namespace fa

@@ -54,7 +54,8 @@ setup(
                                               "kv8_api.cpp")]
             + [f"{PKG_DIR}/csrc/{f}" for f in ("fa_abi.hip", "fa_fwd.hip", "fa_bwd.hip", "fa_kvcache.hip",
                                                "fa_diff_fwd.hip", "fa_diff_bwd.hip", "fa_diff_kv.hip",
-                                               "fa_kvpages.hip", "fa_rotary.hip", "fa_kv8.hip")],
+                                               "fa_kvpages.hip", "fa_rotary.hip", "fa_kv8.hip",
+                                               "fa_kv8_fwd.hip")],
         )
     ],
     cmdclass={"build_ext": HipBuild},
