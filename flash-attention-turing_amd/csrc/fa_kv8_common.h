@@ -93,6 +93,63 @@ __device__ __forceinline__ int kv8_err(const fa_kv8_cache &c, int b, int L0, int
     return err;
 }
 
+// The place of a wave-uniform walk over a sequence's keys in steps of a multiple of 32: first bytes of a head's codes of K and
+// V, and their scales.  Nothing is divided in the walk, and a table's entry is loaded a step ahead of its use.
+template <int STEP>
+struct Kv8Walk {
+    const char *k, *v;
+    const float *ks, *vs;
+    int at, page, next, pg;  // token in the page or row, its size, the table's entry for the next step and its index
+    __device__ __forceinline__ void place(const fa_kv8_cache &c, int hk, int64_t line) {
+        k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
+        v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
+        const int blk = at >> __builtin_ctz(c.scale_block);
+        ks = c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride;
+        vs = c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride;
+    }
+    // To key p0 (a multiple of 32) of sequence b, whose cache row is row.  most: the last key that there is.
+    __device__ __forceinline__ void init(const fa_kv8_cache &c, int b, int row, int hk, int p0, int most) {
+        at = p0;
+        int64_t line = row;
+        page = INT_MAX;
+        if (c.block_table) {
+            page = c.page_block_size;
+            pg = p0 / page;
+            at = p0 - pg * page;
+            line = checked_page(scalar_load(c.block_table + int64_t(b) * c.block_table_stride + pg), c.num_pages, c.status);
+            ahead(c, b, most);
+        }
+        place(c, hk, line);
+    }
+    __device__ __forceinline__ void ahead(const fa_kv8_cache &c, int b, int most) {
+        int p = pg, x = at + STEP;
+        while (x >= page) {
+            x -= page;
+            ++p;
+        }
+        // (Entries behind the sequence are not looked at: the last step's would lie there.)
+        if (p != pg && pg * page + at + STEP <= most) next = scalar_load_ahead(c.block_table + int64_t(b) * c.block_table_stride + p);
+    }
+    // One step on, to a key that there is.
+    __device__ __forceinline__ void step(const fa_kv8_cache &c, int b, int hk, int most) {
+        at += STEP;
+        if (at >= page) {
+            do {
+                at -= page;
+                ++pg;
+            } while (at >= page);
+            place(c, hk, checked_page(next, c.num_pages, c.status));
+        } else {
+            k += STEP * c.k.row_stride;
+            v += STEP * c.v.row_stride;
+            const int lg = __builtin_ctz(c.scale_block), blks = (at >> lg) - ((at - STEP) >> lg);
+            ks += blks * c.k_scale.row_stride;
+            vs += blks * c.v_scale.row_stride;
+        }
+        if (c.block_table) ahead(c, b, most);
+    }
+};
+
 // Attention's plan, made by one workgroup of the launch before: the keys of each sequence cut into equal pieces, so
 // many that the chip has work for all its places.  All pieces have `piece` keys (the last ones of a
 // sequence fewer), whatever the capacity is; a sequence without keys has one empty piece.

@@ -12,7 +12,7 @@
 
 namespace fa {
 
-constexpr int kKcThreads = 256, kKcKeys = 64;
+constexpr int kKcThreads = 256, kKcKeys = 64, kKcHalves = kKcThreads;
 // P is kept times 2^7 and its maximum within 2^8 of the reference, so at most 2^15 in fp16; it loses bits under 2^-21.
 constexpr float kKcRaise = 8.f, kKcLift = 7.f;
 
@@ -22,6 +22,14 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     constexpr int CPT = kKcKeys * CH / kKcThreads;  // chunks of 16 codes a thread for K or V of a tile
     constexpr int DT = HD / 32;
     __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+    // Halves of tiles (32 keys, which lie in one page and one block of scales): where their codes begin, k's scale with the
+    // softmax's, V's as what it adds to the exponents of P and takes from their sum, and what it adds to scores: 0 or NaN.
+    struct Half {
+        const char *k, *v;
+        float k_scale, lift, unlift, nan;
+    };
+    __shared__ __attribute__((aligned(16))) Half halves[kKcHalves];
+    __shared__ float tops[4];
     __shared__ int ticket;
 
     const fa_kv8_cache &c = a.cache;
@@ -40,7 +48,6 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     const int g_lo = rt * kKcRows / G, g_hi = (min(rt * kKcRows + kKcRows, R) - 1) / G;
     const int w_lo = min(w_row0, R - 1) / G, w_hi = (min(w_row0 + 32, R) - 1) / G;
     const int s0 = max(sl.begin, kv8_first(a, g_lo + shift)) / 32 * 32, s1 = min(sl.end, kv8_last(a, g_hi + shift, L) + 1);
-    const int n_tiles = s0 < s1 ? (s1 - s0 + kKcKeys - 1) / kKcKeys : 0;
     // Keys that some row of the wave sees, and that all see.
     const int any_first = kv8_first(a, w_lo + shift), any_last = w_row0 < R ? kv8_last(a, w_hi + shift, L) : -1;
     const int all_first = kv8_first(a, w_hi + shift), all_last = min(kv8_last(a, w_lo + shift, L), s1 - 1);
@@ -59,164 +66,211 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
         }
     }
 
-    // Codes of a tile in registers, the scales of its halves of 32 keys.  A half lies in one page and one block of scales.
+    // A thread's row of a half tile and its chunk of 16 codes.  Sixteen lanes that write together take rows whose swizzles
+    // differ in the lowest bit, so that they cover all banks.
+    const int lr = tid / CH, my_ch = tid % CH;
+    const int my_row = HD == 128 ? (lr >> 1 & 7) | (lr & 1) << 3 | (lr & 16) : (lr & 1) | (lr >> 1 & 1) << 2 | (lr >> 2 & 1) << 1 | (lr & ~7);
+    const uint32_t krs = uint32_t(c.k.row_stride), vrs = uint32_t(c.v.row_stride);  // (at most 2^23)
+    // Codes in registers: of V's tile x, and of K's stage x, which is half a tile ahead: halves 2 x - 1 and 2 x.
     u32x4 kr[CPT], vr[CPT];
-    struct Half {
-        float k, v;
-    } next[2], now[2];
-    const int my_row = tid / CH, my_ch = tid % CH;
-    auto load = [&](int t) FA_INLINE {
-        const char *kb[2], *vb[2];
+    auto load = [&](u32x4 (&to)[CPT], bool is_v, int x, int base) FA_INLINE {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int p0 = min(s0 + t * kKcKeys + 32 * h, (L - 1) / 32 * 32);  // keys past the sequence: any of its blocks
+        for (int i = 0; i < CPT; ++i) {  // HD 128: part i; HD 64: part wave / 2
+            const int h = min(max(2 * x + (CPT == 2 ? i : wave >> 1) - (is_v ? 0 : 1), 0), kKcHalves - 1);
+            // Rows past the sequence re-read its last one, so that no stale code reaches a product.
+            const int most = L - 1 - min(base + 32 * h, (L - 1) / 32 * 32);
+            const uint32_t off = __umul24(min(my_row & 31, most), is_v ? vrs : krs) + 16 * my_ch;
+            typedef const __attribute__((address_space(1))) char *global;
+            const global from = (global)uniform(is_v ? halves[h].v : halves[h].k);
+            to[i] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>(from + off);
+        }
+    };
+    // Eight codes in 16 bits to LDS.
+    const int st0 = my_row * (HD * 2) + (((2 * my_ch) ^ swz<HD / 8>(my_row)) << 4);
+    constexpr int VT = 2 * TILE;  // V's tiles lie behind K's
+    auto store_k = [&](int i, int part, int buf) FA_INLINE {
+        const u32x2 q = part ? u32x2{kr[i][2], kr[i][3]} : u32x2{kr[i][0], kr[i][1]};
+        *reinterpret_cast<f16x8 *>(smem + buf * TILE + i * 32 * (HD * 2) + (part ? st0 ^ 16 : st0)) = kv8_decode<INT8, BF>(q);
+    };
+    auto store_v = [&](int i, int part, int buf) FA_INLINE {
+        const u32x2 q = part ? u32x2{vr[i][2], vr[i][3]} : u32x2{vr[i][0], vr[i][1]};
+        *reinterpret_cast<f16x8 *>(smem + VT + buf * TILE + i * 32 * (HD * 2) + (part ? st0 ^ 16 : st0)) = kv8_decode<INT8, false>(q);
+    };
+    auto store_all = [&](bool is_v, int buf) FA_INLINE {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i)
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                if (is_v)
+                    store_v(i, part, buf);
+                else
+                    store_k(i, part, buf);
+            }
+    };
+    TileReader<HD> rd;
+    rd.init(lane);
+    f32x16 o[DT], s[2];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = zero16();
+    float m = -INFINITY, l = 0.f, vref = 0.f;
+    // Operand reads run PIPE - 1 steps ahead behind scheduling fences, from the lane's bases with the buffer added once a
+    // tile (opaque, so that no read address is held in registers through the loop).
+    constexpr int PIPE = 4, NS = HD / 16, NPV = 2 * DT, EPS = 16 / NS;  // EPS: exponentials of a step
+    f16x8 op[PIPE];
+    for (int base = s0; base < s1; base += 32 * kKcHalves) {
+        const int n_tiles = (min(s1 - base, 32 * kKcHalves) + kKcKeys - 1) / kKcKeys;
+        {
+            // The places and scales of the next halves, one a thread; halves behind the sequence repeat its last.
+            const int p0 = min(base + 32 * tid, (L - 1) / 32 * 32);
             int64_t line = sl.row;
             int at = p0;
             if (c.block_table) {
                 const int pg = p0 / c.page_block_size;
-                line = checked_page(scalar_load_ahead(c.block_table + int64_t(sl.b) * c.block_table_stride + pg), c.num_pages, c.status);
                 at = p0 - pg * c.page_block_size;
-            }
-            const int blk = at / c.scale_block;
-            next[h].k = scalar_float(c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride +
-                                     int64_t(hk) * c.k_scale.head_stride);
-            next[h].v = scalar_float(c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride +
-                                     int64_t(hk) * c.v_scale.head_stride);
-            kb[h] = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
-            vb[h] = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
-        }
-#pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            const int r = i * (kKcThreads / CH) + my_row;  // HD 128: half i; HD 64: half wave / 2
-            const int h = CPT == 2 ? i : wave >> 1;
-            // Rows past the sequence re-read its last one, so that no stale code reaches a product.
-            const int p0 = min(s0 + t * kKcKeys + 32 * h, (L - 1) / 32 * 32), rr = min(r & 31, L - 1 - p0);
-            kr[i] = *reinterpret_cast<const u32x4 *>(kb[h] + int64_t(rr) * c.k.row_stride + 16 * my_ch);
-            vr[i] = *reinterpret_cast<const u32x4 *>(vb[h] + int64_t(rr) * c.v.row_stride + 16 * my_ch);
-        }
-    };
-    // The codes in 16 bits to LDS.  Odd rows write their upper eight first: 16 lanes then cover all banks.
-    auto store = [&](int st) FA_INLINE {
-#pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            const int r = i * (kKcThreads / CH) + my_row, odd = r & 1, sw = swz<HD / 8>(r);
-            char *const base = smem + st * STAGE + r * (HD * 2);
-            const int c0 = ((2 * my_ch + odd) ^ sw) << 4, c1 = ((2 * my_ch + 1 - odd) ^ sw) << 4;
-            const f16x8 k0 = kv8_decode<INT8, BF>(u32x2{kr[i][0], kr[i][1]}), k1 = kv8_decode<INT8, BF>(u32x2{kr[i][2], kr[i][3]});
-            const f16x8 v0 = kv8_decode<INT8, false>(u32x2{vr[i][0], vr[i][1]}), v1 = kv8_decode<INT8, false>(u32x2{vr[i][2], vr[i][3]});
-            *reinterpret_cast<f16x8 *>(base + c0) = odd ? k1 : k0;
-            *reinterpret_cast<f16x8 *>(base + c1) = odd ? k0 : k1;
-            *reinterpret_cast<f16x8 *>(base + TILE + c0) = odd ? v1 : v0;
-            *reinterpret_cast<f16x8 *>(base + TILE + c1) = odd ? v0 : v1;
-        }
-    };
-    TileReader<HD> rd;
-    rd.init(lane);
-    f32x16 o[DT];
-#pragma unroll
-    for (int i = 0; i < DT; ++i) o[i] = zero16();
-    float m = -INFINITY, l = 0.f, vref = 0.f;
-    if (n_tiles > 0) {
-        load(0);
-        store(0);
-        now[0] = next[0];
-        now[1] = next[1];
-        if (n_tiles > 1) load(1);
-        __syncthreads();
-    }
-    for (int t = 0; t < n_tiles; ++t) {
-        const int p0 = s0 + t * kKcKeys;
-        const char *ks = smem + (t & 1) * STAGE, *vs = ks + TILE;
-        const bool some = p0 <= any_last && p0 + kKcKeys > any_first;  // (of the wave)
-        f32x16 s[2];
-        if (some) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s[h] = mfma16<BF>(rd.a_operand(ks, 32 * h, 0), qB[0], zero16());
-#pragma unroll
-                for (int g = 1; g < HD / 16; ++g) s[h] = mfma16<BF>(rd.a_operand(ks, 32 * h, g), qB[g], s[h]);
-            }
-        }
-        const Half cur[2] = {now[0], now[1]};
-        if (t + 1 < n_tiles) {
-            store((t + 1) & 1);
-            now[0] = next[0];
-            now[1] = next[1];
-            if (t + 2 < n_tiles) load(t + 2);
-        }
-        if (some) {
-            // V's scale over a reference of the workgroup's, as a power of P; where it is not finite, it reaches the scores
-            // of its keys as NaN.
-            float lift[2], sv0[2], sk[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sv0[h] = cur[h].v * 0.f;
-                sk[h] = cur[h].k * cscale;
-                const float sv = sv0[h] == 0.f ? cur[h].v : 0.f;
-                if (sv > vref) {
-                    const float f = vref / (4.f * sv);  // room for scales that grow a little
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-                    vref = 4.f * sv;
+                line = c.block_table[int64_t(sl.b) * c.block_table_stride + pg];
+                if (line < 0 || line >= c.num_pages) {
+                    if (c.status) atomicOr(c.status, FA_KV_BAD_PAGE);
+                    line = 0;
                 }
-                lift[h] = sv > 0.f ? sv : 0.f;
             }
+            const int blk = at >> __builtin_ctz(c.scale_block);
+            const float ks = c.k_scale.ptr[line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride];
+            float vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
+            Half h;
+            h.k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
+            h.v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
+            // V's scale over a reference, the largest one, as a power of P; where it is not finite, it reaches the scores of
+            // its keys as NaN.
+            h.nan = vs * 0.f;
+            if (!(h.nan == 0.f) || !(vs > 0.f)) vs = 0.f;
+            float top = vs;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) lift[h] = fmaxf(log2_fast(lift[h] / fmaxf(vref, kKv8MinScale)), -64.f) + kKcLift;
-            const bool cut = p0 < all_first || p0 + kKcKeys - 1 > all_last;
-            float top = -INFINITY;
-            if (cut) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int key = p0 + 32 * h + acc_lrow(r, hh);
-                        const float x = fmaf(s[h][r], sk[h], sv0[h]);
-                        s[h][r] = key < first || key > last || key >= s1 ? -INFINITY : x;
-                    }
-                sk[0] = sk[1] = 1.f;
-                sv0[0] = sv0[1] = 0.f;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float x = max3(s[h][0], s[h][1], s[h][2]);
-#pragma unroll
-                for (int r = 3; r < 15; r += 2) x = max3(x, s[h][r], s[h][r + 1]);
-                x = max3(x, s[h][15], x);
-                top = fmaxf(top, cut ? x : x * sk[h]);
-            }
-            if (__builtin_amdgcn_ballot_w64(top > m + kKcRaise) != 0) {
-                const float m_new = fmaxf(m, max2_xor32(top));
-                const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-                l *= alpha;
+            for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+            if (lane == 0) tops[wave] = top;
+            __syncthreads();
+            const float before = vref;
+            vref = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(before, kKv8MinScale));
+            h.k_scale = ks * cscale;
+            h.lift = fmaxf(log2_fast(vs / vref), -64.f) + kKcLift;
+            h.unlift = exp2_fast(-h.lift);
+            halves[tid] = h;
+            if (base > s0) {
+                const float f = before / vref;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-                m = m_new;
+                    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
             }
-            const float m_use = m == -INFINITY ? 0.f : m;
+            __syncthreads();
+        }
+        load(kr, false, 0, base);
+        load(vr, true, 0, base);
+        store_all(false, 0);
+        load(kr, false, 1, base);
+        store_all(true, 0);
+        load(vr, true, 1, base);
+        store_all(false, 1);
+        load(kr, false, 2, base);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NS; ++u) s[0] = mfma16<BF>(rd.a_operand(smem, 32, u), qB[u], u < 1 ? zero16() : s[0]);
+        __syncthreads();
+        for (int t = 0; t < n_tiles; ++t) {
+            // Half h of tile t, with its scores in s[h]: its softmax runs between the products of the next half's scores, the
+            // conversion of the codes of K's stage t + 2 and V's tile t + 1 between the products with V.
+            const int kbuf = (t + 1) & 1, vbuf = t & 1;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float d = lift[h] - m_use + sv0[h];
-                float sum = 0.f;
+                f32x16 &sc = s[h], &sn = s[1 - h];
+                const int p0 = base + t * kKcKeys + 32 * h;
+                const bool some = p0 <= any_last && p0 + 32 > any_first;  // (of the wave)
+                int ab = rd.a_base + kbuf * TILE, tb0 = rd.tr_base[0] + vbuf * TILE, tb1 = rd.tr_base[1] + vbuf * TILE;
+                asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
+                auto rd_k = [&](int u) FA_INLINE { op[u % PIPE] = rd.a_operand_at(smem + 32 * h * (HD * 2), ab, u); };
+                // Step u: channel tile u % DT, 16 keys u / DT.
+                auto rd_v = [&](int u) FA_INLINE {
+                    op[u % PIPE] = rd.tr_operand_at(smem + VT + (32 * h + 16 * (u / DT)) * (HD * 2), tb0, tb1, u % DT);
+                };
+                auto store_some = [&](int x) FA_INLINE {  // x of 2 CPT
+                    if (h == 0)
+                        store_k(x / 2, x % 2, 1 - kbuf);
+                    else
+                        store_v(x / 2, x % 2, 1 - vbuf);
+                };
+                if (some) {
+                    const f32x4 x4 = *reinterpret_cast<const f32x4 *>(&halves[2 * t + h].k_scale);
+                    float sk = uniform(x4[0]), d = x4[1] + x4[3];
+                    if (p0 < all_first || p0 + 31 > all_last) {
+                        const int lo = first - p0 - 8 * hh, hi = min(last, s1 - 1) - p0 - 8 * hh;
+                        d = x4[1];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[h][r] = exp2_fast(fmaf(s[h][r], sk[h], d));
-                    sum += s[h][r];
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = acc_lrow(r, 0);
+                            const float x = fmaf(sc[r], sk, x4[3]);
+                            sc[r] = key < lo || key > hi ? -INFINITY : x;
+                        }
+                        sk = 1.f;
+                    }
+                    float top = max3(sc[0], sc[1], sc[2]);
+#pragma unroll
+                    for (int r = 3; r < 15; r += 2) top = max3(top, sc[r], sc[r + 1]);
+                    top = max3(top, sc[15], top);
+                    top = top == -INFINITY ? top : top * sk;
+                    if (__builtin_amdgcn_ballot_w64(top > m + kKcRaise) != 0) {
+                        const float m_new = fmaxf(m, max2_xor32(top));
+                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+                        l *= alpha;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+                        m = m_new;
+                    }
+                    d -= m == -INFINITY ? 0.f : m;
+                    float sum = 0.f;
+                    f16x8 pB[2];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int u = 0; u < PIPE - 1; ++u) rd_k(u);
+#pragma unroll
+                    for (int u = 0; u < NS; ++u) {
+                        if (u + PIPE - 1 < NS) rd_k(u + PIPE - 1);
+                        sn = mfma16<BF>(op[u % PIPE], qB[u], u < 1 ? zero16() : sn);
+#pragma unroll
+                        for (int e = u * EPS; e < u * EPS + EPS; ++e) {
+                            sc[e] = exp2_fast(fmaf(sc[e], sk, d));
+                            sum += sc[e];
+                            if (e % 8 == 7) pB[e / 8] = pack8(sc, e - 7);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int u = 0; u < PIPE - 1; ++u) rd_v(u);
+                    l = fmaf(sum, x4[2], l);
+                    __builtin_amdgcn_sched_barrier(0);
+                    constexpr int EVERY = NPV / (2 * CPT);  // products between two stores
+#pragma unroll
+                    for (int u = 0; u < NPV; ++u) {
+                        if (u + PIPE - 1 < NPV) rd_v(u + PIPE - 1);
+                        o[u % DT] = mfma16<false>(op[u % PIPE], pB[u / DT], o[u % DT]);
+                        if (u % EVERY == EVERY - 1) store_some(u / EVERY);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2 * CPT; ++x) store_some(x);
+#pragma unroll
+                    for (int u = 0; u < NS; ++u)
+                        sn = mfma16<BF>(rd.a_operand_at(smem + 32 * h * (HD * 2), ab, u), qB[u], u < 1 ? zero16() : sn);
                 }
-                l = fmaf(sum, exp2_fast(-lift[h]), l);
-#pragma unroll
-                for (int gg = 0; gg < 2; ++gg) {
-                    const f16x8 p = pack8(s[h], 8 * gg);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[dt] = mfma16<false>(rd.tr_operand(vs, 32 * h + 16 * gg, dt), p, o[dt]);
+                if (h == 0) {
+                    if (t + 3 <= n_tiles) load(kr, false, t + 3, base);
+                } else {
+                    if (t + 2 < n_tiles) load(vr, true, t + 2, base);
                 }
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 
     // P's lift and the reference of V's scales leave O.
@@ -257,10 +311,14 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             }
         }
     }
-    if (!row_ok) return;
+    // Opaque to the optimiser: the row's output addresses are formed here, not before the loop and held through it.
+    int orow = row;
+    asm volatile("" : "+v"(orow));
+    if (orow >= R) return;
+    const int oq = orow / G, oh = hk * G + orow - oq * G;
     // A sum of 0 is that of a row without a visible key (or with scores of -infinity alone); NaN goes on to the output.
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    f16 *out = (f16 *)a.o.ptr + int64_t(sl.b) * a.o.batch_stride + int64_t(qpos) * a.o.row_stride + int64_t(hq) * a.o.head_stride + 4 * hh;
+    f16 *out = (f16 *)a.o.ptr + int64_t(sl.b) * a.o.batch_stride + int64_t(oq) * a.o.row_stride + int64_t(oh) * a.o.head_stride + 4 * hh;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -269,7 +327,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             if (l == 0.f) y = pack4<BF>(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<f16x4 *>(out + 32 * dt + 2 * r) = y;
         }
-    if (hh == 0) a.lse[(int64_t(sl.b) * a.nheads + hq) * a.seqlen_q + qpos] = l == 0.f ? 0.f : (m + log2_fast(l)) * kLn2;
+    if (hh == 0) a.lse[(int64_t(sl.b) * a.nheads + oh) * a.seqlen_q + oq] = l == 0.f ? 0.f : (m + log2_fast(l)) * kLn2;
 }
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s) {
