@@ -214,26 +214,6 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read
 
 constexpr int kKdTile = 32;
 
-// Chunk c of row r of a 32-row tile of codes sits at chunk c ^ kd_swz(r): the K reads (16 rows that differ in bits 0, 1, 3 and
-// 4, one chunk) and the transposed V reads (16 rows that differ in bits 0 to 3) then take each bank once.
-template <int HD>
-__device__ __forceinline__ int kd_swz(int r) {
-    if constexpr (HD == 128)
-        return (r >> 1 & 1) | (r >> 3 & 1) << 1 | ((r >> 4 ^ r >> 2) & 1) << 2;
-    else
-        return (r >> 3 & 1) | ((r >> 4 ^ r >> 2) & 1) << 1;
-}
-
-typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
-
-// ds_read_b64_tr_b8: within 16 lanes, lane i gets byte i % 8 of the 8-byte words at the addresses of lanes 2 j + i / 8,
-// j = 0..7.  With lane 2 j + h at row j, bytes 8 h, lane i so holds column i of 8 rows.
-__device__ __forceinline__ u32x2 lds_tr8(const char *base, int off) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t *)(base + off)));
-}
-
 template <bool BF>
 __device__ __forceinline__ f32x4 kd_mfma(const f16x8 a, const f16x8 b, const f32x4 c) {
     if constexpr (BF)
@@ -308,7 +288,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
         char *const base = slot + st * STAGE;
 #pragma unroll
         for (int i = 0; i < CPW; ++i) {
-            const int r = i * (64 / CH) + p_row, rc = min(r, most), ch = 16 * (p_ch ^ kd_swz<HD>(r));
+            const int r = i * (64 / CH) + p_row, rc = min(r, most), ch = 16 * (p_ch ^ kv8_swz<HD>(r));
             g2l16(kb + int64_t(rc) * krs + ch, base + i * 1024);
             g2l16(vb + int64_t(rc) * vrs + ch, base + TILE + i * 1024);
         }
@@ -350,10 +330,10 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
 #pragma unroll
                 for (int j = 0; j < HD / 64; ++j) {
                     const int r = k_row0 + 4 * t;
-                    kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kd_swz<HD>(r)));
+                    kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kv8_swz<HD>(r)));
                 }
 #pragma unroll
-            for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kd_swz<HD>(v_row)) + v_half);
+            for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kv8_swz<HD>(v_row)) + v_half);
             // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
             const float sk = ks[st] * cscale, sv0 = vs[st] * 0.f, sv = sv0 == 0.f ? vs[st] : 0.f;
             wait_lds();

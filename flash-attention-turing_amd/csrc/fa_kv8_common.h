@@ -53,6 +53,25 @@ __device__ __forceinline__ f16x8 kv8_decode(const u32x2 c) {
     return as_h8(r);
 }
 
+// Chunk c (16 bytes) of row r of 32 rows of codes in LDS sits at chunk c ^ kv8_swz(r).  Every operand read then takes each
+// bank once: 16 bytes of one chunk from 16 rows that differ in bits 0 to 3 or in bits 0, 1, 3 and 4, and transposed reads of one
+// chunk from 16 rows (bits 0 to 3) or of a pair of chunks from 8 (bits 0 to 2).
+template <int HD>
+__device__ __forceinline__ int kv8_swz(int r) {
+    if constexpr (HD == 128)
+        return (r >> 3 & 1) | (r >> 1 & 1) << 1 | ((r >> 4 ^ r >> 2) & 1) << 2;
+    else
+        return (r >> 3 & 1) | ((r >> 4 ^ r >> 2) & 1) << 1;
+}
+
+// ds_read_b64_tr_b8: within 16 lanes, lane i gets byte i % 8 of the 8-byte words at the addresses of lanes 2 j + i / 8,
+// j = 0..7.  With lane 2 j + h at row j, bytes 8 h, lane i so holds column i of 8 rows.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
+__device__ __forceinline__ u32x2 lds_tr8(const char *base, int off) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t *)(base + off)));
+}
+
 // Four codes from and to fp32 values in the codes' own units.
 template <bool INT8>
 __device__ __forceinline__ f32x4 kv8_values(uint32_t c) {

@@ -18,10 +18,10 @@ constexpr float kKcRaise = 8.f, kKcLift = 7.f;
 
 template <int HD, bool BF, bool INT8>
 __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_args a, const Kv8Plan plan) {
-    constexpr int CH = HD / 16, TILE = kKcKeys * HD * 2, STAGE = 2 * TILE;
+    constexpr int CH = HD / 16, TILE = kKcKeys * HD, STAGE = 2 * TILE, NST = 4;
     constexpr int CPT = kKcKeys * CH / kKcThreads;  // chunks of 16 codes a thread for K or V of a tile
     constexpr int DT = HD / 32;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
     // Halves of tiles (32 keys, which lie in one page and one block of scales): where their codes begin, k's scale with the
     // softmax's, V's as what it adds to the exponents of P and takes from their sum, and what it adds to scores: 0 or NaN.
     struct Half {
@@ -55,68 +55,43 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     // Q^T as B operands.
     const bool neg = a.softmax_scale < 0.f;
     const float cscale = fabsf(a.softmax_scale) * kLog2e;
-    f16x8 qB[HD / 16];
+    f16x8 qB[HD / 16];  // step g: channels 32 (g / 2) + 16 hh + 8 (g % 2) + 0..7
     {
         const f16 *qp = (const f16 *)a.q.ptr + int64_t(sl.b) * a.q.batch_stride + int64_t(qpos) * a.q.row_stride +
-                        int64_t(hq) * a.q.head_stride + 8 * hh;
+                        int64_t(hq) * a.q.head_stride + 16 * hh;
 #pragma unroll
         for (int g = 0; g < HD / 16; ++g) {
-            u32x4 v = row_ok ? ldg16(qp + 16 * g) : zero_u4();
+            u32x4 v = row_ok ? ldg16(qp + 32 * (g / 2) + 8 * (g % 2)) : zero_u4();
             qB[g] = as_h8(neg ? neg_h8(v) : v);
         }
     }
 
-    // A thread's row of a half tile and its chunk of 16 codes.  Sixteen lanes that write together take rows whose swizzles
-    // differ in the lowest bit, so that they cover all banks.
-    const int lr = tid / CH, my_ch = tid % CH;
-    const int my_row = HD == 128 ? (lr >> 1 & 7) | (lr & 1) << 3 | (lr & 16) : (lr & 1) | (lr >> 1 & 1) << 2 | (lr >> 2 & 1) << 1 | (lr & ~7);
+    // Copies of a tile's codes to LDS, straight from memory: chunk c of row r of a half lies at chunk c ^ kv8_swz(r).
     const uint32_t krs = uint32_t(c.k.row_stride), vrs = uint32_t(c.v.row_stride);  // (at most 2^23)
-    // Codes in registers: of V's tile x, and of K's stage x, which is half a tile ahead: halves 2 x - 1 and 2 x.
-    u32x4 kr[CPT], vr[CPT];
-    auto load = [&](u32x4 (&to)[CPT], bool is_v, int x, int base) FA_INLINE {
+    const int my_row = tid / CH & 31, my_ch = 16 * (tid % CH ^ kv8_swz<HD>(my_row));
+    const uint32_t lds0 = lds_addr(smem) + wave * 1024;
+    auto issue = [&](int x, int base) FA_INLINE {
+        const uint32_t to = lds0 + (x % NST) * STAGE;
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {  // HD 128: part i; HD 64: part wave / 2
-            const int h = min(max(2 * x + (CPT == 2 ? i : wave >> 1) - (is_v ? 0 : 1), 0), kKcHalves - 1);
+        for (int i = 0; i < CPT; ++i) {  // HD 128: half i; HD 64: half wave / 2
+            const int h = 2 * x + (CPT == 2 ? i : wave >> 1);
             // Rows past the sequence re-read its last one, so that no stale code reaches a product.
-            const int most = L - 1 - min(base + 32 * h, (L - 1) / 32 * 32);
-            const uint32_t off = __umul24(min(my_row & 31, most), is_v ? vrs : krs) + 16 * my_ch;
-            typedef const __attribute__((address_space(1))) char *global;
-            const global from = (global)uniform(is_v ? halves[h].v : halves[h].k);
-            to[i] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>(from + off);
+            const int most = min(my_row, L - 1 - min(base + 32 * h, (L - 1) / 32 * 32));
+            g2l16_at((const f16 *)uniform(halves[h].k), __umul24(most, krs) + my_ch, to + i * 4096);
+            g2l16_at((const f16 *)uniform(halves[h].v), __umul24(most, vrs) + my_ch, to + TILE + i * 4096);
         }
     };
-    // Eight codes in 16 bits to LDS.
-    const int st0 = my_row * (HD * 2) + (((2 * my_ch) ^ swz<HD / 8>(my_row)) << 4);
-    constexpr int VT = 2 * TILE;  // V's tiles lie behind K's
-    auto store_k = [&](int i, int part, int buf) FA_INLINE {
-        const u32x2 q = part ? u32x2{kr[i][2], kr[i][3]} : u32x2{kr[i][0], kr[i][1]};
-        *reinterpret_cast<f16x8 *>(smem + buf * TILE + i * 32 * (HD * 2) + (part ? st0 ^ 16 : st0)) = kv8_decode<INT8, BF>(q);
-    };
-    auto store_v = [&](int i, int part, int buf) FA_INLINE {
-        const u32x2 q = part ? u32x2{vr[i][2], vr[i][3]} : u32x2{vr[i][0], vr[i][1]};
-        *reinterpret_cast<f16x8 *>(smem + VT + buf * TILE + i * 32 * (HD * 2) + (part ? st0 ^ 16 : st0)) = kv8_decode<INT8, false>(q);
-    };
-    auto store_all = [&](bool is_v, int buf) FA_INLINE {
-#pragma unroll
-        for (int i = 0; i < CPT; ++i)
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                if (is_v)
-                    store_v(i, part, buf);
-                else
-                    store_k(i, part, buf);
-            }
-    };
-    TileReader<HD> rd;
-    rd.init(lane);
+    // Operand reads: rows sigma(col) of K, 16 codes of two steps; V transposed, eight keys of a channel.
+    const int kr = sigma(col), k_at = kr * HD + ((hh ^ kv8_swz<HD>(kr)) << 4);
+    const int vr = 8 * hh + (lane & 15) / 2, v_at = vr * HD + ((((lane >> 4) & 1) ^ kv8_swz<HD>(vr)) << 4) + 8 * (lane & 1);
     f32x16 o[DT], s[2];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = zero16();
     float m = -INFINITY, l = 0.f, vref = 0.f;
-    // Operand reads run PIPE - 1 steps ahead behind scheduling fences, from the lane's bases with the buffer added once a
-    // tile (opaque, so that no read address is held in registers through the loop).
-    constexpr int PIPE = 4, NS = HD / 16, NPV = 2 * DT, EPS = 16 / NS;  // EPS: exponentials of a step
-    f16x8 op[PIPE];
+    constexpr int NS = HD / 16, NPV = 2 * DT, EPS = 16 / NS;  // EPS: exponentials of a step
+    constexpr int KP = HD == 128 ? 3 : 2, VP = 4;  // reads in flight, and the next
+    u32x4 kc[KP];
+    u32x2 vc[VP];
     for (int base = s0; base < s1; base += 32 * kKcHalves) {
         const int n_tiles = (min(s1 - base, 32 * kKcHalves) + kKcKeys - 1) / kKcKeys;
         {
@@ -163,40 +138,39 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             }
             __syncthreads();
         }
-        load(kr, false, 0, base);
-        load(vr, true, 0, base);
-        store_all(false, 0);
-        load(kr, false, 1, base);
-        store_all(true, 0);
-        load(vr, true, 1, base);
-        store_all(false, 1);
-        load(kr, false, 2, base);
+        for (int x = 0; x < min(3, n_tiles); ++x) issue(x, base);
+        wait_vmem();
         __syncthreads();
+        // Scores of 32 keys: step u of NS, a read of 16 codes for two.
+        auto k_read = [&](const char *tile, int j) FA_INLINE { kc[j % KP] = *reinterpret_cast<const u32x4 *>(tile + (k_at ^ (j << 5))); };
+        auto k_operand = [&](int u) FA_INLINE {
+            const u32x4 q = kc[u / 2 % KP];
+            return kv8_decode<INT8, BF>(u % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]});
+        };
 #pragma unroll
-        for (int u = 0; u < NS; ++u) s[0] = mfma16<BF>(rd.a_operand(smem, 32, u), qB[u], u < 1 ? zero16() : s[0]);
-        __syncthreads();
+        for (int u = 0; u < NS; ++u) {
+            if (u % 2 == 0) k_read(smem, u / 2);
+            s[0] = mfma16<BF>(k_operand(u), qB[u], u < 1 ? zero16() : s[0]);
+        }
         for (int t = 0; t < n_tiles; ++t) {
-            // Half h of tile t, with its scores in s[h]: its softmax runs between the products of the next half's scores, the
-            // conversion of the codes of K's stage t + 2 and V's tile t + 1 between the products with V.
-            const int kbuf = (t + 1) & 1, vbuf = t & 1;
+            // Tile t + 1 has landed for this wave, and after the barrier for all (t + 2 may be on its way); every wave is done
+            // with tile t - 1, whose place t + 3 takes.
+            if (t + 2 < n_tiles)
+                wait_vmem_n<2 * CPT>();
+            else
+                wait_vmem();
+            __syncthreads();
+            if (t + 3 < n_tiles) issue(t + 3, base);
+            // Half h of tile t, with its scores in s[h]: its softmax runs between the products of the next half's scores.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 f32x16 &sc = s[h], &sn = s[1 - h];
                 const int p0 = base + t * kKcKeys + 32 * h;
                 const bool some = p0 <= any_last && p0 + 32 > any_first;  // (of the wave)
-                int ab = rd.a_base + kbuf * TILE, tb0 = rd.tr_base[0] + vbuf * TILE, tb1 = rd.tr_base[1] + vbuf * TILE;
-                asm volatile("" : "+v"(ab), "+v"(tb0), "+v"(tb1));
-                auto rd_k = [&](int u) FA_INLINE { op[u % PIPE] = rd.a_operand_at(smem + 32 * h * (HD * 2), ab, u); };
-                // Step u: channel tile u % DT, 16 keys u / DT.
-                auto rd_v = [&](int u) FA_INLINE {
-                    op[u % PIPE] = rd.tr_operand_at(smem + VT + (32 * h + 16 * (u / DT)) * (HD * 2), tb0, tb1, u % DT);
-                };
-                auto store_some = [&](int x) FA_INLINE {  // x of 2 CPT
-                    if (h == 0)
-                        store_k(x / 2, x % 2, 1 - kbuf);
-                    else
-                        store_v(x / 2, x % 2, 1 - vbuf);
-                };
+                const char *kt = smem + (h == 0 ? t % NST : (t + 1) % NST) * STAGE + (h == 0 ? 32 * HD : 0);
+                const char *vt = smem + t % NST * STAGE + TILE + 32 * h * HD;
+                // Step u: channel tile u % DT, 16 keys u / DT (row bit 4 is bit HD / 2 of the swizzle).
+                auto v_read = [&](int u) FA_INLINE { vc[u % VP] = lds_tr8(vt, 16 * (u / DT) * HD + (v_at ^ (u % DT << 5) ^ u / DT * (HD / 2))); };
                 if (some) {
                     const f32x4 x4 = *reinterpret_cast<const f32x4 *>(&halves[2 * t + h].k_scale);
                     float sk = uniform(x4[0]), d = x4[1] + x4[3];
@@ -231,11 +205,12 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                     f16x8 pB[2];
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int u = 0; u < PIPE - 1; ++u) rd_k(u);
+                    for (int j = 0; j < KP - 1; ++j) k_read(kt, j);
 #pragma unroll
                     for (int u = 0; u < NS; ++u) {
-                        if (u + PIPE - 1 < NS) rd_k(u + PIPE - 1);
-                        sn = mfma16<BF>(op[u % PIPE], qB[u], u < 1 ? zero16() : sn);
+                        if (u % 2 == 0 && u / 2 + KP - 1 < NS / 2) k_read(kt, u / 2 + KP - 1);
+                        if (u >= NS - (VP - 1)) v_read(u - (NS - (VP - 1)));
+                        sn = mfma16<BF>(k_operand(u), qB[u], u < 1 ? zero16() : sn);
 #pragma unroll
                         for (int e = u * EPS; e < u * EPS + EPS; ++e) {
                             sc[e] = exp2_fast(fmaf(sc[e], sk, d));
@@ -244,33 +219,24 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     }
-#pragma unroll
-                    for (int u = 0; u < PIPE - 1; ++u) rd_v(u);
                     l = fmaf(sum, x4[2], l);
-                    __builtin_amdgcn_sched_barrier(0);
-                    constexpr int EVERY = NPV / (2 * CPT);  // products between two stores
 #pragma unroll
                     for (int u = 0; u < NPV; ++u) {
-                        if (u + PIPE - 1 < NPV) rd_v(u + PIPE - 1);
-                        o[u % DT] = mfma16<false>(op[u % PIPE], pB[u / DT], o[u % DT]);
-                        if (u % EVERY == EVERY - 1) store_some(u / EVERY);
+                        const f16x8 v = kv8_decode<INT8, false>(vc[u % VP]);
+                        if (u + VP - 1 < NPV) v_read(u + VP - 1);
+                        o[u % DT] = mfma16<false>(v, pB[u / DT], o[u % DT]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 } else {
 #pragma unroll
-                    for (int x = 0; x < 2 * CPT; ++x) store_some(x);
-#pragma unroll
-                    for (int u = 0; u < NS; ++u)
-                        sn = mfma16<BF>(rd.a_operand_at(smem + 32 * h * (HD * 2), ab, u), qB[u], u < 1 ? zero16() : sn);
-                }
-                if (h == 0) {
-                    if (t + 3 <= n_tiles) load(kr, false, t + 3, base);
-                } else {
-                    if (t + 2 < n_tiles) load(vr, true, t + 2, base);
+                    for (int u = 0; u < NS; ++u) {
+                        if (u % 2 == 0) k_read(kt, u / 2);
+                        sn = mfma16<BF>(k_operand(u), qB[u], u < 1 ? zero16() : sn);
+                    }
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();  // every wave is done with the table and the tiles
     }
 
     // P's lift and the reference of V's scales leave O.
