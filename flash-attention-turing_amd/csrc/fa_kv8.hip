@@ -245,7 +245,9 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int HI = c.nheads_k * plan.row_tiles;
-    const int slot_i = blockIdx.x / HI, hi_i = blockIdx.x % HI, hk = hi_i / plan.row_tiles, rt = hi_i % plan.row_tiles;
+    int slot_i, hk, rt;
+    if (!kv8_item(plan, c.nheads_k, blockIdx.x, slot_i, hk, rt)) return;
+    const int hi_i = hk * plan.row_tiles + rt;
     const Kv8Slot sl = kv8_slot(a, plan, slot_i);
     if (sl.b < 0) return;
     const int G = a.nheads / c.nheads_k, R = G * a.seqlen_q, L = sl.keys;
@@ -572,7 +574,7 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (a.seqlen_q == 0) return launch_kv8_append(a, nullptr, s);
     const Kv8Plan plan = kv8_plan(a);
-    const int64_t grid = int64_t(plan.slots) * a.cache.nheads_k * plan.row_tiles;
+    const int64_t grid = kv8_grid(plan, a.cache.nheads_k);
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     if ((rc = launch_kv8_append(a, &plan, s))) return rc;
     if (plan.many) return kv8_chunk(a, plan, s);

@@ -196,6 +196,28 @@ struct Kv8Plan {
     int64_t at_slots, at_ml, at_o, bytes;
 };
 
+// Workgroups of an attention call: its (slot, KV head) groups times row tiles.  The tiles of a group read the same codes, so
+// they are dealt to one of the eight XCDs (workgroups go to them in turn), where there are groups enough for all.
+__host__ __device__ __forceinline__ bool kv8_by_xcd(const Kv8Plan &p, int nheads_k) {
+    return p.row_tiles > 1 && (nheads_k % 8 == 0 || int64_t(p.slots) * nheads_k >= 64);
+}
+static inline int64_t kv8_grid(const Kv8Plan &p, int nheads_k) {
+    const int64_t groups = int64_t(p.slots) * nheads_k;
+    return (kv8_by_xcd(p, nheads_k) ? (groups + 7) / 8 * 8 : groups) * p.row_tiles;
+}
+__device__ __forceinline__ bool kv8_item(const Kv8Plan &p, int nheads_k, int wg, int &slot, int &hk, int &rt) {
+    int group = wg / p.row_tiles;
+    rt = wg - group * p.row_tiles;
+    if (kv8_by_xcd(p, nheads_k)) {
+        const int turn = wg / (8 * p.row_tiles), in = wg - turn * 8 * p.row_tiles;
+        group = turn * 8 + in % 8;
+        rt = in / 8;
+    }
+    slot = group / nheads_k;
+    hk = group - slot * nheads_k;
+    return slot < p.slots;
+}
+
 // First key that a row at position p sees, and its last one.
 __device__ __forceinline__ int kv8_first(const fa_kv8_args &a, int p) { return a.window_left >= 0 ? max(p - a.window_left, 0) : 0; }
 __device__ __forceinline__ int kv8_last(const fa_kv8_args &a, int p, int L) {

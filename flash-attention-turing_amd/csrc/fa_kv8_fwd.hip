@@ -13,13 +13,13 @@
 namespace fa {
 
 constexpr int kKcThreads = 256, kKcKeys = 64, kKcHalves = kKcThreads;
-// P is kept times 2^7 and its maximum within 2^8 of the reference, so at most 2^15 in fp16; it loses bits under 2^-21.
-constexpr float kKcRaise = 8.f, kKcLift = 7.f;
+// P is kept times at most 2^5, and its reference is raised when the sum of a lane's 16 passes 2^15: fp16 holds it, with all its
+// bits down to 2^-19.
+constexpr float kKcTop = 32768.f, kKcLift = 5.f;
 
 template <int HD, bool BF, bool INT8>
 __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_args a, const Kv8Plan plan) {
     constexpr int CH = HD / 16, TILE = kKcKeys * HD, STAGE = 2 * TILE, NST = 4;
-    constexpr int CPT = kKcKeys * CH / kKcThreads;  // chunks of 16 codes a thread for K or V of a tile
     constexpr int DT = HD / 32;
     __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
     // Halves of tiles (32 keys, which lie in one page and one block of scales): where their codes begin, k's scale with the
@@ -36,7 +36,9 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int HI = c.nheads_k * plan.row_tiles;
-    const int slot_i = blockIdx.x / HI, hi_i = blockIdx.x % HI, hk = hi_i / plan.row_tiles, rt = hi_i % plan.row_tiles;
+    int slot_i, hk, rt;
+    if (!kv8_item(plan, c.nheads_k, blockIdx.x, slot_i, hk, rt)) return;
+    const int hi_i = hk * plan.row_tiles + rt;
     const Kv8Slot sl = kv8_slot(a, plan, slot_i);
     if (sl.b < 0) return;
     const int G = a.nheads / c.nheads_k, R = G * a.seqlen_q, L = sl.keys, shift = L - a.seqlen_q;
@@ -53,7 +55,6 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     const int all_first = kv8_first(a, w_hi + shift), all_last = min(kv8_last(a, w_lo + shift, L), s1 - 1);
 
     // Q^T as B operands.
-    const bool neg = a.softmax_scale < 0.f;
     const float cscale = fabsf(a.softmax_scale) * kLog2e;
     f16x8 qB[HD / 16];  // step g: channels 32 (g / 2) + 16 hh + 8 (g % 2) + 0..7
     {
@@ -61,24 +62,31 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                         int64_t(hq) * a.q.head_stride + 16 * hh;
 #pragma unroll
         for (int g = 0; g < HD / 16; ++g) {
-            u32x4 v = row_ok ? ldg16(qp + 32 * (g / 2) + 8 * (g % 2)) : zero_u4();
-            qB[g] = as_h8(neg ? neg_h8(v) : v);
+            qB[g] = as_h8(row_ok ? ldg16(qp + 32 * (g / 2) + 8 * (g % 2)) : zero_u4());
         }
     }
 
-    // Copies of a tile's codes to LDS, straight from memory: chunk c of row r of a half lies at chunk c ^ kv8_swz(r).
-    const uint32_t krs = uint32_t(c.k.row_stride), vrs = uint32_t(c.v.row_stride);  // (at most 2^23)
-    const int my_row = tid / CH & 31, my_ch = 16 * (tid % CH ^ kv8_swz<HD>(my_row));
-    const uint32_t lds0 = lds_addr(smem) + wave * 1024;
-    auto issue = [&](int x, int base) FA_INLINE {
-        const uint32_t to = lds0 + (x % NST) * STAGE;
+    // Copies of a tile's codes to LDS, straight from memory: chunk c of row r of a half lies at chunk c ^ kv8_swz(r).  A wave
+    // takes one half of K (waves 0, 1) or V.
+    constexpr int RPC = 1024 / HD, CPH = 32 / RPC;  // rows of a copy, copies of a half
+    const int64_t rs = wave < 2 ? c.k.row_stride : c.v.row_stride;  // (at most 2^23)
+    const int row0 = lane / CH;
+    uint32_t off[CPH];
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {  // HD 128: half i; HD 64: half wave / 2
-            const int h = 2 * x + (CPT == 2 ? i : wave >> 1);
+    for (int i = 0; i < CPH; ++i) off[i] = uint32_t(row0) * uint32_t(rs) + 16 * (lane % CH ^ kv8_swz<HD>(row0 + i * RPC));
+    const uint32_t lds0 = lds_addr(smem) + wave * (32 * HD);
+    auto issue = [&](int x, int base) FA_INLINE {
+        const int h = 2 * x + (wave & 1), most = L - 1 - min(base + 32 * h, (L - 1) / 32 * 32);
+        const uint32_t to = lds0 + (x % NST) * STAGE;
+        const char *from = uniform(wave < 2 ? halves[h].k : halves[h].v);
+        if (most >= 31) {
+#pragma unroll
+            for (int i = 0; i < CPH; ++i) g2l16_at((const f16 *)(from + i * RPC * rs), off[i], to + i * 1024);
+        } else {
             // Rows past the sequence re-read its last one, so that no stale code reaches a product.
-            const int most = min(my_row, L - 1 - min(base + 32 * h, (L - 1) / 32 * 32));
-            g2l16_at((const f16 *)uniform(halves[h].k), __umul24(most, krs) + my_ch, to + i * 4096);
-            g2l16_at((const f16 *)uniform(halves[h].v), __umul24(most, vrs) + my_ch, to + TILE + i * 4096);
+#pragma unroll
+            for (int i = 0; i < CPH; ++i)
+                g2l16_at((const f16 *)from, uint32_t(min(row0 + i * RPC, most)) * uint32_t(rs) + off[i] - uint32_t(row0) * uint32_t(rs), to + i * 1024);
         }
     };
     // Operand reads: rows sigma(col) of K, 16 codes of two steps; V transposed, eight keys of a channel.
@@ -111,36 +119,39 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             const int blk = at >> __builtin_ctz(c.scale_block);
             const float ks = c.k_scale.ptr[line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride];
             float vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
-            Half h;
-            h.k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
-            h.v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
+            halves[tid].k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
+            halves[tid].v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
+            __syncthreads();
+            for (int x = 0; x < min(3, n_tiles); ++x) issue(x, base);  // (the waits below are theirs, too)
             // V's scale over a reference, the largest one, as a power of P; where it is not finite, it reaches the scores of
             // its keys as NaN.
-            h.nan = vs * 0.f;
-            if (!(h.nan == 0.f) || !(vs > 0.f)) vs = 0.f;
+            f32x4 h;
+            h[3] = vs * 0.f;
+            if (!(h[3] == 0.f) || !(vs > 0.f)) vs = 0.f;
             float top = vs;
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
             if (lane == 0) tops[wave] = top;
+            wait_vmem();
             __syncthreads();
             const float before = vref;
             vref = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(before, kKv8MinScale));
-            h.k_scale = ks * cscale;
-            h.lift = fmaxf(log2_fast(vs / vref), -64.f) + kKcLift;
-            h.unlift = exp2_fast(-h.lift);
-            halves[tid] = h;
+            h[0] = ks * cscale;
+            h[1] = fmaxf(log2_fast(vs / vref), -64.f) + kKcLift;
+            h[2] = exp2_fast(-h[1]);
+            *reinterpret_cast<f32x4 *>(&halves[tid].k_scale) = h;
             if (base > s0) {
                 const float f = before / vref;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+            } else if (a.softmax_scale < 0.f) {
+#pragma unroll
+                for (int g = 0; g < HD / 16; ++g) qB[g] = as_h8(neg_h8(__builtin_bit_cast(u32x4, qB[g])));
             }
             __syncthreads();
         }
-        for (int x = 0; x < min(3, n_tiles); ++x) issue(x, base);
-        wait_vmem();
-        __syncthreads();
         // Scores of 32 keys: step u of NS, a read of 16 codes for two.
         auto k_read = [&](const char *tile, int j) FA_INLINE { kc[j % KP] = *reinterpret_cast<const u32x4 *>(tile + (k_at ^ (j << 5))); };
         auto k_operand = [&](int u) FA_INLINE {
@@ -156,7 +167,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             // Tile t + 1 has landed for this wave, and after the barrier for all (t + 2 may be on its way); every wave is done
             // with tile t - 1, whose place t + 3 takes.
             if (t + 2 < n_tiles)
-                wait_vmem_n<2 * CPT>();
+                wait_vmem_n<CPH>();
             else
                 wait_vmem();
             __syncthreads();
@@ -185,24 +196,11 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                         }
                         sk = 1.f;
                     }
-                    float top = max3(sc[0], sc[1], sc[2]);
-#pragma unroll
-                    for (int r = 3; r < 15; r += 2) top = max3(top, sc[r], sc[r + 1]);
-                    top = max3(top, sc[15], top);
-                    top = top == -INFINITY ? top : top * sk;
-                    if (__builtin_amdgcn_ballot_w64(top > m + kKcRaise) != 0) {
-                        const float m_new = fmaxf(m, max2_xor32(top));
-                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-                        l *= alpha;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-                        m = m_new;
-                    }
-                    d -= m == -INFINITY ? 0.f : m;
-                    float sum = 0.f;
+                    // Exponentials of the half, with its largest at most 2^15 over the reference, which is that of the last
+                    // raise: their sum says so.
+                    float dm = d - (m == -INFINITY ? 0.f : m), sum = 0.f;
                     f16x8 pB[2];
+                    __builtin_amdgcn_s_setprio(1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int j = 0; j < KP - 1; ++j) k_read(kt, j);
@@ -213,11 +211,47 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                         sn = mfma16<BF>(k_operand(u), qB[u], u < 1 ? zero16() : sn);
 #pragma unroll
                         for (int e = u * EPS; e < u * EPS + EPS; ++e) {
-                            sc[e] = exp2_fast(fmaf(sc[e], sk, d));
+                            sc[e] = exp2_fast(fmaf(sc[e], sk, dm));
                             sum += sc[e];
                             if (e % 8 == 7) pB[e / 8] = pack8(sc, e - 7);
                         }
                         __builtin_amdgcn_sched_barrier(0);
+                    }
+                    // (m is -infinity until a key is visible: a sum over 0 then, too.  NaN goes on.)
+                    if (__builtin_amdgcn_ballot_w64(sum > kKcTop || (m == -INFINITY && sum > 0.f)) != 0) {
+                        // The scores again, their maximum as the new reference.
+                        const char *kt0 = smem + t % NST * STAGE + 32 * h * HD;
+                        f32x16 x = zero16();
+#pragma unroll
+                        for (int u = 0; u < NS; ++u) {
+                            const u32x4 q = *reinterpret_cast<const u32x4 *>(kt0 + (k_at ^ (u / 2 << 5)));
+                            x = mfma16<BF>(kv8_decode<INT8, BF>(u % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[u], x);
+                        }
+                        const int lo = first - p0 - 8 * hh, hi = min(last, s1 - 1) - p0 - 8 * hh;
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = acc_lrow(r, 0);
+                            x[r] = key < lo || key > hi ? -INFINITY : fmaf(x[r], x4[0], x4[3]);
+                            top = fmaxf(top, x[r]);
+                        }
+                        const float m_new = fmaxf(m, max2_xor32(top));
+                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+                        l *= alpha;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+                        m = m_new;
+                        dm = x4[1] - (m == -INFINITY ? 0.f : m);
+                        sum = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            x[r] = exp2_fast(x[r] + dm);
+                            sum += x[r];
+                        }
+                        pB[0] = pack8(x, 0);
+                        pB[1] = pack8(x, 8);
                     }
                     l = fmaf(sum, x4[2], l);
 #pragma unroll
@@ -227,6 +261,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
                         o[u % DT] = mfma16<false>(v, pB[u / DT], o[u % DT]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
+                    __builtin_amdgcn_s_setprio(0);
                 } else {
 #pragma unroll
                     for (int u = 0; u < NS; ++u) {
@@ -258,24 +293,39 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             for (int r = 0; r < 16; r += 2) kv8_put(o_at(sl.ch, dt * 8 + r / 2), f32x2{o[dt][r], o[dt][r + 1]});
         int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
         if (!kv8_count(count, sl.n_pieces, &ticket)) return;
-        m = -INFINITY;
-        for (int i = 0; i < sl.n_pieces; ++i) m = fmaxf(m, kv8_get(ml_at(i))[0]);
-        l = 0.f;
+        // All pieces in their order; this one's are still in registers.
+        float mm = m;
+        for (int i = 0; i < sl.n_pieces; ++i)
+            if (i != sl.ch) mm = fmaxf(mm, kv8_get(ml_at(i))[0]);
+        const float own = m == -INFINITY ? 0.f : exp2_fast(m - mm), l_own = l;
+        f32x16 sum[DT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
+        for (int dt = 0; dt < DT; ++dt) sum[dt] = zero16();
+        l = 0.f;
         for (int i = 0; i < sl.n_pieces; ++i) {
+            if (i == sl.ch) {
+                l = fmaf(l_own, own, l);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[dt][r] = fmaf(own, o[dt][r], sum[dt][r]);
+                continue;
+            }
             const f32x2 ml = kv8_get(ml_at(i));
-            const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - m);
-            l = fmaf(ml[1], f, l);
             f32x2 y[DT * 8];
 #pragma unroll
             for (int j = 0; j < DT * 8; ++j) y[j] = kv8_get(o_at(i, j));
+            const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - mm);
+            l = fmaf(ml[1], f, l);
 #pragma unroll
             for (int j = 0; j < DT * 8; ++j) {
-                o[j / 8][j % 8 * 2] = fmaf(f, y[j][0], o[j / 8][j % 8 * 2]);
-                o[j / 8][j % 8 * 2 + 1] = fmaf(f, y[j][1], o[j / 8][j % 8 * 2 + 1]);
+                sum[j / 8][j % 8 * 2] = fmaf(f, y[j][0], sum[j / 8][j % 8 * 2]);
+                sum[j / 8][j % 8 * 2 + 1] = fmaf(f, y[j][1], sum[j / 8][j % 8 * 2 + 1]);
             }
         }
+        m = mm;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = sum[dt];
     }
     // Opaque to the optimiser: the row's output addresses are formed here, not before the loop and held through it.
     int orow = row;
@@ -297,7 +347,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
 }
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s) {
-    const unsigned grid = unsigned(plan.slots) * unsigned(a.cache.nheads_k * plan.row_tiles);
+    const unsigned grid = unsigned(kv8_grid(plan, a.cache.nheads_k));
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
         hipLaunchKernelGGL((kv8_chunk_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>), dim3(grid),
                            dim3(kKcThreads), 0, s, a, plan);
