@@ -214,6 +214,21 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read
 
 constexpr int kKdTile = 32;
 
+// g2l16_at (fa_diff_common.h); once: for bytes that no other workgroup reads, which the caches are asked not to keep.
+__device__ __forceinline__ void kd_copy(const char *base, uint32_t off, uint32_t l, bool once) {
+    if (!once) return g2l16_at((const f16 *)base, off, l);
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2 nt\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(off), "s"(base), "s"(l)
+        : "memory");
+}
+
 template <bool BF>
 __device__ __forceinline__ f32x4 kd_mfma(const f16x8 a, const f16x8 b, const f32x4 c) {
     if constexpr (BF)
@@ -264,40 +279,17 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     const int my_first = t_first + wave;
     const int n_my = my_first < t_end ? (t_end - my_first + 3) / 4 : 0;
 
-    const int krs = int(c.k.row_stride), vrs = int(c.v.row_stride);
     char *const slot = smem + wave * WAVE_LDS;
-    const int p_row = lane / CH, p_ch = lane % CH;  // of copy 0; copy i: rows 64 / CH further
+    constexpr int RPC = 1024 / HD;  // rows of a copy
+    const int64_t krs = c.k.row_stride, vrs = c.v.row_stride;  // (at most 2^23)
+    const int row0 = lane / CH;
+    uint32_t ch[CPW];
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) ch[i] = 16 * (lane % CH ^ kv8_swz<HD>(row0 + i * RPC));
+    const uint32_t k_off = uint32_t(row0) * uint32_t(krs), v_off = uint32_t(row0) * uint32_t(vrs);
+    const uint32_t lds0 = lds_addr(slot);
     const float cscale = a.softmax_scale * kLog2e;
-    float ks[NST], vs[NST];
-    auto issue = [&](int t, int st) FA_INLINE {
-        const int p0 = t * kKdTile;
-        int64_t line = sl.row;
-        int at = p0;
-        if (c.block_table) {
-            const int pg = p0 / c.page_block_size;
-            line = checked_page(scalar_load(c.block_table + int64_t(sl.b) * c.block_table_stride + pg), c.num_pages, c.status);
-            at = p0 - pg * c.page_block_size;
-        }
-        const char *kb = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * krs + int64_t(hk) * c.k.head_stride;
-        const char *vb = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * vrs + int64_t(hk) * c.v.head_stride;
-        const int blk = at / c.scale_block;
-        ks[st] = scalar_float(c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride +
-                              int64_t(hk) * c.k_scale.head_stride);
-        vs[st] = scalar_float(c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride +
-                              int64_t(hk) * c.v_scale.head_stride);
-        // Rows past the sequence re-read its last one, so that no stale code reaches a product.
-        const int most = min(L - 1 - p0, kKdTile - 1);
-        char *const base = slot + st * STAGE;
-#pragma unroll
-        for (int i = 0; i < CPW; ++i) {
-            const int r = i * (64 / CH) + p_row, rc = min(r, most), ch = 16 * (p_ch ^ kv8_swz<HD>(r));
-            g2l16(kb + int64_t(rc) * krs + ch, base + i * 1024);
-            g2l16(vb + int64_t(rc) * vrs + ch, base + TILE + i * 1024);
-        }
-    };
-#pragma unroll
-    for (int st = 0; st < NST; ++st)
-        if (st < n_my) issue(my_first + 4 * st, st);
+    const bool once = plan.row_tiles == 1;
     // Q^T as B operands: step st takes channels 64 (st / 2) + 16 g + 8 (st % 2) + 0..7.
     f16x8 qB[STEPS];
     {
@@ -306,7 +298,6 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) qB[st] = as_h8(row_ok ? ldg16(qp + 64 * (st / 2) + 8 * (st % 2)) : zero_u4());
     }
-    wait_vmem();  // only tile copies are in flight inside the loop
     f32x4 o[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -314,85 +305,141 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     // LDS addresses: K rows of the tile's two MFMAs, and the transposed V reads.
     const int k_row0 = 8 * (col >> 2) + (col & 3), v_row = 8 * g + (col >> 1), v_half = 8 * (col & 1);
 
-    for (int k0 = 0; k0 < n_my; k0 += NST) {
-#pragma unroll
-        for (int st = 0; st < NST; ++st) {
-            const int k = k0 + st;
-            if (k >= n_my) break;
-            const int p0 = (my_first + 4 * k) * kKdTile;
-            if (k + 1 < n_my)
-                wait_vmem_n<(NST - 1) * 2 * CPW>();
-            else
-                wait_vmem();
-            const char *kt = slot + st * STAGE, *vt = kt + TILE;
-            u32x4 kc[2][HD / 64];
-            u32x2 vc[CH];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < HD / 64; ++j) {
-                    const int r = k_row0 + 4 * t;
-                    kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kv8_swz<HD>(r)));
+    // 64 tiles of the wave at a time: lane i looks up where tile i's codes begin, and its scales.
+    for (int k_base = 0; k_base < n_my; k_base += 64) {
+        const int n = min(n_my - k_base, 64), t_base = my_first + 4 * k_base;
+        uint64_t ka, va;
+        float ks, vs;
+        {
+            const int p0 = (t_base + 4 * min(lane, n - 1)) * kKdTile;
+            int64_t line = sl.row;
+            int at = p0;
+            if (c.block_table) {
+                const int pg = p0 / c.page_block_size;
+                at = p0 - pg * c.page_block_size;
+                line = c.block_table[int64_t(sl.b) * c.block_table_stride + pg];
+                if (line < 0 || line >= c.num_pages) {
+                    if (c.status) atomicOr(c.status, FA_KV_BAD_PAGE);
+                    line = 0;
                 }
-#pragma unroll
-            for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kv8_swz<HD>(v_row)) + v_half);
-            // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
-            const float sk = ks[st] * cscale, sv0 = vs[st] * 0.f, sv = sv0 == 0.f ? vs[st] : 0.f;
-            wait_lds();
-            if (k + NST < n_my) issue(my_first + 4 * (k + NST), st);
-            f32x4 s[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const u32x4 q = kc[t][i / 2];
-                    s[t] = kd_mfma<BF>(kv8_decode<INT8, BF>(i % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[i], s[t]);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], sk, sv0);
             }
-            if (p0 < all_first || p0 + kKdTile - 1 > all_last) {
+            const int blk = at >> __builtin_ctz(c.scale_block);
+            ka = reinterpret_cast<uint64_t>(c.k.ptr) + line * c.k.batch_stride + int64_t(at) * krs + int64_t(hk) * c.k.head_stride;
+            va = reinterpret_cast<uint64_t>(c.v.ptr) + line * c.v.batch_stride + int64_t(at) * vrs + int64_t(hk) * c.v.head_stride;
+            ks = c.k_scale.ptr[line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride];
+            vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
+        }
+        auto of_lane = [](uint64_t x, int i) FA_INLINE {
+            return reinterpret_cast<const char *>(uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(x), i))) |
+                                                  uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(x >> 32), i))) << 32);
+        };
+        auto issue = [&](int k, int st) FA_INLINE {
+            const char *kb = of_lane(ka, k), *vb = of_lane(va, k);
+            const uint32_t to = lds0 + st * STAGE;
+            const int most = L - 1 - (t_base + 4 * k) * kKdTile;
+            if (most >= kKdTile - 1) {
+#pragma unroll
+                for (int i = 0; i < CPW; ++i) {
+                    kd_copy(kb + i * RPC * krs, k_off + ch[i], to + i * 1024, once);
+                    kd_copy(vb + i * RPC * vrs, v_off + ch[i], to + TILE + i * 1024, once);
+                }
+            } else {
+                // Rows past the sequence re-read its last one, so that no stale code reaches a product.
+#pragma unroll
+                for (int i = 0; i < CPW; ++i) {
+                    const uint32_t r = min(row0 + i * RPC, most);
+                    kd_copy(kb, r * uint32_t(krs) + ch[i], to + i * 1024, once);
+                    kd_copy(vb, r * uint32_t(vrs) + ch[i], to + TILE + i * 1024, once);
+                }
+            }
+        };
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+            if (st < n) issue(st, st);
+        wait_vmem();  // only tile copies are in flight inside the loop
+        asm volatile("" : "+v"(ks), "+v"(vs));
+        for (int k0 = 0; k0 < n; k0 += NST) {
+#pragma unroll
+            for (int st = 0; st < NST; ++st) {
+                const int k = k0 + st;
+                if (k >= n) break;
+                const int p0 = (t_base + 4 * k) * kKdTile;
+                if (k + 1 < n)
+                    wait_vmem_n<(NST - 1) * 2 * CPW>();
+                else
+                    wait_vmem();
+                const char *kt = slot + st * STAGE, *vt = kt + TILE;
+                u32x4 kc[2][HD / 64];
+                u32x2 vc[CH];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = p0 + 8 * g + 4 * t + r;
-                        if (key < first || key > last) s[t][r] = -INFINITY;
+                    for (int j = 0; j < HD / 64; ++j) {
+                        const int r = k_row0 + 4 * t;
+                        kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kv8_swz<HD>(r)));
                     }
-            }
-            // The maximum is raised only when a score passes it by 2^8: sums and products keep 32 bits.
-            const float top = max3(max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]), max3(s[1][1], s[1][2], s[1][3]), -INFINITY);
-            if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
-                const float m_new = fmaxf(m, kd_max4(top));
-                const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-                l *= alpha;
 #pragma unroll
-                for (int d = 0; d < CH; ++d)
+                for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kv8_swz<HD>(v_row)) + v_half);
+                // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
+                const float vsk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), k));
+                const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), k)) * cscale, sv0 = vsk * 0.f,
+                            sv = sv0 == 0.f ? vsk : 0.f;
+                wait_lds();
+                if (k + NST < n) issue(k + NST, st);
+                f32x4 s[2];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
-                m = m_new;
-            }
-            const float m_use = m == -INFINITY ? 0.f : m;
-            float e[8];
+                for (int t = 0; t < 2; ++t) {
+                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = exp2_fast(s[i / 4][i % 4] - m_use);
-                l += e[i];
-            }
-            // P times V's scale in bf16, which has fp32's range, as hi + lo: 16 bits.
-            bf16x8 hi, lo;
+                    for (int i = 0; i < STEPS; ++i) {
+                        const u32x4 q = kc[t][i / 2];
+                        s[t] = kd_mfma<BF>(kv8_decode<INT8, BF>(i % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[i], s[t]);
+                    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = e[i] * sv;
-                hi[i] = (__bf16)w;
-                lo[i] = (__bf16)(w - float(hi[i]));
-            }
+                    for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], sk, sv0);
+                }
+                if (p0 < all_first || p0 + kKdTile - 1 > all_last) {
 #pragma unroll
-            for (int d = 0; d < CH; ++d) {
-                const f16x8 v = kv8_decode<INT8, true>(vc[d]);
-                o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, hi), o[d]);
-                o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, lo), o[d]);
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int key = p0 + 8 * g + 4 * t + r;
+                            if (key < first || key > last) s[t][r] = -INFINITY;
+                        }
+                }
+                // The maximum is raised only when a score passes it by 2^8: sums and products keep 32 bits.
+                const float top = max3(max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]), max3(s[1][1], s[1][2], s[1][3]), -INFINITY);
+                if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
+                    const float m_new = fmaxf(m, kd_max4(top));
+                    const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+                    l *= alpha;
+#pragma unroll
+                    for (int d = 0; d < CH; ++d)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
+                    m = m_new;
+                }
+                const float m_use = m == -INFINITY ? 0.f : m;
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = exp2_fast(s[i / 4][i % 4] - m_use);
+                    l += e[i];
+                }
+                // P times V's scale in bf16, which has fp32's range, as hi + lo: 16 bits.
+                bf16x8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float w = e[i] * sv;
+                    hi[i] = (__bf16)w;
+                    lo[i] = (__bf16)(w - float(hi[i]));
+                }
+#pragma unroll
+                for (int d = 0; d < CH; ++d) {
+                    const f16x8 v = kv8_decode<INT8, true>(vc[d]);
+                    o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, hi), o[d]);
+                    o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, lo), o[d]);
+                }
             }
         }
     }
@@ -440,8 +487,12 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     }
     int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
     if (!kv8_count(count, sl.n_pieces, &ticket)) return;
-    kv8_join<HD, BF, kKdRows>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, reinterpret_cast<float *>(smem),
-                              [&](int i) { return part + int64_t(i - sl.ch) * HI; });
+    const auto place = [&](int i) { return part + int64_t(i - sl.ch) * HI; };
+    float *scratch = reinterpret_cast<float *>(smem);
+    if (rows * (HD / 2) <= kKv8Threads)
+        kv8_join<HD, BF, 1>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, scratch, place);
+    else
+        kv8_join<HD, BF, HD / 32>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, scratch, place);
 }
 
 // ---------------------------------------------------------------------------
@@ -460,7 +511,7 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     p.items = a.cache.batch * heads;
     p.round = 128;
     p.least = 256;
-    p.want = int(std::max<int64_t>((p.many ? 2 : 3) * device_cus() / heads, 1));
+    p.want = int(std::max<int64_t>((p.many || a.cache.batch == 1 ? 2 : 3) * device_cus() / heads, 1));
     int64_t slots;
     if (a.num_splits > 0) {
         p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + p.round - 1) / p.round * p.round);

@@ -112,63 +112,6 @@ __device__ __forceinline__ int kv8_err(const fa_kv8_cache &c, int b, int L0, int
     return err;
 }
 
-// The place of a wave-uniform walk over a sequence's keys in steps of a multiple of 32: first bytes of a head's codes of K and
-// V, and their scales.  Nothing is divided in the walk, and a table's entry is loaded a step ahead of its use.
-template <int STEP>
-struct Kv8Walk {
-    const char *k, *v;
-    const float *ks, *vs;
-    int at, page, next, pg;  // token in the page or row, its size, the table's entry for the next step and its index
-    __device__ __forceinline__ void place(const fa_kv8_cache &c, int hk, int64_t line) {
-        k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
-        v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
-        const int blk = at >> __builtin_ctz(c.scale_block);
-        ks = c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride;
-        vs = c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride;
-    }
-    // To key p0 (a multiple of 32) of sequence b, whose cache row is row.  most: the last key that there is.
-    __device__ __forceinline__ void init(const fa_kv8_cache &c, int b, int row, int hk, int p0, int most) {
-        at = p0;
-        int64_t line = row;
-        page = INT_MAX;
-        if (c.block_table) {
-            page = c.page_block_size;
-            pg = p0 / page;
-            at = p0 - pg * page;
-            line = checked_page(scalar_load(c.block_table + int64_t(b) * c.block_table_stride + pg), c.num_pages, c.status);
-            ahead(c, b, most);
-        }
-        place(c, hk, line);
-    }
-    __device__ __forceinline__ void ahead(const fa_kv8_cache &c, int b, int most) {
-        int p = pg, x = at + STEP;
-        while (x >= page) {
-            x -= page;
-            ++p;
-        }
-        // (Entries behind the sequence are not looked at: the last step's would lie there.)
-        if (p != pg && pg * page + at + STEP <= most) next = scalar_load_ahead(c.block_table + int64_t(b) * c.block_table_stride + p);
-    }
-    // One step on, to a key that there is.
-    __device__ __forceinline__ void step(const fa_kv8_cache &c, int b, int hk, int most) {
-        at += STEP;
-        if (at >= page) {
-            do {
-                at -= page;
-                ++pg;
-            } while (at >= page);
-            place(c, hk, checked_page(next, c.num_pages, c.status));
-        } else {
-            k += STEP * c.k.row_stride;
-            v += STEP * c.v.row_stride;
-            const int lg = __builtin_ctz(c.scale_block), blks = (at >> lg) - ((at - STEP) >> lg);
-            ks += blks * c.k_scale.row_stride;
-            vs += blks * c.v_scale.row_stride;
-        }
-        if (c.block_table) ahead(c, b, most);
-    }
-};
-
 // Attention's plan, made by one workgroup of the launch before: the keys of each sequence cut into equal pieces, so
 // many that the chip has work for all its places.  All pieces have `piece` keys (the last ones of a
 // sequence fewer), whatever the capacity is; a sequence without keys has one empty piece.
@@ -353,48 +296,67 @@ __device__ __forceinline__ bool kv8_count(int32_t *count, int n_pieces, int *tic
     return *ticket == n_pieces - 1;
 }
 
-// Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels).  scratch: LDS of
-// ROWS * (kKv8Join + 2) floats.  part(i) is the place of piece i's partial results.
-constexpr int kKv8Join = 32;  // pieces whose weights are in LDS at a time
-template <int HD, bool BF, int ROWS, class Part>
+// Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels), kKv8Join pieces at a
+// time, whose loads are in flight together.  scratch: LDS of 16 (kKv8Join + 2) floats.  part(i) is the place of piece i's partial
+// results.  UNITS: of a thread, for all rows of the tile.
+constexpr int kKv8Join = 64;
+template <int HD, bool BF, int UNITS, class Part>
 __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &plan, int b, int hk, int row0, int rows, int n,
                                          float *scratch, Part part) {
-    constexpr int UNITS = ROWS * (HD / 2) / 256, T = 256 / ROWS < 1 ? 1 : 256 / ROWS;  // T threads a row look for its maximum
-    float *top = scratch, *sum = scratch + ROWS, *weight = scratch + 2 * ROWS;
+    constexpr int T = 256 / kKdRows, PER = kKv8Join / T;  // threads a row that weigh its pieces, pieces of each
+    constexpr int AHEAD = 32 / UNITS;
+    float *old = scratch, *sum = scratch + kKdRows, *weight = scratch + 2 * kKdRows;
     const int tid = threadIdx.x, r = tid / T, t = tid % T;
     float mm = -INFINITY, ll = 0.f;
-    if (r < rows)
-        for (int i = t; i < n; i += T) mm = fmaxf(mm, kv8_get(kv8_ml(a, plan, part(i)) + r)[0]);
-#pragma unroll
-    for (int d = 1; d < T; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     f32x2 x[UNITS] = {};
     for (int i0 = 0; i0 < n; i0 += kKv8Join) {
         const int k = min(kKv8Join, n - i0);
-        __syncthreads();  // the weights before are used up
-        if (r < rows)
-            for (int i = t; i < k; i += T) {
-                const f32x2 ml = kv8_get(kv8_ml(a, plan, part(i0 + i)) + r);
-                const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - mm);
-                weight[i * ROWS + r] = f;
-                ll = fmaf(ml[1], f, ll);
-            }
-        __syncthreads();
-        constexpr int AHEAD = UNITS >= 16 ? 1 : 8;
-        for (int i = 0; i < k; i += AHEAD) {
-            f32x2 y[AHEAD][UNITS];
+        f32x2 ml[PER], y[AHEAD][UNITS];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = t + j * T;
+            ml[j] = r < rows && i < k ? kv8_get(kv8_ml(a, plan, part(i0 + i)) + r) : f32x2{-INFINITY, 0.f};
+        }
+        auto load = [&](int i) FA_INLINE {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
-                    const int e = u * 256 + tid, row = e / (HD / 2);
-                    y[j][u] = i + j < k && row < rows ? kv8_get(kv8_o<HD>(a, plan, part(i0 + i + j)) + e) : f32x2{0.f, 0.f};
+                    const int e = u * 256 + tid;
+                    y[j][u] = i + j < k && e < rows * (HD / 2) ? kv8_get(kv8_o<HD>(a, plan, part(i0 + i + j)) + e) : f32x2{0.f, 0.f};
                 }
+        };
+        load(0);
+        float top = mm;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) top = fmaxf(top, ml[j][0]);
+#pragma unroll
+        for (int d = 1; d < T; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float f0 = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
+        ll *= f0;
+        mm = top;
+        __syncthreads();  // the weights before are used up
+        if (t == 0) old[r] = f0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const float f = ml[j][0] == -INFINITY ? 0.f : exp2_fast(ml[j][0] - top);
+            weight[(t + j * T) * kKdRows + r] = f;
+            ll = fmaf(ml[j][1], f, ll);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const float f = old[min((u * 256 + tid) / (HD / 2), kKdRows - 1)];
+            x[u][0] *= f;
+            x[u][1] *= f;
+        }
+        for (int i = 0; i < k; i += AHEAD) {
+            if (i > 0) load(i);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
-                    const int row = (u * 256 + tid) / (HD / 2);
-                    const float f = i + j < k && row < rows ? weight[(i + j) * ROWS + row] : 0.f;
+                    const float f = i + j < k ? weight[(i + j) * kKdRows + min((u * 256 + tid) / (HD / 2), kKdRows - 1)] : 0.f;
                     x[u][0] = fmaf(f, y[j][u][0], x[u][0]);
                     x[u][1] = fmaf(f, y[j][u][1], x[u][1]);
                 }
@@ -402,15 +364,16 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
     }
 #pragma unroll
     for (int d = 1; d < T; d <<= 1) ll += __shfl_xor(ll, d);
-    if (t == 0 && r < ROWS) {
-        top[r] = mm;
+    __syncthreads();
+    if (t == 0) {
+        old[r] = mm;
         sum[r] = ll;
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int e = u * 256 + tid, row = e / (HD / 2);
-        if (row < rows) kv8_store<HD, BF>(a, b, hk, row0 + row, 2 * (e % (HD / 2)), x[u], top[row], sum[row]);
+        if (row < rows) kv8_store<HD, BF>(a, b, hk, row0 + row, 2 * (e % (HD / 2)), x[u], old[row], sum[row]);
     }
 }
 
