@@ -244,31 +244,31 @@ __device__ __forceinline__ float kd_sum4(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-template <int HD, bool BF, bool INT8>
+template <int HD, bool BF, bool INT8, int NH>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8_args a, const Kv8Plan plan) {
-    constexpr int CH = HD / 16, TILE = kKdTile * HD, STAGE = 2 * TILE, NST = 2;
-    constexpr int CPW = TILE / 1024;  // copies a lane for K or V of a tile
+    constexpr int CH = HD / 16, TILE = kKdTile * HD, STAGE = 2 * NH * TILE, NST = NH * HD == 256 ? 1 : 2;
+    constexpr int CPW = TILE / 1024;  // copies a lane for a head's K or V of a tile
     constexpr int MERGE = 17;         // row stride of the waves' O^T at the merge
     constexpr int WAVE_LDS = NST * STAGE > HD * MERGE * 4 ? NST * STAGE : HD * MERGE * 4;
-    constexpr int STEPS = HD / 32;
+    constexpr int STEPS = HD / 32, ROWS = NH * kKdRows;
     __shared__ __attribute__((aligned(1024))) char smem[4 * WAVE_LDS];
     __shared__ f32x2 ml[4][16];
     __shared__ int ticket;
-    static_assert(4 * WAVE_LDS >= 16 * (kKv8Join + 2) * 4, "the join's scratch");
+    static_assert(4 * WAVE_LDS >= ROWS * (kKv8Join + 2) * 4, "the join's scratch");
 
     const fa_kv8_cache &c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int HI = c.nheads_k * plan.row_tiles;
-    int slot_i, hk, rt;
-    if (!kv8_item(plan, c.nheads_k, blockIdx.x, slot_i, hk, rt)) return;
-    const int hi_i = hk * plan.row_tiles + rt;
+    const int HI = c.nheads_k / NH * plan.row_tiles;
+    int slot_i, hg, rt;
+    if (!kv8_item(plan, c.nheads_k / NH, blockIdx.x, slot_i, hg, rt)) return;
+    const int hi_i = hg * plan.row_tiles + rt, hk0 = hg * NH;
     const Kv8Slot sl = kv8_slot(a, plan, slot_i);
     if (sl.b < 0) return;
     const int G = a.nheads / c.nheads_k, R = G * a.seqlen_q, L = sl.keys;
     const int row = rt * kKdRows + col;
     const bool row_ok = row < R;
-    const int qpos = row_ok ? row / G : 0, hq = hk * G + (row_ok ? row - qpos * G : 0);
+    const int qpos = row_ok ? row / G : 0, gq = row_ok ? row - qpos * G : 0;
     const int shift = L - a.seqlen_q;  // position of query 0
     const int first = kv8_first(a, qpos + shift), last = kv8_last(a, qpos + shift, L);
     // Keys that every row of the tile sees, and that any does.
@@ -291,17 +291,23 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     const float cscale = a.softmax_scale * kLog2e;
     const bool once = plan.row_tiles == 1;
     // Q^T as B operands: step st takes channels 64 (st / 2) + 16 g + 8 (st % 2) + 0..7.
-    f16x8 qB[STEPS];
-    {
+    f16x8 qB[NH][STEPS];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
         const f16 *qp = (const f16 *)a.q.ptr + int64_t(sl.b) * a.q.batch_stride + int64_t(qpos) * a.q.row_stride +
-                        int64_t(hq) * a.q.head_stride + 16 * g;
+                        int64_t((hk0 + h) * G + gq) * a.q.head_stride + 16 * g;
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) qB[st] = as_h8(row_ok ? ldg16(qp + 64 * (st / 2) + 8 * (st % 2)) : zero_u4());
+        for (int st = 0; st < STEPS; ++st) qB[h][st] = as_h8(row_ok ? ldg16(qp + 64 * (st / 2) + 8 * (st % 2)) : zero_u4());
     }
-    f32x4 o[CH];
+    f32x4 o[NH][CH];
+    float m[NH], l[NH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int h = 0; h < NH; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) o[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     // LDS addresses: K rows of the tile's two MFMAs, and the transposed V reads.
     const int k_row0 = 8 * (col >> 2) + (col & 3), v_row = 8 * g + (col >> 1), v_half = 8 * (col & 1);
 
@@ -309,7 +315,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     for (int k_base = 0; k_base < n_my; k_base += 64) {
         const int n = min(n_my - k_base, 64), t_base = my_first + 4 * k_base;
         uint64_t ka, va;
-        float ks, vs;
+        float ks[NH], vs[NH];
         {
             const int p0 = (t_base + 4 * min(lane, n - 1)) * kKdTile;
             int64_t line = sl.row;
@@ -324,10 +330,15 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
                 }
             }
             const int blk = at >> __builtin_ctz(c.scale_block);
-            ka = reinterpret_cast<uint64_t>(c.k.ptr) + line * c.k.batch_stride + int64_t(at) * krs + int64_t(hk) * c.k.head_stride;
-            va = reinterpret_cast<uint64_t>(c.v.ptr) + line * c.v.batch_stride + int64_t(at) * vrs + int64_t(hk) * c.v.head_stride;
-            ks = c.k_scale.ptr[line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride];
-            vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
+            ka = reinterpret_cast<uint64_t>(c.k.ptr) + line * c.k.batch_stride + int64_t(at) * krs + int64_t(hk0) * c.k.head_stride;
+            va = reinterpret_cast<uint64_t>(c.v.ptr) + line * c.v.batch_stride + int64_t(at) * vrs + int64_t(hk0) * c.v.head_stride;
+            const float *kp = c.k_scale.ptr + line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride;
+            const float *vp = c.v_scale.ptr + line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                ks[h] = kp[int64_t(hk0 + h) * c.k_scale.head_stride];
+                vs[h] = vp[int64_t(hk0 + h) * c.v_scale.head_stride];
+            }
         }
         auto of_lane = [](uint64_t x, int i) FA_INLINE {
             return reinterpret_cast<const char *>(uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(x), i))) |
@@ -339,17 +350,22 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
             const int most = L - 1 - (t_base + 4 * k) * kKdTile;
             if (most >= kKdTile - 1) {
 #pragma unroll
-                for (int i = 0; i < CPW; ++i) {
-                    kd_copy(kb + i * RPC * krs, k_off + ch[i], to + i * 1024, once);
-                    kd_copy(vb + i * RPC * vrs, v_off + ch[i], to + TILE + i * 1024, once);
-                }
+                for (int i = 0; i < CPW; ++i)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) {  // (neighbouring heads are neighbouring bytes)
+                        kd_copy(kb + i * RPC * krs + h * c.k.head_stride, k_off + ch[i], to + h * TILE + i * 1024, once);
+                        kd_copy(vb + i * RPC * vrs + h * c.v.head_stride, v_off + ch[i], to + (NH + h) * TILE + i * 1024, once);
+                    }
             } else {
                 // Rows past the sequence re-read its last one, so that no stale code reaches a product.
 #pragma unroll
                 for (int i = 0; i < CPW; ++i) {
                     const uint32_t r = min(row0 + i * RPC, most);
-                    kd_copy(kb, r * uint32_t(krs) + ch[i], to + i * 1024, once);
-                    kd_copy(vb, r * uint32_t(vrs) + ch[i], to + TILE + i * 1024, once);
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) {
+                        kd_copy(kb + h * c.k.head_stride, r * uint32_t(krs) + ch[i], to + h * TILE + i * 1024, once);
+                        kd_copy(vb + h * c.v.head_stride, r * uint32_t(vrs) + ch[i], to + (NH + h) * TILE + i * 1024, once);
+                    }
                 }
             }
         };
@@ -357,7 +373,8 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
         for (int st = 0; st < NST; ++st)
             if (st < n) issue(st, st);
         wait_vmem();  // only tile copies are in flight inside the loop
-        asm volatile("" : "+v"(ks), "+v"(vs));
+#pragma unroll
+        for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(ks[h]), "+v"(vs[h]));
         for (int k0 = 0; k0 < n; k0 += NST) {
 #pragma unroll
             for (int st = 0; st < NST; ++st) {
@@ -365,134 +382,139 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
                 if (k >= n) break;
                 const int p0 = (t_base + 4 * k) * kKdTile;
                 if (k + 1 < n)
-                    wait_vmem_n<(NST - 1) * 2 * CPW>();
+                    wait_vmem_n<(NST - 1) * 2 * NH * CPW>();
                 else
                     wait_vmem();
-                const char *kt = slot + st * STAGE, *vt = kt + TILE;
-                u32x4 kc[2][HD / 64];
-                u32x2 vc[CH];
+                u32x4 kc[NH][2][HD / 64];
+                u32x2 vc[NH][CH];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < HD / 64; ++j) {
-                        const int r = k_row0 + 4 * t;
-                        kc[t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kv8_swz<HD>(r)));
-                    }
-#pragma unroll
-                for (int d = 0; d < CH; ++d) vc[d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kv8_swz<HD>(v_row)) + v_half);
-                // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
-                const float vsk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), k));
-                const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), k)) * cscale, sv0 = vsk * 0.f,
-                            sv = sv0 == 0.f ? vsk : 0.f;
-                wait_lds();
-                if (k + NST < n) issue(k + NST, st);
-                f32x4 s[2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < STEPS; ++i) {
-                        const u32x4 q = kc[t][i / 2];
-                        s[t] = kd_mfma<BF>(kv8_decode<INT8, BF>(i % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[i], s[t]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], sk, sv0);
-                }
-                if (p0 < all_first || p0 + kKdTile - 1 > all_last) {
+                for (int h = 0; h < NH; ++h) {
+                    const char *kt = slot + st * STAGE + h * TILE, *vt = kt + NH * TILE;
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int key = p0 + 8 * g + 4 * t + r;
-                            if (key < first || key > last) s[t][r] = -INFINITY;
+                        for (int j = 0; j < HD / 64; ++j) {
+                            const int r = k_row0 + 4 * t;
+                            kc[h][t][j] = *reinterpret_cast<const u32x4 *>(kt + r * HD + 16 * ((4 * j + g) ^ kv8_swz<HD>(r)));
                         }
+#pragma unroll
+                    for (int d = 0; d < CH; ++d) vc[h][d] = lds_tr8(vt, v_row * HD + 16 * (d ^ kv8_swz<HD>(v_row)) + v_half);
                 }
-                // The maximum is raised only when a score passes it by 2^8: sums and products keep 32 bits.
-                const float top = max3(max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]), max3(s[1][1], s[1][2], s[1][3]), -INFINITY);
-                if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
-                    const float m_new = fmaxf(m, kd_max4(top));
-                    const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-                    l *= alpha;
+                wait_lds();
+                if (k + NST < n) issue(k + NST, st);
 #pragma unroll
-                    for (int d = 0; d < CH; ++d)
+                for (int h = 0; h < NH; ++h) {
+                    // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
+                    const float vsk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs[h]), k));
+                    const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks[h]), k)) * cscale, sv0 = vsk * 0.f,
+                                sv = sv0 == 0.f ? vsk : 0.f;
+                    f32x4 s[2];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
-                    m = m_new;
-                }
-                const float m_use = m == -INFINITY ? 0.f : m;
-                float e[8];
+                    for (int t = 0; t < 2; ++t) {
+                        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = exp2_fast(s[i / 4][i % 4] - m_use);
-                    l += e[i];
-                }
-                // P times V's scale in bf16, which has fp32's range, as hi + lo: 16 bits.
-                bf16x8 hi, lo;
+                        for (int i = 0; i < STEPS; ++i) {
+                            const u32x4 q = kc[h][t][i / 2];
+                            s[t] = kd_mfma<BF>(kv8_decode<INT8, BF>(i % 2 ? u32x2{q[2], q[3]} : u32x2{q[0], q[1]}), qB[h][i], s[t]);
+                        }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float w = e[i] * sv;
-                    hi[i] = (__bf16)w;
-                    lo[i] = (__bf16)(w - float(hi[i]));
-                }
+                        for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], sk, sv0);
+                    }
+                    if (p0 < all_first || p0 + kKdTile - 1 > all_last) {
 #pragma unroll
-                for (int d = 0; d < CH; ++d) {
-                    const f16x8 v = kv8_decode<INT8, true>(vc[d]);
-                    o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, hi), o[d]);
-                    o[d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, lo), o[d]);
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int key = p0 + 8 * g + 4 * t + r;
+                                if (key < first || key > last) s[t][r] = -INFINITY;
+                            }
+                    }
+                    // The maximum is raised only when a score passes it by 2^8: sums and products keep 32 bits.
+                    const float top = max3(max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]), max3(s[1][1], s[1][2], s[1][3]), -INFINITY);
+                    if (__builtin_amdgcn_ballot_w64(top > m[h] + 8.f) != 0) {
+                        const float m_new = fmaxf(m[h], kd_max4(top));
+                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m[h] - m_new);
+                        l[h] *= alpha;
+#pragma unroll
+                        for (int d = 0; d < CH; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[h][d][r] *= alpha;
+                        m[h] = m_new;
+                    }
+                    const float m_use = m[h] == -INFINITY ? 0.f : m[h];
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        e[i] = exp2_fast(s[i / 4][i % 4] - m_use);
+                        l[h] += e[i];
+                    }
+                    // P times V's scale in bf16, which has fp32's range, as hi + lo: 16 bits.
+                    bf16x8 hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float w = e[i] * sv;
+                        hi[i] = (__bf16)w;
+                        lo[i] = (__bf16)(w - float(hi[i]));
+                    }
+#pragma unroll
+                    for (int d = 0; d < CH; ++d) {
+                        const f16x8 v = kv8_decode<INT8, true>(vc[h][d]);
+                        o[h][d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, hi), o[h][d]);
+                        o[h][d] = kd_mfma<true>(v, __builtin_bit_cast(f16x8, lo), o[h][d]);
+                    }
                 }
             }
         }
     }
 
-    // Merge the four waves: O^T to LDS, then every thread sums pairs of channels of a row.
-    l = kd_sum4(l);
-    float *ow = reinterpret_cast<float *>(slot);
-#pragma unroll
-    for (int d = 0; d < CH; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ow[(16 * d + 4 * g + r) * MERGE + col] = o[d][r];
-    if (g == 0) ml[wave][col] = f32x2{m, l};
-    __syncthreads();
+    // Merge the four waves, a head after the other: O^T to LDS, then every thread sums pairs of channels of a row.
     const int rows = min(kKdRows, R - rt * kKdRows);
-    auto merged = [&](int r, int d, float &mm, float &ll) FA_INLINE {
-        mm = fmaxf(fmaxf(ml[0][r][0], ml[1][r][0]), fmaxf(ml[2][r][0], ml[3][r][0]));
-        ll = 0.f;
-        f32x2 x = {0.f, 0.f};
+    const int64_t part = int64_t(slot_i) * HI + hi_i;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = ml[w][r][0] == -INFINITY ? 0.f : exp2_fast(ml[w][r][0] - mm);
-            const float *q = reinterpret_cast<const float *>(smem + w * WAVE_LDS);
-            ll = fmaf(ml[w][r][1], f, ll);
-            x[0] = fmaf(q[d * MERGE + r], f, x[0]);
-            x[1] = fmaf(q[(d + 1) * MERGE + r], f, x[1]);
-        }
-        return x;
-    };
-    if (sl.n_pieces == 1) {
+    for (int h = 0; h < NH; ++h) {
+        if (h > 0) __syncthreads();
+        const float lh = kd_sum4(l[h]);
+        float *ow = reinterpret_cast<float *>(slot);
+#pragma unroll
+        for (int d = 0; d < CH; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ow[(16 * d + 4 * g + r) * MERGE + col] = o[h][d][r];
+        if (g == 0) ml[wave][col] = f32x2{m[h], lh};
+        __syncthreads();
         for (int e = tid; e < rows * (HD / 2); e += kKv8Threads) {
             const int r = e / (HD / 2), d = 2 * (e % (HD / 2));
-            float mm, ll;
-            const f32x2 x = merged(r, d, mm, ll);
-            kv8_store<HD, BF>(a, sl.b, hk, rt * kKdRows + r, d, x, mm, ll);
+            const float mm = fmaxf(fmaxf(ml[0][r][0], ml[1][r][0]), fmaxf(ml[2][r][0], ml[3][r][0]));
+            float ll = 0.f;
+            f32x2 x = {0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = ml[w][r][0] == -INFINITY ? 0.f : exp2_fast(ml[w][r][0] - mm);
+                const float *q = reinterpret_cast<const float *>(smem + w * WAVE_LDS);
+                ll = fmaf(ml[w][r][1], f, ll);
+                x[0] = fmaf(q[d * MERGE + r], f, x[0]);
+                x[1] = fmaf(q[(d + 1) * MERGE + r], f, x[1]);
+            }
+            if (sl.n_pieces == 1) {
+                kv8_store<HD, BF>(a, sl.b, hk0 + h, rt * kKdRows + r, d, x, mm, ll);
+            } else {
+                kv8_put(kv8_o<HD>(a, plan, part) + h * rows * (HD / 2) + e, x);
+                if (d == 0) kv8_put(kv8_ml(a, plan, part) + h * rows + r, f32x2{mm, ll});
+            }
         }
-        return;
     }
-    const int64_t part = int64_t(slot_i) * HI + hi_i;
-    for (int e = tid; e < rows * (HD / 2); e += kKv8Threads) {
-        const int r = e / (HD / 2), d2 = e % (HD / 2);
-        float mm, ll;
-        const f32x2 x = merged(r, 2 * d2, mm, ll);
-        kv8_put(kv8_o<HD>(a, plan, part) + e, x);
-        if (d2 == 0) kv8_put(kv8_ml(a, plan, part) + r, f32x2{mm, ll});
-    }
+    if (sl.n_pieces == 1) return;
     int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
     if (!kv8_count(count, sl.n_pieces, &ticket)) return;
     const auto place = [&](int i) { return part + int64_t(i - sl.ch) * HI; };
+    const auto write = [&](int r, int d, f32x2 x, float mm, float ll) {
+        const int h = r / rows;
+        kv8_store<HD, BF>(a, sl.b, hk0 + h, rt * kKdRows + r - h * rows, d, x, mm, ll);
+    };
     float *scratch = reinterpret_cast<float *>(smem);
-    if (rows * (HD / 2) <= kKv8Threads)
-        kv8_join<HD, BF, 1>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, scratch, place);
+    if (NH * rows * (HD / 2) <= 2 * kKv8Threads)
+        kv8_join<HD, ROWS, 2>(a, plan, NH * rows, sl.n_pieces, scratch, place, write);
     else
-        kv8_join<HD, BF, HD / 32>(a, plan, sl.b, hk, rt * kKdRows, rows, sl.n_pieces, scratch, place);
+        kv8_join<HD, ROWS, ROWS * (HD / 2) / kKv8Threads>(a, plan, NH * rows, sl.n_pieces, scratch, place, write);
 }
 
 // ---------------------------------------------------------------------------
@@ -500,14 +522,21 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s);  // fa_kv8_fwd.hip
 
+// KV heads that a workgroup of few rows takes together.
+static int kv8_heads(const fa_kv8_args &a) {
+    const int most = 256 / a.cache.head_dim;
+    return a.cache.nheads_k % most == 0 ? most : a.cache.nheads_k % 2 == 0 ? 2 : 1;
+}
+
 static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     Kv8Plan p{};
     const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q, cap = std::max(a.cache.cache_capacity, 1);
     p.many = rows >= 64;
     const int tile = p.many ? kKcRows : kKdRows;
     p.row_tiles = int((rows + tile - 1) / tile);
-    p.rows_max = p.many ? tile : int(std::min<int64_t>(rows, tile));
-    const int64_t heads = int64_t(a.cache.nheads_k) * p.row_tiles;
+    p.heads = p.many ? 1 : kv8_heads(a);
+    p.rows_max = p.many ? tile : p.heads * int(std::min<int64_t>(rows, tile));
+    const int64_t heads = int64_t(a.cache.nheads_k / p.heads) * p.row_tiles;
     p.items = a.cache.batch * heads;
     p.round = 128;
     p.least = 256;
@@ -625,14 +654,21 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (a.seqlen_q == 0) return launch_kv8_append(a, nullptr, s);
     const Kv8Plan plan = kv8_plan(a);
-    const int64_t grid = kv8_grid(plan, a.cache.nheads_k);
+    const int64_t grid = kv8_grid(plan, a.cache.nheads_k / plan.heads);
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     if ((rc = launch_kv8_append(a, &plan, s))) return rc;
     if (plan.many) return kv8_chunk(a, plan, s);
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
-        hipLaunchKernelGGL((kv8_decode_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),
-                           dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, plan);
-        return int(hipGetLastError());
+        constexpr int HD = decltype(hd)::value;
+        auto go = [&](auto nh) {
+            hipLaunchKernelGGL((kv8_decode_kernel<HD, decltype(bf)::value, decltype(int8)::value, decltype(nh)::value>),
+                               dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, plan);
+            return int(hipGetLastError());
+        };
+        if constexpr (HD == 64)
+            if (plan.heads == 4) return go(std::integral_constant<int, 4>{});
+        if (plan.heads == 2) return go(std::integral_constant<int, 2>{});
+        return go(std::integral_constant<int, 1>{});
     });
 }
 

@@ -124,10 +124,11 @@ struct Kv8Slot {
 };
 static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
 
-// Workspace: counters of the (sequence, KV head, row tile) items, the slots, then the partial results.
+// Workspace: counters of the (sequence, KV heads, row tile) items, the slots, then the partial results.
 constexpr int kKdRows = 16, kKcRows = 128;  // rows of a tile: few rows, many
 struct Kv8Plan {
     bool many;          // the kernel of many rows (fa_kv8_fwd.hip)
+    int heads;          // KV heads that a workgroup takes together
     int row_tiles;      // of a KV head
     int rows_max;       // rows of a tile whose partial results are kept
     int slots;          // at most
@@ -135,7 +136,7 @@ struct Kv8Plan {
     int fixed;          // keys of a piece, where the call says so, or 0
     int want;           // slots that fill the chip
     int least;          // keys of a piece at least
-    int64_t items;      // batch * nheads_k * row_tiles
+    int64_t items;      // batch * nheads_k / heads * row_tiles
     int64_t at_slots, at_ml, at_o, bytes;
 };
 
@@ -297,15 +298,16 @@ __device__ __forceinline__ bool kv8_count(int32_t *count, int n_pieces, int *tic
 }
 
 // Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels), kKv8Join pieces at a
-// time, whose loads are in flight together.  scratch: LDS of 16 (kKv8Join + 2) floats.  part(i) is the place of piece i's partial
-// results.  UNITS: of a thread, for all rows of the tile.
+// time, whose loads are in flight together.  scratch: LDS of ROWS (kKv8Join + 2) floats.  part(i) is the place of piece i's partial
+// results, write(row, channel, its and the next one's unnormalised O, maximum, sum) takes the joined ones.
 constexpr int kKv8Join = 64;
-template <int HD, bool BF, int UNITS, class Part>
-__device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &plan, int b, int hk, int row0, int rows, int n,
-                                         float *scratch, Part part) {
-    constexpr int T = 256 / kKdRows, PER = kKv8Join / T;  // threads a row that weigh its pieces, pieces of each
+template <int HD, int ROWS, int UNITS, class Part, class Write>
+__device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &plan, int rows, int n, float *scratch, Part part,
+                                         Write write) {
+    constexpr int T = 256 / ROWS, PER = kKv8Join / T;  // threads a row that weigh its pieces, pieces of each
     constexpr int AHEAD = 32 / UNITS;
-    float *old = scratch, *sum = scratch + kKdRows, *weight = scratch + 2 * kKdRows;
+    static_assert(AHEAD >= 1 && kKv8Join % AHEAD == 0 && kKv8Join % T == 0, "whole rounds");
+    float *old = scratch, *sum = scratch + ROWS, *weight = scratch + 2 * ROWS;
     const int tid = threadIdx.x, r = tid / T, t = tid % T;
     float mm = -INFINITY, ll = 0.f;
     f32x2 x[UNITS] = {};
@@ -340,13 +342,13 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const float f = ml[j][0] == -INFINITY ? 0.f : exp2_fast(ml[j][0] - top);
-            weight[(t + j * T) * kKdRows + r] = f;
+            weight[(t + j * T) * ROWS + r] = f;
             ll = fmaf(ml[j][1], f, ll);
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const float f = old[min((u * 256 + tid) / (HD / 2), kKdRows - 1)];
+            const float f = old[min((u * 256 + tid) / (HD / 2), ROWS - 1)];
             x[u][0] *= f;
             x[u][1] *= f;
         }
@@ -356,7 +358,7 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
             for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
-                    const float f = i + j < k ? weight[(i + j) * kKdRows + min((u * 256 + tid) / (HD / 2), kKdRows - 1)] : 0.f;
+                    const float f = i + j < k ? weight[(i + j) * ROWS + min((u * 256 + tid) / (HD / 2), ROWS - 1)] : 0.f;
                     x[u][0] = fmaf(f, y[j][u][0], x[u][0]);
                     x[u][1] = fmaf(f, y[j][u][1], x[u][1]);
                 }
@@ -373,7 +375,7 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int e = u * 256 + tid, row = e / (HD / 2);
-        if (row < rows) kv8_store<HD, BF>(a, b, hk, row0 + row, 2 * (e % (HD / 2)), x[u], old[row], sum[row]);
+        if (row < rows) write(row, 2 * (e % (HD / 2)), x[u], old[row], sum[row]);
     }
 }
 
