@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_append_kernel(const fa_kv8_ar
     if (int(blockIdx.x) < plan_wgs) return kv8_make_plan(a, plan);
     if (int(blockIdx.x) < plan_wgs + clear_wgs) {
         const int64_t i = int64_t(blockIdx.x - plan_wgs) * kKv8Threads + threadIdx.x;
-        if (i < plan.items) static_cast<int32_t *>(a.ws)[i] = 0;
+        if (i < plan.counters) static_cast<int32_t *>(a.ws)[i] = 0;
         return;
     }
     constexpr int KCH = HD / 8;  // units of a row: 8 elements
@@ -503,18 +503,31 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
         }
     }
     if (sl.n_pieces == 1) return;
-    int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
-    if (!kv8_count(count, sl.n_pieces, &ticket)) return;
-    const auto place = [&](int i) { return part + int64_t(i - sl.ch) * HI; };
+    const int F = kv8_group(sl.n_pieces, NH * rows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
+    const int64_t part0 = part - int64_t(sl.ch) * HI, group_part = part0 + int64_t(g0) * HI;
+    float *scratch = reinterpret_cast<float *>(smem);
+    const auto join = [&](int n, auto place, auto write) FA_INLINE {
+        if (NH * rows * (HD / 2) <= 2 * kKv8Threads)
+            kv8_join<HD, ROWS, 2>(a, plan, NH * rows, n, scratch, place, write);
+        else
+            kv8_join<HD, ROWS, ROWS * (HD / 2) / kKv8Threads>(a, plan, NH * rows, n, scratch, place, write);
+    };
     const auto write = [&](int r, int d, f32x2 x, float mm, float ll) {
         const int h = r / rows;
         kv8_store<HD, BF>(a, sl.b, hk0 + h, rt * kKdRows + r - h * rows, d, x, mm, ll);
     };
-    float *scratch = reinterpret_cast<float *>(smem);
-    if (NH * rows * (HD / 2) <= 2 * kKv8Threads)
-        kv8_join<HD, ROWS, 2>(a, plan, NH * rows, sl.n_pieces, scratch, place, write);
-    else
-        kv8_join<HD, ROWS, ROWS * (HD / 2) / kKv8Threads>(a, plan, NH * rows, sl.n_pieces, scratch, place, write);
+    if (!kv8_count(kv8_counter(a, plan.items + group_part), in_group, &ticket)) return;
+    if (groups == 1) {
+        join(in_group, [&](int i) { return group_part + int64_t(i) * HI; }, write);
+        return;
+    }
+    join(in_group, [&](int i) { return group_part + int64_t(i) * HI; },
+         [&](int r, int d, f32x2 x, float mm, float ll) {
+             kv8_put(kv8_o<HD>(a, plan, group_part) + r * (HD / 2) + d / 2, x);
+             if (d == 0) kv8_put(kv8_ml(a, plan, group_part) + r, f32x2{mm, ll});
+         });
+    if (!kv8_count(kv8_counter(a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
+    join(groups, [&](int i) { return part0 + int64_t(i) * F * HI; }, write);
 }
 
 // ---------------------------------------------------------------------------
@@ -522,10 +535,15 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s);  // fa_kv8_fwd.hip
 
-// KV heads that a workgroup of few rows takes together.
+// KV heads that a workgroup of few rows takes together: their codes of a token are neighbours in memory, which
+// reads runs of 256 bytes faster, but there are fewer items to share a short call.
 static int kv8_heads(const fa_kv8_args &a) {
-    const int most = 256 / a.cache.head_dim;
-    return a.cache.nheads_k % most == 0 ? most : a.cache.nheads_k % 2 == 0 ? 2 : 1;
+    const int64_t bytes = int64_t(a.cache.batch) * a.cache.cache_capacity * a.cache.nheads_k * a.cache.head_dim * 2;
+    int most = 256 / a.cache.head_dim;
+    if (bytes < 256 << 20) most /= 2;
+    if (bytes < 32 << 20) most = 1;
+    while (a.cache.nheads_k % most != 0) most /= 2;
+    return most;
 }
 
 static Kv8Plan kv8_plan(const fa_kv8_args &a) {
@@ -540,19 +558,20 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     p.items = a.cache.batch * heads;
     p.round = 128;
     p.least = 256;
-    p.want = int(std::max<int64_t>((p.many || a.cache.batch == 1 ? 2 : 3) * device_cus() / heads, 1));
+    p.want = int(std::max<int64_t>(2 * device_cus() / heads, 1));
     int64_t slots;
     if (a.num_splits > 0) {
         p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + p.round - 1) / p.round * p.round);
         slots = a.cache.batch * ((cap + p.fixed - 1) / p.fixed);
     } else {
-        // Pieces of at least total / want keys: a sequence has at most one short piece.
-        slots = std::min<int64_t>(int64_t(p.want) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
+        // Pieces of at least total / (2 want) keys: a sequence has at most one short piece.
+        slots = std::min<int64_t>(2 * int64_t(p.want) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
     }
     p.slots = int(std::min<int64_t>(slots, INT32_MAX));
     const bool parts = slots > a.cache.batch;
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    p.at_slots = up(p.items * 4);
+    p.counters = parts ? p.items + slots * heads : 0;
+    p.at_slots = up(p.counters * 4);
     p.at_ml = p.at_slots + up(slots * int64_t(sizeof(Kv8Slot)));
     p.at_o = p.at_ml + (parts ? up(slots * heads * p.rows_max * 8) : 0);
     p.bytes = p.at_o + (parts ? slots * heads * p.rows_max * a.cache.head_dim * 4 : 0);
@@ -591,7 +610,7 @@ static int check_kv8_new(const fa_kv8_args &a) {
 static int launch_kv8_append(const fa_kv8_args &a, const Kv8Plan *plan, hipStream_t s) {
     const fa_kv8_cache &c = a.cache;
     const int blocks = a.seqlen_new > 0 ? int((int64_t(a.seqlen_new) + 2 * c.scale_block - 2) / c.scale_block) : 0;
-    const int64_t clear = plan ? (plan->items + kKv8Threads - 1) / kKv8Threads : 0;
+    const int64_t clear = plan ? (plan->counters + kKv8Threads - 1) / kKv8Threads : 0;
     const int64_t grid = (plan ? 1 : 0) + clear + int64_t(c.batch) * blocks * c.nheads_k * 2;
     if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
     if (grid == 0) return FA_OK;

@@ -112,9 +112,9 @@ __device__ __forceinline__ int kv8_err(const fa_kv8_cache &c, int b, int L0, int
     return err;
 }
 
-// Attention's plan, made by one workgroup of the launch before: the keys of each sequence cut into equal pieces, so
-// many that the chip has work for all its places.  All pieces have `piece` keys (the last ones of a
-// sequence fewer), whatever the capacity is; a sequence without keys has one empty piece.
+// Attention's plan, made by one workgroup of the launch before, whatever the capacity is: each sequence's keys cut into as
+// many pieces as it has times the batch's keys by the places on the chip, all of one length; a sequence without keys has one
+// empty piece.
 struct Kv8Slot {
     int b, row;         // sequence, its cache row
     int begin, end;     // keys
@@ -124,7 +124,8 @@ struct Kv8Slot {
 };
 static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
 
-// Workspace: counters of the (sequence, KV heads, row tile) items, the slots, then the partial results.
+// Workspace: counters of the (sequence, KV heads, row tile) items and of every piece of them (a group of pieces counts at its
+// first one's), the slots, then the partial results.
 constexpr int kKdRows = 16, kKcRows = 128;  // rows of a tile: few rows, many
 struct Kv8Plan {
     bool many;          // the kernel of many rows (fa_kv8_fwd.hip)
@@ -137,7 +138,7 @@ struct Kv8Plan {
     int want;           // slots that fill the chip
     int least;          // keys of a piece at least
     int64_t items;      // batch * nheads_k / heads * row_tiles
-    int64_t at_slots, at_ml, at_o, bytes;
+    int64_t counters, at_slots, at_ml, at_o, bytes;
 };
 
 // Workgroups of an attention call: its (slot, KV head) groups times row tiles.  The tiles of a group read the same codes, so
@@ -195,7 +196,7 @@ __device__ __forceinline__ int64_t kv8_scan(int64_t x, int64_t &total) {
 // One workgroup: the slots of an attention call.
 __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Plan &plan) {
     __shared__ int64_t before[257];
-    __shared__ int keys_of[256], begin_of[256], row_of[256];
+    __shared__ int keys_of[256], begin_of[256], row_of[256], piece_of[256];
     const int tid = threadIdx.x;
     Kv8Slot *slots = reinterpret_cast<Kv8Slot *>(static_cast<char *>(a.ws) + plan.at_slots);
     auto sequence = [&](int b, int &begin, int &L, int &row) {
@@ -213,8 +214,33 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
             sum += L - begin;
         }
         kv8_scan(sum, total);
-        const int64_t c = (total + plan.want - 1) / plan.want;
-        piece = int(max(int64_t(plan.least), (c + plan.round - 1) / plan.round * plan.round));
+        // The even share, a little more for the rounding of 32 bits, in whole rounds.
+        auto length = [&](float x) {
+            const float share = float(total) * x / float(plan.want) * 1.000001f;
+            return int(min(2147483392u, max(uint32_t(plan.least), (uint32_t(share) / plan.round + 1) * plan.round)));
+        };
+        piece = length(1.f);
+        // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, and
+        // where none fits, as with lengths far apart, half the share: twice the pieces, started as places become free.
+        if (!plan.many && a.cache.batch > 1) {
+            const int at[4] = {piece, length(1.0625f), length(1.125f), length(1.25f)};
+            int64_t n01 = 0, n23 = 0;  // two counts each
+            for (int b = tid; b < a.cache.batch; b += 256) {
+                int begin, L, row;
+                sequence(b, begin, L, row);
+                auto pieces = [&](int i) { return int64_t(max(1, (L - begin - 1) / at[i] + 1)); };
+                n01 += pieces(0) << 32 | pieces(1);
+                n23 += pieces(2) << 32 | pieces(3);
+            }
+            int64_t t01, t23;
+            kv8_scan(n01, t01);
+            kv8_scan(n23, t23);
+            const int64_t n[4] = {t01 >> 32, t01 & 0xffffffff, t23 >> 32, t23 & 0xffffffff};
+            piece = length(0.5f);
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (n[i] <= plan.want) piece = at[i];
+        }
     }
     int64_t done = 0;
     for (int b0 = 0; b0 < a.cache.batch; b0 += 256) {
@@ -230,6 +256,10 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         keys_of[tid] = L;
         begin_of[tid] = begin;
         row_of[tid] = row;
+        // Pieces of few rows are equal: they end together.  Those of many rows keep the length, whose places run one each, and
+        // the short last ones fill what is left: 3 + 2 pieces on 4 places took 204 us equal and 172 us so.
+        const int64_t even = (int64_t(L) - begin + max(n, 1) - 1) / max(n, 1);
+        piece_of[tid] = plan.fixed || plan.many ? piece : int(min(int64_t(INT_MAX), (even + plan.round - 1) / plan.round * plan.round));
         if (tid == 0) before[256] = total;
         __syncthreads();
         for (int64_t s = tid; s < total && done + s < plan.slots; s += 256) {
@@ -243,8 +273,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
             x.ch = int(s - before[lo]);
             x.keys = keys_of[lo];
             x.n_pieces = int(before[lo + 1] - before[lo]);
-            x.begin = begin_of[lo] + x.ch * piece;
-            x.end = min(x.keys, x.begin + piece);
+            x.begin = min(x.keys, begin_of[lo] + x.ch * piece_of[lo]);
+            x.end = min(x.keys, x.begin + piece_of[lo]);
             x.pad = 0;
             slots[done + s] = x;
         }
@@ -288,14 +318,22 @@ __device__ __forceinline__ f32x2 kv8_get(const uint64_t *p) {
     return __builtin_bit_cast(f32x2, __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// Counts a piece whose partial results are stored; true in the workgroup that counts last, which joins them all.
-__device__ __forceinline__ bool kv8_count(int32_t *count, int n_pieces, int *ticket) {
+// Counts a piece whose partial results are stored; true in the workgroup that counts last of n.
+__device__ __forceinline__ bool kv8_count(int32_t *count, int n, int *ticket) {
     wait_vmem();
     __syncthreads();  // every wave's stores have completed
     if (threadIdx.x == 0) *ticket = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    return *ticket == n_pieces - 1;
+    return *ticket == n - 1;
 }
+
+// Pieces of an item are joined in one step, or, where their partial results (bytes each) are many, eight at a time by the last
+// workgroup of the eight, whose result takes the place of the first one's, and then these: one workgroup would read too long.
+// Measured (us, one step and two): 40 pieces of 8 KB 58 and 47, 40 of 2 KB 26.6 and 27.5, 64 of 2 KB 31.8 and 31.8.
+__device__ __forceinline__ int kv8_group(int n_pieces, int bytes) {
+    return n_pieces <= 8 || int64_t(n_pieces) * bytes <= 160 << 10 ? n_pieces : 8;
+}
+__device__ __forceinline__ int32_t *kv8_counter(const fa_kv8_args &a, int64_t i) { return static_cast<int32_t *>(a.ws) + i; }
 
 // Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels), kKv8Join pieces at a
 // time, whose loads are in flight together.  scratch: LDS of ROWS (kKv8Join + 2) floats.  part(i) is the place of piece i's partial

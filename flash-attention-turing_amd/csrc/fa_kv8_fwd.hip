@@ -283,49 +283,61 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     l = sum_xor32(l);
     if (sl.n_pieces > 1) {
         // Partial results lane by lane: (maximum, sum) of every row, then register pairs of O by wave and lane.
-        const int64_t part = int64_t(slot_i) * HI + hi_i;
-        auto ml_at = [&](int i) { return kv8_ml(a, plan, part + int64_t(i - sl.ch) * HI) + wave * 32 + col; };
-        auto o_at = [&](int i, int j) { return kv8_o<HD>(a, plan, part + int64_t(i - sl.ch) * HI) + (wave * (HD / 4) + j) * 64 + lane; };
-        if (hh == 0) kv8_put(ml_at(sl.ch), f32x2{m, l});
+        const int F = kv8_group(sl.n_pieces, kKcRows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
+        const int64_t part0 = int64_t(slot_i - sl.ch) * HI + hi_i;
+        auto ml_at = [&](int i) { return kv8_ml(a, plan, part0 + int64_t(i) * HI) + wave * 32 + col; };
+        auto o_at = [&](int i, int j) { return kv8_o<HD>(a, plan, part0 + int64_t(i) * HI) + (wave * (HD / 4) + j) * 64 + lane; };
+        auto put = [&](int i) FA_INLINE {
+            if (hh == 0) kv8_put(ml_at(i), f32x2{m, l});
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) kv8_put(o_at(sl.ch, dt * 8 + r / 2), f32x2{o[dt][r], o[dt][r + 1]});
-        int32_t *count = static_cast<int32_t *>(a.ws) + int64_t(sl.b) * HI + hi_i;
-        if (!kv8_count(count, sl.n_pieces, &ticket)) return;
-        // All pieces in their order; this one's are still in registers.
-        float mm = m;
-        for (int i = 0; i < sl.n_pieces; ++i)
-            if (i != sl.ch) mm = fmaxf(mm, kv8_get(ml_at(i))[0]);
-        const float own = m == -INFINITY ? 0.f : exp2_fast(m - mm), l_own = l;
-        f32x16 sum[DT];
+                for (int r = 0; r < 16; r += 2) kv8_put(o_at(i, dt * 8 + r / 2), f32x2{o[dt][r], o[dt][r + 1]});
+        };
+        // Pieces first, first + step, .. (n of them) in their order; the own one's results are still in registers.
+        auto join = [&](int first, int step, int n, int own_i) FA_INLINE {
+            float mm = m;
+            for (int k = 0; k < n; ++k)
+                if (first + k * step != own_i) mm = fmaxf(mm, kv8_get(ml_at(first + k * step))[0]);
+            const float own = m == -INFINITY ? 0.f : exp2_fast(m - mm), l_own = l;
+            f32x16 sum[DT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) sum[dt] = zero16();
-        l = 0.f;
-        for (int i = 0; i < sl.n_pieces; ++i) {
-            if (i == sl.ch) {
-                l = fmaf(l_own, own, l);
+            for (int dt = 0; dt < DT; ++dt) sum[dt] = zero16();
+            l = 0.f;
+            for (int k = 0; k < n; ++k) {
+                const int i = first + k * step;
+                if (i == own_i) {
+                    l = fmaf(l_own, own, l);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[dt][r] = fmaf(own, o[dt][r], sum[dt][r]);
-                continue;
+                        for (int r = 0; r < 16; ++r) sum[dt][r] = fmaf(own, o[dt][r], sum[dt][r]);
+                    continue;
+                }
+                const f32x2 ml = kv8_get(ml_at(i));
+                f32x2 y[DT * 8];
+#pragma unroll
+                for (int j = 0; j < DT * 8; ++j) y[j] = kv8_get(o_at(i, j));
+                const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - mm);
+                l = fmaf(ml[1], f, l);
+#pragma unroll
+                for (int j = 0; j < DT * 8; ++j) {
+                    sum[j / 8][j % 8 * 2] = fmaf(f, y[j][0], sum[j / 8][j % 8 * 2]);
+                    sum[j / 8][j % 8 * 2 + 1] = fmaf(f, y[j][1], sum[j / 8][j % 8 * 2 + 1]);
+                }
             }
-            const f32x2 ml = kv8_get(ml_at(i));
-            f32x2 y[DT * 8];
+            m = mm;
 #pragma unroll
-            for (int j = 0; j < DT * 8; ++j) y[j] = kv8_get(o_at(i, j));
-            const float f = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - mm);
-            l = fmaf(ml[1], f, l);
-#pragma unroll
-            for (int j = 0; j < DT * 8; ++j) {
-                sum[j / 8][j % 8 * 2] = fmaf(f, y[j][0], sum[j / 8][j % 8 * 2]);
-                sum[j / 8][j % 8 * 2 + 1] = fmaf(f, y[j][1], sum[j / 8][j % 8 * 2 + 1]);
-            }
+            for (int dt = 0; dt < DT; ++dt) o[dt] = sum[dt];
+        };
+        put(sl.ch);
+        if (!kv8_count(kv8_counter(a, plan.items + part0 + int64_t(g0) * HI), in_group, &ticket)) return;
+        join(g0, 1, in_group, sl.ch);
+        if (groups > 1) {
+            put(g0);
+            if (!kv8_count(kv8_counter(a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
+            join(0, F, groups, g0);
         }
-        m = mm;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = sum[dt];
     }
     // Opaque to the optimiser: the row's output addresses are formed here, not before the loop and held through it.
     int orow = row;
