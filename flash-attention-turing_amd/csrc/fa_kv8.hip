@@ -55,12 +55,12 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_append_kernel(const fa_kv8_ar
     constexpr int KCH = HD / 8;  // units of a row: 8 elements
     __shared__ uint32_t part[kKv8Threads / 64];
     const fa_kv8_cache &c = a.cache;
-    int64_t rest = blockIdx.x - plan_wgs - clear_wgs;
+    int rest = int(blockIdx.x) - plan_wgs - clear_wgs;
     const bool is_v = rest & 1;
     rest >>= 1;
-    const int hk = int(rest % c.nheads_k);
+    const int hk = rest % c.nheads_k;
     rest /= c.nheads_k;
-    const int j = int(rest % blocks), b = int(rest / blocks);
+    const int j = rest % blocks, b = rest / blocks;
     const int L0 = a.cache_seqlens[b], n = a.seqlens_new ? a.seqlens_new[b] : a.seqlen_new;
     int row;
     const int err = kv8_err(c, b, L0, n, a.seqlen_new, row);
@@ -141,62 +141,96 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_append_kernel(const fa_kv8_ar
 }
 
 // ---------------------------------------------------------------------------
-// Read back: a wave takes kKv8Rows packed rows, all heads of K and of V, 16 codes a lane.
+// Read back: a workgroup takes some packed rows, all heads of K and of V.  Its first threads find the rows' places, one each;
+// then every thread has kKv8Reads loads of eight codes under way before the first is used.
 
-constexpr int kKv8Rows = 4;
+constexpr int kKv8Reads = 8, kKv8ReadRows = 64;
+
+// Rows of a workgroup: one batch of loads.
+static inline int kv8_read_rows(int units) { return std::min(std::max(kKv8Reads * kKv8Threads / units, 1), kKv8ReadRows); }
 
 template <int HD, bool BF, bool INT8>
-__global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read_args a) {
-    constexpr int CH = HD / 16;
+__global__ __launch_bounds__(kKv8Threads) void kv8_read_kernel(const fa_kv8_read_args a, const int rows) {
+    constexpr int CH = HD / 8;
     const fa_kv8_cache &c = a.cache;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t r0 = (int64_t(blockIdx.x) * (kKv8Threads / 64) + wave) * kKv8Rows;
-    if (r0 >= a.total) return;
-    for (int64_t r = r0; r < min(r0 + kKv8Rows, int64_t(a.total)); ++r) {
-        const int b = packed_sequence(a.cu_seqlens, c.batch, int(r));
-        bool ok = b >= 0 && b < c.batch;
+    __shared__ int64_t line_of[kKv8ReadRows];
+    __shared__ int at_of[kKv8ReadRows];  // -1: zeros
+    const int tid = threadIdx.x;
+    const int64_t r0 = int64_t(blockIdx.x) * rows;
+    const int n_rows = int(min(int64_t(rows), a.total - r0));
+    const int b0 = tid < 64 ? packed_sequence(a.cu_seqlens, c.batch, int(r0)) : 0;
+    if (tid < n_rows) {
+        // The row's sequence is the first row's or a later one: the last that starts at or before the row.
+        const int r = int(r0) + tid;
+        int b = b0;
+        if (b < c.batch && a.cu_seqlens[b + 1] <= r) {
+            int out = c.batch + 1;  // starts behind the row, or the end
+            for (++b; out - b > 1;) {
+                const int mid = b + (out - b) / 2;
+                if (a.cu_seqlens[mid] <= r)
+                    b = mid;
+                else
+                    out = mid;
+            }
+        }
         int64_t line = 0;
-        int at = 0;
-        if (ok) {
+        int at = -1;
+        if (b >= 0 && b < c.batch) {
             const int start = a.cu_seqlens[b];
             int row;
             const int n = a.cu_seqlens[b + 1] - start, err = kv8_err(c, b, 0, n, INT_MAX, row);
-            if (err && c.status && lane == 0) atomicOr(c.status, err);
-            ok = !err && r - start < n;
-            at = ok ? int(r) - start : 0;
-            line = row;
-            if (ok && c.block_table) {
-                const int pg = at / c.page_block_size;
-                line = c.block_table[int64_t(b) * c.block_table_stride + pg];
-                at -= pg * c.page_block_size;
-                if (line < 0 || line >= c.num_pages) {
-                    if (c.status && lane == 0) atomicOr(c.status, FA_KV_BAD_PAGE);
-                    line = 0;
+            if (err && c.status) atomicOr(c.status, err);
+            if (!err && r - start < n) {
+                at = r - start;
+                line = row;
+                if (c.block_table) {
+                    const int pg = at / c.page_block_size;
+                    line = c.block_table[int64_t(b) * c.block_table_stride + pg];
+                    at -= pg * c.page_block_size;
+                    if (line < 0 || line >= c.num_pages) {
+                        if (c.status) atomicOr(c.status, FA_KV_BAD_PAGE);
+                        line = 0;
+                    }
                 }
             }
         }
-        for (int u = lane; u < 2 * c.nheads_k * CH; u += 64) {
-            const bool is_v = u >= c.nheads_k * CH;
-            const int x = is_v ? u - c.nheads_k * CH : u, h = x / CH, ch = x % CH;
-            const fa_tensor &t = is_v ? c.v : c.k, &o = is_v ? a.v_out : a.k_out;
-            const fa_kv8_scales &sc = is_v ? c.v_scale : c.k_scale;
-            u32x4 lo = zero_u4(), hi = zero_u4();
-            if (ok) {
-                const u32x4 q = *reinterpret_cast<const u32x4 *>((const char *)t.ptr + line * t.batch_stride +
-                                                                 int64_t(at) * t.row_stride + int64_t(h) * t.head_stride + 16 * ch);
-                const float s = sc.ptr[line * sc.batch_stride + int64_t(at / c.scale_block) * sc.row_stride + int64_t(h) * sc.head_stride];
-                f16x4 y[4];
+        line_of[tid] = line;
+        at_of[tid] = at;
+    }
+    __syncthreads();
+    const uint32_t half = c.nheads_k * CH, units = 2 * half, n = n_rows * units;
+    for (uint32_t e0 = tid; e0 < n; e0 += kKv8Reads * kKv8Threads) {
+        u32x2 q[kKv8Reads];
+        float s[kKv8Reads];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 v = kv8_values<INT8>(q[i]);
-                    y[i] = pack4<BF>(v[0] * s, v[1] * s, v[2] * s, v[3] * s);
-                }
-                lo = __builtin_bit_cast(u32x4, f16x8(__builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7)));
-                hi = __builtin_bit_cast(u32x4, f16x8(__builtin_shufflevector(y[2], y[3], 0, 1, 2, 3, 4, 5, 6, 7)));
-            }
-            u32x4 *p = reinterpret_cast<u32x4 *>((f16 *)o.ptr + r * o.row_stride + int64_t(h) * o.head_stride + 16 * ch);
-            p[0] = lo;
-            p[1] = hi;
+        for (int i = 0; i < kKv8Reads; ++i) {
+            q[i] = u32x2{0u, 0u};
+            s[i] = 0.f;
+            const uint32_t e = e0 + i * kKv8Threads, r = e / units, x = e - r * units;
+            if (e >= n || at_of[r] < 0) continue;
+            const bool is_v = x >= half;
+            const uint32_t y = is_v ? x - half : x, h = y / CH, ch = y % CH;
+            const fa_tensor &t = is_v ? c.v : c.k;
+            const fa_kv8_scales &sc = is_v ? c.v_scale : c.k_scale;
+            const int64_t line = line_of[r];
+            const int at = at_of[r];
+            q[i] = *reinterpret_cast<const u32x2 *>((const char *)t.ptr + line * t.batch_stride + int64_t(at) * t.row_stride +
+                                                    int64_t(h) * t.head_stride + 8 * ch);
+            s[i] = sc.ptr[line * sc.batch_stride + int64_t(uint32_t(at) / uint32_t(c.scale_block)) * sc.row_stride +
+                          int64_t(h) * sc.head_stride];
+        }
+#pragma unroll
+        for (int i = 0; i < kKv8Reads; ++i) {
+            const uint32_t e = e0 + i * kKv8Threads, r = e / units, x = e - r * units;
+            if (e >= n) continue;
+            const bool is_v = x >= half;
+            const uint32_t y = is_v ? x - half : x, h = y / CH, ch = y % CH;
+            const fa_tensor &o = is_v ? a.v_out : a.k_out;
+            const f32x4 lo = kv8_values<INT8>(q[i][0]), hi = kv8_values<INT8>(q[i][1]);
+            const f16x4 y0 = pack4<BF>(lo[0] * s[i], lo[1] * s[i], lo[2] * s[i], lo[3] * s[i]);
+            const f16x4 y1 = pack4<BF>(hi[0] * s[i], hi[1] * s[i], hi[2] * s[i], hi[3] * s[i]);
+            f16 *p = (f16 *)o.ptr + (r0 + r) * o.row_stride + int64_t(h) * o.head_stride + 8 * ch;
+            *reinterpret_cast<f16x8 *>(p) = __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 }
@@ -245,7 +279,10 @@ __device__ __forceinline__ float kd_sum4(float x) {
 }
 
 template <int HD, bool BF, bool INT8, int NH>
-__global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8_args a, const Kv8Plan plan) {
+__global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const Kv8Call call) {
+    kv8_early();
+    const fa_kv8_args &a = call.a;
+    const Kv8Plan &plan = call.plan;
     constexpr int CH = HD / 16, TILE = kKdTile * HD, STAGE = 2 * NH * TILE, NST = NH * HD == 256 ? 1 : 2;
     constexpr int CPW = TILE / 1024;  // copies a lane for a head's K or V of a tile
     constexpr int MERGE = 17;         // row stride of the waves' O^T at the merge
@@ -468,6 +505,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     }
 
     // Merge the four waves, a head after the other: O^T to LDS, then every thread sums pairs of channels of a row.
+    const Kv8Call &late = kv8_late();
     const int rows = min(kKdRows, R - rt * kKdRows);
     const int64_t part = int64_t(slot_i) * HI + hi_i;
 #pragma unroll
@@ -495,10 +533,10 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
                 x[1] = fmaf(q[(d + 1) * MERGE + r], f, x[1]);
             }
             if (sl.n_pieces == 1) {
-                kv8_store<HD, BF>(a, sl.b, hk0 + h, rt * kKdRows + r, d, x, mm, ll);
+                kv8_store<HD, BF>(late.a, sl.b, hk0 + h, rt * kKdRows + r, d, x, mm, ll);
             } else {
-                kv8_put(kv8_o<HD>(a, plan, part) + h * rows * (HD / 2) + e, x);
-                if (d == 0) kv8_put(kv8_ml(a, plan, part) + h * rows + r, f32x2{mm, ll});
+                kv8_put(kv8_o<HD>(late.a, late.plan, part) + h * rows * (HD / 2) + e, x);
+                if (d == 0) kv8_put(kv8_ml(late.a, late.plan, part) + h * rows + r, f32x2{mm, ll});
             }
         }
     }
@@ -506,28 +544,35 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const fa_kv8
     const int F = kv8_group(sl.n_pieces, NH * rows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
     const int64_t part0 = part - int64_t(sl.ch) * HI, group_part = part0 + int64_t(g0) * HI;
     float *scratch = reinterpret_cast<float *>(smem);
-    const auto join = [&](int n, auto place, auto write) FA_INLINE {
-        if (NH * rows * (HD / 2) <= 2 * kKv8Threads)
-            kv8_join<HD, ROWS, 2>(a, plan, NH * rows, n, scratch, place, write);
-        else
-            kv8_join<HD, ROWS, ROWS * (HD / 2) / kKv8Threads>(a, plan, NH * rows, n, scratch, place, write);
+    if (!kv8_count(kv8_counter(late.a, late.plan.items + group_part), in_group, &ticket)) return;
+    // (One copy of the join for both steps: a workgroup comes here with its instructions still in memory.)
+    const auto join = [&](auto units) FA_INLINE {
+        bool last = groups == 1;
+        int64_t from = group_part, step = HI;
+        int n = in_group;
+        for (;;) {
+            kv8_join<HD, ROWS, decltype(units)::value>(
+                late.a, late.plan, NH * rows, n, scratch, [&](int i) { return from + i * step; },
+                [&](int r, int d, f32x2 x, float mm, float ll) {
+                    if (last) {
+                        const int h = r / rows;
+                        kv8_store<HD, BF>(late.a, sl.b, hk0 + h, rt * kKdRows + r - h * rows, d, x, mm, ll);
+                    } else {
+                        kv8_put(kv8_o<HD>(late.a, late.plan, group_part) + r * (HD / 2) + d / 2, x);
+                        if (d == 0) kv8_put(kv8_ml(late.a, late.plan, group_part) + r, f32x2{mm, ll});
+                    }
+                });
+            if (last || !kv8_count(kv8_counter(late.a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
+            last = true;
+            from = part0;
+            step = int64_t(F) * HI;
+            n = groups;
+        }
     };
-    const auto write = [&](int r, int d, f32x2 x, float mm, float ll) {
-        const int h = r / rows;
-        kv8_store<HD, BF>(a, sl.b, hk0 + h, rt * kKdRows + r - h * rows, d, x, mm, ll);
-    };
-    if (!kv8_count(kv8_counter(a, plan.items + group_part), in_group, &ticket)) return;
-    if (groups == 1) {
-        join(in_group, [&](int i) { return group_part + int64_t(i) * HI; }, write);
-        return;
-    }
-    join(in_group, [&](int i) { return group_part + int64_t(i) * HI; },
-         [&](int r, int d, f32x2 x, float mm, float ll) {
-             kv8_put(kv8_o<HD>(a, plan, group_part) + r * (HD / 2) + d / 2, x);
-             if (d == 0) kv8_put(kv8_ml(a, plan, group_part) + r, f32x2{mm, ll});
-         });
-    if (!kv8_count(kv8_counter(a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
-    join(groups, [&](int i) { return part0 + int64_t(i) * F * HI; }, write);
+    if (NH * rows * (HD / 2) <= kKv8Threads)
+        join(std::integral_constant<int, 1>{});
+    else
+        join(std::integral_constant<int, ROWS * (HD / 2) / kKv8Threads>{});
 }
 
 // ---------------------------------------------------------------------------
@@ -661,6 +706,7 @@ extern "C" int fa_kv8_append(const fa_kv8_args *args, void *stream) {
 
 extern "C" size_t fa_kv8_ws_bytes(const fa_kv8_args *a) {
     if (!a || a->cache.batch <= 0 || a->seqlen_q <= 0 || a->nheads <= 0 || a->cache.nheads_k <= 0) return 0;
+    if (a->cache.head_dim != 64 && a->cache.head_dim != 128) return 0;
     return size_t(fa::kv8_plan(*a).bytes);
 }
 
@@ -681,7 +727,7 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
         constexpr int HD = decltype(hd)::value;
         auto go = [&](auto nh) {
             hipLaunchKernelGGL((kv8_decode_kernel<HD, decltype(bf)::value, decltype(int8)::value, decltype(nh)::value>),
-                               dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, plan);
+                               dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, Kv8Call{a, plan});
             return int(hipGetLastError());
         };
         if constexpr (HD == 64)
@@ -701,11 +747,12 @@ extern "C" int fa_kv8_read(const fa_kv8_read_args *args, void *stream) {
     if (rc) return rc;
     if (a.dtype != FA_FP16 && a.dtype != FA_BF16) return FA_ERR_UNSUPPORTED;
     if (!a.cu_seqlens || check_tensor(a.k_out, true) || check_tensor(a.v_out, true)) return FA_ERR_INVALID_ARG;
-    const int64_t per = kKv8Rows * (kKv8Threads / 64), grid = (int64_t(a.total) + per - 1) / per;
+    const int per = kv8_read_rows(2 * a.cache.nheads_k * (a.cache.head_dim / 8));
+    const int64_t grid = (int64_t(a.total) + per - 1) / per;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
         hipLaunchKernelGGL((kv8_read_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),
-                           dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a);
+                           dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, a, per);
         return int(hipGetLastError());
     });
 }

@@ -222,8 +222,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         piece = length(1.f);
         // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, and
         // where none fits, as with lengths far apart, half the share: twice the pieces, started as places become free.
-        if (!plan.many && a.cache.batch > 1) {
-            const int at[4] = {piece, length(1.0625f), length(1.125f), length(1.25f)};
+        const int at[4] = {piece, length(1.0625f), length(1.125f), length(1.25f)};
+        if (!plan.many && a.cache.batch > 1 && at[3] > plan.least) {
             int64_t n01 = 0, n23 = 0;  // two counts each
             for (int b = tid; b < a.cache.batch; b += 256) {
                 int begin, L, row;
@@ -282,6 +282,30 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         __syncthreads();
     }
     for (int64_t s = done + tid; s < plan.slots; s += 256) slots[s].b = -1;
+}
+
+// What the attention kernels are called with.  kv8_late reads it anew from where it is used: all of it at once does not fit the
+// scalar registers, and what does not is moved to vector lanes and back, which cost a call of one token 1.3 us.
+struct Kv8Call {
+    fa_kv8_args a;
+    Kv8Plan plan;
+};
+__device__ __forceinline__ const Kv8Call &kv8_late() {
+    typedef const __attribute__((address_space(4))) void *Args;
+    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Kv8Call *)p;
+}
+
+// Brings the whole of it to the scalar cache at a kernel's start, where all the lines' latencies are one (0.6 us of a call of one token).
+__device__ __forceinline__ void kv8_early() {
+    typedef const __attribute__((address_space(4))) uint32_t *Args;
+    const Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    uint32_t x[(sizeof(Kv8Call) + 63) / 64];
+#pragma unroll
+    for (size_t i = 0; i < sizeof(x) / 4; ++i) x[i] = p[16 * i];
+#pragma unroll
+    for (size_t i = 0; i < sizeof(x) / 4; ++i) asm volatile("" ::"s"(x[i]));
 }
 
 // A wave-uniform slot, through the scalar cache.
