@@ -541,7 +541,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const Kv8Cal
         }
     }
     if (sl.n_pieces == 1) return;
-    const int F = kv8_group(sl.n_pieces, NH * rows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
+    const int F = kv8_group(sl.n_pieces, rows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
     const int64_t part0 = part - int64_t(sl.ch) * HI, group_part = part0 + int64_t(g0) * HI;
     float *scratch = reinterpret_cast<float *>(smem);
     if (!kv8_count(kv8_counter(late.a, late.plan.items + group_part), in_group, &ticket)) return;
@@ -594,7 +594,12 @@ static int kv8_heads(const fa_kv8_args &a) {
 static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     Kv8Plan p{};
     const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q, cap = std::max(a.cache.cache_capacity, 1);
-    p.many = rows >= 64;
+    // The kernel of many rows reads and converts the codes once for 128 rows, the other one for 16, but it starts later and its
+    // pieces' results are large.  Measured, by the 16-row tiles' keys (us, few and many): 32 rows of 8 heads x 8192 keys 26 and 37,
+    // 512 rows x 8192 55 and 50, 1024 x 32768 319 and 164; batch of 32 x 20 rows x 6144 131 and 144, 16 x 32 x 8192 86 and 79.
+    const int64_t few_keys = (rows + kKdRows - 1) / kKdRows * a.cache.nheads_k * a.cache.batch * cap;
+    // A given number of pieces asks for sums that do not depend on the batch.
+    p.many = a.num_splits > 0 ? rows >= 4 * kKdRows : rows >= 2 * kKdRows && few_keys >= int64_t(6144) * device_cus();
     const int tile = p.many ? kKcRows : kKdRows;
     p.row_tiles = int((rows + tile - 1) / tile);
     p.heads = p.many ? 1 : kv8_heads(a);
@@ -602,7 +607,7 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     const int64_t heads = int64_t(a.cache.nheads_k / p.heads) * p.row_tiles;
     p.items = a.cache.batch * heads;
     p.round = 128;
-    p.least = 256;
+    p.least = p.many ? 512 : 256;  // fewer and longer: 8 heads x 512 rows x 2048 keys took 36 us at 256 and 31 us at 512
     p.want = int(std::max<int64_t>(2 * device_cus() / heads, 1));
     int64_t slots;
     if (a.num_splits > 0) {

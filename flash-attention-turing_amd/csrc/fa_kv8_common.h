@@ -351,11 +351,11 @@ __device__ __forceinline__ bool kv8_count(int32_t *count, int n, int *ticket) {
     return *ticket == n - 1;
 }
 
-// Pieces of an item are joined in one step, or, where their partial results (bytes each) are many, eight at a time by the last
-// workgroup of the eight, whose result takes the place of the first one's, and then these: one workgroup would read too long.
-// Measured (us, one step and two): 40 pieces of 8 KB 58 and 47, 40 of 2 KB 26.6 and 27.5, 64 of 2 KB 31.8 and 31.8.
+// Pieces of an item are joined in one step, or, where their partial results (bytes each for a KV head) are many, eight at a time
+// by the last workgroup of the eight, whose result takes the place of the first one's, and then these: one workgroup would read
+// too long.  Measured (us, one step and two): 40 pieces of 4 KB 58 and 47, 40 of 2 KB 26.6 and 27.5, 64 of 2 KB 31.8 and 31.8.
 __device__ __forceinline__ int kv8_group(int n_pieces, int bytes) {
-    return n_pieces <= 8 || int64_t(n_pieces) * bytes <= 160 << 10 ? n_pieces : 8;
+    return n_pieces <= 8 || int64_t(n_pieces) * bytes <= 128 << 10 ? n_pieces : 8;
 }
 __device__ __forceinline__ int32_t *kv8_counter(const fa_kv8_args &a, int64_t i) { return static_cast<int32_t *>(a.ws) + i; }
 

@@ -18,7 +18,10 @@ constexpr int kKcThreads = 256, kKcKeys = 64, kKcHalves = kKcThreads;
 constexpr float kKcTop = 32768.f, kKcLift = 5.f;
 
 template <int HD, bool BF, bool INT8>
-__global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_args a, const Kv8Plan plan) {
+__global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call call) {
+    kv8_early();
+    const fa_kv8_args &a = call.a;
+    const Kv8Plan &plan = call.plan;
     constexpr int CH = HD / 16, TILE = kKcKeys * HD, STAGE = 2 * TILE, NST = 4;
     constexpr int DT = HD / 32;
     __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
@@ -274,6 +277,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
         __syncthreads();  // every wave is done with the table and the tiles
     }
 
+    const Kv8Call &late = kv8_late();
     // P's lift and the reference of V's scales leave O.
     const float out_scale = vref * exp2_fast(-kKcLift);
 #pragma unroll
@@ -285,8 +289,8 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
         // Partial results lane by lane: (maximum, sum) of every row, then register pairs of O by wave and lane.
         const int F = kv8_group(sl.n_pieces, kKcRows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
         const int64_t part0 = int64_t(slot_i - sl.ch) * HI + hi_i;
-        auto ml_at = [&](int i) { return kv8_ml(a, plan, part0 + int64_t(i) * HI) + wave * 32 + col; };
-        auto o_at = [&](int i, int j) { return kv8_o<HD>(a, plan, part0 + int64_t(i) * HI) + (wave * (HD / 4) + j) * 64 + lane; };
+        auto ml_at = [&](int i) { return kv8_ml(late.a, late.plan, part0 + int64_t(i) * HI) + wave * 32 + col; };
+        auto o_at = [&](int i, int j) { return kv8_o<HD>(late.a, late.plan, part0 + int64_t(i) * HI) + (wave * (HD / 4) + j) * 64 + lane; };
         auto put = [&](int i) FA_INLINE {
             if (hh == 0) kv8_put(ml_at(i), f32x2{m, l});
 #pragma unroll
@@ -331,11 +335,11 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             for (int dt = 0; dt < DT; ++dt) o[dt] = sum[dt];
         };
         put(sl.ch);
-        if (!kv8_count(kv8_counter(a, plan.items + part0 + int64_t(g0) * HI), in_group, &ticket)) return;
+        if (!kv8_count(kv8_counter(late.a, late.plan.items + part0 + int64_t(g0) * HI), in_group, &ticket)) return;
         join(g0, 1, in_group, sl.ch);
         if (groups > 1) {
             put(g0);
-            if (!kv8_count(kv8_counter(a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
+            if (!kv8_count(kv8_counter(late.a, int64_t(sl.b) * HI + hi_i), groups, &ticket)) return;
             join(0, F, groups, g0);
         }
     }
@@ -346,7 +350,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
     const int oq = orow / G, oh = hk * G + orow - oq * G;
     // A sum of 0 is that of a row without a visible key (or with scores of -infinity alone); NaN goes on to the output.
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    f16 *out = (f16 *)a.o.ptr + int64_t(sl.b) * a.o.batch_stride + int64_t(oq) * a.o.row_stride + int64_t(oh) * a.o.head_stride + 4 * hh;
+    f16 *out = (f16 *)late.a.o.ptr + int64_t(sl.b) * late.a.o.batch_stride + int64_t(oq) * late.a.o.row_stride + int64_t(oh) * late.a.o.head_stride + 4 * hh;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -355,14 +359,14 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const fa_kv8_a
             if (l == 0.f) y = pack4<BF>(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<f16x4 *>(out + 32 * dt + 2 * r) = y;
         }
-    if (hh == 0) a.lse[(int64_t(sl.b) * a.nheads + oh) * a.seqlen_q + oq] = l == 0.f ? 0.f : (m + log2_fast(l)) * kLn2;
+    if (hh == 0) late.a.lse[(int64_t(sl.b) * late.a.nheads + oh) * late.a.seqlen_q + oq] = l == 0.f ? 0.f : (m + log2_fast(l)) * kLn2;
 }
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s) {
     const unsigned grid = unsigned(kv8_grid(plan, a.cache.nheads_k));
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
         hipLaunchKernelGGL((kv8_chunk_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>), dim3(grid),
-                           dim3(kKcThreads), 0, s, a, plan);
+                           dim3(kKcThreads), 0, s, Kv8Call{a, plan});
         return int(hipGetLastError());
     });
 }

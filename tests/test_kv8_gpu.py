@@ -532,3 +532,141 @@ def test_as_it_is_used(device, kind, dtype):
     exact = {name: s.oracle(name) for name in "kv"}
     assert torch.equal(k[: int(lens[0])].cpu().double(), exact["k"].tokens(0, int(lens[0])))
     assert torch.equal(v[int(lens[0]):].cpu().double(), exact["v"].tokens(1, int(lens[1])))
+
+
+def _widen(s, tokens, page):
+    """The same cache behind a table of a larger capacity, whose further entries are no pages."""
+    more = torch.full((s.table.shape[0], tokens // page), -1, dtype=torch.int32, device=s.device)
+    s.table = torch.cat((s.table, more), 1)
+
+
+@pytest.mark.parametrize("splits", [1, 3, 200])
+@pytest.mark.parametrize("kind,dtype", [("e4m3", "bf16"), ("int8", "fp16"), ("e4m3", "fp16"), ("int8", "bf16")])
+@pytest.mark.parametrize("d,block,page", [(64, 32, 32), (128, 32, 96), (128, 64, 64), (64, 256, 256)])
+def test_attention_of_many_rows(device, d, block, page, kind, dtype, splits):
+    """At least 64 rows a KV head and a given number of pieces: the kernel of many rows, whatever the size; heads that the
+    eight XCDs do not share evenly, and more queries than keys."""
+    for i, (lens, sq, h, hk, causal, window) in enumerate((
+            ([0, 95, 900], 64, 3, 3, True, (-1, -1)), ([33, 20], 130, 4, 2, True, (-1, -1)), ([600, 31], 70, 6, 1, True, (200, -1)),
+            ([400, 1], 65, 4, 4, False, (50, 20)), ([257], 129, 2, 2, False, (-1, 0)), ([1200], 40, 8, 1, False, (-1, -1)))):
+        s = Setup(device, lens, 0, hk, d, kind, block, "paged", page=page, seed=i)
+        q = s.normal(len(lens), sq, h, d).to(DTYPES[dtype]).to(device)
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=causal, window_size=window,
+                                                  num_splits=splits, return_softmax_lse=True, **s.places)
+        _check(s, q, out, lse, lens, causal, window, d ** -0.5)
+
+
+@pytest.mark.parametrize("d,kind", [(64, "e4m3"), (128, "int8")])
+def test_long_pieces(device, d, kind):
+    """Pieces longer than a table of places holds, with and without a window, in both kernels."""
+    s = Setup(device, [17000, 8200], 0, 1, d, kind, 64, "paged", page=64)
+    for sq, splits in ((4, 1), (70, 1), (70, 2), (4, 60), (70, 60)):
+        q = s.normal(2, sq, 2, d).bfloat16().to(device)
+        for window in ((-1, -1), (9000, -1)):
+            out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, window_size=window,
+                                                      num_splits=splits, return_softmax_lse=True, **s.places)
+            _check(s, q, out, lse, [17000, 8200], True, window, d ** -0.5)
+
+
+@pytest.mark.parametrize("d,hk,capacity", [(128, 4, 0), (128, 4, 200 << 10), (128, 3, 400 << 10), (64, 4, 200 << 10),
+                                           (64, 4, 800 << 10), (64, 6, 800 << 10), (64, 3, 800 << 10)])
+def test_heads_of_a_workgroup(device, d, hk, capacity):
+    """Few rows over capacities where a workgroup takes one, two or four KV heads."""
+    lens, page = [700, 0, 77, 2000], 64
+    s = Setup(device, lens, 0, hk, d, "e4m3", 64, "paged", page=page)
+    for sq in (1, 3, 9):
+        q = s.normal(4, sq, 4 * hk, d).bfloat16().to(device)
+        args = dict(cache_seqlens=s.lens, causal=True, num_splits=0, return_softmax_lse=True)
+        want = fai.flash_attn_with_kvcache_q8(q, *s.caches, block_table=s.table, **args)
+        _check(s, q, *want, lens, True, (-1, -1), d ** -0.5)
+        if capacity:
+            table = s.table
+            _widen(s, capacity, page)
+            got = fai.flash_attn_with_kvcache_q8(q, *s.caches, block_table=s.table, **args)
+            _check(s, q, *got, lens, True, (-1, -1), d ** -0.5)
+            s.table = table
+
+
+def test_many_rows_by_the_work(device):
+    """The same call on both sides of the amount of work where the kernel of many rows takes over."""
+    lens, page = [3000, 400, 1100], 64
+    s = Setup(device, lens, 0, 4, 128, "e4m3", 64, "paged", page=page)
+    table = s.table
+    for sq, h in ((8, 16), (33, 4), (100, 8)):
+        q = s.normal(3, sq, h, 128).half().to(device)
+        for wide in (0, 1 << 20):
+            s.table = table
+            if wide:
+                _widen(s, wide, page)
+            out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, return_softmax_lse=True,
+                                                      **s.places)
+            _check(s, q, out, lse, lens, True, (-1, -1), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("kind,dtype", [("e4m3", "fp16"), ("e4m3", "bf16"), ("int8", "fp16"), ("int8", "bf16")])
+def test_any_scales_of_few_and_many_rows(device, kind, dtype, rows):
+    """Scales of another quantiser, 0, far apart; a softmax_scale of either sign and 0; scores that grow along the keys."""
+    lens, d = [700, 97], 64
+    for i, (scale, growth) in enumerate(((0.125, 1), (-0.3, 1), (0.0, 1), (0.5, 40), (-0.5, 40))):
+        s = Setup(device, lens, 0, 2, d, kind, 32, "contiguous", seed=i)
+        for name in ("ks", "vs"):
+            x = getattr(s, name)
+            x.copy_(torch.rand(x.shape, generator=s.g) * (0.02 if kind == "e4m3" else 0.05))
+        s.vs[0, 1] = 0
+        s.vs[0, 2] = 2.0 ** -40
+        s.vs[0, 5] *= 300
+        s.ks[0, 3] = 0
+        s.ks *= torch.linspace(1 / growth, growth ** 0.5, s.ks.shape[1], device=device)[None, :, None]
+        q = s.normal(2, rows, 4, d).to(DTYPES[dtype]).to(device)
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, softmax_scale=scale,
+                                                  num_splits=i % 2 + 1, return_softmax_lse=True)
+        _check(s, q, out, lse, lens, True, (-1, -1), scale)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_not_a_number_and_infinity(device, kind, rows):
+    """A block that is not finite makes those rows NaN that see it, and no others."""
+    lens, d, block = [300, 300], 128, 32
+    for bad in ("k", "v"):
+        s = Setup(device, lens, 0, 2, d, kind, block, "contiguous")
+        q = s.normal(2, rows, 4, d).bfloat16().to(device)
+        args = dict(cache_seqlens=s.lens, causal=True, window_size=(60, -1), num_splits=1)
+        want = fai.flash_attn_with_kvcache_q8(q, *s.caches, **args)
+        getattr(s, bad + "s")[0, 7, 1] = math.nan  # keys 224 .. 255 of KV head 1
+        getattr(s, bad + "s")[1, 2, 0] = math.nan  # keys 64 .. 95: no window reaches back to them from here
+        got = fai.flash_attn_with_kvcache_q8(q, *s.caches, **args)
+        assert torch.equal(got[1], want[1])
+        for r in range(rows):
+            pos = 300 - rows + r
+            hit = pos >= 224 and pos - 60 <= 255
+            assert torch.equal(got[0, r, :2], want[0, r, :2])
+            assert got[0, r, 2:].isnan().all() if hit else torch.equal(got[0, r, 2:], want[0, r, 2:])
+
+
+def test_offsets_past_32_bits(device):
+    """The last pages of a pool of 4.6 GB of codes each for K and V, against the same pages in a small one."""
+    page, hk, d, pages = 64, 8, 128, 70000
+    small = Setup(device, [150, 64], 0, hk, d, "e4m3", 64, "paged", page=page, capacity=320)
+    big = [torch.empty(pages, *x.shape[1:], dtype=x.dtype, device=device) for x in small.caches]
+    n = small.kc.shape[0]
+    for x, y in zip(big, small.caches):
+        x[-n:] = y
+    far = torch.where(small.table >= 0, small.table + pages - n, small.table)
+    table = small.table
+    q = small.normal(2, 70, 16, d).bfloat16().to(device)
+    cu = torch.tensor([0, 150, 214], dtype=torch.int32, device=device)
+    for splits, rows in ((0, 1), (1, 70), (0, 70)):
+        args = dict(cache_seqlens=small.lens, causal=True, num_splits=splits)
+        want = fai.flash_attn_with_kvcache_q8(q[:, :rows], *small.caches, block_table=table, **args)
+        assert torch.equal(fai.flash_attn_with_kvcache_q8(q[:, :rows], *big, block_table=far, **args), want)
+    for x, y in zip(fai.flash_attn_kvcache_read_q8(*big, cu, 214, block_table=far),
+                    fai.flash_attn_kvcache_read_q8(*small.caches, cu, 214, block_table=table)):
+        assert torch.equal(x, y)
+    k = small.normal(2, 10, hk, d).bfloat16().to(device)
+    lens = small.lens - 10
+    fai.flash_attn_kvcache_append_q8(k, k, *small.caches, lens, block_table=table)
+    fai.flash_attn_kvcache_append_q8(k, k, *big, lens, block_table=far)
+    for x, y in zip(big, small.caches):
+        assert torch.equal(x[-n:].float().nan_to_num(-1), y.float().nan_to_num(-1))
