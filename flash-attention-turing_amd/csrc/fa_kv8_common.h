@@ -98,11 +98,6 @@ __device__ __forceinline__ uint32_t kv8_codes(const f32x4 v) {
     }
 }
 
-// A wave-uniform float of memory that no kernel in flight writes, through the scalar cache.
-__device__ __forceinline__ float scalar_float(const float *p) {
-    return *(const __attribute__((address_space(4))) float *)uniform(p);
-}
-
 // Cache row of sequence b, and what is wrong with it and with its lengths (0: nothing).
 __device__ __forceinline__ int kv8_err(const fa_kv8_cache &c, int b, int L0, int n, int most_new, int &row) {
     row = c.cache_batch_idx ? c.cache_batch_idx[b] : b;

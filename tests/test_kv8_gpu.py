@@ -670,3 +670,37 @@ def test_offsets_past_32_bits(device):
     fai.flash_attn_kvcache_append_q8(k, k, *big, lens, block_table=far)
     for x, y in zip(big, small.caches):
         assert torch.equal(x[-n:].float().nan_to_num(-1), y.float().nan_to_num(-1))
+
+
+def test_copied_pages(device):
+    """copy_pages moves codes and, as pools of their own, scales: attention over the copies is attention over the originals."""
+    s = Setup(device, [150, 64], 0, 4, 64, "e4m3", 32, "paged", page=64)
+    pages = s.kc.shape[0]
+    pools = [torch.cat((x, torch.zeros_like(x))) for x in s.caches]
+    src = torch.arange(pages, dtype=torch.int32, device=device)
+    fai.flash_attn_kvcache_copy_pages(pools[0], pools[1], src, src + pages)
+    fai.flash_attn_kvcache_copy_pages(*(x.view(2 * pages, 1, 1, -1) for x in pools[2:]), src, src + pages)
+    q = s.normal(2, 3, 8, 64).half().to(device)
+    want = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, **s.places)
+    table = torch.where(s.table >= 0, s.table + pages, s.table)
+    assert torch.equal(fai.flash_attn_with_kvcache_q8(q, *pools, cache_seqlens=s.lens, causal=True, block_table=table), want)
+
+
+def test_c_entry_points(device):
+    """The plain C calls: what they refuse before anything is launched, and workspace sizes of calls that have none."""
+    import ctypes
+
+    import fa_capi
+
+    lib = fa_capi.load()
+    a = fa_capi.FaKv8Args()
+    assert lib.fa_kv8_attention(None, None) < 0 and lib.fa_kv8_append(None, None) < 0 and lib.fa_kv8_read(None, None) < 0
+    for head_dim in (0, 48, 512, -64):
+        a.cache.batch, a.cache.nheads_k, a.nheads, a.seqlen_q, a.cache.head_dim = 2, 2, 4, 1, head_dim
+        assert lib.fa_kv8_ws_bytes(ctypes.byref(a)) == 0
+        assert lib.fa_kv8_attention(ctypes.byref(a), None) < 0
+    a.cache.head_dim, a.cache.cache_capacity, a.cache.nheads_k = 64, 256, 8
+    assert lib.fa_kv8_ws_bytes(ctypes.byref(a)) == 0  # more KV heads than heads
+    a.cache.nheads_k = 2
+    assert lib.fa_kv8_ws_bytes(ctypes.byref(a)) > 0
+    assert lib.fa_kv8_attention(ctypes.byref(a), None) < 0  # (no tensors)
