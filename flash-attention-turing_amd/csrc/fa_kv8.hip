@@ -19,6 +19,7 @@ namespace fa {
 // tokens 16 us at 4.4 TB/s, a copy's rate at that size.
 
 constexpr int kKv8Threads = 256;
+constexpr int64_t kKv8MaxGrid = 0xffffffffu / kKv8Threads;  // a launch has less than 2^32 threads
 
 // The smallest power of two s >= 2^-126 with x <= most * s, from the bits of |x| in the tensors' type; NaN if x is not finite.
 template <bool BF, bool INT8>
@@ -673,7 +674,7 @@ static int launch_kv8_append(const fa_kv8_args &a, const Kv8Plan *plan, hipStrea
     const int blocks = a.seqlen_new > 0 ? int((int64_t(a.seqlen_new) + 2 * c.scale_block - 2) / c.scale_block) : 0;
     const int64_t clear = plan ? (plan->counters + kKv8Threads - 1) / kKv8Threads : 0;
     const int64_t grid = (plan ? 1 : 0) + clear + int64_t(c.batch) * blocks * c.nheads_k * 2;
-    if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    if (grid > kKv8MaxGrid) return FA_ERR_INVALID_ARG;
     if (grid == 0) return FA_OK;
     const int most = std::min(c.scale_block, std::max(a.seqlen_new, 1)) * (c.head_dim / 8);  // units of a workgroup
     return kv8_by_type(c.head_dim, a.dtype, c.kind, [&](auto hd, auto bf, auto int8) {
@@ -730,13 +731,14 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
     using namespace fa;
     int rc = check_kv8(args);
     if (rc) return rc;
-    const fa_kv8_args &a = *args;
+    fa_kv8_args a = *args;
     if (a.cache.batch == 0) return FA_OK;
+    a.window_left = std::min(a.window_left, INT32_MAX / 2);  // positions less a window stay in 32 bits
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (a.seqlen_q == 0) return launch_kv8_append(a, nullptr, s);
     const Kv8Plan plan = kv8_plan(a);
     const int64_t grid = kv8_grid(plan, a.cache.nheads_k / plan.heads);
-    if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    if (grid > kKv8MaxGrid) return FA_ERR_INVALID_ARG;
     if ((rc = launch_kv8_append(a, &plan, s))) return rc;
     if (plan.many) return kv8_chunk(a, plan, s);
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
@@ -765,6 +767,7 @@ extern "C" int fa_kv8_read(const fa_kv8_read_args *args, void *stream) {
     if (!a.cu_seqlens || check_tensor(a.k_out, true) || check_tensor(a.v_out, true)) return FA_ERR_INVALID_ARG;
     const int per = kv8_read_rows(2 * a.cache.nheads_k * (a.cache.head_dim / 8));
     const int64_t grid = (int64_t(a.total) + per - 1) / per;
+    if (grid > kKv8MaxGrid) return FA_ERR_INVALID_ARG;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     return kv8_by_type(a.cache.head_dim, a.dtype, a.cache.kind, [&](auto hd, auto bf, auto int8) {
         hipLaunchKernelGGL((kv8_read_kernel<decltype(hd)::value, decltype(bf)::value, decltype(int8)::value>),

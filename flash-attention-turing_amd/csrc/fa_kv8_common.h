@@ -211,8 +211,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         kv8_scan(sum, total);
         // The even share, a little more for the rounding of 32 bits, in whole rounds.
         auto length = [&](float x) {
-            const float share = float(total) * x / float(plan.want) * 1.000001f;
-            return int(min(2147483392u, max(uint32_t(plan.least), (uint32_t(share) / plan.round + 1) * plan.round)));
+            const float share = fminf(float(total) * x / float(plan.want) * 1.000001f, 2147483520.f);
+            return int(min(2147483647u, max(uint32_t(plan.least), (uint32_t(share) / plan.round + 1) * plan.round)));
         };
         piece = length(1.f);
         // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, and

@@ -266,7 +266,7 @@ extern "C" int fa_rotary(const fa_rotary_args *args, void *stream) {
     for (const fa_tensor *t : {&a.k, &a.k_out})
         if (check_tensor(*t, a.nheads_k > 0)) return FA_ERR_INVALID_ARG;
     const int64_t grid = (rows + kRtThreads / 64 - 1) / (kRtThreads / 64);
-    if (grid > 0x7fffffff) return FA_ERR_INVALID_ARG;
+    if (grid > 0xffffffffu / kRtThreads) return FA_ERR_INVALID_ARG;  // a launch has less than 2^32 threads
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     auto go = [&](auto hd, auto bf, auto inter) {
         hipLaunchKernelGGL((rotary_kernel<decltype(hd)::value, decltype(bf)::value, decltype(inter)::value>),

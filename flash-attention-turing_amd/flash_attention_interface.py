@@ -969,7 +969,8 @@ def flash_attn_kvcache_append_q8(
 ) -> None:
     """Quantise k and v (batch, seqlen_new, nheads_k, headdim; fp16 or bf16) into a cache in 8 bits at cache_seqlens
     (int32 (batch,), which the caller advances).  seqlens_new (int32 (batch,)): new tokens of each sequence of a padded
-    batch, the rows of k and v behind them are not looked at; None: all of them.
+    batch, the rows of k and v behind them are not looked at; None: all of them.  No two sequences of a call may append to one
+    block of tokens.
 
     validate as in flash_diff_attn_with_kvcache: True checks lengths, rows and pages on the host; False leaves that to the
     kernels, which append nothing where something is wrong and record it for flash_attn_kvcache_check()."""
