@@ -590,17 +590,14 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const Kv8Cal
 
 int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s);  // fa_kv8_fwd.hip
 
-// KV heads that a workgroup of few rows takes together: their codes of a token are neighbours in memory, which
-// reads runs of 256 bytes faster, but there are fewer items to share a short call.  Measured (us, one head and so many): 64 x 8192
-// tokens of 8 heads of 128 203 and 187 (two), of 64 171 and 122 (four); 4 x 48000, 4 heads of 64, 50 and 47 (two; four 70);
-// 8 x 8000, 8 heads of 128, 37.8 and 39.5 (two).
+// KV heads that a workgroup of few rows takes together, one or two: their codes of a token are neighbours in memory, which reads
+// longer runs faster, but there are fewer items to share a short call.  Measured (us, one and two), 8 heads of 128 channels:
+// 64 x 8192 tokens 192 and 173, 8 x 32000 102 and 98, 2 x 131072 105 and 107, 1 x 131072 62 and 77; heads of 64, whose codes are
+// half a line: 8 heads 64 x 8192 174 and 117, 1 x 131072 57 and 45, 4 heads 4 x 48000 47 and 44.  (Four of 64: 114, 81 and 58.)
 static int kv8_heads(const fa_kv8_args &a) {
     const int64_t bytes = int64_t(a.cache.batch) * a.cache.cache_capacity * a.cache.nheads_k * a.cache.head_dim * 2;
-    int most = 256 / a.cache.head_dim;
-    if (bytes < 256 << 20) most /= 2;
-    if (bytes < 32 << 20) most = 1;
-    while (a.cache.nheads_k % most != 0) most /= 2;
-    return most;
+    const bool two = a.cache.head_dim == 64 ? bytes >= 32 << 20 : bytes >= 256 << 20 && a.cache.batch >= 4;
+    return two && a.cache.nheads_k % 2 == 0 ? 2 : 1;
 }
 
 static Kv8Plan kv8_plan(const fa_kv8_args &a) {
@@ -618,16 +615,18 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     p.rows_max = p.many ? tile : p.heads * int(std::min<int64_t>(rows, tile));
     const int64_t heads = int64_t(a.cache.nheads_k / p.heads) * p.row_tiles;
     p.items = a.cache.batch * heads;
-    p.round = 128;
     p.least = p.many ? 512 : 256;  // fewer and longer: 8 heads x 512 rows x 2048 keys took 36 us at 256 and 31 us at 512
-    p.want = int(std::max<int64_t>(2 * device_cus() / heads, 1));
+    // Two workgroups run on a CU.  One reads memory as fast, but more rows compute, too (us, one a CU and two): 24 rows x 9000 keys
+    // 25 and 28.5, 64 rows x 2000 keys of 8 sequences 37 and 29, 256 rows x 8192 keys 47 and 39.
+    p.most = int(std::max<int64_t>(2 * device_cus() / heads, 1));
+    p.want = p.many || p.row_tiles > 2 ? p.most : int(std::max<int64_t>(device_cus() / heads, 1));
     int64_t slots;
     if (a.num_splits > 0) {
-        p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + p.round - 1) / p.round * p.round);
+        p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + kKv8Round - 1) / kKv8Round * kKv8Round);
         slots = a.cache.batch * ((cap + p.fixed - 1) / p.fixed);
     } else {
-        // Pieces of at least total / (2 want) keys: a sequence has at most one short piece.
-        slots = std::min<int64_t>(2 * int64_t(p.want) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
+        // Pieces of at least total / (2 most) keys: a sequence has at most one short piece.
+        slots = std::min<int64_t>(2 * int64_t(p.most) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
     }
     p.slots = int(std::min<int64_t>(slots, INT32_MAX));
     const bool parts = slots > a.cache.batch;
@@ -748,8 +747,6 @@ extern "C" int fa_kv8_attention(const fa_kv8_args *args, void *stream) {
                                dim3(unsigned(grid)), dim3(kKv8Threads), 0, s, Kv8Call{a, plan});
             return int(hipGetLastError());
         };
-        if constexpr (HD == 64)
-            if (plan.heads == 4) return go(std::integral_constant<int, 4>{});
         if (plan.heads == 2) return go(std::integral_constant<int, 2>{});
         return go(std::integral_constant<int, 1>{});
     });

@@ -122,15 +122,15 @@ static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
 // Workspace: counters of the (sequence, KV heads, row tile) items and of every piece of them (a group of pieces counts at its
 // first one's), the slots, then the partial results.
 constexpr int kKdRows = 16, kKcRows = 128;  // rows of a tile: few rows, many
+constexpr int kKv8Round = 128;              // pieces have a multiple of so many keys: a tile of every wave, or two of a workgroup's
 struct Kv8Plan {
     bool many;          // the kernel of many rows (fa_kv8_fwd.hip)
     int heads;          // KV heads that a workgroup takes together
     int row_tiles;      // of a KV head
     int rows_max;       // rows of a tile whose partial results are kept
     int slots;          // at most
-    int round;          // piece lengths are multiples of it
     int fixed;          // keys of a piece, where the call says so, or 0
-    int want;           // slots that fill the chip
+    int want, most;     // slots that fill the chip, and that run at once
     int least;          // keys of a piece at least
     int64_t items;      // batch * nheads_k / heads * row_tiles
     int64_t counters, at_slots, at_ml, at_o, bytes;
@@ -188,6 +188,22 @@ __device__ __forceinline__ int64_t kv8_scan(int64_t x, int64_t &total) {
     return base + inc - x;
 }
 
+// Sums of four counts over the 256 threads of a workgroup.
+__device__ __forceinline__ void kv8_sums(int64_t (&x)[4]) {
+    __shared__ int64_t part[4][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], d);
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][i] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = part[0][i] + part[1][i] + part[2][i] + part[3][i];
+}
+
 // One workgroup: the slots of an attention call.
 __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Plan &plan) {
     __shared__ int64_t before[257];
@@ -209,32 +225,36 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
             sum += L - begin;
         }
         kv8_scan(sum, total);
-        // The even share, a little more for the rounding of 32 bits, in whole rounds.
-        auto length = [&](float x) {
-            const float share = fminf(float(total) * x / float(plan.want) * 1.000001f, 2147483520.f);
-            return int(min(2147483647u, max(uint32_t(plan.least), (uint32_t(share) / plan.round + 1) * plan.round)));
+        // x times the even share of n places, a little more for the rounding of 32 bits, in whole rounds.
+        auto length = [&](float x, int n) {
+            const float share = fminf(float(total) * x / float(n) * 1.000001f, 2147483520.f);
+            return int(min(2147483647u, max(uint32_t(plan.least), (uint32_t(share) / kKv8Round + 1) * kKv8Round)));
         };
-        piece = length(1.f);
-        // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, and
-        // where none fits, as with lengths far apart, half the share: twice the pieces, started as places become free.
-        const int at[4] = {piece, length(1.0625f), length(1.125f), length(1.25f)};
+        piece = length(1.f, plan.want);
+        // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, at one
+        // workgroup a CU or else at two; where none fits, as with lengths far apart, half the share of these: pieces that start as
+        // places become free.  Measured (us, one and two a CU): 64 x 8192 173 and 186, 4 x 48000 43 and 48, 2 x 9000 25 and 28.5;
+        // two a CU and half their share: 64 x 1024-16384 202 and 172.
+        const int at[8] = {piece, length(1.0625f, plan.want), length(1.125f, plan.want), length(1.25f, plan.want),
+                           length(1.f, plan.most), length(1.0625f, plan.most), length(1.125f, plan.most), length(1.25f, plan.most)};
         if (!plan.many && a.cache.batch > 1 && at[3] > plan.least) {
-            int64_t n01 = 0, n23 = 0;  // two counts each
+            float inv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) inv[i] = 1.f / float(at[i]);
+            // (Counts of 32-bit quotients: a length that is wrongly taken for fitting, or not, is as good.)
+            int64_t n[4] = {};  // two counts each
             for (int b = tid; b < a.cache.batch; b += 256) {
                 int begin, L, row;
                 sequence(b, begin, L, row);
-                auto pieces = [&](int i) { return int64_t(max(1, (L - begin - 1) / at[i] + 1)); };
-                n01 += pieces(0) << 32 | pieces(1);
-                n23 += pieces(2) << 32 | pieces(3);
-            }
-            int64_t t01, t23;
-            kv8_scan(n01, t01);
-            kv8_scan(n23, t23);
-            const int64_t n[4] = {t01 >> 32, t01 & 0xffffffff, t23 >> 32, t23 & 0xffffffff};
-            piece = length(0.5f);
+                auto pieces = [&](int i) { return int64_t(max(1, int(float(L - begin - 1) * inv[i]) + 1)); };
 #pragma unroll
-            for (int i = 3; i >= 0; --i)
-                if (n[i] <= plan.want) piece = at[i];
+                for (int i = 0; i < 4; ++i) n[i] += pieces(2 * i) << 32 | pieces(2 * i + 1);
+            }
+            kv8_sums(n);
+            piece = length(0.5f, plan.most);
+#pragma unroll
+            for (int i = 7; i >= 0; --i)
+                if ((i % 2 ? n[i / 2] & 0xffffffff : n[i / 2] >> 32) <= (i < 4 ? plan.want : plan.most)) piece = at[i];
         }
     }
     int64_t done = 0;
@@ -243,7 +263,7 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         int begin = 0, L = 0, row = 0, n = 0;
         if (b < a.cache.batch) {
             sequence(b, begin, L, row);
-            n = max(1, int((int64_t(L) - begin + piece - 1) / piece));
+            n = max(1, int((uint32_t(L - begin) + uint32_t(piece) - 1) / uint32_t(piece)));
         }
         int64_t total;
         const int64_t at = kv8_scan(n, total);
@@ -253,8 +273,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         row_of[tid] = row;
         // Pieces of few rows are equal: they end together.  Those of many rows keep the length, whose places run one each, and
         // the short last ones fill what is left: 3 + 2 pieces on 4 places took 204 us equal and 172 us so.
-        const int64_t even = (int64_t(L) - begin + max(n, 1) - 1) / max(n, 1);
-        piece_of[tid] = plan.fixed || plan.many ? piece : int(min(int64_t(INT_MAX), (even + plan.round - 1) / plan.round * plan.round));
+        const uint32_t parts = max(n, 1), even = (uint32_t(L - begin) + parts - 1) / parts;
+        piece_of[tid] = plan.fixed || plan.many ? piece : int(min(uint32_t(INT_MAX), (even + kKv8Round - 1) / kKv8Round * kKv8Round));
         if (tid == 0) before[256] = total;
         __syncthreads();
         for (int64_t s = tid; s < total && done + s < plan.slots; s += 256) {
