@@ -617,7 +617,7 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     p.items = a.cache.batch * heads;
     p.least = p.many ? 512 : 256;  // fewer and longer: 8 heads x 512 rows x 2048 keys took 36 us at 256 and 31 us at 512
     // Two workgroups run on a CU.  One reads memory as fast, but more rows compute, too (us, one a CU and two): 24 rows x 9000 keys
-    // 25 and 28.5, 64 rows x 2000 keys of 8 sequences 37 and 29, 256 rows x 8192 keys 47 and 39.
+    // 25 and 28.5, but 64 rows x 2000 keys of 8 sequences 37 and 29, 256 rows x 8192 keys 47 and 39.
     p.most = int(std::max<int64_t>(2 * device_cus() / heads, 1));
     p.want = p.many || p.row_tiles > 2 ? p.most : int(std::max<int64_t>(device_cus() / heads, 1));
     int64_t slots;
@@ -643,7 +643,8 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
 static int check_kv8_cache(const fa_kv8_cache &c) {
     if (c.head_dim != 64 && c.head_dim != 128) return FA_ERR_UNSUPPORTED;
     if (c.kind != FA_KV8_E4M3 && c.kind != FA_KV8_INT8) return FA_ERR_UNSUPPORTED;
-    if (c.batch < 0 || c.nheads_k <= 0 || c.cache_capacity < 0) return FA_ERR_INVALID_ARG;
+    // (2^30 tokens: a position and a table of places behind it stay in 32 bits.)
+    if (c.batch < 0 || c.nheads_k <= 0 || c.cache_capacity < 0 || c.cache_capacity > 1 << 30) return FA_ERR_INVALID_ARG;
     if (c.scale_block != 32 && c.scale_block != 64 && c.scale_block != 128 && c.scale_block != 256) return FA_ERR_INVALID_ARG;
     if (c.block_table ? c.cache_batch_idx || c.page_block_size <= 0 || c.page_block_size % c.scale_block || c.num_pages <= 0
                       : c.cache_capacity % c.scale_block != 0)

@@ -227,8 +227,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         kv8_scan(sum, total);
         // x times the even share of n places, a little more for the rounding of 32 bits, in whole rounds.
         auto length = [&](float x, int n) {
-            const float share = fminf(float(total) * x / float(n) * 1.000001f, 2147483520.f);
-            return int(min(2147483647u, max(uint32_t(plan.least), (uint32_t(share) / kKv8Round + 1) * kKv8Round)));
+            const float share = fminf(float(total) * x / float(n) * 1.000001f, float(1 << 30));
+            return int(max(uint32_t(plan.least), (uint32_t(share) / kKv8Round + 1) * kKv8Round));
         };
         piece = length(1.f, plan.want);
         // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, at one
@@ -274,7 +274,7 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         // Pieces of few rows are equal: they end together.  Those of many rows keep the length, whose places run one each, and
         // the short last ones fill what is left: 3 + 2 pieces on 4 places took 204 us equal and 172 us so.
         const uint32_t parts = max(n, 1), even = (uint32_t(L - begin) + parts - 1) / parts;
-        piece_of[tid] = plan.fixed || plan.many ? piece : int(min(uint32_t(INT_MAX), (even + kKv8Round - 1) / kKv8Round * kKv8Round));
+        piece_of[tid] = plan.fixed || plan.many ? piece : int((even + kKv8Round - 1) / kKv8Round * kKv8Round);
         if (tid == 0) before[256] = total;
         __syncthreads();
         for (int64_t s = tid; s < total && done + s < plan.slots; s += 256) {

@@ -704,3 +704,22 @@ def test_c_entry_points(device):
     a.cache.nheads_k = 2
     assert lib.fa_kv8_ws_bytes(ctypes.byref(a)) > 0
     assert lib.fa_kv8_attention(ctypes.byref(a), None) < 0  # (no tensors)
+
+
+def test_the_largest_capacity(device):
+    """2^30 tokens behind a table; one page more is refused."""
+    page = 1 << 10
+    s = Setup(device, [3000, 1], 0, 2, 64, "e4m3", 32, "paged", page=page)
+    q = s.normal(2, 1, 4, 64).half().to(device)
+    table = s.table
+    for cols, rows in ((1 << 20, 1), (1 << 20, 70)):
+        s.table = table
+        _widen(s, cols * page - table.shape[1] * page, page)
+        q = s.normal(2, rows, 4, 64).half().to(device)
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, return_softmax_lse=True,
+                                                  validate=False, **s.places)
+        _check(s, q, out, lse, [3000, 1], True, (-1, -1), 0.125)
+    fai.flash_attn_kvcache_check()
+    _widen(s, page, page)
+    with pytest.raises(RuntimeError):
+        fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, validate=False, **s.places)
