@@ -16,7 +16,7 @@ namespace fa {
 // raised at most a few times however many appends fill it.
 //
 // One token for each of 64 sequences takes 5 us, a chain of four latencies (length, page, rows, scale); 4 prompts of up to 4096
-// tokens 16 us at 4.4 TB/s, a copy's rate at that size.
+// tokens 15 us at 4.8 TB/s, a copy's rate at that size.
 
 constexpr int kKv8Threads = 256;
 constexpr int64_t kKv8MaxGrid = 0xffffffffu / kKv8Threads;  // a launch has less than 2^32 threads
@@ -685,8 +685,13 @@ static int launch_kv8_append(const fa_kv8_args &a, const Kv8Plan *plan, hipStrea
                                s, a, plan ? *plan : Kv8Plan{}, plan ? 1 : 0, int(clear), std::max(blocks, 1));
             return int(hipGetLastError());
         };
+        // As many units a thread as a block or the call has at most: registers for more cost waves.  4 x 2048 tokens, 8 heads (us,
+        // so many and the most): blocks of 32, 64 channels, 12.8 and 15.3 (1 and 8); of 64, 128 channels, 11.4 and 15.4 (4 and 16);
+        // 4 prompts of up to 4096 tokens, blocks of 128, 15.3 and 16.9 (8 and 16).
         if (most <= kKv8Threads) return go(std::integral_constant<int, 1>{});
         if (most <= 4 * kKv8Threads) return go(std::integral_constant<int, 4>{});
+        if constexpr (HD == 128)
+            if (most <= 8 * kKv8Threads) return go(std::integral_constant<int, 8>{});
         return go(std::integral_constant<int, 256 * HD / 8 / kKv8Threads>{});
     });
 }
