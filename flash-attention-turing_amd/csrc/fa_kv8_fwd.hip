@@ -225,8 +225,10 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    // (m is -infinity until a key is visible: a sum over 0 then, too.  NaN goes on.)
-                    if (__builtin_amdgcn_ballot_w64(sum > kKcTop || (m == -INFINITY && sum > 0.f)) != 0) {
+                    // A row without a reference gets one from the first half that shows it a key, whatever the sum: scores far
+                    // below 0 leave a sum of 0.
+                    const bool fresh = m == -INFINITY && max(first, p0) <= min(min(last, s1 - 1), p0 + 31);
+                    if (__builtin_amdgcn_ballot_w64(sum > kKcTop || fresh) != 0) {
                         // The scores again, their maximum as the new reference.
                         const char *kt0 = smem + t % NST * STAGE + 32 * h * HD;
                         f32x16 x = zero16();

@@ -1,0 +1,63 @@
+"""Attention over a KV cache in 8 bits where its softmax can go wrong: scores far from 0, in the kernels of few and of many
+query rows, whole and in pieces, elementwise within the roundings that oracle/kv8.py counts."""
+
+import pytest
+import torch
+
+import flash_attention_interface as fai
+from test_kv8_gpu import Setup, _check
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [1, 70]  # query rows of a KV head: the kernel of few, and of many
+
+
+def _put(s, k, v):
+    """Write k and v [batch][tokens, heads, dim] into an empty cache."""
+    for name, x in (("k", k), ("v", v)):
+        o = s.oracle(name)
+        for i, t in enumerate(x):
+            o.append(i, 0, t.to(torch.bfloat16))
+        s.put(name, o)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("kind,d", [("e4m3", 64), ("e4m3", 128), ("int8", 64), ("int8", 128)])
+@pytest.mark.parametrize("levels", [(-120, -120), (-150, -150), (-92, -90), (-90, -92), (-1000, -1000), (-200, -100), (-60, 40)])
+def test_scores_far_from_zero(device, levels, kind, d, rows, splits):
+    """Every row of a wave has scores near levels[0] in the first half of its keys and near levels[1] in the second: a common
+    offset, which softmax does not see.  Some blocks of V are small, or 0."""
+    lens, hk, scale = [256, 700], 2, 1 / 16
+    s = Setup(device, lens, 0, hk, d, kind, 32, "contiguous", held=False)
+    sign = torch.randint(0, 2, (d,), generator=s.g).float() * 2 - 1
+    ks, vs = [], []
+    for n in lens:
+        size = torch.where(torch.arange(n) < n // 2, *(abs(x) / (4 * d * scale) for x in levels))
+        turn = torch.where(torch.arange(n) < n // 2, *(torch.tensor(1.0 if x > 0 else -1.0) for x in levels))
+        ks.append((size * turn)[:, None, None] * sign + 0.01 * s.normal(n, hk, d))
+        v = s.normal(n, hk, d)
+        v[64:96] *= 2.0 ** -20
+        v[128:160] = 0
+        vs.append(v)
+    _put(s, ks, vs)
+    q = (4 * sign + 0.01 * s.normal(2, rows, 2 * hk, d)).half().to(device)
+    out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, softmax_scale=scale,
+                                              num_splits=splits, return_softmax_lse=True)
+    assert (lse < -50).all() or max(levels) > 0
+    _check(s, q, out, lse, lens, True, (-1, -1), scale)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_scores_far_from_zero_behind_a_window(device, rows):
+    """The first keys that a row sees lie in the middle of a tile that other rows see from its start."""
+    d, lens, scale = 128, [500], 1 / 16
+    s = Setup(device, lens, 0, 1, d, "e4m3", 64, "paged", held=False)
+    sign = torch.randint(0, 2, (d,), generator=s.g).float() * 2 - 1
+    level = torch.linspace(180, 100, 500)
+    _put(s, [-(level / (4 * d * scale))[:, None, None] * sign + 0.01 * s.normal(500, 1, d)], [s.normal(500, 1, d)])
+    q = (4 * sign + 0.01 * s.normal(1, rows, 3, d)).bfloat16().to(device)
+    for window, causal in (((40, -1), True), ((3, 0), False), ((0, -1), True)):
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=causal, window_size=window,
+                                                  softmax_scale=scale, num_splits=2, return_softmax_lse=True, **s.places)
+        _check(s, q, out, lse, lens, causal, window, scale)
