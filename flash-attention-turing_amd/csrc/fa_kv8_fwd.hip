@@ -5,8 +5,14 @@
 // LDS traffic, and each wave converts what it reads.  (Converted once for the workgroup, through registers and 16-bit LDS, the same
 // call took 183 us against 172: the barriers and writes cost more than the conversions.)  Scales multiply scores and
 // probabilities.  Four waves of 32 rows: S^T = K Q^T, so that a lane owns a row, and P^T feeds O^T += V^T P^T from the
-// accumulators, half a tile behind.  P is fp16 for both types of q, which codes allow: exact products and 11 bits
-// where bf16 has 8.
+// accumulators, half a tile behind.
+//
+// P times V's scale is rounded to fp16 for both types of q, as P is in the forward kernels: codes make the products exact,
+// and 11 bits are no fewer than the output keeps.  (As hi + lo, which the kernel of few rows has, where the
+// product with V costs nothing, 1160 -> 1590 us at 2048 queries over 32768 keys, 179 -> 238 at 2 x 512 over 4k to 12k.)  fp16's
+// range suffices because O has a reference of its own, a row's largest score + log2(V's scale) so far: keys that a row does
+// not see, or whose probability is small, take no bits from the others, whatever their V is.  What rounds to 0 is 2^-30 of the
+// row's largest p * scale.
 //
 // What bounds it: matrix and vector instructions of the same SIMDs, 43 and 62 % of the cycles at 2 x 512 queries over 4k to
 // 12k tokens (32/8 heads of 128, e4m3: 166 us of a call's 172, 0.86 PFLOP/s), 0.99 PFLOP/s at 2048 queries over 32768; int8 takes
@@ -18,9 +24,9 @@
 namespace fa {
 
 constexpr int kKcThreads = 256, kKcKeys = 64, kKcHalves = kKcThreads;
-// P is kept times at most 2^5, and its reference is raised when the sum of a lane's 16 passes 2^15: fp16 holds it, with all its
-// bits down to 2^-19.
-constexpr float kKcTop = 32768.f, kKcLift = 5.f;
+// P is 2^5 at its reference, which is raised when the sum of a lane's 16, or their softmax sum, passes 2^15: fp16 holds it,
+// with all its bits down to 2^-19 of the reference.
+constexpr float kKcTop = 32768.f, kKcLift = 5.f, kKcNoLift = -160.f;
 
 template <int HD, bool BF, bool INT8>
 __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call call) {
@@ -31,13 +37,12 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
     constexpr int DT = HD / 32;
     __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
     // Halves of tiles (32 keys, which lie in one page and one block of scales): where their codes begin, k's scale with the
-    // softmax's, V's as what it adds to the exponents of P and takes from their sum, and what it adds to scores: 0 or NaN.
+    // softmax's, V's as what it adds to the exponents of P, and what it adds to scores: 0 or NaN.
     struct Half {
         const char *k, *v;
-        float k_scale, lift, unlift, nan;
+        float k_scale, lift, nan, pad;
     };
     __shared__ __attribute__((aligned(16))) Half halves[kKcHalves];
-    __shared__ float tops[4];
     __shared__ int ticket;
 
     const fa_kv8_cache &c = a.cache;
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
     f32x16 o[DT], s[2];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = zero16();
-    float m = -INFINITY, l = 0.f, vref = 0.f;
+    float m = -INFINITY, mo = -INFINITY, l = 0.f;  // references of the sum and of O, the sum
     constexpr int NS = HD / 16, NPV = 2 * DT, EPS = 16 / NS;  // EPS: exponentials of a step
     constexpr int KP = HD == 128 ? 3 : 2, VP = 4;  // reads in flight, and the next
     u32x4 kc[KP];
@@ -126,35 +131,21 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
             }
             const int blk = at >> __builtin_ctz(c.scale_block);
             const float ks = c.k_scale.ptr[line * c.k_scale.batch_stride + int64_t(blk) * c.k_scale.row_stride + int64_t(hk) * c.k_scale.head_stride];
-            float vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
+            const float vs = c.v_scale.ptr[line * c.v_scale.batch_stride + int64_t(blk) * c.v_scale.row_stride + int64_t(hk) * c.v_scale.head_stride];
             halves[tid].k = (const char *)c.k.ptr + line * c.k.batch_stride + int64_t(at) * c.k.row_stride + int64_t(hk) * c.k.head_stride;
             halves[tid].v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
             __syncthreads();
             for (int x = 0; x < min(3, n_tiles); ++x) issue(x, base);  // (the waits below are theirs, too)
-            // V's scale over a reference, the largest one, as a power of P; where it is not finite, it reaches the scores of
-            // its keys as NaN.
+            // V's scale as a power of P (of 0: under that of any number); where it is not finite, it reaches the scores of its
+            // keys as NaN.
             f32x4 h;
-            h[3] = vs * 0.f;
-            if (!(h[3] == 0.f) || !(vs > 0.f)) vs = 0.f;
-            float top = vs;
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-            if (lane == 0) tops[wave] = top;
-            wait_vmem();
-            __syncthreads();
-            const float before = vref;
-            vref = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(before, kKv8MinScale));
             h[0] = ks * cscale;
-            h[1] = fmaxf(log2_fast(vs / vref), -64.f) + kKcLift;
-            h[2] = exp2_fast(-h[1]);
+            h[2] = vs * 0.f;
+            h[1] = fmaxf(log2_fast(h[2] == 0.f ? vs : 0.f), kKcNoLift);
+            h[3] = 0.f;
             *reinterpret_cast<f32x4 *>(&halves[tid].k_scale) = h;
-            if (base > s0) {
-                const float f = before / vref;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-            } else if (a.softmax_scale < 0.f) {
+            wait_vmem();
+            if (base == s0 && a.softmax_scale < 0.f) {
 #pragma unroll
                 for (int g = 0; g < HD / 16; ++g) qB[g] = as_h8(neg_h8(__builtin_bit_cast(u32x4, qB[g])));
             }
@@ -192,21 +183,24 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
                 auto v_read = [&](int u) FA_INLINE { vc[u % VP] = lds_tr8(vt, 16 * (u / DT) * HD + (v_at ^ (u % DT << 5) ^ u / DT * (HD / 2))); };
                 if (some) {
                     const f32x4 x4 = *reinterpret_cast<const f32x4 *>(&halves[2 * t + h].k_scale);
-                    float sk = uniform(x4[0]), d = x4[1] + x4[3];
+                    float sk = uniform(x4[0]), d = x4[2];
                     if (p0 < all_first || p0 + 31 > all_last) {
                         const int lo = first - p0 - 8 * hh, hi = min(last, s1 - 1) - p0 - 8 * hh;
-                        d = x4[1];
+                        d = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int key = acc_lrow(r, 0);
-                            const float x = fmaf(sc[r], sk, x4[3]);
+                            const float x = fmaf(sc[r], sk, x4[2]);
                             sc[r] = key < lo || key > hi ? -INFINITY : x;
                         }
                         sk = 1.f;
                     }
-                    // Exponentials of the half, with its largest at most 2^15 over the reference, which is that of the last
-                    // raise: their sum says so.
-                    float dm = d - (m == -INFINITY ? 0.f : m), sum = 0.f;
+                    // Exponentials of the half, with its largest at most 2^15 over the references, which are those of the last
+                    // raise: their sum says so.  p is what scores are raised by: V's scale over O's reference, or 2^-64 over
+                    // the sum's where that is more.  (Such keys are 0 in P, and still all there in the sum.)
+                    auto power = [&]() FA_INLINE { return m == -INFINITY ? 0.f : fmaxf(x4[1] - mo, -64.f - m); };
+                    float p = power(), sum = 0.f;
+                    const float dm = p + d;
                     f16x8 pB[2];
                     __builtin_amdgcn_s_setprio(1);
                     __builtin_amdgcn_sched_barrier(0);
@@ -228,8 +222,9 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
                     // A row without a reference gets one from the first half that shows it a key, whatever the sum: scores far
                     // below 0 leave a sum of 0.
                     const bool fresh = m == -INFINITY && max(first, p0) <= min(min(last, s1 - 1), p0 + 31);
-                    if (__builtin_amdgcn_ballot_w64(sum > kKcTop || fresh) != 0) {
-                        // The scores again, their maximum as the new reference.
+                    float sum_l = m == -INFINITY ? sum : sum * exp2_fast(-p - m);
+                    if (__builtin_amdgcn_ballot_w64(sum > kKcTop || sum_l > kKcTop || fresh) != 0) {
+                        // The scores again, their maximum as the new reference; with V's scale for O's.
                         const char *kt0 = smem + t % NST * STAGE + 32 * h * HD;
                         f32x16 x = zero16();
 #pragma unroll
@@ -242,28 +237,31 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int key = acc_lrow(r, 0);
-                            x[r] = key < lo || key > hi ? -INFINITY : fmaf(x[r], x4[0], x4[3]);
+                            x[r] = key < lo || key > hi ? -INFINITY : fmaf(x[r], x4[0], x4[2]);
                             top = fmaxf(top, x[r]);
                         }
-                        const float m_new = fmaxf(m, max2_xor32(top));
-                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-                        l *= alpha;
+                        top = max2_xor32(top);
+                        const float m_new = fmaxf(m, top), mo_new = fmaxf(mo, top + x4[1] - kKcLift);
+                        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(mo - mo_new);
+                        l *= m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
                         m = m_new;
-                        dm = x4[1] - (m == -INFINITY ? 0.f : m);
+                        mo = mo_new;
+                        p = power();
                         sum = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            x[r] = exp2_fast(x[r] + dm);
+                            x[r] = exp2_fast(x[r] + p);
                             sum += x[r];
                         }
                         pB[0] = pack8(x, 0);
                         pB[1] = pack8(x, 8);
+                        sum_l = m == -INFINITY ? sum : sum * exp2_fast(-p - m);
                     }
-                    l = fmaf(sum, x4[2], l);
+                    l += sum_l;
 #pragma unroll
                     for (int u = 0; u < NPV; ++u) {
                         const f16x8 v = kv8_decode<INT8, false>(vc[u % VP]);
@@ -285,8 +283,8 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
     }
 
     const Kv8Call &late = kv8_late();
-    // P's lift and the reference of V's scales leave O.
-    const float out_scale = vref * exp2_fast(-kKcLift);
+    // O on the sum's reference.
+    const float out_scale = m == -INFINITY ? 1.f : exp2_fast(mo - m);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

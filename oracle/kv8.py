@@ -3,8 +3,9 @@
 ``append`` and ``read`` are exact: scales are powers of two, so that codes and scales have one right value each.
 ``attention`` gives every output with the error that a kernel may have which computes as documented: scores of exact
 products summed in fp32 (e = 2^-23 an operation), scaled, exponentials off by 2^-21 (|s| + |lse| + 1) more, probabilities
-times V's scale rounded to fp16 or better (2^-11 relatively, 2^-30 of the largest value absolutely), sums in fp32, one
-rounding of the output (u = eps / 2, t half of the type's smallest step).
+times V's scale rounded to fp16 or better (2^-11 relatively; absolutely 2^-30 of the row's largest probability times scale over
+the keys that it sees, for each of them), sums in fp32, one rounding of the output (u = eps / 2, t half of the type's smallest
+step).  A scale times the largest code is at most twice the largest value of its block, which lies in one of 256 tokens.
 """
 
 import math
@@ -120,7 +121,9 @@ def attention(q, k, v, scale, causal, window=(-1, -1)):
         row = err.amax(1, keepdim=True)
         o = torch.where(keep, p, 0.0) @ torch.where(keep.any(0)[:, None], vv, 0.0)
         a = p @ torch.where(keep.any(0)[:, None], vv.abs(), 0.0)
-        acc = (2.0 ** -11 + 2 * row + (2 * sk + 24) * E) * a + 2.0 ** -30 * keep.sum(1, keepdim=True) * vv.abs().max()
+        size = torch.nn.functional.pad(vv.abs().amax(1), (0, -sk % 256)).view(-1, 256).amax(1).repeat_interleave(256)[:sk]
+        floor = 2.0 ** -30 * (torch.where(keep, p, 0.0) * torch.where(keep.any(0), 2 * size, 0.0)).amax(1, keepdim=True)
+        acc = (2.0 ** -11 + 2 * row + (2 * sk + 24) * E) * a + floor * keep.sum(1, keepdim=True)
         out[:, i], out_b[:, i] = o, torch.where(empty[:, None], 0.0, acc + u * (o.abs() + acc) + t)
         lse[i], lse_b[i] = l[:, 0], torch.where(empty, 0.0, row[:, 0] + (sk + 16) * E + 2.0 ** -21 * l[:, 0].abs())
     return {"out": (out, out_b), "lse": (lse, lse_b)}

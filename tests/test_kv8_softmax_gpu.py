@@ -61,3 +61,57 @@ def test_scores_far_from_zero_behind_a_window(device, rows):
         out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=causal, window_size=window,
                                                   softmax_scale=scale, num_splits=2, return_softmax_lse=True, **s.places)
         _check(s, q, out, lse, lens, causal, window, scale)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("kind,d", [("e4m3", 64), ("e4m3", 128), ("int8", 64), ("int8", 128)])
+@pytest.mark.parametrize("power", [16, 24, 60])
+def test_values_that_a_row_does_not_see(device, power, kind, d, rows, splits):
+    """Blocks whose V is 2^power times the others': one that rows before it do not see (causal), one that no row's window
+    reaches, and one whose keys have no probability to speak of.  The other rows keep all their bits."""
+    n, hk, block = 1000, 2, 32
+    for where in ("future", "window", "score"):
+        s = Setup(device, [n], 0, hk, d, kind, block, "contiguous", held=False)
+        k, v = s.normal(n, hk, d), s.normal(n, hk, d)
+        q, window = s.normal(1, rows, 2 * hk, d), (-1, -1)
+        if where == "future":  # the last block: rows before it see nothing of the 256 tokens from 768 on, or some of them
+            v[992:] *= 2.0 ** power
+        elif where == "window":
+            v[480:512] *= 2.0 ** power  # (of the 256 tokens from 256 on, which rows do not see)
+            window = (300, -1)
+        else:
+            sign = torch.randint(0, 2, (d,), generator=s.g).float() * 2 - 1
+            q, k = q + 2 * sign, k + sign
+            k[256:288] -= 40 * sign  # exp(-2 40 d / sqrt d): 2^-900 and less
+            v[256:288] *= 2.0 ** power
+        _put(s, [k], [v])
+        q = q.bfloat16().to(device)
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, window_size=window,
+                                                  num_splits=splits, return_softmax_lse=True)
+        _check(s, q, out, lse, [n], True, window, d ** -0.5)
+        if where == "future":  # what the rows before it are without it
+            s.vc[:, 992:], s.vs[:, 31] = 0, 2.0 ** -126
+            few = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, num_splits=splits)
+            before = [r for r in range(rows) if n - rows + r < 992]
+            a, b = out[:, before].double(), few[:, before].double()
+            # Two roundings to bf16, and what fp16's of P may differ by.
+            assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 2.0 ** -10 * 4).all()
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_values_from_small_to_large(device, kind, rows):
+    """V grows 2^4 a block, so that every block is another reference, and shrinks again; scores grow and shrink against it."""
+    n, d, hk = 640, 64, 1
+    for slope in (0.0, 2.0, -2.0, 6.0, -6.0):
+        s = Setup(device, [n], 0, hk, d, kind, 32, "contiguous", held=False)
+        step = (torch.arange(n) // 32).float()
+        v = s.normal(n, hk, d) * 2.0 ** (40 - 4 * (step - 10).abs())[:, None, None]
+        sign = torch.randint(0, 2, (d,), generator=s.g).float() * 2 - 1
+        k = (slope * (step - 10).abs() / 64)[:, None, None] * sign + 0.1 * s.normal(n, hk, d)
+        _put(s, [k], [v])
+        q = (sign + 0.1 * s.normal(1, rows, 2, d)).bfloat16().to(device)
+        out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, softmax_scale=1.0,
+                                                  num_splits=1, return_softmax_lse=True)
+        _check(s, q, out, lse, [n], True, (-1, -1), 1.0)
