@@ -451,10 +451,11 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const Kv8Cal
                 if (k + NST < n) issue(k + NST, st);
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
-                    // V's scale reaches the scores of its keys as 0, or as NaN where it is not finite, and then has done its part.
+                    // Scales reach the scores of their keys as 0, or as NaN where one is not finite (of infinity times a score of
+                    // either sign, softmax would pass over half), and V's then has done its part.
+                    const float ksk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks[h]), k));
                     const float vsk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs[h]), k));
-                    const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks[h]), k)) * cscale, sv0 = vsk * 0.f,
-                                sv = sv0 == 0.f ? vsk : 0.f;
+                    const float sk = ksk * cscale, sv0 = fmaf(vsk, 0.f, ksk * 0.f), sv = sv0 == 0.f ? vsk : 0.f;
                     f32x4 s[2];
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {

@@ -136,11 +136,11 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
             halves[tid].v = (const char *)c.v.ptr + line * c.v.batch_stride + int64_t(at) * c.v.row_stride + int64_t(hk) * c.v.head_stride;
             __syncthreads();
             for (int x = 0; x < min(3, n_tiles); ++x) issue(x, base);  // (the waits below are theirs, too)
-            // V's scale as a power of P (of 0: under that of any number); where it is not finite, it reaches the scores of its
-            // keys as NaN.
+            // V's scale as a power of P (of 0: under that of any number); where one of the two is not finite, the scores of its
+            // keys are NaN.
             f32x4 h;
             h[0] = ks * cscale;
-            h[2] = vs * 0.f;
+            h[2] = ks * 0.f + vs * 0.f;
             h[1] = fmaxf(log2_fast(h[2] == 0.f ? vs : 0.f), kKcNoLift);
             h[3] = 0.f;
             *reinterpret_cast<f32x4 *>(&halves[tid].k_scale) = h;

@@ -924,7 +924,8 @@ def flash_attn_rotary_func(
 # clearing.  The appends make scales powers of two: the smallest s >= 2 ** -126 with max|x| <= most * s (most is 448 for
 # e4m3, 127 for int8), or the old one where the block holds earlier tokens and that is larger; codes are x / s, rounded to
 # nearest even, and earlier tokens' codes are rounded again where a scale grows.  A NaN or an infinity among a block's new
-# values makes its scale NaN.  The readers take any scales that are not negative.
+# values makes its scale NaN.  The readers take any finite codes and scales that are not negative; a scale that is NaN or
+# infinite makes NaN those rows of attention that see its block.
 
 
 def _q8_places(batch, k_cache, lens, seqlen_new, cache_batch_idx, block_table, validate):

@@ -478,7 +478,8 @@ int fa_rotary(const fa_rotary_args *args, void *stream);
  * the old scale where the block holds earlier tokens and that is larger, and codes are x / s rounded to
  * nearest even; earlier tokens' codes are rounded again where the scale grows.  A NaN or an
  * infinity among the new values makes the scale NaN, and so every value of the block.
- * Attention takes any scales >= 0.  Lengths, rows and pages are checked on the device as in
+ * Attention takes any finite codes and scales >= 0; rows that see a block with a scale that is NaN or infinite become
+ * NaN.  Lengths, rows and pages are checked on the device as in
  * fa_diff_kvcache_args.  No counterpart in the reference.
  */
 enum { FA_KV8_E4M3 = 0, FA_KV8_INT8 = 1 };

@@ -115,3 +115,31 @@ def test_values_from_small_to_large(device, kind, rows):
         out, lse = fai.flash_attn_with_kvcache_q8(q, *s.caches, cache_seqlens=s.lens, causal=True, softmax_scale=1.0,
                                                   num_splits=1, return_softmax_lse=True)
         _check(s, q, out, lse, [n], True, (-1, -1), 1.0)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_scales_that_are_not_finite(device, which, bad, kind, rows):
+    """Rows that see a block with such a scale are NaN, also where all of its scores would be -infinity; no others are."""
+    n, d, hk = 300, 128, 2
+    for alike in (False, True):
+        s = Setup(device, [n, n], 0, hk, d, kind, 32, "contiguous", held=False)
+        sign = torch.randint(0, 2, (d,), generator=s.g).float() * 2 - 1
+        k = [s.normal(n, hk, d) - (4 * sign if alike else 0) for _ in range(2)]
+        _put(s, k, [s.normal(n, hk, d) for _ in range(2)])
+        q = (s.normal(2, rows, 4, d) + (4 * sign if alike else 0)).bfloat16().to(device)
+        args = dict(cache_seqlens=s.lens, causal=True, window_size=(60, -1), num_splits=1)
+        want = fai.flash_attn_with_kvcache_q8(q, *s.caches, **args)
+        getattr(s, which + "s")[0, 7, 1] = bad  # keys 224 .. 255 of KV head 1
+        getattr(s, which + "s")[1, 2, 0] = bad  # keys 64 .. 95: no window reaches back to them from here
+        got = fai.flash_attn_with_kvcache_q8(q, *s.caches, **args)
+        assert torch.equal(got[1], want[1])
+        for r in range(rows):
+            pos = n - rows + r
+            assert torch.equal(got[0, r, :2], want[0, r, :2])
+            if pos >= 224 and pos - 60 <= 255:
+                assert got[0, r, 2:].isnan().all(), r
+            else:
+                assert torch.equal(got[0, r, 2:], want[0, r, 2:]), r
