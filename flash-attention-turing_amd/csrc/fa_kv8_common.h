@@ -377,16 +377,18 @@ __device__ __forceinline__ int32_t *kv8_counter(const fa_kv8_args &a, int64_t i)
 // Joins the n pieces of an item in their order, by the 256 threads: thread units of (row, two channels), kKv8Join pieces at a
 // time, whose loads are in flight together.  scratch: LDS of ROWS (kKv8Join + 2) floats.  part(i) is the place of piece i's partial
 // results, write(row, channel, its and the next one's unnormalised O, maximum, sum) takes the joined ones.
-constexpr int kKv8Join = 64;
+// A row's bits are the same for any ROWS: sums of pieces i, i + 16, .. are kept apart and added in one order.
+constexpr int kKv8Join = 64, kKv8Apart = 16;
 template <int HD, int ROWS, int UNITS, class Part, class Write>
 __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &plan, int rows, int n, float *scratch, Part part,
                                          Write write) {
     constexpr int T = 256 / ROWS, PER = kKv8Join / T;  // threads a row that weigh its pieces, pieces of each
     constexpr int AHEAD = 32 / UNITS;
-    static_assert(AHEAD >= 1 && kKv8Join % AHEAD == 0 && kKv8Join % T == 0, "whole rounds");
+    constexpr int A = kKv8Apart / T;  // sums of a thread
+    static_assert(AHEAD >= 1 && kKv8Join % AHEAD == 0 && kKv8Join % T == 0 && kKv8Apart % T == 0 && PER % A == 0, "whole rounds");
     float *old = scratch, *sum = scratch + ROWS, *weight = scratch + 2 * ROWS;
     const int tid = threadIdx.x, r = tid / T, t = tid % T;
-    float mm = -INFINITY, ll = 0.f;
+    float mm = -INFINITY, ll[A] = {};
     f32x2 x[UNITS] = {};
     for (int i0 = 0; i0 < n; i0 += kKv8Join) {
         const int k = min(kKv8Join, n - i0);
@@ -412,7 +414,8 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
 #pragma unroll
         for (int d = 1; d < T; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
         const float f0 = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
-        ll *= f0;
+#pragma unroll
+        for (int j = 0; j < A; ++j) ll[j] *= f0;
         mm = top;
         __syncthreads();  // the weights before are used up
         if (t == 0) old[r] = f0;
@@ -420,7 +423,7 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
         for (int j = 0; j < PER; ++j) {
             const float f = ml[j][0] == -INFINITY ? 0.f : exp2_fast(ml[j][0] - top);
             weight[(t + j * T) * ROWS + r] = f;
-            ll = fmaf(ml[j][1], f, ll);
+            ll[j % A] = fmaf(ml[j][1], f, ll[j % A]);
         }
         __syncthreads();
 #pragma unroll
@@ -441,12 +444,17 @@ __device__ __forceinline__ void kv8_join(const fa_kv8_args &a, const Kv8Plan &pl
                 }
         }
     }
+    // (Sums i and i + 8 first, whether they are one thread's or two threads'.)
 #pragma unroll
-    for (int d = 1; d < T; d <<= 1) ll += __shfl_xor(ll, d);
+    for (int d = A / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int j = 0; j < d; ++j) ll[j] += ll[j + d];
+#pragma unroll
+    for (int d = T / 2; d > 0; d >>= 1) ll[0] += __shfl_xor(ll[0], d);
     __syncthreads();
     if (t == 0) {
         old[r] = mm;
-        sum[r] = ll;
+        sum[r] = ll[0];
     }
     __syncthreads();
 #pragma unroll
