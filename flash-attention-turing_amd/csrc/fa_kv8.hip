@@ -518,7 +518,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_decode_kernel(const Kv8Cal
     // Merge the four waves, a head after the other: O^T to LDS, then every thread sums pairs of channels of a row.
     const Kv8Call &late = kv8_late();
     const int rows = min(kKdRows, R - rt * kKdRows);
-    const int64_t part = int64_t(slot_i) * HI + hi_i;
+    const int64_t part = int64_t(sl.part) * HI + hi_i;
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
         if (h > 0) __syncthreads();
@@ -621,22 +621,27 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     // 25 and 28.5, but 64 rows x 2000 keys of 8 sequences 37 and 29, 256 rows x 8192 keys 47 and 39.
     p.most = int(std::max<int64_t>(2 * device_cus() / heads, 1));
     p.want = p.many || p.row_tiles > 2 ? p.most : int(std::max<int64_t>(device_cus() / heads, 1));
-    int64_t slots;
+    int64_t slots, parts;
     if (a.num_splits > 0) {
         p.fixed = int(((cap + a.num_splits - 1) / a.num_splits + kKv8Round - 1) / kKv8Round * kKv8Round);
         slots = a.cache.batch * ((cap + p.fixed - 1) / p.fixed);
+        parts = cap > p.fixed ? slots : 0;
     } else {
-        // Pieces of at least total / (2 most) keys: a sequence has at most one short piece.
+        // Pieces of more than total / most keys (many rows) or half of that: a sequence has at most one short piece, and a
+        // sequence with several is longer than a piece.  So fewer than most (2 most) sequences have several, of fewer than
+        // most (2 most) pieces and as many again as there are such sequences: none where most is 1.
+        parts = p.many ? 2 * int64_t(p.most) - 2 : 4 * int64_t(p.most) - 2;
         slots = std::min<int64_t>(2 * int64_t(p.most) + a.cache.batch, a.cache.batch * ((cap + p.least - 1) / p.least));
     }
     p.slots = int(std::min<int64_t>(slots, INT32_MAX));
-    const bool parts = slots > a.cache.batch;
+    if (slots == a.cache.batch) parts = 0;
+    parts = std::min(parts, slots);
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    p.counters = parts ? p.items + slots * heads : 0;
+    p.counters = parts ? p.items + parts * heads : 0;
     p.at_slots = up(p.counters * 4);
     p.at_ml = p.at_slots + up(slots * int64_t(sizeof(Kv8Slot)));
-    p.at_o = p.at_ml + (parts ? up(slots * heads * p.rows_max * 8) : 0);
-    p.bytes = p.at_o + (parts ? slots * heads * p.rows_max * a.cache.head_dim * 4 : 0);
+    p.at_o = p.at_ml + up(parts * heads * p.rows_max * 8);
+    p.bytes = p.at_o + parts * heads * p.rows_max * a.cache.head_dim * 4;
     return p;
 }
 

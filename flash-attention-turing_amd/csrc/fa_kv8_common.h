@@ -115,12 +115,12 @@ struct Kv8Slot {
     int begin, end;     // keys
     int keys;           // of the sequence
     int ch, n_pieces;   // this piece, and how many the sequence has
-    int pad;
+    int part;           // the piece among those of sequences with several, whose partial results have places
 };
 static_assert(sizeof(Kv8Slot) == 32, "one scalar load");
 
-// Workspace: counters of the (sequence, KV heads, row tile) items and of every piece of them (a group of pieces counts at its
-// first one's), the slots, then the partial results.
+// Workspace: counters of the (sequence, KV heads, row tile) items and of every piece that is one of several (a group of pieces
+// counts at its first one's), the slots, then those pieces' partial results.
 constexpr int kKdRows = 16, kKcRows = 128;  // rows of a tile: few rows, many
 constexpr int kKv8Round = 128;              // pieces have a multiple of so many keys: a tile of every wave, or two of a workgroup's
 struct Kv8Plan {
@@ -206,7 +206,7 @@ __device__ __forceinline__ void kv8_sums(int64_t (&x)[4]) {
 
 // One workgroup: the slots of an attention call.
 __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Plan &plan) {
-    __shared__ int64_t before[257];
+    __shared__ int before[257], parts_before[256];
     __shared__ int keys_of[256], begin_of[256], row_of[256], piece_of[256];
     const int tid = threadIdx.x;
     Kv8Slot *slots = reinterpret_cast<Kv8Slot *>(static_cast<char *>(a.ws) + plan.at_slots);
@@ -257,7 +257,7 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
                 if ((i % 2 ? n[i / 2] & 0xffffffff : n[i / 2] >> 32) <= (i < 4 ? plan.want : plan.most)) piece = at[i];
         }
     }
-    int64_t done = 0;
+    int64_t done = 0, parts_done = 0;
     for (int b0 = 0; b0 < a.cache.batch; b0 += 256) {
         const int b = b0 + tid;
         int begin = 0, L = 0, row = 0, n = 0;
@@ -265,9 +265,12 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
             sequence(b, begin, L, row);
             n = max(1, int((uint32_t(L - begin) + uint32_t(piece) - 1) / uint32_t(piece)));
         }
-        int64_t total;
-        const int64_t at = kv8_scan(n, total);
-        before[tid] = at;
+        // (Both counts in one sum: a launch has less than 2^24 slots.)
+        int64_t totals;
+        const int64_t at = kv8_scan(int64_t(n > 1 ? n : 0) << 32 | n, totals);
+        const int total = int(totals & 0xffffffff);
+        before[tid] = int(at & 0xffffffff);
+        parts_before[tid] = int(at >> 32);
         keys_of[tid] = L;
         begin_of[tid] = begin;
         row_of[tid] = row;
@@ -285,15 +288,16 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
             Kv8Slot x;
             x.b = b0 + lo;
             x.row = row_of[lo];
-            x.ch = int(s - before[lo]);
+            x.ch = int(s) - before[lo];
             x.keys = keys_of[lo];
-            x.n_pieces = int(before[lo + 1] - before[lo]);
+            x.n_pieces = before[lo + 1] - before[lo];
             x.begin = min(x.keys, begin_of[lo] + x.ch * piece_of[lo]);
             x.end = min(x.keys, x.begin + piece_of[lo]);
-            x.pad = 0;
+            x.part = int(parts_done) + parts_before[lo] + x.ch;
             slots[done + s] = x;
         }
         done += total;
+        parts_done += totals >> 32;
         __syncthreads();
     }
     for (int64_t s = done + tid; s < plan.slots; s += 256) slots[s].b = -1;

@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kKcThreads, 2) void kv8_chunk_kernel(const Kv8Call 
     if (sl.n_pieces > 1) {
         // Partial results lane by lane: (maximum, sum) of every row, then register pairs of O by wave and lane.
         const int F = kv8_group(sl.n_pieces, kKcRows * HD * 4), g0 = sl.ch / F * F, in_group = min(F, sl.n_pieces - g0), groups = (sl.n_pieces + F - 1) / F;
-        const int64_t part0 = int64_t(slot_i - sl.ch) * HI + hi_i;
+        const int64_t part0 = int64_t(sl.part - sl.ch) * HI + hi_i;
         auto ml_at = [&](int i) { return kv8_ml(late.a, late.plan, part0 + int64_t(i) * HI) + wave * 32 + col; };
         auto o_at = [&](int i, int j) { return kv8_o<HD>(late.a, late.plan, part0 + int64_t(i) * HI) + (wave * (HD / 4) + j) * 64 + lane; };
         auto put = [&](int i) FA_INLINE {
