@@ -859,18 +859,21 @@ class FlashAttnRotaryFunc(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(*(x for x in rest if isinstance(x, torch.Tensor)))
         ctx.rest = tuple(None if isinstance(x, torch.Tensor) else (x,) for x in rest)
-        return tuple(flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest, False))
+        return tuple(flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest))
 
     @staticmethod
     def backward(ctx, dq, dk):
         tensors = iter(ctx.saved_tensors)
         rest = tuple(next(tensors) if x is None else x[0] for x in ctx.rest)
-        dq, dk = maybe_contiguous(dq), maybe_contiguous(dk)
-        if dq is None and dk is not None:  # a gradient of k alone
-            dk = flash_attn_gpu.rotary(dk, None, *rest, True)[0]
-        elif dq is not None:
-            dq, dk = flash_attn_gpu.rotary(dq, dk, *rest, True)
-        return (dq, dk) + (None,) * len(rest)
+        back = (*rest[:-1], not rest[-1])
+        # (A gradient of k alone is rotated as q.)
+        x, y = (dk, None) if dq is None else (dq, dk)
+        if x is not None:
+            if torch.is_grad_enabled():  # create_graph: the gradient is a rotation, too, with a gradient of its own
+                x, y = FlashAttnRotaryFunc.apply(x, y, *back)
+            else:
+                x, y = flash_attn_gpu.rotary(maybe_contiguous(x), maybe_contiguous(y), *back)
+        return ((None, x) if dq is None else (x, y)) + (None,) * len(rest)
 
 
 def flash_attn_rotary_func(
@@ -888,7 +891,7 @@ def flash_attn_rotary_func(
     positions (int32, (batch, seqlen) or (total,)), where they say.  A row whose position the tables do not have becomes
     NaN in the rotated channels.
 
-    Returns q and k rotated, new tensors (q alone where k is None); q and k get gradients, the tables none."""
+    Returns q and k rotated, new tensors (q alone where k is None); q and k get gradients of any order, the tables none."""
     for name, t in (("rotary_cos", rotary_cos), ("rotary_sin", rotary_sin)):
         if not isinstance(t, torch.Tensor) or t.dim() != 2:
             raise TypeError(f"{name} must be a 2-D tensor (rows, rotary_dim / 2)")
@@ -903,14 +906,14 @@ def flash_attn_rotary_func(
     elif not isinstance(seqlen_offsets, int):
         raise TypeError("seqlen_offsets must be an int or a torch.int32 tensor")
     rest = (maybe_contiguous(rotary_cos), maybe_contiguous(rotary_sin), rotary_interleaved, positions,
-            maybe_contiguous(offsets), offset, maybe_contiguous(cu_seqlens))
+            maybe_contiguous(offsets), offset, maybe_contiguous(cu_seqlens), False)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
                                     or rotary_cos.requires_grad or rotary_sin.requires_grad):
         if rotary_cos.requires_grad or rotary_sin.requires_grad:
             raise RuntimeError("rotary_cos and rotary_sin get no gradient")
         q, k = FlashAttnRotaryFunc.apply(q, k, *rest)
     else:
-        q, k = flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest, False)
+        q, k = flash_attn_gpu.rotary(maybe_contiguous(q), maybe_contiguous(k), *rest)
     return q if k is None else (q, k)
 
 
