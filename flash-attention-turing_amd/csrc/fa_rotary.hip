@@ -7,6 +7,7 @@
 //
 // A wave takes one row of q and k, all heads: the row's cosines and sines go to registers once (16 a lane) and serve
 // every head, and each load or store of the wave covers whole 128-byte lines.
+#include <algorithm>
 #include <cmath>
 
 #include "fa_diff_common.h"
@@ -163,7 +164,8 @@ struct RotaryTurns {
     double f[FA_ROTARY_MAX_DIM / 2];  // turns a token
 };
 
-// cos and sin of 2 pi t.  t less its nearest quarter turn leaves an angle y of at most pi / 4; the Taylor sums of sine
+// cos and sin of 2 pi t.  A turn count has four roundings of 2^-53: the angle is off by 2^-51 of itself, 2^-25 at the last position
+// that the tables may have (FA_ROTARY_MAX_POSITION), half a step of fp32.  t less its nearest quarter turn leaves an angle y of at most pi / 4; the Taylor sums of sine
 // and cosine to y^11 and y^12 are off by less than 1e-11 there, far under half a step of fp32.
 __device__ __forceinline__ void rt_cos_sin(double t, double &c, double &s) {
     t -= rint(t);
@@ -225,7 +227,8 @@ extern "C" int fa_rotary_tables(const fa_rotary_tables_args *args, void *stream)
     if (a.rotary_dim <= 0 || a.rotary_dim % 16 || a.rotary_dim > FA_ROTARY_MAX_DIM || a.seqlen < 0) return FA_ERR_INVALID_ARG;
     if (a.dtype != FA_FP16 && a.dtype != FA_BF16 && a.dtype != FA_FP32) return FA_ERR_UNSUPPORTED;
     if (!(a.base > 0) || !(a.factor > 0) || !(a.original_seqlen >= 0) || !std::isfinite(a.attention_factor) ||
-        a.offset > (int64_t(1) << 52) || a.offset < -(int64_t(1) << 52) ||
+        a.offset < -FA_ROTARY_MAX_POSITION || a.offset > FA_ROTARY_MAX_POSITION ||
+        a.offset + std::max(a.seqlen, 1) - 1 > FA_ROTARY_MAX_POSITION ||
         (a.original_seqlen > 0 && !(a.high_turns > a.low_turns)))
         return FA_ERR_INVALID_ARG;
     if (a.seqlen == 0) return FA_OK;

@@ -826,7 +826,8 @@ def flash_attn_rotary_tables(
     dtype: torch.dtype = torch.float32, device: Union[torch.device, str, int, None] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """cos and sin (seqlen, rotary_dim / 2) of the angles (offset + i) * f_j, f_j = base ** (-2 j / rotary_dim), computed
-    in 64 bits and rounded once to dtype (float32, float16 or bfloat16); rotary_dim is a multiple of 16.
+    in 64 bits and rounded once to dtype (float32, float16 or bfloat16); rotary_dim is a multiple of 16.  Positions lie
+    within 2 ** 26 of 0, where 64 bits leave the angles right to half a step of float32.
 
     For contexts longer than those of the training by a factor: f_j / factor, or, with original_seqlen (the training's
     length), by the turns t that a pair makes in it: f_j for t >= high_turns, f_j / factor for t <= low_turns, and
@@ -838,6 +839,8 @@ def flash_attn_rotary_tables(
         raise ValueError("rotary_dim must be a multiple of 16 up to 256")
     if seqlen < 0:
         raise ValueError("seqlen must be non-negative")
+    if abs(offset) > 2 ** 26 or offset + max(seqlen, 1) - 1 > 2 ** 26:
+        raise ValueError("positions must be within 2 ** 26 of 0")
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError("dtype must be torch.float32, torch.float16 or torch.bfloat16")
     if not all(math.isfinite(x) for x in (base, factor, attention_factor)) or base <= 0 or factor <= 0:

@@ -432,12 +432,15 @@ int fa_kvpages_compact(const fa_kvpages_args *args, void *stream);
  * No counterpart in the reference.
  */
 #define FA_ROTARY_MAX_DIM 256
+/* Positions of the tables: up to here, to either side, angles in 64 bits are right to half a step of fp32 (2^-25). */
+#define FA_ROTARY_MAX_POSITION (1 << 26)
 
 /* cos and sin, [seqlen][rotary_dim / 2] of dtype: entry (i, j) is attention_factor times the
  * cosine / sine of (offset + i) * f_j, computed in 64 bits, f_j = base ^ (-2 j / rotary_dim).
  * factor != 1 divides the frequencies: all of them (original_seqlen 0), or, by the turns t that
  * a pair makes in original_seqlen tokens, f_j (keep + (1 - keep) / factor) with
- * keep = (t - low_turns) / (high_turns - low_turns) cut to [0, 1]. */
+ * keep = (t - low_turns) / (high_turns - low_turns) cut to [0, 1].  All positions lie within
+ * FA_ROTARY_MAX_POSITION of 0. */
 typedef struct fa_rotary_tables_args {
     void *cos, *sin;                /* 16-byte aligned                           */
     int32_t seqlen, rotary_dim;     /* rotary_dim: a multiple of 16 up to FA_ROTARY_MAX_DIM */
