@@ -766,6 +766,15 @@ def _check_pages(block_table=None, cache_seqlens=None, page_refs=None, **lists) 
             raise RuntimeError(f"{name} must be a CUDA tensor")
 
 
+def _check_whole(what: str, *pools) -> None:
+    """Pools of codes are half of a cache in 8 bits: a call that plans its copies itself would leave their scales behind."""
+    for c in pools:
+        if isinstance(c, torch.Tensor) and c.dtype in (torch.float8_e4m3fn, torch.int8):
+            raise NotImplementedError(
+                f"{what} would leave the scales of a cache in 8 bits behind; use flash_attn_kvcache_copy_pages for codes and "
+                "scales (pools of bytes without scales: .view(torch.uint8))")
+
+
 def flash_attn_kvcache_alloc(block_table, cache_seqlens, page_refs, seqlen_new: Union[int, torch.Tensor],
                              page_block_size: int, validate: bool = True) -> None:
     """Give every row the pages that its next seqlen_new tokens (an int, or int32 [rows], 0 for none) need and its
@@ -793,7 +802,9 @@ def flash_attn_kvcache_fork(k_cache, v_cache, block_table, cache_seqlens, page_r
                             children: torch.Tensor, validate: bool = True) -> None:
     """Make row children[i] (empty, in the list once, no parent itself) a fork of row parents[i]: it shares the
     parent's full pages, and where the parent's last page is partly filled it gets a free page (lowest first, in the
-    list's order) with a copy of that page's tokens; the rest of that page is left as it was."""
+    list's order) with a copy of that page's tokens; the rest of that page is left as it was.  Not for the codes of a cache
+    in 8 bits, whose scales would stay behind."""
+    _check_whole("flash_attn_kvcache_fork", k_cache, v_cache)
     _check_pages(block_table, cache_seqlens, page_refs, parents=parents, children=children)
     _kv_pages_call(flash_attn_gpu.kvpages_fork, block_table.device, validate, k_cache, v_cache, block_table,
                    cache_seqlens, page_refs, parents, children)
@@ -811,7 +822,8 @@ def flash_attn_kvcache_compact(k_cache, v_cache, block_table, page_refs) -> Tupl
     """Move the pages in use to the front of the pools: with n of them, the k-th free page below n takes the contents
     of the k-th used page from n on.  Returns the table and the counts afterwards (new tensors) and n (int32 [1]).
     The moved pages stay as they were in their old places, so the old table stays right for work that is already
-    queued, until those pages are given out again."""
+    queued, until those pages are given out again.  Not for the codes of a cache in 8 bits, whose scales would stay behind."""
+    _check_whole("flash_attn_kvcache_compact", k_cache, v_cache)
     _check_pages(block_table, page_refs=page_refs)
     return flash_attn_gpu.kvpages_compact(k_cache, v_cache, block_table, page_refs)
 
