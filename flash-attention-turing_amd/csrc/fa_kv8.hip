@@ -15,8 +15,9 @@ namespace fa {
 // two: the quotients are exact, codes that stay in e4m3's normal range keep their bits when a scale grows, and a block is
 // raised at most a few times however many appends fill it.
 //
-// One token for each of 64 sequences takes 5 us, a chain of four latencies (length, page, rows, scale); 4 prompts of up to 4096
-// tokens 15 us at 4.8 TB/s, a copy's rate at that size.
+// One token for each of 64 sequences takes 5 us, a chain of four latencies (length, page, rows, scale), and where it raises the
+// scale of a full block 3 us more (64 tokens) to 10 (256); 4 prompts of up to 4096 tokens 15 us at 4.8 TB/s, a copy's rate
+// at that size.
 
 constexpr int kKv8Threads = 256;
 constexpr int64_t kKv8MaxGrid = 0xffffffffu / kKv8Threads;  // a launch has less than 2^32 threads
@@ -593,8 +594,8 @@ int kv8_chunk(const fa_kv8_args &a, const Kv8Plan &plan, hipStream_t s);  // fa_
 
 // KV heads that a workgroup of few rows takes together, one or two: their codes of a token are neighbours in memory, which reads
 // longer runs faster, but there are fewer items to share a short call.  Measured (us, one and two), 8 heads of 128 channels:
-// 64 x 8192 tokens 192 and 173, 8 x 32000 102 and 98, 2 x 131072 105 and 107, 1 x 131072 62 and 77; heads of 64, whose codes are
-// half a line: 8 heads 64 x 8192 174 and 117, 1 x 131072 57 and 45, 4 heads 4 x 48000 47 and 44.  (Four of 64: 114, 81 and 58.)
+// 64 x 8192 tokens 193 and 173, 8 x 32000 102 and 98, 2 x 131072 106 and 106, 1 x 131072 60 and 76; heads of 64, whose codes are
+// half a line: 8 heads 64 x 8192 173 and 116, 1 x 131072 56 and 45, 4 heads 4 x 48000 43 and 35.
 static int kv8_heads(const fa_kv8_args &a) {
     const int64_t bytes = int64_t(a.cache.batch) * a.cache.cache_capacity * a.cache.nheads_k * a.cache.head_dim * 2;
     const bool two = a.cache.head_dim == 64 ? bytes >= 32 << 20 : bytes >= 256 << 20 && a.cache.batch >= 4;
@@ -605,8 +606,8 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     Kv8Plan p{};
     const int64_t rows = int64_t(a.nheads / a.cache.nheads_k) * a.seqlen_q, cap = std::max(a.cache.cache_capacity, 1);
     // The kernel of many rows reads and converts the codes once for 128 rows, the other one for 16, but it starts later and its
-    // pieces' results are large.  Measured, by the 16-row tiles' keys (us, few and many): 32 rows of 8 heads x 8192 keys 26 and 37,
-    // 512 rows x 8192 55 and 50, 1024 x 32768 319 and 164; batch of 32 x 20 rows x 6144 131 and 144, 16 x 32 x 8192 86 and 79.
+    // pieces' results are large.  Measured, by the 16-row tiles' keys (us, few and many): 32 rows of 8 heads x 8192 keys 25 and 37,
+    // 512 rows x 8192 57 and 50, 1024 x 32768 323 and 164; batch of 32 x 20 rows x 6144 101 and 110, 16 x 32 x 8192 80 and 74.
     const int64_t few_keys = (rows + kKdRows - 1) / kKdRows * a.cache.nheads_k * a.cache.batch * cap;
     // A given number of pieces asks for sums that do not depend on the batch.
     p.many = a.num_splits > 0 ? rows >= 4 * kKdRows : rows >= 2 * kKdRows && few_keys >= int64_t(6144) * device_cus();
@@ -618,7 +619,7 @@ static Kv8Plan kv8_plan(const fa_kv8_args &a) {
     p.items = a.cache.batch * heads;
     p.least = p.many ? 512 : 256;  // fewer and longer: 8 heads x 512 rows x 2048 keys took 36 us at 256 and 31 us at 512
     // Two workgroups run on a CU.  One reads memory as fast, but more rows compute, too (us, one a CU and two): 24 rows x 9000 keys
-    // 25 and 28.5, but 64 rows x 2000 keys of 8 sequences 37 and 29, 256 rows x 8192 keys 47 and 39.
+    // 24 and 27, 64 rows x 2000 keys of 8 sequences 29 and 30, but 256 rows x 8192 keys 49 and 39.
     p.most = int(std::max<int64_t>(2 * device_cus() / heads, 1));
     p.want = p.many || p.row_tiles > 2 ? p.most : int(std::max<int64_t>(device_cus() / heads, 1));
     int64_t slots, parts;
@@ -692,7 +693,7 @@ static int launch_kv8_append(const fa_kv8_args &a, const Kv8Plan *plan, hipStrea
             return int(hipGetLastError());
         };
         // As many units a thread as a block or the call has at most: registers for more cost waves.  4 x 2048 tokens, 8 heads (us,
-        // so many and the most): blocks of 32, 64 channels, 12.8 and 15.3 (1 and 8); of 64, 128 channels, 11.4 and 15.4 (4 and 16);
+        // so many and the most): blocks of 32, 64 channels, 12.8 and 15.2 (1 and 8); of 64, 128 channels, 11.2 and 15.5 (4 and 16);
         // 4 prompts of up to 4096 tokens, blocks of 128, 15.3 and 16.9 (8 and 16).
         if (most <= kKv8Threads) return go(std::integral_constant<int, 1>{});
         if (most <= 4 * kKv8Threads) return go(std::integral_constant<int, 4>{});

@@ -233,8 +233,8 @@ __device__ __forceinline__ void kv8_make_plan(const fa_kv8_args &a, const Kv8Pla
         piece = length(1.f, plan.want);
         // Few rows, where a piece costs little besides its codes: the shortest of four lengths whose pieces all run at once, at one
         // workgroup a CU or else at two; where none fits, as with lengths far apart, half the share of these: pieces that start as
-        // places become free.  Measured (us, one and two a CU): 64 x 8192 173 and 186, 4 x 48000 43 and 48, 2 x 9000 25 and 28.5;
-        // two a CU and half their share: 64 x 1024-16384 202 and 172.
+        // places become free.  Measured (us, one and two a CU): 64 x 8192 172 and 186, 4 x 48000 37 and 40, 2 x 9000 22 and 24;
+        // two a CU and half their share: 64 x 1024-16384 188 and 172.
         const int at[8] = {piece, length(1.0625f, plan.want), length(1.125f, plan.want), length(1.25f, plan.want),
                            length(1.f, plan.most), length(1.0625f, plan.most), length(1.125f, plan.most), length(1.25f, plan.most)};
         if (!plan.many && a.cache.batch > 1 && at[3] > plan.least) {
@@ -372,7 +372,8 @@ __device__ __forceinline__ bool kv8_count(int32_t *count, int n, int *ticket) {
 
 // Pieces of an item are joined in one step, or, where their partial results (bytes each for a KV head) are many, eight at a time
 // by the last workgroup of the eight, whose result takes the place of the first one's, and then these: one workgroup would read
-// too long.  Measured (us, one step and two): 40 pieces of 4 KB 58 and 47, 40 of 2 KB 26.6 and 27.5, 64 of 2 KB 31.8 and 31.8.
+// too long.  Measured (us, one step and two): 4 x 48000 tokens in 40 pieces of 4 KB 51.5 and 49.5, 1 x 65536 in 64 pieces of 4 KB
+// 38 and 33; 8 heads of 128 channels, 1 x 65536 in 40 pieces of 2 KB 45 and 47.
 __device__ __forceinline__ int kv8_group(int n_pieces, int bytes) {
     return n_pieces <= 8 || int64_t(n_pieces) * bytes <= 128 << 10 ? n_pieces : 8;
 }

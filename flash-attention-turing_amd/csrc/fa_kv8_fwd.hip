@@ -2,21 +2,23 @@
 //
 // A workgroup takes 128 rows of a KV head (its query heads times the query positions) and one piece of the
 // sequence's keys, 64 at a time.  Codes go from memory straight to a ring of four LDS stages and stay 8 bits there: half the
-// LDS traffic, and each wave converts what it reads.  (Converted once for the workgroup, through registers and 16-bit LDS, the same
+// LDS traffic, and each wave converts what it reads.  (Converted once for the workgroup, through registers and 16-bit LDS, a
 // call took 183 us against 172: the barriers and writes cost more than the conversions.)  Scales multiply scores and
 // probabilities.  Four waves of 32 rows: S^T = K Q^T, so that a lane owns a row, and P^T feeds O^T += V^T P^T from the
 // accumulators, half a tile behind.
 //
 // P times V's scale is rounded to fp16 for both types of q, as P is in the forward kernels: codes make the products exact,
-// and 11 bits are no fewer than the output keeps.  (As hi + lo, which the kernel of few rows has, where the
-// product with V costs nothing, 1160 -> 1590 us at 2048 queries over 32768 keys, 179 -> 238 at 2 x 512 over 4k to 12k.)  fp16's
-// range suffices because O has a reference of its own, a row's largest score + log2(V's scale) so far: keys that a row does
-// not see, or whose probability is small, take no bits from the others, whatever their V is.  What rounds to 0 is 2^-30 of the
-// row's largest p * scale.
+// and 11 bits are no fewer than the output keeps.  Against 64 bits a bf16 output is as far off as one that is rounded alone
+// (0.0017 of its norm), an fp16 output up to 1.4 times (0.00027 and 0.00021).  P as hi + lo, which the kernel of few rows has, where
+// the product with V costs nothing, would not add that, but half of the products: 175 -> 238 us at 2 x 512 queries over 4k to
+// 12k keys, 1145 -> 1605 at 2048 over 32768.  fp16's range suffices because O has a reference of its own, a row's largest
+// score + log2(V's scale) so far: keys that a row does not see, or whose probability is small, take no bits from the others,
+// whatever their V is.  What rounds to 0 is 2^-30 of the row's largest p * scale.
 //
-// What bounds it: matrix and vector instructions of the same SIMDs, 43 and 62 % of the cycles at 2 x 512 queries over 4k to
-// 12k tokens (32/8 heads of 128, e4m3: 166 us of a call's 172, 0.86 PFLOP/s), 0.99 PFLOP/s at 2048 queries over 32768; int8 takes
-// a quarter longer, four conversions an operand where e4m3 has two.  Row tiles of a KV head share an XCD's L2 (kv8_item).
+// What bounds it: matrix and vector instructions of the same SIMDs, 43 and 65 % of the cycles at 2 x 512 queries over 4k to
+// 12k tokens (32/8 heads of 128, e4m3, bf16: 173 us a call, 0.86 PFLOP/s), 0.99 PFLOP/s at 2048 queries over 32768 (1148 us); int8
+// takes a quarter to a third longer (218 and 1482): 10 or 12 instructions convert an operand where e4m3 has 4.  Row tiles of a
+// KV head share an XCD's L2 (kv8_item).
 #include <algorithm>
 
 #include "fa_kv8_common.h"
