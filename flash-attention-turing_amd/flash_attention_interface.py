@@ -1068,7 +1068,9 @@ def flash_attn_with_kvcache_q8(
 
     The keys are cut into pieces on the device by the lengths of the whole batch; num_splits > 0 cuts the cache's capacity
     into that many instead, and a row's bits then do not depend on the batch.  return_softmax_lse adds the log-sum-exp,
-    fp32 (batch, nheads, seqlen_q).  A q without rows (seqlen_q 0) appends alone.  For rotary positions rotate q and k by
+    fp32 (batch, nheads, seqlen_q).  Calls with few query rows a KV head (nheads / nheads_k * seqlen_q) keep 16 bits of the
+    probabilities in the product with v, calls with many 11, as flash_attn_func does: many are 64 where num_splits is given,
+    else from 32 on by the work that the cache's capacity allows.  A q without rows (seqlen_q 0) appends alone.  For rotary positions rotate q and k by
     flash_attn_rotary_func(..., seqlen_offsets=cache_seqlens) first.
 
     validate as in flash_attn_kvcache_append_q8; with False a call can be captured in a graph, a sequence with a bad length

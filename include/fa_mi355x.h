@@ -417,7 +417,7 @@ int fa_kvpages_alloc(const fa_kvpages_args *args, void *stream);
 /* Page to[i] = page from[i], all at once; pairs that touch each other's pages are not copied (FA_KV_BAD_LIST). */
 int fa_kvpages_copy(const fa_kvpages_args *args, void *stream);
 /* Row to[i] (empty) shares the full pages of row from[i] and gets a page with a copy of the tokens of a last, partly
- * filled one. */
+ * filled one.  (This and compact move one pair of pools: not the codes of a cache in 8 bits, whose scales would stay.) */
 int fa_kvpages_fork(const fa_kvpages_args *args, void *stream);
 /* Rows from[i] give their pages back and become empty. */
 int fa_kvpages_free(const fa_kvpages_args *args, void *stream);
